@@ -41,7 +41,14 @@ class Tile(ctypes.Structure):
                 ("stride", ctypes.c_int * 4), ("size", ctypes.c_int * 4)]
 
 
+class Array(ctypes.Structure):
+    """fbfft_array of include/fbfft_amd.h."""
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_longlong * MAX_DIM),
+                ("size", ctypes.c_longlong * MAX_DIM), ("dim", ctypes.c_int), ("type", ctypes.c_int)]
+
+
 assert ctypes.sizeof(Tile) == 48
+assert ctypes.sizeof(Array) == 96
 
 _lib = None
 _calls = None
@@ -56,7 +63,13 @@ EXPORTS = (
     "fbfft_conv_choose_fft_size", "fbfft_conv_workspace", "fbfft_conv_workspace_image", "fbfft_conv_fprop_workspace", "fbfft_conv_fprop", "fbfft_conv_bprop",
     "fbfft_conv_accgrad", "fbfft_conv_fprop_static", "fbfft_bench_copy", "fbfft_error_string",
     "fbfft_twiddle_table",
+    "fbfft_group_norm_workspace", "fbfft_group_norm_fprop", "fbfft_group_norm_bprop",
+    "fbfft_linear_workspace", "fbfft_linear_fprop", "fbfft_linear_bprop",
+    "fbfft_dropout_fprop", "fbfft_dropout_bprop",
 )
+
+# enum fbfft_activation of include/fbfft_amd.h
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 def lib():
@@ -106,6 +119,18 @@ def lib():
         L.fbfft_conv_accgrad.argtypes = [tp, tp, tp, ctypes.c_int, ctypes.c_float, ctypes.c_int, vp,
                                          ctypes.c_size_t, vp]
         L.fbfft_conv_fprop_static.argtypes = [tp, tp, tp, ctypes.c_int, vp]
+        ap, ll, ull, i32, size = (ctypes.POINTER(Array), ctypes.c_longlong, ctypes.c_ulonglong, ctypes.c_int,
+                                  ctypes.c_size_t)
+        L.fbfft_group_norm_workspace.argtypes = [i32] + [ll] * 4
+        L.fbfft_group_norm_workspace.restype = size
+        L.fbfft_group_norm_fprop.argtypes = [ap] * 6 + [ll, ctypes.c_float, i32, vp, size, vp]
+        L.fbfft_group_norm_bprop.argtypes = [ap] * 9 + [ll, i32, vp, size, vp]
+        L.fbfft_linear_workspace.argtypes = [i32] + [ll] * 3 + [i32]
+        L.fbfft_linear_workspace.restype = size
+        L.fbfft_linear_fprop.argtypes = [ap] * 6 + [i32, vp, size, vp]
+        L.fbfft_linear_bprop.argtypes = [ap] * 7 + [i32, vp, size, vp]
+        L.fbfft_dropout_fprop.argtypes = [ap] * 3 + [ctypes.c_double, ull, ull, vp, vp]
+        L.fbfft_dropout_bprop.argtypes = [ap] * 2 + [ctypes.c_double, ull, ull, vp, vp]
         L.fbfft_bench_copy.argtypes = [vp, vp, ctypes.c_size_t, vp]
         L.fbfft_error_string.argtypes = [ctypes.c_int]
         L.fbfft_error_string.restype = ctypes.c_char_p
@@ -472,3 +497,160 @@ def conv_accgrad(input, gradOutput, gradWeight, fftSize, workspace, scale=1.0, a
                                        scale, int(bool(accumulate)),
                                        workspace.data_ptr(),
                                        workspace.numel() * workspace.element_size(), _stream(stream))
+
+
+# ---- operators around a convolution layer: float32, float16 and bfloat16, any strides ----
+
+def _types():
+    import torch
+    return {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def array(t):
+    """fbfft_array describing a float32, float16 or bfloat16 torch tensor; None for None."""
+    if t is None:
+        return None
+    kind = _types().get(t.dtype)
+    if kind is None:
+        raise TypeError("operands are float32, float16 or bfloat16, not %s" % t.dtype)
+    if t.dim() > MAX_DIM:
+        raise ValueError("rank > %d" % MAX_DIM)
+    a = Array()
+    a.data, a.dim, a.type = t.data_ptr(), t.dim(), kind
+    a.size[:t.dim()], a.stride[:t.dim()] = t.size(), t.stride()
+    return a
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError("activation is one of %s, not %r" % (", ".join(ACTIVATIONS), name))
+    return ACTIVATIONS[name]
+
+
+def _space(workspace):
+    """(address, bytes) of a workspace, which may be None."""
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
+def _given(*ts):
+    _on_gpu(*(t for t in ts if t is not None))
+    return [array(t) for t in ts]
+
+
+def group_norm_workspace(pass_, input, groups):
+    """Workspace bytes of group_norm_fprop (pass 0) or group_norm_bprop (1) on this input [B][C][H][W]."""
+    b, c, h, w = input.shape
+    return lib().fbfft_group_norm_workspace(int(pass_), b, c, h * w, groups)
+
+
+def group_norm_fprop(input, weight, bias, output, groups, workspace, activation="none", eps=1e-5, mean=None, rstd=None,
+                     stream=None):
+    """output = activation((input - mean) * rstd * weight + bias), mean and rstd = 1 / sqrt(var + eps) over each
+    image's groups of channels.
+
+    input, output: [B][C][H][W] of one type, any strides (channels last: `.permute(0, 3, 1, 2)` of [B][H][W][C]).
+    weight, bias: [C] of any type, or None.  mean, rstd: float32 [B][groups], written for group_norm_bprop, or None.
+    output may be input."""
+    act = _activation(activation)
+    if stream is None:
+        rc = (_native or _load_native()).group_norm_fprop(input, weight, bias, output, mean, rstd, groups, float(eps), act,
+                                                          workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_group_norm_fprop(*_given(input, weight, bias, output, mean, rstd), groups, float(eps), act,
+                                        *_space(workspace), _stream(stream))
+
+
+def group_norm_bprop(input, weight, bias, mean, rstd, gradOutput, gradInput, gradWeight, gradBias, groups, workspace,
+                     activation="none", stream=None):
+    """The gradients of group_norm_fprop from its input, mean and rstd.  gradInput, gradWeight, gradBias: any of them
+    None where it is not wanted; gradInput may be gradOutput."""
+    act = _activation(activation)
+    if stream is None:
+        rc = (_native or _load_native()).group_norm_bprop(input, weight, bias, mean, rstd, gradOutput, gradInput, gradWeight,
+                                                          gradBias, groups, act, workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_group_norm_bprop(
+        *_given(input, weight, bias, mean, rstd, gradOutput, gradInput, gradWeight, gradBias), groups, act,
+        *_space(workspace), _stream(stream))
+
+
+def linear_workspace(pass_, rows, inputs, outputs, dtype):
+    """Workspace bytes of linear_fprop (pass 0) or linear_bprop (1) on input [rows][inputs], weight [outputs][inputs]."""
+    kind = _types().get(dtype)
+    if kind is None:
+        raise TypeError("operands are float32, float16 or bfloat16, not %s" % dtype)
+    return lib().fbfft_linear_workspace(int(pass_), rows, inputs, outputs, kind)
+
+
+def linear_fprop(input, weight, bias, output, workspace, activation="none", residual=None, preactivation=None,
+                 stream=None):
+    """z = input weight^T + bias, output = activation(z) + residual.
+
+    input [M][K], weight [N][K], residual, preactivation, output [M][N] of one type, any strides; bias [N] of any
+    type.  bias, residual: or None.  preactivation: z is written there for linear_bprop, or None.  The rows are the pixels of a
+    channels-last image for a 1 x 1 projection.  residual may be output."""
+    act = _activation(activation)
+    if stream is None:
+        rc = (_native or _load_native()).linear_fprop(input, weight, bias, residual, output, preactivation, act, workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_linear_fprop(*_given(input, weight, bias, residual, output, preactivation), act, *_space(workspace),
+                                    _stream(stream))
+
+
+def linear_bprop(input, weight, gradOutput, preactivation, gradInput, gradWeight, gradBias, workspace, activation="none",
+                 stream=None):
+    """The gradients of linear_fprop: with dz = gradOutput * activation'(preactivation), gradInput = dz weight,
+    gradWeight = dz^T input, gradBias = sum of dz's rows; any of the three None where it is not wanted.  (The
+    residual's gradient is gradOutput itself.)"""
+    act = _activation(activation)
+    if stream is None:
+        rc = (_native or _load_native()).linear_bprop(input, weight, gradOutput, preactivation, gradInput, gradWeight, gradBias,
+                                                      act, workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_linear_bprop(*_given(input, weight, gradOutput, preactivation, gradInput, gradWeight, gradBias), act,
+                                    *_space(workspace), _stream(stream))
+
+
+def _step(step):
+    """The address of a step: an int64 GPU tensor of one element, or None."""
+    if step is None:
+        return None
+    import torch
+    _on_gpu(step)
+    if step.dtype != torch.int64 or step.numel() != 1:
+        raise TypeError("a step is one int64")
+    return step.data_ptr()
+
+
+def dropout_fprop(input, output, p, seed, offset, residual=None, step=None, stream=None):
+    """output = (input / (1 - p) where a number of the counter-based generator keeps it, 0 elsewhere) + residual.
+
+    The mask follows from seed, offset (+ step, one int64 in GPU memory that a captured graph may add to) and an element's
+    place in the shape alone, whatever the strides; p is rounded to a 65536th, and the factor is that of the rounded
+    value.  output may be input or residual."""
+    if stream is None and step is None:
+        rc = (_native or _load_native()).dropout(input, residual, output, float(p), seed, offset)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_dropout_fprop(*_given(input, residual, output), float(p), _word(seed), _word(offset), _step(step),
+                                     _stream(stream))
+
+
+def dropout_bprop(gradOutput, gradInput, p, seed, offset, step=None, stream=None):
+    """gradInput = gradOutput under the mask and factor of dropout_fprop with the same p, seed, offset and step."""
+    if stream is None and step is None:
+        rc = (_native or _load_native()).dropout(gradOutput, None, gradInput, float(p), seed, offset)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_dropout_bprop(*_given(gradOutput, gradInput), float(p), _word(seed), _word(offset), _step(step),
+                                     _stream(stream))
+
+
+def _word(v):
+    if not 0 <= v < 2 ** 64:
+        raise ValueError("seed and offset are 64-bit unsigned integers")
+    return v

@@ -6,7 +6,8 @@
 // of this module).  Here a descriptor is filled from the tensor itself.
 //
 // Each function takes plain calls only - float32 GPU tensors of exact type Tensor or Parameter and
-// rank up to 5 whose extents fit 32 bits, integers that fit, the current stream - and returns
+// rank up to 5 whose extents fit 32 bits (the operators around a layer: any of their three types, 64
+// bits), integers that fit, the current stream - and returns
 // NotImplemented for any other, which its caller then makes by the general way with that way's
 // results and errors.  The C entry point runs without the interpreter lock, as under ctypes.
 #define PY_SSIZE_T_CLEAN
@@ -171,6 +172,133 @@ PyObject* accgrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- operators around a convolution layer: arrays of three types, any of them possibly None ----
+
+struct Arrays {
+  fbfft_array filled[9];
+  const fbfft_array* at[9];
+};
+
+// None, or a tensor of one of the three types
+bool arrayOf(PyObject* o, fbfft_array* a, const fbfft_array** at) {
+  *at = nullptr;
+  if (o == Py_None) return true;
+  if (!THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() > FBFFT_MAX_DIM) return false;
+  *a = fbfft_array{};
+  switch (t.scalar_type()) {
+    case at::kFloat: a->type = FBFFT_FLOAT32; break;
+    case at::kHalf: a->type = FBFFT_FLOAT16; break;
+    case at::kBFloat16: a->type = FBFFT_BFLOAT16; break;
+    default: return false;
+  }
+  a->dim = (int)t.dim();
+  for (int i = 0; i < a->dim; ++i) {
+    a->size[i] = t.size(i);
+    a->stride[i] = t.stride(i);
+  }
+  a->data = t.data_ptr();
+  *at = a;
+  return true;
+}
+
+bool arraysOf(PyObject* const* objects, int n, Arrays* to) {
+  for (int i = 0; i < n; ++i)
+    if (!arrayOf(objects[i], &to->filled[i], &to->at[i])) return false;
+  return true;
+}
+
+bool space(PyObject* o, void** p, size_t* bytes) {
+  *p = nullptr;
+  *bytes = 0;
+  return o == Py_None || memory(o, p, bytes);
+}
+
+bool word(PyObject* o, unsigned long long* v) {
+  if (!PyLong_Check(o)) return false;
+  *v = PyLong_AsUnsignedLongLong(o);
+  if (!PyErr_Occurred()) return true;
+  PyErr_Clear();
+  return false;
+}
+
+// (input, weight, bias, output, mean, rstd, groups, eps, activation, workspace)
+PyObject* normForward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 10, [&]() -> PyObject* {
+    Arrays x;
+    int groups, activation;
+    float eps;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 6, &x) || !integer(a[6], &groups) || !real(a[7], &eps) || !integer(a[8], &activation) ||
+        !space(a[9], &ws, &bytes))
+      Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_group_norm_fprop(x.at[0], x.at[1], x.at[2], x.at[3], x.at[4], x.at[5], groups, eps, activation, ws,
+                                    bytes, (fbfft_stream_t)s);
+    });
+  });
+}
+
+// (input, weight, bias, mean, rstd, gradOutput, gradInput, gradWeight, gradBias, groups, activation, workspace)
+PyObject* normBackward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 12, [&]() -> PyObject* {
+    Arrays x;
+    int groups, activation;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 9, &x) || !integer(a[9], &groups) || !integer(a[10], &activation) || !space(a[11], &ws, &bytes))
+      Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_group_norm_bprop(x.at[0], x.at[1], x.at[2], x.at[3], x.at[4], x.at[5], x.at[6], x.at[7], x.at[8],
+                                    groups, activation, ws, bytes, (fbfft_stream_t)s);
+    });
+  });
+}
+
+// (input, weight, bias, residual, output, preactivation, activation, workspace)
+PyObject* linearForward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    Arrays x;
+    int activation;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 6, &x) || !integer(a[6], &activation) || !space(a[7], &ws, &bytes)) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_linear_fprop(x.at[0], x.at[1], x.at[2], x.at[3], x.at[4], x.at[5], activation, ws, bytes, (fbfft_stream_t)s);
+    });
+  });
+}
+
+// (input, weight, gradOutput, preactivation, gradInput, gradWeight, gradBias, activation, workspace)
+PyObject* linearBackward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    Arrays x;
+    int activation;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 7, &x) || !integer(a[7], &activation) || !space(a[8], &ws, &bytes)) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_linear_bprop(x.at[0], x.at[1], x.at[2], x.at[3], x.at[4], x.at[5], x.at[6], activation, ws, bytes,
+                                (fbfft_stream_t)s);
+    });
+  });
+}
+
+// (input, residual, output, p, seed, offset); a step in device memory goes the general way
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    Arrays x;
+    unsigned long long seed, offset;
+    if (!arraysOf(a, 3, &x) || !PyFloat_Check(a[3]) || !word(a[4], &seed) || !word(a[5], &offset)) Py_RETURN_NOTIMPLEMENTED;
+    const double p = PyFloat_AS_DOUBLE(a[3]);
+    return call([&](void* s) {
+      return fbfft_dropout_fprop(x.at[0], x.at[1], x.at[2], p, seed, offset, nullptr, (fbfft_stream_t)s);
+    });
+  });
+}
+
 // (getDevice, rawStream): how torch names the current stream; kept for the life of the process
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) {
@@ -197,6 +325,11 @@ PyMethodDef methods[] = {
     FBFFT_METHOD("conv_fprop", layer<fbfft_conv_fprop>),
     FBFFT_METHOD("conv_bprop", layer<fbfft_conv_bprop>),
     FBFFT_METHOD("conv_accgrad", accgrad),
+    FBFFT_METHOD("group_norm_fprop", normForward),
+    FBFFT_METHOD("group_norm_bprop", normBackward),
+    FBFFT_METHOD("linear_fprop", linearForward),
+    FBFFT_METHOD("linear_bprop", linearBackward),
+    FBFFT_METHOD("dropout", dropout),
     {nullptr, nullptr, 0, nullptr}};
 #undef FBFFT_METHOD
 

@@ -1,0 +1,131 @@
+// Dropout whose mask is drawn from a counter-based generator, forward and backward.
+//
+//   y[i] = (u(i) >= T ? x[i] * 65536 / (65536 - T) : 0) + residual[i]
+//
+// u(i): 16 bits of Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) at the counter (i / 8, offset).  Sixteen bits per
+// element instead of 32 halve the generator, whose 20 products of 32 x 32 bits per counter run at a quarter of the
+// rate of other vector instructions; T is the probability rounded to 16 bits, and the factor is that of T, so the
+// expectation is exact.
+#include "operators.h"
+
+#include <algorithm>
+
+namespace fbfft_amd {
+namespace {
+
+struct DropoutArgs {
+  const void *x, *residual;
+  void* y;
+  long size[FBFFT_MAX_DIM], xs[FBFFT_MAX_DIM], rs[FBFFT_MAX_DIM], ys[FBFFT_MAX_DIM];
+  long total;
+  unsigned threshold, seedLow, seedHigh;
+  unsigned long long offset;
+  const unsigned long long* step;
+  float factor;
+};
+
+struct Words {
+  unsigned w[4];
+};
+
+// The multipliers and key increments are those of the published generator.
+__device__ __forceinline__ Words philox(unsigned long long block, unsigned long long offset, unsigned k0, unsigned k1) {
+  unsigned a = (unsigned)block, b = (unsigned)(block >> 32), c = (unsigned)offset, d = (unsigned)(offset >> 32);
+#pragma unroll
+  for (int r = 0; r < 10; ++r) {
+    const unsigned long long p = (unsigned long long)a * 0xD2511F53u, q = (unsigned long long)c * 0xCD9E8D57u;
+    a = (unsigned)(q >> 32) ^ b ^ k0;
+    b = (unsigned)q;
+    c = (unsigned)(p >> 32) ^ d ^ k1;
+    d = (unsigned)p;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  return {{a, b, c, d}};
+}
+
+// A thread takes the eight elements of one counter.  DENSE: they are neighbours in every operand.
+template <class T, bool DENSE>
+__global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
+  const long block = (long)blockIdx.x * 256 + threadIdx.x, first = block * 8;
+  if (first >= g.total) return;
+  const Words words = philox(block, g.offset + (g.step ? *g.step : 0), g.seedLow, g.seedHigh);
+  const T* const x = static_cast<const T*>(g.x);
+  const T* const residual = static_cast<const T*>(g.residual);
+  T* const y = static_cast<T*>(g.y);
+  auto result = [&](int j, float v, float r) __attribute__((always_inline)) {
+    const unsigned u = j % 2 ? words.w[j / 2] >> 16 : words.w[j / 2] & 0xFFFFu;
+    return (u >= g.threshold ? v * g.factor : 0.f) + r;
+  };
+  if (DENSE && first + 8 <= g.total) {
+    float v[8], r[8] = {};
+    loadPack<T, 8>(x + first, v);
+    if (residual) loadPack<T, 8>(residual + first, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = result(j, v[j], r[j]);
+    storePack<T, 8>(y + first, v);
+    return;
+  }
+  long at[FBFFT_MAX_DIM];
+  long rest = first;
+#pragma unroll
+  for (int d = FBFFT_MAX_DIM - 1; d > 0; --d) {
+    at[d] = g.size[d] == 1 ? 0 : rest % g.size[d];
+    rest = g.size[d] == 1 ? rest : rest / g.size[d];
+  }
+  at[0] = rest;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (first + j >= g.total) break;
+    long xo = 0, ro = 0, yo = 0;
+#pragma unroll
+    for (int d = 0; d < FBFFT_MAX_DIM; ++d) xo += at[d] * g.xs[d], ro += at[d] * g.rs[d], yo += at[d] * g.ys[d];
+    y[yo] = (T)result(j, (float)x[xo], residual ? (float)residual[ro] : 0.f);
+    bool carry = true;
+#pragma unroll
+    for (int d = FBFFT_MAX_DIM - 1; d >= 0; --d) {
+      at[d] += carry;
+      carry = carry && at[d] == g.size[d];
+      if (carry) at[d] = 0;
+    }
+  }
+}
+
+template <class T>
+void launch(const DropoutArgs& g, bool dense, hipStream_t s) {
+  const dim3 grid((unsigned)((g.total + 2047) / 2048));
+  if (dense)
+    dropout<T, true><<<grid, 256, 0, s>>>(g);
+  else
+    dropout<T, false><<<grid, 256, 0, s>>>(g);
+}
+
+}  // namespace
+
+int launchDropout(const DropoutProblem& p, hipStream_t s) {
+  DropoutArgs g{};
+  g.x = p.x, g.residual = p.residual, g.y = p.y, g.total = p.total;
+  std::copy(p.size, p.size + FBFFT_MAX_DIM, g.size);
+  std::copy(p.xs, p.xs + FBFFT_MAX_DIM, g.xs);
+  std::copy(p.rs, p.rs + FBFFT_MAX_DIM, g.rs);
+  std::copy(p.ys, p.ys + FBFFT_MAX_DIM, g.ys);
+  g.threshold = p.threshold;
+  // (65536 dropped of 65536: no element is kept, and the factor is never used)
+  g.factor = p.threshold < 65536u ? (float)(65536.0 / (65536.0 - p.threshold)) : 0.f;
+  g.seedLow = (unsigned)p.seed, g.seedHigh = (unsigned)(p.seed >> 32), g.offset = p.offset, g.step = p.step;
+  bool dense = true;
+  long run = 1;
+  for (int d = FBFFT_MAX_DIM - 1; d >= 0; --d) {
+    if (g.size[d] != 1) dense = dense && g.xs[d] == run && g.ys[d] == run && (!g.residual || g.rs[d] == run);
+    run *= g.size[d];
+  }
+  if (p.type == FBFFT_FLOAT32)
+    launch<float>(g, dense, s);
+  else if (p.type == FBFFT_FLOAT16)
+    launch<half16>(g, dense, s);
+  else
+    launch<brain16>(g, dense, s);
+  return launchStatus();
+}
+
+}  // namespace fbfft_amd

@@ -326,6 +326,100 @@ int fbfft_conv_accgrad(const fbfft_tensor* input, const fbfft_tensor* gradOutput
 int fbfft_conv_fprop_static(const fbfft_tensor* input, const fbfft_tensor* weight,
                             const fbfft_tensor* output, int fftSize, fbfft_stream_t stream);
 
+/* ---- Operators around a convolution layer: group norm, products with an epilogue, dropout ----
+ *
+ * None has a counterpart in the reference.  Like everything above they enqueue on the caller's
+ * stream, allocate nothing and synchronise nothing; unlike it they take three element types and
+ * 64-bit extents.  Sums, statistics and every intermediate value are held in at least 32 bits,
+ * and a result is rounded once, to its array's type, except where a comment says otherwise. */
+
+enum fbfft_type { FBFFT_FLOAT32 = 0, FBFFT_FLOAT16 = 1, FBFFT_BFLOAT16 = 2 };
+
+/* none: z;  ReLU: max(z, 0);  SiLU: z / (1 + exp(-z));  GELU: z (1 + erf(z / sqrt 2)) / 2 */
+enum fbfft_activation {
+  FBFFT_ACTIVATION_NONE = 0,
+  FBFFT_ACTIVATION_RELU = 1,
+  FBFFT_ACTIVATION_SILU = 2,
+  FBFFT_ACTIVATION_GELU = 3
+};
+
+/* A non-owning strided view of elements of one type, strides in elements.  Any strides: channels
+ * last is a matter of strides, not of another entry point.  data is aligned to the element. */
+typedef struct fbfft_array {
+  void* data;
+  long long stride[FBFFT_MAX_DIM];
+  long long size[FBFFT_MAX_DIM];
+  int dim;
+  int type; /* enum fbfft_type */
+} fbfft_array;
+
+/* Group norm with an activation.  input, output [B][C][H][W] of one type; C = groups * D:
+ *   mean, var: over the n = D H W values of image b and group g (var divides by n)
+ *   z = (input - mean) / sqrt(var + eps) * weight[c] + bias[c],  output = activation(z)
+ * weight, bias: [C] of any type, or NULL for 1 and 0.  mean, rstd (= 1 / sqrt(var + eps)): float32
+ * [B][groups], written for the backward pass, or NULL.  output may be input itself (same address and
+ * strides); any other overlap is not defined.  workspace: fbfft_group_norm_workspace(0, ...) bytes,
+ * 256-byte aligned, NULL where that is 0; its contents need not survive. */
+size_t fbfft_group_norm_workspace(int pass, long long batch, long long channels, long long pixels, long long groups);
+int fbfft_group_norm_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
+                           const fbfft_array* output, const fbfft_array* mean, const fbfft_array* rstd,
+                           long long groups, float eps, int activation, void* workspace, size_t workspaceBytes,
+                           fbfft_stream_t stream);
+
+/* Its gradients, from the input and the mean and rstd that the forward pass wrote (xh = (input - mean) rstd):
+ *   dz = gradOutput activation'(z),  gradBias[c] = sum dz,  gradWeight[c] = sum dz xh  over images and pixels
+ *   gradInput = rstd (weight dz - sum_group(weight dz) / n - xh sum_group(weight dz xh) / n)
+ * ReLU's derivative at 0 is 0.  gradInput, gradWeight, gradBias: any of them NULL where it is not wanted; the
+ * latter two are overwritten.  gradInput may be gradOutput or input itself.  Reproducible bit for bit.
+ * workspace: fbfft_group_norm_workspace(1, ...). */
+int fbfft_group_norm_bprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
+                           const fbfft_array* mean, const fbfft_array* rstd, const fbfft_array* gradOutput,
+                           const fbfft_array* gradInput, const fbfft_array* gradWeight, const fbfft_array* gradBias,
+                           long long groups, int activation, void* workspace, size_t workspaceBytes,
+                           fbfft_stream_t stream);
+
+/* Rows times a weight matrix, with its epilogue:
+ *   z[m][n] = sum_k input[m][k] weight[n][k] + bias[n],  output = activation(z) + residual
+ * input [M][K], weight [N][K], residual, preactivation, output [M][N], all of one type; bias [N] of any
+ * type.  bias, residual: NULL for none.  preactivation: z, rounded, for the backward pass, or NULL; output is
+ * computed from z before that rounding.  residual may be output itself; no other operand may overlap it.
+ * K = 0 gives activation(bias) + residual.  float32 operands are multiplied as three bf16 pieces each,
+ * in six products that leave out terms below 2^-24 of a product; a value that is not finite reaches every
+ * result that it is a factor of, as infinity or NaN.
+ * workspace: fbfft_linear_workspace(0, ...) bytes, 256-byte aligned, NULL where that is 0. */
+size_t fbfft_linear_workspace(int pass, long long M, long long K, long long N, int type);
+int fbfft_linear_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
+                       const fbfft_array* residual, const fbfft_array* output, const fbfft_array* preactivation,
+                       int activation, void* workspace, size_t workspaceBytes, fbfft_stream_t stream);
+
+/* Its gradients.  dz = gradOutput activation'(preactivation) (the residual's gradient is gradOutput):
+ *   gradInput = dz weight,  gradWeight = dz^T input,  gradBias = sum_m dz
+ * preactivation: NULL where activation is none.  Any of the three gradients is NULL where it is not wanted, and
+ * weight without gradInput and input without gradWeight may be NULL; all are overwritten.  Between dz and the two
+ * products stands one rounding to the operands' type, which the matrix instructions take; gradBias sums dz before
+ * it.  Reproducible bit for bit.  workspace: fbfft_linear_workspace(1, ...). */
+int fbfft_linear_bprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* gradOutput,
+                       const fbfft_array* preactivation, const fbfft_array* gradInput, const fbfft_array* gradWeight,
+                       const fbfft_array* gradBias, int activation, void* workspace, size_t workspaceBytes,
+                       fbfft_stream_t stream);
+
+/* Dropout whose mask is never stored:
+ *   output = (u >= T ? input * 65536 / (65536 - T) : 0) + residual,   T = p * 65536, rounded to nearest
+ * u is a 16-bit number of the counter-based generator Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random
+ * numbers: as easy as 1, 2, 3; 2011): element i, counted row-major over the logical extents whatever the strides,
+ * takes number i % 8 (words in order, the lower half of each first) of the counter whose low 64 bits are i / 8 and
+ * whose high 64 bits are offset + (step ? *step : 0); the key is seed.  So the element is kept with the probability
+ * 1 - T / 65536 that its factor makes up for.  A dropped element is 0 whatever it holds.  input, residual
+ * (or NULL), output: rank 1 to 5, of one type and one shape; output may be either of the others.  step: a device
+ * address, or NULL: a captured graph that adds to it draws another mask with every replay.  0 <= p <= 1. */
+int fbfft_dropout_fprop(const fbfft_array* input, const fbfft_array* residual, const fbfft_array* output, double p,
+                        unsigned long long seed, unsigned long long offset, const unsigned long long* step,
+                        fbfft_stream_t stream);
+
+/* gradInput = (u >= T ? gradOutput * 65536 / (65536 - T) : 0): the forward pass's mask, drawn again. */
+int fbfft_dropout_bprop(const fbfft_array* gradOutput, const fbfft_array* gradInput, double p, unsigned long long seed,
+                        unsigned long long offset, const unsigned long long* step, fbfft_stream_t stream);
+
 /* Measurement aid with no counterpart in the reference: a plain device-to-device copy
  * of `bytes` (a multiple of 16, both pointers 16-byte aligned) on `stream`, in the
  * shape that moves a batch the size of a transform's operands fastest from HBM to HBM.

@@ -1,0 +1,223 @@
+"""Group norm with an activation, forward and backward, against its plain form in 64 bits."""
+import pytest
+import torch
+
+import fbcuda_amd as F
+from gpu_util import dev
+from operators_util import ACTS, NAMES, R, TYPES, norm, norm_grads, randn, rounded, within
+
+pytestmark = pytest.mark.gpu
+
+LAYOUTS = ["last", "planes", "crop", "slice", "turned"]
+
+
+def images(values, dtype, layout):
+    """values [B][C][H][W] on the GPU with the strides that `layout` names."""
+    b, c, h, w = values.shape
+    v = values.to(dtype).to(dev())
+    if layout == "last":
+        return v.permute(0, 2, 3, 1).contiguous().permute(0, 3, 1, 2)
+    if layout == "planes":
+        return v.contiguous()
+    if layout == "crop":  # a window of larger planes: rows apart
+        t = torch.zeros((b, c, h + 2, w + 3), dtype=dtype, device=dev())[:, :, 1:1 + h, 2:2 + w]
+    elif layout == "slice":  # some channels of more, channels last, off any 16-byte boundary
+        t = torch.zeros((b, h, w, c + 5), dtype=dtype, device=dev())[..., 3:3 + c].permute(0, 3, 1, 2)
+    else:  # images innermost
+        t = torch.zeros((c, w, h, b), dtype=dtype, device=dev()).permute(3, 0, 2, 1)
+    return t.copy_(v)
+
+
+def space(pass_, x, groups):
+    return torch.empty(F.group_norm_workspace(pass_, x, groups), dtype=torch.uint8, device=dev())
+
+
+def make(shape, groups, dtype, layout, seed, params=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    b, c, h, w = shape
+    x = randn(gen, b, c, h, w) * (0.5 + randn(gen, 1, c, 1, 1).abs()) + randn(gen, 1, c, 1, 1, std=0.7)
+    weight, bias = randn(gen, c, std=0.3, mean=1.0), randn(gen, c, std=0.3)
+    gy = randn(gen, b, c, h, w, std=0.1)
+    return (images(x, dtype, layout), weight.to(params).to(dev()), bias.to(params).to(dev()), images(gy, dtype, layout))
+
+
+def check_forward(x, weight, bias, groups, name, layout, eps=1e-5, out=None):
+    y = out if out is not None else images(torch.full(x.shape, 7.0, dtype=torch.float64), x.dtype, layout)
+    mean, rstd = (torch.full((x.shape[0], groups), 7.0, device=dev()) for _ in range(2))
+    want, wm, wr, bound = norm(x, weight, bias, groups, eps, name)
+    assert F.group_norm_fprop(x, weight, bias, y, groups, space(0, x, groups), activation=name, eps=eps, mean=mean,
+                              rstd=rstd) == F.Success
+    torch.cuda.synchronize()
+    within(y, want, rounded(want, x.dtype) + bound)
+    within(mean, wm, 4 * R * wm.abs() + 1e-12)
+    within(rstd, wr, 8 * R * wr)
+    return mean, rstd
+
+
+def check_backward(x, weight, bias, gy, mean, rstd, groups, name, layout, params=torch.float32):
+    gx = images(torch.full(x.shape, 7.0, dtype=torch.float64), x.dtype, layout)
+    c = x.shape[1]
+    gw, gb = (torch.full((c,), 7.0, dtype=params, device=dev()) for _ in range(2))
+    (wx, bx), (ww, bw), (wb, bb) = norm_grads(x, weight, bias, mean, rstd, gy, groups, name)
+    assert F.group_norm_bprop(x, weight, bias, mean, rstd, gy, gx, gw, gb, groups, space(1, x, groups),
+                              activation=name) == F.Success
+    torch.cuda.synchronize()
+    within(gx, wx, rounded(wx, x.dtype) + bx)
+    within(gw, ww, rounded(ww, params) + bw)
+    within(gb, wb, rounded(wb, params) + bb)
+    return gx, gw, gb
+
+
+# (B, C, H, W, groups): one value a group, one pixel, odd planes, groups of six channels in words of eight and four, one
+# group of all, every channel its own, groups wider than a workgroup, images larger than one
+SHAPES = [(1, 1, 1, 1, 1), (2, 8, 1, 1, 2), (3, 12, 1, 7, 3), (2, 64, 27, 27, 8), (4, 192, 23, 23, 32), (2, 48, 9, 11, 8),
+          (1, 32, 64, 64, 1), (2, 30, 5, 5, 30), (1, 4100, 3, 2, 1), (2, 40, 33, 31, 4), (1, 16, 150, 131, 2),
+          (70, 24, 4, 4, 4)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("layout", LAYOUTS)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_forward_and_backward(shape, layout, dtype):
+    groups = shape[4]
+    name = ACTS[(shape[1] + LAYOUTS.index(layout)) % 4]
+    x, weight, bias, gy = make(shape[:4], groups, dtype, layout, 1)
+    mean, rstd = check_forward(x, weight, bias, groups, name, layout)
+    check_backward(x, weight, bias, gy, mean, rstd, groups, name, layout)
+
+
+@pytest.mark.parametrize("name", ACTS)
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("layout", ["last", "planes"])
+@pytest.mark.parametrize("shape", [(2, 32, 12, 13, 4), (2, 32, 140, 140, 4)], ids=str)
+def test_activations(shape, layout, dtype, name):
+    x, weight, bias, gy = make(shape[:4], shape[4], dtype, layout, 2, params=dtype)
+    mean, rstd = check_forward(x, weight, bias, shape[4], name, layout)
+    check_backward(x, weight, bias, gy, mean, rstd, shape[4], name, layout, params=dtype)
+
+
+@pytest.mark.parametrize("shape", [(2, 24, 10, 10, 4), (2, 24, 200, 190, 4)], ids=str)
+@pytest.mark.parametrize("layout", ["last", "planes"])
+def test_without_parameters_and_in_place(layout, shape):
+    x, _, _, gy = make(shape[:4], shape[4], torch.float32, layout, 3)
+    mean, rstd = check_forward(x.clone(memory_format=torch.preserve_format), None, None, shape[4], "silu", layout)
+    check_backward(x, None, None, gy, mean, rstd, shape[4], "silu", layout)
+    want, _, _, bound = norm(x, None, None, shape[4], 1e-5, "gelu")
+    assert F.group_norm_fprop(x, None, None, x, shape[4], space(0, x, shape[4]), activation="gelu") == F.Success
+    within(x, want, rounded(want, x.dtype) + bound)
+    # gradInput in the place of gradOutput, without the parameters' gradients
+    (wx, bx), _, _ = norm_grads(x, None, None, mean, rstd, gy, shape[4], "silu")
+    assert F.group_norm_bprop(x, None, None, mean, rstd, gy, gy, None, None, shape[4], space(1, x, shape[4]),
+                              activation="silu") == F.Success
+    within(gy, wx, rounded(wx, x.dtype) + bx)
+
+
+@pytest.mark.parametrize("layout", ["last", "planes"])
+@pytest.mark.parametrize("side", [16, 160])
+def test_variance_far_below_the_squared_mean(layout, side):
+    """Means of 1000 deviations: a difference of fp32 sums would leave nothing of the variance.  And a corner far
+    from everything else."""
+    gen = torch.Generator().manual_seed(4)
+    v = randn(gen, 2, 16, side, side, std=0.01, mean=10.0)
+    v[1, :, 0, 0] = 0.0
+    x = images(v, torch.float32, layout)
+    check_forward(x, None, None, 4, "none", layout)
+
+
+@pytest.mark.parametrize("layout", ["last", "planes"])
+@pytest.mark.parametrize("side", [4, 180])
+def test_constant_groups_and_values_that_are_not_finite(layout, side):
+    gen = torch.Generator().manual_seed(5)
+    v = randn(gen, 4, 16, side, side)
+    v[0] = 3.0                       # no variance: the bias's activation
+    v[1, 3, 0, 0] = float("nan")     # reaches its own group of its own image
+    v[2, 9, -1, -1] = float("inf")
+    x = images(v, torch.float32, layout)
+    bias = torch.randn(16, generator=gen).to(dev())
+    y = torch.empty_like(x)
+    assert F.group_norm_fprop(x, None, bias, y, 4, space(0, x, 4), activation="silu") == F.Success
+    want, _, _, bound = norm(x, None, bias, 4, 1e-5, "silu")
+    got = y.cpu().double()
+    within(got[0], want[0], rounded(want[0], x.dtype) + bound[0])
+    within(got[3], want[3], rounded(want[3], x.dtype) + bound[3])
+    for image, group in ((1, 0), (2, 2)):
+        for g in range(4):
+            part = slice(4 * g, 4 * g + 4)
+            if g == group:
+                assert bool(torch.isnan(got[image, part]).all())
+            else:
+                within(got[image, part], want[image, part], rounded(want[image, part], x.dtype) + bound[image, part])
+
+
+@pytest.mark.parametrize("layout", ["last", "planes"])
+@pytest.mark.parametrize("side", [6, 170])
+def test_gradients_are_differences(layout, side):
+    """The sum of r * output, at x + h d and x - h d."""
+    gen = torch.Generator().manual_seed(6)
+    shape, groups, h = (2, 12, side, side), 3, 1e-2
+    v, d, r = (randn(gen, *shape) for _ in range(3))
+    weight, bias = randn(gen, 12, mean=1.0), randn(gen, 12)
+    dw, db = randn(gen, 12), randn(gen, 12)
+    to = lambda t: images(t, torch.float32, layout) if t.dim() == 4 else t.float().to(dev())  # noqa: E731
+
+    def loss(s):
+        x, w, b = to(v + s * d), to(weight + s * dw), to(bias + s * db)
+        y, mean, rstd = torch.empty_like(x), *(torch.empty((2, groups), device=dev()) for _ in range(2))
+        assert F.group_norm_fprop(x, w, b, y, groups, space(0, x, groups), activation="silu", mean=mean,
+                                  rstd=rstd) == F.Success
+        return float((y.double().cpu() * r).sum()), (x, w, b, mean, rstd)
+
+    _, (x, w, b, mean, rstd) = loss(0.0)
+    gx, gw, gb = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    assert F.group_norm_bprop(x, w, b, mean, rstd, to(r), gx, gw, gb, groups, space(1, x, groups),
+                              activation="silu") == F.Success
+    slope = sum(float((g.double().cpu() * e).sum()) for g, e in ((gx, d), (gw, dw), (gb, db)))
+    # what the difference leaves out is h^2 / 6 times a third derivative, of the sum's size sqrt(n) times about 10
+    # in products of normal numbers; fp32 results add 2^-24 sqrt(n) / h
+    n = v.numel()
+    allowed = (h * h / 6 * 40 + 8 * R / h) * n ** 0.5
+    assert abs((loss(h)[0] - loss(-h)[0]) / (2 * h) - slope) <= allowed
+
+
+@pytest.mark.parametrize("layout", ["last", "planes"])
+def test_empty_and_partial_calls(layout):
+    x = torch.empty((0, 8, 4, 4), device=dev())
+    stats = torch.empty((0, 2), device=dev())
+    gw, gb = torch.full((8,), 7.0, device=dev()), torch.full((8,), 7.0, device=dev())
+    assert F.group_norm_fprop(x, None, None, x, 2, None) == F.Success
+    assert F.group_norm_bprop(x, None, None, stats, stats, x, x, gw, gb, 2, None) == F.Success
+    assert not bool(gw.any()) and not bool(gb.any())  # sums over no images
+    x, weight, bias, gy = make((2, 8, 30, 30), 2, torch.float32, layout, 7)
+    mean, rstd = check_forward(x, weight, bias, 2, "silu", layout)
+    gx, gw, gb = check_backward(x, weight, bias, gy, mean, rstd, 2, "silu", layout)
+    only = [torch.full_like(t, 7.0) for t in (gx, gw, gb)]
+    for i in range(3):
+        args = [t if i == k else None for k, t in enumerate(only)]
+        assert F.group_norm_bprop(x, weight, bias, mean, rstd, gy, *args, 2, space(1, x, 2), activation="silu") == F.Success
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(only, (gx, gw, gb)))  # and reproducible
+
+
+def test_other_streams_and_the_general_way():
+    x, weight, bias, gy = make((3, 32, 40, 40), 4, torch.bfloat16, "last", 8)
+    y, z = torch.empty_like(x), torch.empty_like(x)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    assert F.group_norm_fprop(x, weight, bias, y, 4, space(0, x, 4), activation="silu") == F.Success
+    ws = space(0, x, 4)
+    torch.cuda.synchronize()
+    assert F.group_norm_fprop(x, weight, bias, z, 4, ws, activation="silu", stream=stream) == F.Success
+    torch.cuda.synchronize()
+    assert torch.equal(y, z)
+
+
+def test_offsets_past_32_bits():
+    """Two images and the pixels of an image more than 2^32 elements apart."""
+    far = (1 << 32) + 24
+    store = torch.zeros(2 * far + 4096, dtype=torch.bfloat16, device=dev())
+    x = store.as_strided((2, 8, 1, 2), (64, 1, 8, far))
+    gen = torch.Generator().manual_seed(9)
+    v = randn(gen, 2, 8, 1, 2)
+    x.copy_(v.to(dev()))
+    check_forward(x, None, None, 2, "silu", "planes")
+    del store
