@@ -6,7 +6,15 @@
 //   dx = rstd (w dz - sum(w dz) / n - xh sum(w dz xh) / n)
 //
 // Sums of x and x^2 are taken in 64 bits: their difference then keeps a variance that is far smaller than the
-// squared mean, without a second pass over the data.
+// squared mean, without a second pass over the data (64-bit additions run at the rate of 32-bit ones here).
+//
+// Three sets of kernels:
+//   Last    a lane holds a few neighbouring channels and walks over pixels (channels contiguous, or any strides)
+//   Planes  a lane walks over the contiguous values of a group (planes without gaps)
+//   Any     a group, or a channel, to a workgroup, element by element: groups wider than Last's lanes
+// The first two hold what a workgroup reads in registers where that suffices for a whole group, so that memory sees
+// one read and one write in one launch; else a first launch leaves sums of pieces of a group, and a second one joins
+// them and reads again, backwards, what the last-level cache still holds.
 #include "operators.h"
 
 #include <algorithm>
@@ -20,12 +28,23 @@ struct NormArgs {
   float *mean, *rstd;
   long meanB, meanG, rstdB, rstdG;
   long B, C, G, D, H, W, P;
+  Divisor byW, byP, byD, byLanes, byPieces, byBands;
+  double share;  // 1 / (D P)
   int activation;
   float eps;
-  float2* channels;  // backward: sums of dz and dz xh of each image and channel
+  // channels-last plan: channels of a workgroup, rows of lanes and lanes of a row, pixels of a piece; planes: values of one
+  int band, rows, lanes, pieces;
+  long piece;
+  double2* sums;     // forward: of x and x^2, [image][group][piece]
+  float2* groups;    // backward: sums of w dz and w dz xh, [image][group][piece]
+  float2* channels;  // backward: sums of dz and dz xh, [image][piece][channel]
 };
 
-__device__ __forceinline__ long pixelAt(const Image& i, long p, long W) { return p / W * i.h + p % W * i.w; }
+__device__ __forceinline__ long pixelAt(const NormArgs& a, const Image& i, int p) {
+  if (i.h == a.W * i.w) return (long)p * i.w;
+  const int row = quotient(p, a.byW);
+  return (long)row * i.h + (long)(p - row * (int)a.W) * i.w;
+}
 
 // The activation's argument, from a product and a sum that are rounded apart: both passes, and a program that writes
 // the formula down, then agree on which values a ReLU lets through.
@@ -34,15 +53,831 @@ __device__ __forceinline__ float affine(float xh, float w, float shift) {
   return xh * w + shift;
 }
 
-// the sum over the workgroup's 256 lanes, in every lane
-__device__ __forceinline__ double groupSum(double v, double* space) {
-#pragma unroll
-  for (int k = 32; k > 0; k /= 2) v += __shfl_xor(v, k);
+struct Moments {
+  float mean, rstd;
+};
+__device__ __forceinline__ Moments momentsOf(const NormArgs& a, double s1, double s2) {
+  const double centre = s1 * a.share, variance = s2 * a.share - centre * centre;
+  // (not a maximum: a group that holds NaN keeps it)
+  return {(float)centre, 1.f / sqrtf((float)((variance < 0.0 ? 0.0 : variance) + a.eps))};
+}
+
+// the sum over a workgroup of NT lanes, in every lane
+template <int NT, class S>
+__device__ __forceinline__ S teamSum(S v, S* space) {
+  v = waveSum(v);
+  if (NT == 64) return v;
   __syncthreads();
   if (threadIdx.x % 64 == 0) space[threadIdx.x / 64] = v;
   __syncthreads();
-  return space[0] + space[1] + space[2] + space[3];
+  v = 0;
+#pragma unroll
+  for (int k = 0; k < NT / 64; ++k) v += space[k];
+  return v;
 }
+
+// The gradients of weight and bias: the sums over images and pieces.  256 lanes: eight channels, 32 lanes to each.
+constexpr int kParameters = 8;
+__device__ __forceinline__ void parameterGradients(const NormArgs& a, int block, float2 (&part)[32][kParameters]) {
+  const int lane = threadIdx.x % kParameters, slice = threadIdx.x / kParameters;
+  const long c = (long)block * kParameters + lane, rows = a.B * a.pieces;
+  float s1 = 0, s2 = 0;
+  if (c < a.C)
+#pragma unroll 8
+    for (long r = slice; r < rows; r += 32) {
+      const float2 s = a.channels[r * a.C + c];
+      s1 += s.x;
+      s2 += s.y;
+    }
+  part[slice][lane] = float2{s1, s2};
+  __syncthreads();
+  if (slice > 0 || c >= a.C) return;
+  s1 = s2 = 0;
+  for (int r = 0; r < 32; ++r) {
+    s1 += part[r][lane].x;
+    s2 += part[r][lane].y;
+  }
+  if (a.gradBias.data) storeAny(a.gradBias.data, a.gradBias.type, c * a.gradBias.stride, s1);
+  if (a.gradWeight.data) storeAny(a.gradWeight.data, a.gradWeight.type, c * a.gradWeight.stride, s2);
+}
+
+__global__ __launch_bounds__(256) void normParameters(NormArgs a) {
+  __shared__ float2 part[32][kParameters];
+  parameterGradients(a, blockIdx.x, part);
+}
+
+// ---- Last ----
+
+constexpr int kBand = 1024;  // channels of a workgroup at most
+constexpr int kAhead = 4;    // pixels whose loads a lane has in flight where it walks over a piece
+
+template <int NT, int VEC, class S>
+struct Columns {
+  S lane[NT * VEC], part[NT];
+};
+
+// A workgroup's band of whole groups: lane t holds VEC channels from VEC (t % lanes) of every rows-th pixel.  Adds what
+// each lane has of its channels over the rows of lanes; sums[i] is then that of lane column i (SLOTS values of a lane
+// side by side).  Where rows of lanes divide a wave its rows meet in registers first (64 sums by one lane from LDS
+// took 7 us of the smallest call's 14), and what waits in LDS is summed in two stages.
+template <int NT, int SLOTS, int VEC, class S>
+__device__ __forceinline__ void joinRows(const NormArgs& a, int lanes, int column, int r, S (&v)[SLOTS],
+                                         Columns<NT, VEC, S>& space, S* sums) {
+  const int t = threadIdx.x, columns = lanes * SLOTS;
+  const bool divides = a.lanes <= 32 && (a.lanes & (a.lanes - 1)) == 0;
+  const int rows = divides ? NT / 64 : a.rows, row = divides ? t / 64 : r;
+  if (divides) {
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) v[j] = waveSumEvery(v[j], a.lanes);
+  }
+  __syncthreads();
+  if (column < lanes && (divides ? t % 64 < a.lanes : r < a.rows))
+#pragma unroll
+    for (int j = 0; j < SLOTS; ++j) space.lane[row * columns + column * SLOTS + j] = v[j];
+  __syncthreads();
+  if (rows <= 16 || columns > NT / 2) {
+    for (int i = t; i < columns; i += NT) {
+      S sum = 0;
+#pragma unroll 4
+      for (int k = 0; k < rows; ++k) sum += space.lane[k * columns + i];
+      sums[i] = sum;
+    }
+    return;
+  }
+  const int parts = min(NT / columns, 16), part = t / columns, i = t - part * columns;
+  if (part < parts) {
+    S sum = 0;
+#pragma unroll 4
+    for (int k = part; k < rows; k += parts) sum += space.lane[k * columns + i];
+    space.part[t] = sum;
+  }
+  __syncthreads();
+  if (t < columns) {
+    S sum = 0;
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) sum += space.part[k * columns + t];
+    sums[t] = sum;
+  }
+}
+
+// What a workgroup of Last, and a lane of it, work on.
+struct Band {
+  int b, piece, first, firstGroup;  // image, piece, channels and groups in front of the band
+  int channels, lanes, groups;      // of the band; lanes: of a row, with channels
+  int column, r;                    // of this lane: its place in a row of lanes, and the row
+  bool live;
+};
+template <int VEC>
+__device__ __forceinline__ Band bandOf(const NormArgs& a, int index) {
+  Band w;
+  const int row = quotient(index, a.byPieces);
+  w.piece = index - row * a.pieces;
+  w.b = quotient(row, a.byBands);
+  w.first = (row - w.b * (int)a.byBands.value) * a.band;
+  w.channels = min(a.band, (int)a.C - w.first);
+  w.lanes = w.channels / VEC;
+  w.firstGroup = quotient(w.first, a.byD);
+  w.groups = quotient(w.channels, a.byD);
+  w.r = quotient(threadIdx.x, a.byLanes);
+  w.column = threadIdx.x - w.r * a.lanes;
+  w.live = w.r < a.rows && w.column < w.lanes;
+  return w;
+}
+template <class T>
+__device__ __forceinline__ T* laneOf(const NormArgs& a, const Image& i, const Band& band, int vec) {
+  return static_cast<T*>(i.data) + band.b * i.b + (long)(band.first + band.column * vec) * i.c;
+}
+
+// weight and bias of the band's channels, into LDS
+__device__ __forceinline__ void bandParameters(const NormArgs& a, const Band& band, float2* to, int threads) {
+  for (int c = threadIdx.x; c < band.channels; c += threads)
+    to[c] = float2{lineOr(a.weight, band.first + c, 1.f), lineOr(a.bias, band.first + c, 0.f)};
+}
+
+template <int VEC>
+struct Channel {
+  float mean[VEC], rstd[VEC], w[VEC], shift[VEC];
+
+  __device__ __forceinline__ void load(const NormArgs& a, const Band& band, const Moments* stats, const float2* params) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int c = min(band.column * VEC + j, band.channels - 1);
+      const Moments m = stats[quotient(c, a.byD)];
+      const float2 p = params[c];
+      mean[j] = m.mean;
+      rstd[j] = m.rstd;
+      w[j] = p.x;
+      shift[j] = p.y;
+    }
+  }
+  // x is replaced by the normalised values, z by the activation's arguments
+  __device__ __forceinline__ void arguments(float (&x)[VEC], float (&z)[VEC]) const {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      x[j] = (x[j] - mean[j]) * rstd[j];
+      z[j] = affine(x[j], w[j], shift[j]);
+    }
+  }
+};
+
+// the statistics of the band's groups from sums over their columns; space holds 64-bit sums
+template <int NT, int VEC>
+__device__ __forceinline__ void joinMoments(const NormArgs& a, const Band& band, double (&s1)[VEC], double (&s2)[VEC],
+                                            Columns<NT, VEC, double>& space, double* sums, Moments* stats, bool raw) {
+  // where a lane's channels are all of one group, they are added before they go through LDS
+  const int D = (int)a.D, t = threadIdx.x;
+  const bool whole = VEC > 1 && D % VEC == 0;
+  const int wide = whole ? D / VEC : D;
+  auto one = [&](double(&s)[VEC]) __attribute__((always_inline)) {
+    if (whole) {
+      double v[1] = {0};
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[0] += s[j];
+      joinRows<NT, 1, VEC>(a, band.lanes, band.column, band.r, v, space, sums);
+    } else {
+      joinRows<NT, VEC, VEC>(a, band.lanes, band.column, band.r, s, space, sums);
+    }
+    __syncthreads();
+    // a wave to a group (as many as a wave has lanes, or fewer, to each: NT groups at most)
+    double kept = 0;
+    for (int g = t / 64, k = 0; g < band.groups; g += NT / 64, ++k) {
+      double v = 0;
+      for (int i = t % 64; i < wide; i += 64) v += sums[g * wide + i];
+      v = waveSum(v);
+      if (t % 64 == k) kept = v;
+    }
+    return kept;
+  };
+  const double first = one(s1), second = one(s2);
+  const int g = t / 64 + t % 64 * (NT / 64);
+  if (g < band.groups) {
+    const long group = band.firstGroup + g;
+    if (raw) {
+      a.sums[(band.b * a.G + group) * a.pieces + band.piece] = double2{first, second};
+    } else {
+      const Moments m = momentsOf(a, first, second);
+      stats[g] = m;
+      if (a.mean) a.mean[band.b * a.meanB + group * a.meanG] = m.mean;
+      if (a.rstd) a.rstd[band.b * a.rstdB + group * a.rstdG] = m.rstd;
+    }
+  }
+  __syncthreads();
+}
+
+template <int VEC>
+__device__ __forceinline__ void moments(const float (&v)[VEC], double (&s1)[VEC], double (&s2)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const double x = v[j];
+    s1[j] += x;
+    s2[j] = __builtin_fma(x, x, s2[j]);
+  }
+}
+
+// N elements of one word
+template <int VEC, class R>
+__device__ __forceinline__ void unpack(const R raw, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = (float)raw;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (float)raw[j];
+  }
+}
+
+// Workgroups are dealt out to the eight XCDs in turn; those of one XCD take neighbouring work, so that lines that two
+// bands of an image share are read into one L2.
+__device__ __forceinline__ int nearWork(int total) {
+  const int per = (total + 7) / 8;
+  const int index = (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
+  return (int)blockIdx.x / 8 < per && index < total ? index : -1;
+}
+
+// All pixels of a band in registers: one read, one write.
+template <class T, int VEC, int NT, int ITEMS>
+__global__ __launch_bounds__(NT) void lastForward(NormArgs a, int total) {
+  __shared__ Columns<NT, VEC, double> space;
+  __shared__ double sums[kBand];
+  __shared__ Moments stats[NT];
+  __shared__ float2 params[kBand];
+  const int index = nearWork(total);
+  if (index < 0) return;
+  const Band band = bandOf<VEC>(a, index);
+  const T* const x = laneOf<const T>(a, a.x, band, VEC);
+  T* const y = laneOf<T>(a, a.y, band, VEC);
+  const int P = (int)a.P;
+  typename Pack<T, VEC>::type raw[ITEMS];
+  if (band.live)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int p = band.r + i * a.rows;
+      if (p < P) raw[i] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, p));
+    }
+  bandParameters(a, band, params, NT);
+  double s1[VEC] = {}, s2[VEC] = {};
+  if (band.live)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (band.r + i * a.rows < P) {
+        float v[VEC];
+        unpack(raw[i], v);
+        moments(v, s1, s2);
+      }
+  joinMoments<NT, VEC>(a, band, s1, s2, space, sums, stats, false);
+  if (!band.live) return;
+  Channel<VEC> ch;
+  ch.load(a, band, stats, params);
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int p = band.r + i * a.rows;
+    if (p >= P) break;
+    float v[VEC], z[VEC];
+    unpack(raw[i], v);
+    ch.arguments(v, z);
+    activateAll(z, a.activation);
+    storePack<T, VEC>(y + pixelAt(a, a.y, p), z);
+  }
+}
+
+// The sums of a piece of each group.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void lastSums(NormArgs a) {
+  __shared__ Columns<256, VEC, double> space;
+  __shared__ double sums[kBand];
+  const Band band = bandOf<VEC>(a, blockIdx.x);
+  const T* const x = laneOf<const T>(a, a.x, band, VEC);
+  const int end = (int)min((band.piece + 1) * a.piece, a.P);
+  double s1[VEC] = {}, s2[VEC] = {};
+  if (band.live) {
+    for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
+      typename Pack<T, VEC>::type raw[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) raw[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, min(p + k * a.rows, end - 1)));
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (p + k * a.rows < end) {
+          float v[VEC];
+          unpack(raw[k], v);
+          moments(v, s1, s2);
+        }
+    }
+  }
+  joinMoments<256, VEC>(a, band, s1, s2, space, sums, nullptr, true);
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void lastApply(NormArgs a) {
+  __shared__ Moments stats[256];
+  __shared__ float2 params[kBand];
+  const Band band = bandOf<VEC>(a, gridDim.x - 1 - blockIdx.x);
+  bandParameters(a, band, params, 256);
+  for (int g = threadIdx.x / 64; g < band.groups; g += 4) {
+    const long group = band.firstGroup + g;
+    double s1 = 0, s2 = 0;
+    for (int i = threadIdx.x % 64; i < a.pieces; i += 64) {
+      const double2 s = a.sums[(band.b * a.G + group) * a.pieces + i];
+      s1 += s.x;
+      s2 += s.y;
+    }
+    const Moments m = momentsOf(a, waveSum(s1), waveSum(s2));
+    if (threadIdx.x % 64 == 0) {
+      stats[g] = m;
+      if (band.piece == 0 && a.mean) a.mean[band.b * a.meanB + group * a.meanG] = m.mean;
+      if (band.piece == 0 && a.rstd) a.rstd[band.b * a.rstdB + group * a.rstdG] = m.rstd;
+    }
+  }
+  __syncthreads();
+  if (!band.live) return;
+  Channel<VEC> ch;
+  ch.load(a, band, stats, params);
+  const T* const x = laneOf<const T>(a, a.x, band, VEC);
+  T* const y = laneOf<T>(a, a.y, band, VEC);
+  const int end = (int)min((band.piece + 1) * a.piece, a.P);
+  for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
+    typename Pack<T, VEC>::type raw[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) raw[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, min(p + k * a.rows, end - 1)));
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (p + k * a.rows < end) {
+        float v[VEC], z[VEC];
+        unpack(raw[k], v);
+        ch.arguments(v, z);
+        activateAll(z, a.activation);
+        storePack<T, VEC>(y + pixelAt(a, a.y, p + k * a.rows), z);
+      }
+  }
+}
+
+// the statistics that the forward pass kept
+__device__ __forceinline__ void keptMoments(const NormArgs& a, const Band& band, Moments* stats, int threads) {
+  for (int g = threadIdx.x; g < band.groups; g += threads) {
+    const long group = band.firstGroup + g;
+    stats[g] = Moments{a.mean[band.b * a.meanB + group * a.meanG], a.rstd[band.b * a.rstdB + group * a.rstdG]};
+  }
+  __syncthreads();
+}
+
+// Sums of dz and dz xh per channel of the band, kept for the gradients of weight and bias; then those of w dz and
+// w dz xh per group: done(group of the band, sum, sum) in one lane.
+template <int NT, int VEC, class F>
+__device__ __forceinline__ void joinGradients(const NormArgs& a, const Band& band, float (&s1)[VEC], float (&s2)[VEC],
+                                              Columns<NT, VEC, float>& space, float (&sums)[2][kBand], const float2* params, F done) {
+  joinRows<NT, VEC, VEC>(a, band.lanes, band.column, band.r, s1, space, sums[0]);
+  joinRows<NT, VEC, VEC>(a, band.lanes, band.column, band.r, s2, space, sums[1]);
+  // (a lane reads what it has written)
+  for (int c = threadIdx.x; c < band.channels; c += NT) {
+    const float2 s{sums[0][c], sums[1][c]};
+    a.channels[((long)band.b * a.pieces + band.piece) * a.C + band.first + c] = s;
+    const float w = params[c].x;
+    sums[0][c] = s.x * w;
+    sums[1][c] = s.y * w;
+  }
+  __syncthreads();
+  const int D = (int)a.D;
+  for (int g = threadIdx.x / 64; g < band.groups; g += NT / 64) {
+    float m1 = 0, m2 = 0;
+    for (int i = threadIdx.x % 64; i < D; i += 64) m1 += sums[0][g * D + i], m2 += sums[1][g * D + i];
+    m1 = waveSum(m1);
+    m2 = waveSum(m2);
+    if (threadIdx.x % 64 == 0) done(g, m1, m2);
+  }
+}
+
+// dx in the place of dz, from xh
+template <int VEC>
+__device__ __forceinline__ void inputGradient(const Channel<VEC>& ch, const float (&m1)[VEC], const float (&m2)[VEC],
+                                              const float (&xh)[VEC], float (&dz)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) dz[j] = ch.rstd[j] * (dz[j] * ch.w[j] - m1[j] - xh[j] * m2[j]);
+}
+
+// All pixels of a band of input and gradient in registers: two reads, one write.
+template <class T, int VEC, int NT, int ITEMS>
+__global__ __launch_bounds__(NT) void lastBackward(NormArgs a, int total) {
+  __shared__ Columns<NT, VEC, float> space;
+  __shared__ float sums[2][kBand];
+  __shared__ Moments stats[NT], means[NT];
+  __shared__ float2 params[kBand];
+  const int index = nearWork(total);
+  if (index < 0) return;
+  const Band band = bandOf<VEC>(a, index);
+  const T* const x = laneOf<const T>(a, a.x, band, VEC);
+  const T* const g = laneOf<const T>(a, a.g, band, VEC);
+  const int P = (int)a.P;
+  typename Pack<T, VEC>::type rx[ITEMS], rg[ITEMS];
+  if (band.live)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const int p = band.r + i * a.rows;
+      if (p < P) {
+        rx[i] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, p));
+        rg[i] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(g + pixelAt(a, a.g, p));
+      }
+    }
+  bandParameters(a, band, params, NT);
+  keptMoments(a, band, stats, NT);
+  float s1[VEC] = {}, s2[VEC] = {};
+  Channel<VEC> ch;
+  ch.load(a, band, stats, params);
+  if (band.live)
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (band.r + i * a.rows < P) {
+        float v[VEC], dz[VEC], z[VEC];
+        unpack(rx[i], v);
+        unpack(rg[i], dz);
+        ch.arguments(v, z);
+        slopeAll(z, dz, a.activation);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          s1[j] += dz[j];
+          s2[j] = __builtin_fmaf(dz[j], v[j], s2[j]);
+        }
+      }
+  joinGradients<NT, VEC>(a, band, s1, s2, space, sums, params,
+                         [&](int k, float m1, float m2) { means[k] = Moments{m1 * (float)a.share, m2 * (float)a.share}; });
+  if (!a.y.data) return;
+  __syncthreads();
+  if (!band.live) return;
+  T* const y = laneOf<T>(a, a.y, band, VEC);
+  float m1[VEC], m2[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const Moments m = means[quotient(band.column * VEC + j, a.byD)];
+    m1[j] = m.mean;
+    m2[j] = m.rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int p = band.r + i * a.rows;
+    if (p >= P) break;
+    float v[VEC], dz[VEC], z[VEC];
+    unpack(rx[i], v);
+    unpack(rg[i], dz);
+    ch.arguments(v, z);
+    slopeAll(z, dz, a.activation);
+    inputGradient(ch, m1, m2, v, dz);
+    storePack<T, VEC>(y + pixelAt(a, a.y, p), dz);
+  }
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void lastGradSums(NormArgs a) {
+  __shared__ Columns<256, VEC, float> space;
+  __shared__ float sums[2][kBand];
+  __shared__ Moments stats[256];
+  __shared__ float2 params[kBand];
+  const Band band = bandOf<VEC>(a, blockIdx.x);
+  const T* const x = laneOf<const T>(a, a.x, band, VEC);
+  const T* const g = laneOf<const T>(a, a.g, band, VEC);
+  bandParameters(a, band, params, 256);
+  keptMoments(a, band, stats, 256);
+  Channel<VEC> ch;
+  ch.load(a, band, stats, params);
+  const int end = (int)min((band.piece + 1) * a.piece, a.P);
+  float s1[VEC] = {}, s2[VEC] = {};
+  if (band.live) {
+    for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
+      typename Pack<T, VEC>::type rx[kAhead], rg[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int at = min(p + k * a.rows, end - 1);
+        rx[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, at));
+        rg[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(g + pixelAt(a, a.g, at));
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (p + k * a.rows < end) {
+          float v[VEC], dz[VEC], z[VEC];
+          unpack(rx[k], v);
+          unpack(rg[k], dz);
+          ch.arguments(v, z);
+          slopeAll(z, dz, a.activation);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            s1[j] += dz[j];
+            s2[j] = __builtin_fmaf(dz[j], v[j], s2[j]);
+          }
+        }
+    }
+  }
+  joinGradients<256, VEC>(a, band, s1, s2, space, sums, params, [&](int k, float m1, float m2) {
+    a.groups[(band.b * a.G + band.firstGroup + k) * a.pieces + band.piece] = float2{m1, m2};
+  });
+}
+
+// (The first `before` workgroups add up the gradients of weight and bias.)
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void lastGradApply(NormArgs a, int before) {
+  __shared__ Moments stats[256], means[256];
+  __shared__ union {
+    float2 params[kBand], part[32][kParameters];
+  } space;
+  if ((int)blockIdx.x < before) return parameterGradients(a, blockIdx.x, space.part);
+  float2* const params = space.params;
+  const Band band = bandOf<VEC>(a, gridDim.x - 1 - blockIdx.x);
+  bandParameters(a, band, params, 256);
+  for (int k = threadIdx.x / 64; k < band.groups; k += 4) {
+    float m1 = 0, m2 = 0;
+    for (int i = threadIdx.x % 64; i < a.pieces; i += 64) {
+      const float2 s = a.groups[(band.b * a.G + band.firstGroup + k) * a.pieces + i];
+      m1 += s.x;
+      m2 += s.y;
+    }
+    m1 = waveSum(m1);
+    m2 = waveSum(m2);
+    if (threadIdx.x % 64 == 0) means[k] = Moments{m1 * (float)a.share, m2 * (float)a.share};
+  }
+  keptMoments(a, band, stats, 256);
+  if (!band.live) return;
+  const T* const x = laneOf<const T>(a, a.x, band, VEC);
+  const T* const g = laneOf<const T>(a, a.g, band, VEC);
+  T* const y = laneOf<T>(a, a.y, band, VEC);
+  Channel<VEC> ch;
+  ch.load(a, band, stats, params);
+  float m1[VEC], m2[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    const Moments m = means[quotient(band.column * VEC + j, a.byD)];
+    m1[j] = m.mean;
+    m2[j] = m.rstd;
+  }
+  const int end = (int)min((band.piece + 1) * a.piece, a.P);
+  for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
+    typename Pack<T, VEC>::type rx[kAhead], rg[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int at = min(p + k * a.rows, end - 1);
+      rx[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, at));
+      rg[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(g + pixelAt(a, a.g, at));
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (p + k * a.rows < end) {
+        float v[VEC], dz[VEC], z[VEC];
+        unpack(rx[k], v);
+        unpack(rg[k], dz);
+        ch.arguments(v, z);
+        slopeAll(z, dz, a.activation);
+        inputGradient(ch, m1, m2, v, dz);
+        storePack<T, VEC>(y + pixelAt(a, a.y, p + k * a.rows), dz);
+      }
+  }
+}
+
+// ---- Planes ----
+
+// Elements e ... e + VEC - 1 of the n of a group: neighbours (VEC > 1), or one by its strides.
+template <class T, int VEC>
+struct Words {
+  typename Pack<T, VEC>::type raw;
+
+  static __device__ __forceinline__ long offset(const NormArgs& a, const Image& i, int e) {
+    const int c = quotient(e, a.byP);
+    return c * i.c + pixelAt(a, i, e - c * (int)a.P);
+  }
+  __device__ __forceinline__ void load(const NormArgs& a, const Image& i, const T* base, int e, int n) {
+    if constexpr (VEC == 1) {
+      raw = e < n ? base[offset(a, i, e)] : (T)0.f;
+    } else if (e + VEC <= n) {
+      raw = *reinterpret_cast<const typename Pack<T, VEC>::type*>(base + e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) raw[j] = e + j < n ? base[e + j] : (T)0.f;
+    }
+  }
+  static __device__ __forceinline__ void store(const NormArgs& a, const Image& i, T* base, int e, int n, const float (&v)[VEC]) {
+    if constexpr (VEC == 1) {
+      if (e < n) base[offset(a, i, e)] = (T)v[0];
+    } else if (e + VEC <= n) {
+      storePack<T, VEC>(base + e, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (e + j < n) base[e + j] = (T)v[j];
+    }
+  }
+};
+
+// weight and bias of elements e ... of group g: of one channel or, over the end of a plane, of two (planes are no
+// smaller than a word)
+template <int VEC>
+struct Along {
+  float w[VEC], shift[VEC];
+
+  __device__ __forceinline__ void load(const NormArgs& a, long group, int e) {
+    const int P = (int)a.P, c = quotient(e, a.byP), left = (c + 1) * P - e;
+    const long first = group * a.D + c, second = c + 1 < a.D ? first + 1 : first;
+    const float w0 = lineOr(a.weight, first, 1.f), shift0 = lineOr(a.bias, first, 0.f);
+    float w1 = w0, shift1 = shift0;
+    if (VEC > 1 && left < VEC) {
+      w1 = lineOr(a.weight, second, 1.f);
+      shift1 = lineOr(a.bias, second, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      w[j] = j < left ? w0 : w1;
+      shift[j] = j < left ? shift0 : shift1;
+    }
+  }
+};
+
+// A team of TEAM lanes holds a group in registers; teams of 64 share a workgroup of 256.
+template <class T, int VEC, int TEAM, int ITEMS>
+__global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void planesForward(NormArgs a) {
+  constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
+  __shared__ double space[TEAM / 64];
+  const int t = threadIdx.x % TEAM, n = (int)(a.D * a.P);
+  const long index = (long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
+  if (index >= a.B * a.G) return;  // (a whole wave: teams of more are a workgroup each)
+  const long b = index / a.G, g = index % a.G;
+  const T* const x = static_cast<const T*>(a.x.data) + b * a.x.b + g * a.D * a.x.c;
+  T* const y = static_cast<T*>(a.y.data) + b * a.y.b + g * a.D * a.y.c;
+  Words<T, VEC> v[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) v[i].load(a, a.x, x, (i * TEAM + t) * VEC, n);
+  double s1[VEC] = {}, s2[VEC] = {};
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {  // (zeros behind the end)
+    float f[VEC];
+    unpack(v[i].raw, f);
+    moments(f, s1, s2);
+  }
+#pragma unroll
+  for (int j = 1; j < VEC; ++j) s1[0] += s1[j], s2[0] += s2[j];
+  s1[0] = teamSum<TEAM>(s1[0], space);
+  s2[0] = teamSum<TEAM>(s2[0], space);
+  const Moments m = momentsOf(a, s1[0], s2[0]);
+  if (t == 0) {
+    if (a.mean) a.mean[b * a.meanB + g * a.meanG] = m.mean;
+    if (a.rstd) a.rstd[b * a.rstdB + g * a.rstdG] = m.rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int e = (i * TEAM + t) * VEC;
+    if (e >= n) break;
+    Along<VEC> p;
+    p.load(a, g, e);
+    float out[VEC];
+    unpack(v[i].raw, out);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = affine((out[j] - m.mean) * m.rstd, p.w[j], p.shift[j]);
+    activateAll(out, a.activation);
+    Words<T, VEC>::store(a, a.y, y, e, n, out);
+  }
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void planesSums(NormArgs a) {
+  __shared__ double space[4];
+  const long piece = blockIdx.x % a.pieces, index = blockIdx.x / a.pieces, b = index / a.G, g = index % a.G;
+  const int n = (int)(a.D * a.P), end = (int)min((piece + 1) * a.piece, (long)n);
+  const T* const x = static_cast<const T*>(a.x.data) + b * a.x.b + g * a.D * a.x.c;
+  double s1[VEC] = {}, s2[VEC] = {};
+#pragma unroll 4
+  for (long e = piece * a.piece + threadIdx.x * VEC; e < end; e += 256 * VEC) {
+    Words<T, VEC> v;
+    v.load(a, a.x, x, (int)e, end);
+    float f[VEC];
+    unpack(v.raw, f);
+    moments(f, s1, s2);
+  }
+#pragma unroll
+  for (int j = 1; j < VEC; ++j) s1[0] += s1[j], s2[0] += s2[j];
+  s1[0] = teamSum<256>(s1[0], space);
+  s2[0] = teamSum<256>(s2[0], space);
+  if (threadIdx.x == 0) a.sums[index * a.pieces + piece] = double2{s1[0], s2[0]};
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void planesApply(NormArgs a) {
+  __shared__ double space[4];
+  const long block = gridDim.x - 1 - blockIdx.x;
+  const long piece = block % a.pieces, index = block / a.pieces, b = index / a.G, g = index % a.G;
+  const int n = (int)(a.D * a.P), end = (int)min((piece + 1) * a.piece, (long)n);
+  double s1 = 0, s2 = 0;
+  for (int i = threadIdx.x; i < a.pieces; i += 256) {
+    const double2 s = a.sums[index * a.pieces + i];
+    s1 += s.x;
+    s2 += s.y;
+  }
+  s1 = teamSum<256>(s1, space);
+  s2 = teamSum<256>(s2, space);
+  const Moments m = momentsOf(a, s1, s2);
+  if (threadIdx.x == 0 && piece == 0) {
+    if (a.mean) a.mean[b * a.meanB + g * a.meanG] = m.mean;
+    if (a.rstd) a.rstd[b * a.rstdB + g * a.rstdG] = m.rstd;
+  }
+  const T* const x = static_cast<const T*>(a.x.data) + b * a.x.b + g * a.D * a.x.c;
+  T* const y = static_cast<T*>(a.y.data) + b * a.y.b + g * a.D * a.y.c;
+#pragma unroll 4
+  for (long e = piece * a.piece + threadIdx.x * VEC; e < end; e += 256 * VEC) {
+    Words<T, VEC> v;
+    v.load(a, a.x, x, (int)e, end);
+    Along<VEC> p;
+    p.load(a, g, (int)e);
+    float out[VEC];
+    unpack(v.raw, out);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = affine((out[j] - m.mean) * m.rstd, p.w[j], p.shift[j]);
+    activateAll(out, a.activation);
+    Words<T, VEC>::store(a, a.y, y, (int)e, end, out);
+  }
+}
+
+// A team sums a piece of one plane.
+template <class T, int VEC, int TEAM>
+__global__ __launch_bounds__(256) void planesGradSums(NormArgs a) {
+  constexpr int TEAMS = 256 / TEAM;
+  __shared__ float space[TEAM / 64];
+  const long block = (long)blockIdx.x * TEAMS + threadIdx.x / TEAM;
+  if (block >= a.B * a.C * a.pieces) return;  // (a whole wave)
+  const long piece = block % a.pieces, index = block / a.pieces, b = index / a.C, c = index % a.C, group = c / a.D;
+  const int t = threadIdx.x % TEAM, end = (int)min((piece + 1) * a.piece, a.P);
+  const float mean = a.mean[b * a.meanB + group * a.meanG], rstd = a.rstd[b * a.rstdB + group * a.rstdG];
+  const float w = lineOr(a.weight, c, 1.f), shift = lineOr(a.bias, c, 0.f);
+  const T* const x = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
+  const T* const g = static_cast<const T*>(a.g.data) + b * a.g.b + c * a.g.c;
+  float s1 = 0, s2 = 0;
+#pragma unroll 2
+  for (long e = piece * a.piece + t * VEC; e < end; e += TEAM * VEC) {
+    Words<T, VEC> vx, vg;
+    vx.load(a, a.x, x, (int)e, end);
+    vg.load(a, a.g, g, (int)e, end);
+    float fx[VEC], fg[VEC];
+    unpack(vx.raw, fx);
+    unpack(vg.raw, fg);
+    float z[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      fx[j] = (fx[j] - mean) * rstd;
+      z[j] = affine(fx[j], w, shift);
+    }
+    slopeAll(z, fg, a.activation);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      // (behind the end nothing, whatever the slope is there)
+      const float dz = e + j < end ? fg[j] : 0.f;
+      s1 += dz;
+      s2 = __builtin_fmaf(dz, fx[j], s2);
+    }
+  }
+  s1 = teamSum<TEAM>(s1, space);
+  s2 = teamSum<TEAM>(s2, space);
+  if (t == 0) a.channels[(b * a.pieces + piece) * a.C + c] = float2{s1, s2};
+}
+
+// A workgroup: 256 VEC elements, times `each`, of a group.  The first `before` of them add up the gradients of weight
+// and bias.
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void planesGradApply(NormArgs a, long blocks, int each, int before) {
+  __shared__ float space[4];
+  __shared__ float2 sums[32][kParameters];
+  if ((int)blockIdx.x < before) return parameterGradients(a, blockIdx.x, sums);
+  const long block = gridDim.x - 1 - blockIdx.x, part = block % blocks, index = block / blocks, b = index / a.G, group = index % a.G;
+  const int n = (int)(a.D * a.P);
+  const float mean = a.mean[b * a.meanB + group * a.meanG], rstd = a.rstd[b * a.rstdB + group * a.rstdG];
+  float m1 = 0, m2 = 0;
+  for (long i = threadIdx.x; i < a.D * a.pieces; i += 256) {
+    const long c = group * a.D + i % a.D;
+    const float2 s = a.channels[(b * a.pieces + i / a.D) * a.C + c];
+    const float w = lineOr(a.weight, c, 1.f);
+    m1 += s.x * w;
+    m2 += s.y * w;
+  }
+  const float scale = 1.f / (float)n;
+  m1 = teamSum<256>(m1, space) * scale;
+  m2 = teamSum<256>(m2, space) * scale;
+  const T* const x = static_cast<const T*>(a.x.data) + b * a.x.b + group * a.D * a.x.c;
+  const T* const g = static_cast<const T*>(a.g.data) + b * a.g.b + group * a.D * a.g.c;
+  T* const y = static_cast<T*>(a.y.data) + b * a.y.b + group * a.D * a.y.c;
+#pragma unroll 2
+  for (int i = 0; i < each; ++i) {
+    const long at = ((part * each + i) * 256 + threadIdx.x) * VEC;
+    if (at >= n) break;
+    const int e = (int)at;
+    Words<T, VEC> vx, vg;
+    vx.load(a, a.x, x, e, n);
+    vg.load(a, a.g, g, e, n);
+    Along<VEC> p;
+    p.load(a, group, e);
+    float fx[VEC], out[VEC], z[VEC];
+    unpack(vx.raw, fx);
+    unpack(vg.raw, out);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      fx[j] = (fx[j] - mean) * rstd;
+      z[j] = affine(fx[j], p.w[j], p.shift[j]);
+    }
+    slopeAll(z, out, a.activation);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = rstd * (out[j] * p.w[j] - m1 - fx[j] * m2);
+    Words<T, VEC>::store(a, a.y, y, e, n, out);
+  }
+}
+
+// ---- Any ----
 
 // A workgroup takes one group of one image, whatever the strides.
 template <class T>
@@ -53,23 +888,24 @@ __global__ __launch_bounds__(256) void normAny(NormArgs a) {
   T* const y = static_cast<T*>(a.y.data) + b * a.y.b + g * a.D * a.y.c;
   double s1 = 0, s2 = 0;
   for (long e = threadIdx.x; e < n; e += 256) {
-    const double v = (float)x[e / a.P * a.x.c + pixelAt(a.x, e % a.P, a.W)];
+    const int c = quotient((int)e, a.byP);
+    const double v = (float)x[c * a.x.c + pixelAt(a, a.x, (int)e - c * (int)a.P)];
     s1 += v;
     s2 += v * v;
   }
-  s1 = groupSum(s1, space);
-  s2 = groupSum(s2, space);
-  const double centre = s1 / n, variance = fmax(s2 / n - centre * centre, 0.0);
-  const float mean = (float)centre, rstd = (float)(1.0 / sqrt(variance + a.eps));
+  s1 = teamSum<256>(s1, space);
+  s2 = teamSum<256>(s2, space);
+  const Moments m = momentsOf(a, s1, s2);
+  const float mean = m.mean, rstd = m.rstd;
   if (threadIdx.x == 0) {
     if (a.mean) a.mean[b * a.meanB + g * a.meanG] = mean;
     if (a.rstd) a.rstd[b * a.rstdB + g * a.rstdG] = rstd;
   }
   for (long e = threadIdx.x; e < n; e += 256) {
-    const long c = e / a.P, p = e % a.P;
-    const float v = (float)x[c * a.x.c + pixelAt(a.x, p, a.W)];
+    const int c = quotient((int)e, a.byP), p = (int)e - c * (int)a.P;
+    const float v = (float)x[c * a.x.c + pixelAt(a, a.x, p)];
     const float w = lineOr(a.weight, g * a.D + c, 1.f), shift = lineOr(a.bias, g * a.D + c, 0.f);
-    y[c * a.y.c + pixelAt(a.y, p, a.W)] = (T)activate(affine((v - mean) * rstd, w, shift), a.activation);
+    y[c * a.y.c + pixelAt(a, a.y, p)] = (T)activate(affine((v - mean) * rstd, w, shift), a.activation);
   }
 }
 
@@ -83,14 +919,14 @@ __global__ __launch_bounds__(256) void normSumsAny(NormArgs a) {
   const T* const x = static_cast<const T*>(a.x.data) + b * a.x.b + c * a.x.c;
   const T* const g = static_cast<const T*>(a.g.data) + b * a.g.b + c * a.g.c;
   double s1 = 0, s2 = 0;
-  for (long p = threadIdx.x; p < a.P; p += 256) {
-    const float xh = ((float)x[pixelAt(a.x, p, a.W)] - mean) * rstd;
-    const float dz = (float)g[pixelAt(a.g, p, a.W)] * slope(affine(xh, w, shift), a.activation);
+  for (int p = threadIdx.x; p < a.P; p += 256) {
+    const float xh = ((float)x[pixelAt(a, a.x, p)] - mean) * rstd;
+    const float dz = (float)g[pixelAt(a, a.g, p)] * slope(affine(xh, w, shift), a.activation);
     s1 += dz;
     s2 += (double)dz * xh;
   }
-  s1 = groupSum(s1, space);
-  s2 = groupSum(s2, space);
+  s1 = teamSum<256>(s1, space);
+  s2 = teamSum<256>(s2, space);
   if (threadIdx.x == 0) a.channels[b * a.C + c] = float2{(float)s1, (float)s2};
 }
 
@@ -111,29 +947,120 @@ __global__ __launch_bounds__(256) void normGradAny(NormArgs a) {
   const T* const g = static_cast<const T*>(a.g.data) + b * a.g.b + group * a.D * a.g.c;
   T* const y = static_cast<T*>(a.y.data) + b * a.y.b + group * a.D * a.y.c;
   for (long e = threadIdx.x; e < n; e += 256) {
-    const long c = e / a.P, p = e % a.P;
+    const int c = quotient((int)e, a.byP), p = (int)e - c * (int)a.P;
     const float w = lineOr(a.weight, group * a.D + c, 1.f), shift = lineOr(a.bias, group * a.D + c, 0.f);
-    const float xh = ((float)x[c * a.x.c + pixelAt(a.x, p, a.W)] - mean) * rstd;
-    const float dz = (float)g[c * a.g.c + pixelAt(a.g, p, a.W)] * slope(affine(xh, w, shift), a.activation);
-    y[c * a.y.c + pixelAt(a.y, p, a.W)] = (T)(rstd * (dz * w - m1 - xh * m2));
+    const float xh = ((float)x[c * a.x.c + pixelAt(a, a.x, p)] - mean) * rstd;
+    const float dz = (float)g[c * a.g.c + pixelAt(a, a.g, p)] * slope(affine(xh, w, shift), a.activation);
+    y[c * a.y.c + pixelAt(a, a.y, p)] = (T)(rstd * (dz * w - m1 - xh * m2));
   }
 }
 
-// The gradients of weight and bias: the sums over the images, in their order.
-__global__ __launch_bounds__(64) void normParameters(NormArgs a) {
-  const long c = (long)blockIdx.x * 64 + threadIdx.x;
-  if (c >= a.C) return;
-  double s1 = 0, s2 = 0;
-  for (long b = 0; b < a.B; ++b) {
-    const float2 s = a.channels[b * a.C + c];
-    s1 += s.x;
-    s2 += s.y;
-  }
-  if (a.gradBias.data) storeAny(a.gradBias.data, a.gradBias.type, c * a.gradBias.stride, (float)s1);
-  if (a.gradWeight.data) storeAny(a.gradWeight.data, a.gradWeight.type, c * a.gradWeight.stride, (float)s2);
+// ---- what runs ----
+
+enum Family { Last, Planes, Any };
+
+// The kernels of a problem: elements of a word, lanes of a workgroup or team and words of a lane where a group stays in
+// registers (items 0: two launches), and the pieces that the first of two launches cuts a group into.
+struct NormPlan {
+  Family family;
+  int vec, threads, items, band, lanes, rows;
+  long pieces, piece;
+};
+
+struct Shape {
+  int threads, items;
+};
+
+bool unitPixels(const Image& i, long C, long H, long W) {
+  return (W == 1 || i.w == 1) && (H == 1 || i.h == W) && (C == 1 || i.c == H * W);
+}
+bool wordsFit(const Image& i, long vec, size_t size) {
+  return i.b % vec == 0 && i.h % vec == 0 && i.w % vec == 0 && aligned(i.data, vec * size);
 }
 
-NormArgs argsOf(const NormProblem& p) {
+constexpr long kMostPieces = 256;
+// (of each image's pixels, or of a group's values; the bound that the workspace is made for)
+long piecesOf(long units, long images) {
+  return std::max(1L, std::min({kMostPieces, 2048 / std::max(1L, images), units}));
+}
+
+NormPlan planOf(const NormProblem& p, bool backward) {
+  const size_t size = p.type == FBFFT_FLOAT32 ? 4 : 2;
+  const int most = 16 / (int)size;
+  const long P = p.H * p.W, D = p.C / p.G, n = D * P;
+  const Image* const used[3] = {&p.x, &p.y, &p.g};
+  const int count = backward ? 3 : 2;
+  bool unit = true, channels = true, nearer = true;
+  for (int i = 0; i < count; ++i) {
+    if (!used[i]->data) continue;
+    unit = unit && unitPixels(*used[i], p.C, p.H, p.W);
+    channels = channels && (p.C == 1 || used[i]->c == 1);
+    nearer = nearer && std::abs(used[i]->w) < std::abs(used[i]->c);
+  }
+  NormPlan plan{};
+  if (unit || (nearer && !channels)) {
+    plan.family = Planes;
+    plan.vec = unit && P >= most ? most : 1;
+    const long words = (n + plan.vec - 1) / plan.vec;
+    if (!backward) {
+      plan.threads = words <= 64 * 4 ? 64 : words <= 256 * 4 ? 256 : 1024;
+      plan.items = words <= plan.threads * 4L ? 4 : words <= plan.threads * 8L ? 8 : 0;
+      if (plan.items == 0) {
+        plan.pieces = piecesOf((n + 4095) / 4096, p.B * p.G);
+        plan.piece = ((n + plan.pieces - 1) / plan.pieces + plan.vec - 1) / plan.vec * plan.vec;
+      }
+    } else {
+      plan.threads = P <= 64 * 4 * plan.vec ? 64 : 256;
+      plan.pieces = piecesOf((P + 4095) / 4096, p.B * p.C);
+      plan.piece = ((P + plan.pieces - 1) / plan.pieces + plan.vec - 1) / plan.vec * plan.vec;
+    }
+    return plan;
+  }
+  plan.family = Last;
+  for (plan.vec = channels ? most : 1; plan.vec > 1; plan.vec = plan.vec > 2 ? 2 : 1) {
+    bool fit = p.C % plan.vec == 0;
+    for (int i = 0; i < count; ++i) fit = fit && (!used[i]->data || wordsFit(*used[i], plan.vec, size));
+    if (fit) break;
+  }
+  const long vec = plan.vec;
+  long least = D;  // channels of the smallest band: whole groups and whole words
+  while (least % vec != 0) least += D;
+  if (least / vec > 256 || least > kBand || (D % vec != 0 && least > 256)) {
+    plan.family = Any;
+    plan.pieces = 1;
+    return plan;
+  }
+  auto setBand = [&](long band, int threads) {
+    plan.band = (int)std::min(band, p.C), plan.threads = threads;
+    plan.lanes = (int)(plan.band / vec), plan.rows = threads / plan.lanes;
+  };
+  // a band of 128 bytes of neighbouring channels or more where this leaves a workgroup for each compute unit, or of 64,
+  // or of whatever a group has
+  const long bytes = least * (long)size;
+  for (long want : {128L, 64L, 1L}) {
+    const long band = std::min(p.C, (want + bytes - 1) / bytes * least), lanes = band / vec, bands = (p.C + band - 1) / band;
+    if (want > 1 && p.B * bands < 256 && band > least) continue;
+    for (const auto& shape : {Shape{256, 4}, Shape{256, 8}, Shape{512, 8}, Shape{1024, 8}}) {
+      if (backward && shape.threads == 1024) break;  // (input, gradient and a lane's sums would not fit its registers)
+      if (lanes > shape.threads || band / D > shape.threads || band > kBand || P > shape.threads / lanes * (long)shape.items) continue;
+      setBand(band, shape.threads);
+      plan.items = shape.items;
+      plan.pieces = 1, plan.piece = P;
+      return plan;
+    }
+  }
+  long band = least;
+  while (band + least <= p.C && (band + least) / vec <= 256 && band + least <= kBand && (band + least) / D <= 256 &&
+         (D % vec == 0 || band + least <= 256))
+    band += least;
+  setBand(band, 256);
+  const long bands = (p.C + plan.band - 1) / plan.band;
+  plan.pieces = piecesOf((P + 4 * plan.rows - 1) / (4 * plan.rows), p.B * bands);
+  plan.piece = (P + plan.pieces - 1) / plan.pieces;
+  return plan;
+}
+
+NormArgs argsOf(const NormProblem& p, const NormPlan& plan, bool backward) {
   NormArgs a{};
   a.x = p.x, a.y = p.y, a.g = p.g;
   a.weight = p.weight, a.bias = p.bias, a.gradWeight = p.gradWeight, a.gradBias = p.gradBias;
@@ -141,32 +1068,141 @@ NormArgs argsOf(const NormProblem& p) {
   a.meanB = p.meanB, a.meanG = p.meanG, a.rstdB = p.rstdB, a.rstdG = p.rstdG;
   a.B = p.B, a.C = p.C, a.G = p.G, a.D = p.C / p.G, a.H = p.H, a.W = p.W, a.P = p.H * p.W;
   a.activation = p.activation, a.eps = p.eps;
-  a.channels = static_cast<float2*>(p.workspace);
+  a.share = 1.0 / ((double)a.D * a.P);
+  a.byW = divisorOf(a.W), a.byP = divisorOf(a.P), a.byD = divisorOf(a.D), a.byLanes = divisorOf(plan.lanes);
+  a.byPieces = divisorOf(plan.pieces), a.byBands = divisorOf(plan.band ? (p.C + plan.band - 1) / plan.band : 1);
+  a.band = plan.band, a.rows = plan.rows, a.lanes = plan.lanes, a.pieces = (int)plan.pieces, a.piece = plan.piece;
+  char* const space = static_cast<char*>(p.workspace);
+  if (!backward) {
+    a.sums = reinterpret_cast<double2*>(space);
+  } else {
+    a.groups = reinterpret_cast<float2*>(space);
+    a.channels = a.groups + (p.B * kMostPieces < 4096 ? p.B * kMostPieces : std::max(4096L, p.B)) * p.G;
+  }
   return a;
+}
+
+unsigned blocksOf(const NormArgs& a) { return (unsigned)(a.B * ((a.C + a.band - 1) / a.band) * a.pieces); }
+
+template <class T, int VEC>
+int forwardLast(const NormPlan& plan, const NormArgs& a, hipStream_t s) {
+  const int total = (int)blocksOf(a);
+  const dim3 grid((unsigned)total), dealt((unsigned)((total + 7) / 8 * 8));
+  if (plan.items == 0) {
+    lastSums<T, VEC><<<grid, 256, 0, s>>>(a);
+    lastApply<T, VEC><<<grid, 256, 0, s>>>(a);
+  } else if (plan.items == 4) {
+    lastForward<T, VEC, 256, 4><<<dealt, 256, 0, s>>>(a, total);
+  } else if (plan.threads == 256) {
+    lastForward<T, VEC, 256, 8><<<dealt, 256, 0, s>>>(a, total);
+  } else if (plan.threads == 512) {
+    lastForward<T, VEC, 512, 8><<<dealt, 512, 0, s>>>(a, total);
+  } else {
+    lastForward<T, VEC, 1024, 8><<<dealt, 1024, 0, s>>>(a, total);
+  }
+  return launchStatus();
+}
+
+template <class T, int VEC>
+int forwardPlanes(const NormPlan& plan, const NormArgs& a, hipStream_t s) {
+  const long groups = a.B * a.G;
+  if (plan.items == 0) {
+    planesSums<T, VEC><<<dim3((unsigned)(groups * a.pieces)), 256, 0, s>>>(a);
+    planesApply<T, VEC><<<dim3((unsigned)(groups * a.pieces)), 256, 0, s>>>(a);
+  } else if (plan.threads == 64) {
+    planesForward<T, VEC, 64, 4><<<dim3((unsigned)((groups + 3) / 4)), 256, 0, s>>>(a);
+  } else if (plan.threads == 256) {
+    planesForward<T, VEC, 256, 4><<<dim3((unsigned)groups), 256, 0, s>>>(a);
+  } else if (plan.items == 4) {
+    planesForward<T, VEC, 1024, 4><<<dim3((unsigned)groups), 1024, 0, s>>>(a);
+  } else {
+    planesForward<T, VEC, 1024, 8><<<dim3((unsigned)groups), 1024, 0, s>>>(a);
+  }
+  return launchStatus();
+}
+
+// (both: whether the gradients of weight and bias are done, by `before` workgroups)
+template <class T, int VEC>
+bool backwardLast(const NormPlan& plan, const NormArgs& a, int before, hipStream_t s) {
+  const int total = (int)blocksOf(a);
+  const dim3 grid((unsigned)total), dealt((unsigned)((total + 7) / 8 * 8));
+  if (plan.items == 0) {
+    lastGradSums<T, VEC><<<grid, 256, 0, s>>>(a);
+    if (!a.y.data) return false;
+    lastGradApply<T, VEC><<<dim3((unsigned)(total + before)), 256, 0, s>>>(a, before);
+    return true;
+  }
+  if (plan.items == 4)
+    lastBackward<T, VEC, 256, 4><<<dealt, 256, 0, s>>>(a, total);
+  else if (plan.threads == 256)
+    lastBackward<T, VEC, 256, 8><<<dealt, 256, 0, s>>>(a, total);
+  else
+    lastBackward<T, VEC, 512, 8><<<dealt, 512, 0, s>>>(a, total);
+  return false;
+}
+
+template <class T, int VEC>
+bool backwardPlanes(const NormPlan& plan, const NormArgs& a, int before, hipStream_t s) {
+  const long planes = a.B * a.C * a.pieces;
+  if (plan.threads == 64)
+    planesGradSums<T, VEC, 64><<<dim3((unsigned)((planes + 3) / 4)), 256, 0, s>>>(a);
+  else
+    planesGradSums<T, VEC, 256><<<dim3((unsigned)planes), 256, 0, s>>>(a);
+  if (!a.y.data) return false;
+  const long words = (a.D * a.P + VEC - 1) / VEC, each = std::max(1L, std::min(8L, words * a.B * a.G / (256 * 4096)));
+  const long blocks = (words + 256 * each - 1) / (256 * each);
+  planesGradApply<T, VEC><<<dim3((unsigned)(a.B * a.G * blocks + before)), 256, 0, s>>>(a, blocks, (int)each, before);
+  return true;
 }
 
 template <class T>
 int forward(const NormProblem& p, hipStream_t s) {
-  const NormArgs a = argsOf(p);
+  constexpr int W = 16 / sizeof(T);
+  const NormPlan plan = planOf(p, false);
+  const NormArgs a = argsOf(p, plan, false);
+  if (plan.family == Planes) return plan.vec == W ? forwardPlanes<T, W>(plan, a, s) : forwardPlanes<T, 1>(plan, a, s);
+  if (plan.family == Last)
+    return plan.vec == W   ? forwardLast<T, W>(plan, a, s)
+           : plan.vec == 2 ? forwardLast<T, 2>(plan, a, s)
+                           : forwardLast<T, 1>(plan, a, s);
   normAny<T><<<dim3((unsigned)(a.B * a.G)), 256, 0, s>>>(a);
   return launchStatus();
 }
 
 template <class T>
 int backward(const NormProblem& p, hipStream_t s) {
-  NormArgs a = argsOf(p);
-  if (a.P == 0) a.B = 0;  // no pixels: the gradients are sums of nothing
-  if (a.B > 0) normSumsAny<T><<<dim3((unsigned)(a.B * a.C)), 256, 0, s>>>(a);
-  if (a.B > 0 && a.y.data) normGradAny<T><<<dim3((unsigned)(a.B * a.G)), 256, 0, s>>>(a);
-  if (a.gradWeight.data || a.gradBias.data)
-    normParameters<<<dim3((unsigned)((a.C + 63) / 64)), 64, 0, s>>>(a);
+  constexpr int W = 16 / sizeof(T);
+  NormPlan plan{Any};
+  NormArgs a = argsOf(p, plan, true);
+  const int parameters = a.gradWeight.data || a.gradBias.data ? (int)((a.C + kParameters - 1) / kParameters) : 0;
+  bool done = parameters == 0;
+  if (a.B == 0 || a.P == 0) {
+    a.B = 0;  // the gradients of weight and bias are sums of nothing
+  } else {
+    plan = planOf(p, true);
+    a = argsOf(p, plan, true);
+    if (plan.family == Planes) {
+      done |= plan.vec == W ? backwardPlanes<T, W>(plan, a, parameters, s) : backwardPlanes<T, 1>(plan, a, parameters, s);
+    } else if (plan.family == Last) {
+      done |= plan.vec == W   ? backwardLast<T, W>(plan, a, parameters, s)
+              : plan.vec == 2 ? backwardLast<T, 2>(plan, a, parameters, s)
+                              : backwardLast<T, 1>(plan, a, parameters, s);
+    } else {
+      normSumsAny<T><<<dim3((unsigned)(a.B * a.C)), 256, 0, s>>>(a);
+      if (a.y.data) normGradAny<T><<<dim3((unsigned)(a.B * a.G)), 256, 0, s>>>(a);
+    }
+  }
+  if (!done) normParameters<<<dim3((unsigned)parameters), 256, 0, s>>>(a);
   return launchStatus();
 }
 
 }  // namespace
 
 size_t normWorkspaceBytes(int pass, long B, long C, long P, long G) {
-  return pass == 0 ? 0 : (size_t)(B * C) * sizeof(float2);
+  // images times pieces: of any plan
+  const long rows = B * kMostPieces < 4096 ? B * kMostPieces : std::max(4096L, B);
+  if (pass == 0) return (size_t)rows * G * sizeof(double2);
+  return (size_t)rows * (G + C) * sizeof(float2);
 }
 
 int launchNormForward(const NormProblem& p, hipStream_t s) {

@@ -56,6 +56,73 @@ __device__ __forceinline__ void storeAny(void* p, int type, long i, float v) {
     static_cast<brain16*>(p)[i] = (brain16)v;
 }
 
+// Division of numbers below 2^31 by one that is fixed before the launch: one product and a shift.
+struct Divisor {
+  unsigned magic, shift, value;
+};
+inline Divisor divisorOf(long value) {
+  Divisor d{0, 0, (unsigned)value};
+  if (value < 2) return d;
+  unsigned bits = 1;
+  while ((1ul << bits) < (unsigned long)value) ++bits;
+  d.magic = (unsigned)(((1ul << (31 + bits)) + value - 1) / value);  // at least 2^31: the value is over 2^(bits - 1)
+  d.shift = bits - 1;
+  return d;
+}
+__device__ __forceinline__ int quotient(int n, const Divisor& d) {
+  return d.value < 2 ? n : (int)(__umulhi((unsigned)n, d.magic) >> d.shift);
+}
+
+// Sums over the 64 lanes of a wave, in every lane: four steps among 16 lanes by data-parallel moves, then rows and
+// halves of the wave swapped against themselves.  Nothing goes through LDS.
+template <int CONTROL>
+__device__ __forceinline__ float moved(float v) {
+  const int i = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CONTROL, 0xF, 0xF, false));
+}
+template <int CONTROL>
+__device__ __forceinline__ double moved(double v) {
+  const long i = __builtin_bit_cast(long, v);
+  const int low = (int)i, high = (int)(i >> 32);
+  const unsigned l = __builtin_amdgcn_update_dpp(low, low, CONTROL, 0xF, 0xF, false);
+  const unsigned h = __builtin_amdgcn_update_dpp(high, high, CONTROL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (unsigned long)h << 32 | l);
+}
+template <bool HALVES>
+__device__ __forceinline__ float swappedSum(float v) {
+  const unsigned i = __builtin_bit_cast(unsigned, v);
+  const auto r = HALVES ? __builtin_amdgcn_permlane32_swap(i, i, false, false) : __builtin_amdgcn_permlane16_swap(i, i, false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+template <bool HALVES>
+__device__ __forceinline__ double swappedSum(double v) {
+  const unsigned long i = __builtin_bit_cast(unsigned long, v);
+  const unsigned low = (unsigned)i, high = (unsigned)(i >> 32);
+  const auto l = HALVES ? __builtin_amdgcn_permlane32_swap(low, low, false, false) : __builtin_amdgcn_permlane16_swap(low, low, false, false);
+  const auto h = HALVES ? __builtin_amdgcn_permlane32_swap(high, high, false, false) : __builtin_amdgcn_permlane16_swap(high, high, false, false);
+  return __builtin_bit_cast(double, (unsigned long)(unsigned)h[0] << 32 | (unsigned)l[0]) +
+         __builtin_bit_cast(double, (unsigned long)(unsigned)h[1] << 32 | (unsigned)l[1]);
+}
+template <class S>
+__device__ __forceinline__ S waveSum(S v) {
+  v += moved<0xB1>(v);   // lanes 1 0 3 2
+  v += moved<0x4E>(v);   // lanes 2 3 0 1
+  v += moved<0x141>(v);  // eight lanes, reversed
+  v += moved<0x140>(v);  // sixteen lanes, reversed
+  return swappedSum<true>(swappedSum<false>(v));
+}
+
+// The same over the lanes whose numbers leave one remainder on division by `period`, a power of two up to 32.
+template <class S>
+__device__ __forceinline__ S waveSumEvery(S v, int period) {
+  if (period <= 8) v += moved<0x128>(v);  // rotations among 16 lanes, by 8
+  if (period <= 4) v += moved<0x124>(v);
+  if (period <= 2) v += moved<0x122>(v);
+  if (period <= 1) v += moved<0x121>(v);
+  if (period <= 16) v = swappedSum<false>(v);
+  return swappedSum<true>(v);
+}
+
 // a vector of parameters, or nothing
 struct Line {
   void* data;
@@ -100,6 +167,21 @@ __device__ __forceinline__ float activate(float z, int activation) {
   return z;
 }
 
+template <int N>
+__device__ __forceinline__ void activateAll(float (&v)[N], int activation) {
+  if (activation == FBFFT_ACTIVATION_NONE) return;
+  if (activation == FBFFT_ACTIVATION_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = activate(v[j], FBFFT_ACTIVATION_RELU);
+  } else if (activation == FBFFT_ACTIVATION_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = activate(v[j], FBFFT_ACTIVATION_SILU);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = activate(v[j], FBFFT_ACTIVATION_GELU);
+  }
+}
+
 __device__ __forceinline__ float slope(float z, int activation) {
   if (activation == FBFFT_ACTIVATION_RELU) return z > 0.f ? 1.f : 0.f;
   if (activation == FBFFT_ACTIVATION_SILU) {
@@ -112,6 +194,22 @@ __device__ __forceinline__ float slope(float z, int activation) {
     return __builtin_fmaf(z, density, cdf);
   }
   return 1.f;
+}
+
+// g[j] times the slope at z[j]
+template <int N>
+__device__ __forceinline__ void slopeAll(const float (&z)[N], float (&g)[N], int activation) {
+  if (activation == FBFFT_ACTIVATION_NONE) return;
+  if (activation == FBFFT_ACTIVATION_RELU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] *= slope(z[j], FBFFT_ACTIVATION_RELU);
+  } else if (activation == FBFFT_ACTIVATION_SILU) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] *= slope(z[j], FBFFT_ACTIVATION_SILU);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) g[j] *= slope(z[j], FBFFT_ACTIVATION_GELU);
+  }
 }
 
 // ---- launchers (each returns an fbfft_error; shapes are checked by the caller) ----

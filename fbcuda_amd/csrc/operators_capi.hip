@@ -57,7 +57,7 @@ int checkNorm(const fbfft_array* input, const fbfft_array* weight, const fbfft_a
   if (groups < 1 || C % groups != 0) return FBFFT_UNSUPPORTED_SIZE;
   if (!okLine(weight, C) || !okLine(bias, C)) return FBFFT_UNSUPPORTED_DIMENSION;
   // (workgroups count images times channels, and lanes the values of a group in 31 bits)
-  if (input->size[0] * C > 0x7fffffff || C / groups * input->size[2] * input->size[3] > 0x7fffffff) return FBFFT_UNSUPPORTED_SIZE;
+  if (input->size[0] * C > 0x7fffffff || C / groups * input->size[2] * input->size[3] > 0x7ffff000) return FBFFT_UNSUPPORTED_SIZE;
   return FBFFT_SUCCESS;
 }
 
