@@ -41,9 +41,8 @@ struct NormArgs {
 };
 
 __device__ __forceinline__ long pixelAt(const NormArgs& a, const Image& i, int p) {
-  if (i.h == a.W * i.w) return (long)p * i.w;
-  const int row = quotient(p, a.byW);
-  return (long)row * i.h + (long)(p - row * (int)a.W) * i.w;
+  // (rows without gaps: the second term is 0; a branch would cost more)
+  return (long)p * i.w + (long)quotient(p, a.byW) * (i.h - a.W * i.w);
 }
 
 // The activation's argument, from a product and a sum that are rounded apart: both passes, and a program that writes
@@ -117,23 +116,30 @@ struct Columns {
 };
 
 // A workgroup's band of whole groups: lane t holds VEC channels from VEC (t % lanes) of every rows-th pixel.  Adds what
-// each lane has of its channels over the rows of lanes; sums[i] is then that of lane column i (SLOTS values of a lane
+// each lane has of its channels over the rows of lanes; sums[i] is then that of lane column i (several values of a lane
 // side by side).  Where rows of lanes divide a wave its rows meet in registers first (64 sums by one lane from LDS
 // took 7 us of the smallest call's 14), and what waits in LDS is summed in two stages.
-template <int NT, int SLOTS, int VEC, class S>
-__device__ __forceinline__ void joinRows(const NormArgs& a, int lanes, int column, int r, S (&v)[SLOTS],
+// `step` of a lane's channels, 1 or a power of two that divides VEC, are added up before that: those of one group.
+template <int NT, int VEC, class S>
+__device__ __forceinline__ void joinRows(const NormArgs& a, int lanes, int column, int r, int step, S (&v)[VEC],
                                          Columns<NT, VEC, S>& space, S* sums) {
-  const int t = threadIdx.x, columns = lanes * SLOTS;
+#pragma unroll
+  for (int d = 1; d < VEC; d *= 2)
+    if (step > d)
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2 * d) v[j] += v[j + d];
+  const int t = threadIdx.x, shift = 31 - __builtin_clz(step), slots = VEC >> shift, columns = lanes * slots;
   const bool divides = a.lanes <= 32 && (a.lanes & (a.lanes - 1)) == 0;
   const int rows = divides ? NT / 64 : a.rows, row = divides ? t / 64 : r;
-  if (divides) {
+  if (divides)
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) v[j] = waveSumEvery(v[j], a.lanes);
-  }
+    for (int j = 0; j < VEC; ++j)
+      if ((j & (step - 1)) == 0) v[j] = waveSumEvery(v[j], a.lanes);
   __syncthreads();
   if (column < lanes && (divides ? t % 64 < a.lanes : r < a.rows))
 #pragma unroll
-    for (int j = 0; j < SLOTS; ++j) space.lane[row * columns + column * SLOTS + j] = v[j];
+    for (int j = 0; j < VEC; ++j)
+      if ((j & (step - 1)) == 0) space.lane[row * columns + column * slots + (j >> shift)] = v[j];
   __syncthreads();
   if (rows <= 16 || columns > NT / 2) {
     for (int i = t; i < columns; i += NT) {
@@ -210,6 +216,13 @@ struct Channel {
       shift[j] = p.y;
     }
   }
+  // The activation's arguments in the place of x.  16-bit results take one multiply-add: what it loses to the mean's
+  // size, 2^-24 mean / deviation, is below their rounding (and that of x, whose bits the mean's size takes, too).
+  template <class T>
+  __device__ __forceinline__ void apply(float (&x)[VEC]) const {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) x[j] = sizeof(T) == 4 ? affine((x[j] - mean[j]) * rstd[j], w[j], shift[j]) : __builtin_fmaf(x[j], rstd[j] * w[j], __builtin_fmaf(-mean[j], rstd[j] * w[j], shift[j]));
+  }
   // x is replaced by the normalised values, z by the activation's arguments
   __device__ __forceinline__ void arguments(float (&x)[VEC], float (&z)[VEC]) const {
 #pragma unroll
@@ -224,19 +237,11 @@ struct Channel {
 template <int NT, int VEC>
 __device__ __forceinline__ void joinMoments(const NormArgs& a, const Band& band, double (&s1)[VEC], double (&s2)[VEC],
                                             Columns<NT, VEC, double>& space, double* sums, Moments* stats, bool raw) {
-  // where a lane's channels are all of one group, they are added before they go through LDS
   const int D = (int)a.D, t = threadIdx.x;
-  const bool whole = VEC > 1 && D % VEC == 0;
-  const int wide = whole ? D / VEC : D;
+  // a lane's channels of one group, where groups and words start together
+  const int step = D % VEC == 0 ? VEC : VEC % D == 0 ? D : 1, wide = D / step;
   auto one = [&](double(&s)[VEC]) __attribute__((always_inline)) {
-    if (whole) {
-      double v[1] = {0};
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[0] += s[j];
-      joinRows<NT, 1, VEC>(a, band.lanes, band.column, band.r, v, space, sums);
-    } else {
-      joinRows<NT, VEC, VEC>(a, band.lanes, band.column, band.r, s, space, sums);
-    }
+    joinRows<NT, VEC>(a, band.lanes, band.column, band.r, step, s, space, sums);
     __syncthreads();
     // a wave to a group (as many as a wave has lanes, or fewer, to each: NT groups at most)
     double kept = 0;
@@ -331,11 +336,11 @@ __global__ __launch_bounds__(NT) void lastForward(NormArgs a, int total) {
   for (int i = 0; i < ITEMS; ++i) {
     const int p = band.r + i * a.rows;
     if (p >= P) break;
-    float v[VEC], z[VEC];
+    float v[VEC];
     unpack(raw[i], v);
-    ch.arguments(v, z);
-    activateAll(z, a.activation);
-    storePack<T, VEC>(y + pixelAt(a, a.y, p), z);
+    ch.template apply<T>(v);
+    activateAll(v, a.activation);
+    storePack<T, VEC>(y + pixelAt(a, a.y, p), v);
   }
 }
 
@@ -400,11 +405,11 @@ __global__ __launch_bounds__(256) void lastApply(NormArgs a) {
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
       if (p + k * a.rows < end) {
-        float v[VEC], z[VEC];
+        float v[VEC];
         unpack(raw[k], v);
-        ch.arguments(v, z);
-        activateAll(z, a.activation);
-        storePack<T, VEC>(y + pixelAt(a, a.y, p + k * a.rows), z);
+        ch.template apply<T>(v);
+        activateAll(v, a.activation);
+        storePack<T, VEC>(y + pixelAt(a, a.y, p + k * a.rows), v);
       }
   }
 }
@@ -423,8 +428,8 @@ __device__ __forceinline__ void keptMoments(const NormArgs& a, const Band& band,
 template <int NT, int VEC, class F>
 __device__ __forceinline__ void joinGradients(const NormArgs& a, const Band& band, float (&s1)[VEC], float (&s2)[VEC],
                                               Columns<NT, VEC, float>& space, float (&sums)[2][kBand], const float2* params, F done) {
-  joinRows<NT, VEC, VEC>(a, band.lanes, band.column, band.r, s1, space, sums[0]);
-  joinRows<NT, VEC, VEC>(a, band.lanes, band.column, band.r, s2, space, sums[1]);
+  joinRows<NT, VEC>(a, band.lanes, band.column, band.r, 1, s1, space, sums[0]);
+  joinRows<NT, VEC>(a, band.lanes, band.column, band.r, 1, s2, space, sums[1]);
   // (a lane reads what it has written)
   for (int c = threadIdx.x; c < band.channels; c += NT) {
     const float2 s{sums[0][c], sums[1][c]};
@@ -981,7 +986,7 @@ bool wordsFit(const Image& i, long vec, size_t size) {
 constexpr long kMostPieces = 256;
 // (of each image's pixels, or of a group's values; the bound that the workspace is made for)
 long piecesOf(long units, long images) {
-  return std::max(1L, std::min({kMostPieces, 2048 / std::max(1L, images), units}));
+  return std::max(1L, std::min({kMostPieces, 1024 / std::max(1L, images), units}));
 }
 
 NormPlan planOf(const NormProblem& p, bool backward) {

@@ -155,15 +155,26 @@ __device__ __forceinline__ void normalOf(float z, float& cdf, float& density) {
   density = 0.398942280f * e;
 }
 
+// z times the normal distribution function, where the density is not wanted: log2(cdf / (1 - cdf)) is z times a
+// polynomial in z^2, fitted the same way up to |z| = 5.6 (and constant behind it) for the least greatest error of the
+// result, 6.6e-8: half of what 32-bit arithmetic loses in z (1 + erf(z / sqrt 2)) / 2.
+__device__ __forceinline__ float gelu(float z) {
+  const float u = __builtin_fminf(z * z, 31.36f);
+  float q = 5.2339035e-09f;
+  q = __builtin_fmaf(q, u, -3.86017405e-07f);
+  q = __builtin_fmaf(q, u, 1.14667555e-05f);
+  q = __builtin_fmaf(q, u, -0.000159485367f);
+  q = __builtin_fmaf(q, u, -9.52946357e-05f);
+  q = __builtin_fmaf(q, u, 0.104838192f);
+  q = __builtin_fmaf(q, u, 2.30220747f);
+  return z * inverse(1.f + __builtin_amdgcn_exp2f(-z * q));
+}
+
 __device__ __forceinline__ float activate(float z, int activation) {
   // (a comparison that keeps NaN)
   if (activation == FBFFT_ACTIVATION_RELU) return z < 0.f ? 0.f : z;
   if (activation == FBFFT_ACTIVATION_SILU) return z * inverse(1.f + expOf(-z));
-  if (activation == FBFFT_ACTIVATION_GELU) {
-    float cdf, density;
-    normalOf(z, cdf, density);
-    return z * cdf;
-  }
+  if (activation == FBFFT_ACTIVATION_GELU) return gelu(z);
   return z;
 }
 
