@@ -25,6 +25,7 @@ struct Epilogue {
   Matrix out, residual, z;  // data null: none of it
   Line bias;
   int activation;
+  bool dense;    // rows of out, residual and z without gaps between neighbours
   float* parts;  // not null: fp32 sums of each range of k, [range][M][N], in place of results
 };
 
@@ -60,31 +61,42 @@ __device__ __forceinline__ float withoutLeading(float v) {
   return v - __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & 0xFFFF0000u);
 }
 
-constexpr int kTile = 128, kStep = 32;  // rows of either operand and k of a step
+constexpr int kStep = 32;  // k of a step
 
-// One step of an operand, [row][k] or [k][row], as 16-bit pieces in LDS: 16-byte words that are permuted so that the
-// lanes of a fragment's read spread over the banks.  KC: k is contiguous.
-template <class T, bool KC>
+// One step of an operand, ROWS rows by kStep of k, [row][k] or [k][row], as 16-bit pieces in LDS: 16-byte words that
+// are permuted so that the lanes of a fragment's read spread over the banks.  KC: k is contiguous.
+template <class T, bool KC, int ROWS>
 struct Stage {
-  static constexpr int per = 16 / sizeof(T), words = kTile * kStep / per / 256, pieceBytes = kTile * kStep * 2;
+  static constexpr int per = 16 / sizeof(T), words = ROWS * kStep / per / 256, pieceBytes = ROWS * kStep * 2;
   typename Pack<T, per>::type v[words];
+  const T* from[words];  // of each word at k = 0
+  bool whole[words];     // its elements are neighbours, and inside
 
-  __device__ __forceinline__ void load(const Matrix& m, long row0, long rows, long k0, long end) {
-    const T* const data = static_cast<const T*>(m.data);
+  static __device__ __forceinline__ int lineOf(int i) { return (threadIdx.x + 256 * i) / ((KC ? kStep : ROWS) / per); }
+  static __device__ __forceinline__ int firstOf(int i) { return (threadIdx.x + 256 * i) % ((KC ? kStep : ROWS) / per) * per; }
+
+  __device__ __forceinline__ void setup(const Matrix& m, long row0, long rows) {
 #pragma unroll
     for (int i = 0; i < words; ++i) {
-      const int w = threadIdx.x + 256 * i;
-      const long row = row0 + (KC ? w / (kStep / per) : w % (kTile / per) * per);
-      const long k = k0 + (KC ? w % (kStep / per) * per : w / (kTile / per));
-      const long inner = KC ? m.col : m.row;
-      if (inner == 1 && (KC ? row < rows && k + per <= end : k < end && row + per <= rows)) {
-        v[i] = *reinterpret_cast<const typename Pack<T, per>::type*>(data + row * m.row + k * m.col);
-      } else {
+      const long row = row0 + (KC ? lineOf(i) : firstOf(i)), k = KC ? firstOf(i) : lineOf(i);
+      // (rows behind the last: the last again, whose results nobody takes)
+      from[i] = static_cast<const T*>(m.data) + min(row, rows - 1) * m.row + k * m.col;
+      whole[i] = KC ? m.col == 1 : m.row == 1 && row + per <= rows;
+    }
+  }
+
+  __device__ __forceinline__ void load(const Matrix& m, long row0, long rows, long k0, long end) {
 #pragma unroll
-        for (int j = 0; j < per; ++j) {
-          const long r = KC ? row : row + j, c = KC ? k + j : k;
-          v[i][j] = r < rows && c < end ? data[r * m.row + c * m.col] : (T)0.f;
-        }
+    for (int i = 0; i < words; ++i) {
+      const long k = k0 + (KC ? firstOf(i) : lineOf(i));
+      const T* const p = from[i] + k0 * m.col;
+      if (whole[i] && (KC ? k + per <= end : k < end)) {
+        v[i] = *reinterpret_cast<const typename Pack<T, per>::type*>(p);
+      } else {
+        const long left = KC ? end - k : rows - row0 - firstOf(i), step = KC ? m.col : m.row;
+        const bool some = KC || k < end;
+#pragma unroll
+        for (int j = 0; j < per; ++j) v[i][j] = some && j < left ? p[j * step] : (T)0.f;
       }
     }
   }
@@ -92,16 +104,14 @@ struct Stage {
   // where element `at` (a multiple of `per`) of line `line` lies: bytes
   static __device__ __forceinline__ int place(int line, int at) {
     if (KC) return line * 64 + ((at / 8 ^ line / 4 % 4) * 16) + at % 8 * 2;
-    return line * 256 + ((at / 16 ^ (line % 4 + line / 8 % 2 * 4)) * 32) + at % 16 * 2;
+    const int spread = line % 4 + line / 8 % 2 * 4;
+    return line * (ROWS * 2) + ((at / 16 ^ (ROWS >= 128 ? spread : spread % 4)) * 32) + at % 16 * 2;
   }
 
   __device__ __forceinline__ void store(char* space) const {
 #pragma unroll
     for (int i = 0; i < words; ++i) {
-      const int w = threadIdx.x + 256 * i;
-      const int line = KC ? w / (kStep / per) : w / (kTile / per);
-      const int at = KC ? w % (kStep / per) * per : w % (kTile / per) * per;
-      char* const to = space + place(line, at);
+      char* const to = space + place(lineOf(i), firstOf(i));
       if constexpr (sizeof(T) == 2) {
         *reinterpret_cast<uintx4*>(to) = __builtin_bit_cast(uintx4, v[i]);
       } else {
@@ -127,10 +137,9 @@ struct Stage {
     uintx4 f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const char* const from = space + place(k + 4 * h, at);
-      const shortx4 q = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) shortx4*)const_cast<char*>(from));
-      const uintx2 u = __builtin_bit_cast(uintx2, q);
+      const char* const q = space + place(k + 4 * h, at);
+      const uintx2 u = __builtin_bit_cast(
+          uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)const_cast<char*>(q)));
       f[2 * h] = u[0];
       f[2 * h + 1] = u[1];
     }
@@ -138,99 +147,338 @@ struct Stage {
   }
 };
 
-// one result from its sum
-template <class T>
-__device__ __forceinline__ void finish(const Epilogue& e, long i, long j, float z) {
-  z += lineOr(e.bias, j, 0.f);
-  if (e.z.data) static_cast<T*>(e.z.data)[i * e.z.row + j * e.z.col] = (T)z;
-  float v = activate(z, e.activation);
-  if (e.residual.data) v += (float)static_cast<const T*>(e.residual.data)[i * e.residual.row + j * e.residual.col];
-  static_cast<T*>(e.out.data)[i * e.out.row + j * e.out.col] = (T)v;
+// v[0 ... 7] plus the biases from j
+__device__ __forceinline__ void addBias(const Line& bias, long j, float (&v)[8]) {
+  float b[8];
+  if (bias.stride == 1 && bias.type == FBFFT_FLOAT32) {
+    loadPack<float, 8>(static_cast<const float*>(bias.data) + j, b);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) b[q] = loadAny(bias.data, bias.type, (j + q) * bias.stride);
+  }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) v[q] += b[q];
 }
 
-// A workgroup: 128 x 128 results over one range of k; a wave a quarter of them.  B's rows lie along the rows of the
-// matrix instruction, so that a lane ends with four neighbouring results of one row.
-template <class T, bool AK, bool BK>
+// Eight neighbouring results of row i, or the `count` of them that are inside, from their sums: all of them at once
+// where neighbours are neighbours in memory, else one by one.
+template <class T, class Eight, class One>
+__device__ __forceinline__ void finish(const Epilogue& e, long i, long j, long count, Eight eight, One one) {
+  T* const out = static_cast<T*>(e.out.data) + i * e.out.row + j * e.out.col;
+  const T* const residual = static_cast<const T*>(e.residual.data) + i * e.residual.row + j * e.residual.col;
+  T* const kept = static_cast<T*>(e.z.data) + i * e.z.row + j * e.z.col;
+  if (e.dense && count >= 8) {
+    float z[8];
+    eight(z);
+    if (e.bias.data) addBias(e.bias, j, z);
+    if (e.z.data) storePack<T, 8>(kept, z);
+    activateAll(z, e.activation);
+    if (e.residual.data) {
+      float r[8];
+      loadPack<T, 8>(residual, r);
+#pragma unroll
+      for (int v = 0; v < 8; ++v) z[v] += r[v];
+    }
+    storePack<T, 8>(out, z);
+    return;
+  }
+#pragma unroll 1
+  for (int v = 0; v < min(count, 8L); ++v) {
+    const float z = one(v) + lineOr(e.bias, j + v, 0.f);
+    if (e.z.data) kept[v * e.z.col] = (T)z;
+    float y = activate(z, e.activation);
+    if (e.residual.data) y += (float)residual[v * e.residual.col];
+    out[v * e.out.col] = (T)y;
+  }
+}
+
+// A wave's sums, RM x RN blocks of 16 x 16 (a lane: four neighbours of row lane % 16 of each), go through its own
+// `space` in LDS, TURN rows of blocks at a time, so that a lane then has eight neighbouring results, and rows of them
+// are whole lines.  The 16-byte words of a row are permuted, so that 16 rows' writes take all banks.
+template <class T, int RM, int RN, int TURN>
+__device__ __forceinline__ void leave(const ProductArgs& g, long range, long m0, long n0, const floatx4 (&sum)[RM][RN], char* space) {
+  constexpr int COLS = RN * 16, WORDS = COLS / 4, LANES = COLS / 8, MASK = WORDS < 16 ? WORDS - 1 : 15;
+  const int lane = threadIdx.x % 64;
+#pragma unroll
+  for (int i0 = 0; i0 < RM; i0 += TURN) {
+    waveExchange();
+#pragma unroll
+    for (int i = 0; i < TURN; ++i)
+#pragma unroll
+      for (int j = 0; j < RN; ++j) {
+        const int row = 16 * i + lane % 16, word = (4 * j + lane / 16) ^ (row & MASK);
+        *reinterpret_cast<floatx4*>(space + (row * WORDS + word) * 16) = sum[i0 + i][j];
+      }
+    waveExchange();
+#pragma unroll 1
+    for (int row = lane / LANES; row < 16 * TURN; row += 64 / LANES) {
+      const long m = m0 + 16 * i0 + row, n = n0 + lane % LANES * 8, count = g.N - n;
+      if (m >= g.M || count <= 0) continue;
+      const char* const line = space + row * (WORDS * 16);
+      const int word = lane % LANES * 2;
+      auto eight = [&](float(&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const floatx4 q = *reinterpret_cast<const floatx4*>(line + ((word + h) ^ (row & MASK)) * 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[4 * h + k] = q[k];
+        }
+      };
+      auto one = [&](int v) __attribute__((always_inline)) {
+        return *reinterpret_cast<const float*>(line + ((word + v / 4) ^ (row & MASK)) * 16 + v % 4 * 4);
+      };
+      if (!g.e.parts) {
+        finish<T>(g.e, m, n, count, eight, one);
+        continue;
+      }
+      float* const to = g.e.parts + (range * g.M + m) * g.N + n;
+      if (count >= 8) {
+        float v[8];
+        eight(v);
+        storePack<float, 8>(to, v);
+      } else {
+#pragma unroll 1
+        for (int v = 0; v < count; ++v) to[v] = one(v);
+      }
+    }
+  }
+}
+
+// Where a workgroup's tile lies.  Neighbouring tiles go to one XCD (workgroups are dealt out to the eight in turn), in
+// strips of four rows of tiles, so that those that run together share lines of both operands in its L2.
+template <int BM, int BN>
+struct Tile {
+  long m0, n0;
+  bool any;
+
+  __device__ __forceinline__ Tile(long M, long N) {
+    constexpr int tall = 4;
+    const int across = (int)((N + BN - 1) / BN), down = (int)((M + BM - 1) / BM), total = across * down, per = (total + 7) / 8;
+    int tile = (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
+    any = (int)blockIdx.x / 8 < per && tile < total;
+    const int strip = tile / (tall * across), height = max(1, min(tall, down - strip * tall));
+    tile -= strip * tall * across;
+    m0 = (long)(strip * tall + tile % height) * BM;
+    n0 = (long)(tile / height) * BN;
+  }
+};
+
+// A workgroup: BM x BN results over one range of k; a wave WM x WN of them.  B's rows lie along the rows of the
+// matrix instruction, so that a lane ends with four neighbouring results of one row.  The next step's words are in
+// registers while this one's pieces are multiplied.
+template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(256) void product(ProductArgs g) {
   typedef typename Pieces<T>::type P;
-  constexpr int PIECES = Pieces<T>::count, BYTES = kTile * kStep * 2;
-  __shared__ __attribute__((aligned(16))) char space[2 * PIECES * BYTES];
-  char *const sa = space, *const sb = space + PIECES * BYTES;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int wm = wave / 2 * 64, wn = wave % 2 * 64;
-  const long m0 = (long)blockIdx.y * kTile, n0 = (long)blockIdx.x * kTile;
-  const long first = blockIdx.z * g.range, end = min(first + g.range, g.K);
+  typedef Stage<T, AK, BM> A;
+  typedef Stage<T, BK, BN> B;
+  constexpr int PIECES = Pieces<T>::count, RM = WM / 16, RN = WN / 16, BYTES = PIECES * (A::pieceBytes + B::pieceBytes);
+  constexpr int SHARE = BYTES / 4 > WN * 64 ? BYTES / 4 : WN * 64;  // of LDS, to a wave
+  static_assert(BM / WM * (BN / WN) == 4, "four waves");
+  __shared__ __attribute__((aligned(16))) char space[4 * SHARE];
+  char *const sa = space, *const sb = space + PIECES * A::pieceBytes;
+  const int wave = threadIdx.x / 64, wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+  const Tile<BM, BN> tile(g.M, g.N);
+  if (!tile.any) return;
+  const long first = blockIdx.y * g.range, end = min(first + g.range, g.K);
 
-  floatx4 sum[4][4];
+  floatx4 sum[RM][RN];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < RM; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < RN; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  Stage<T, AK> a;
-  Stage<T, BK> b;
-  a.load(g.a, m0, g.M, first, end);
-  b.load(g.b, n0, g.N, first, end);
+  A a;
+  B b;
+  a.setup(g.a, tile.m0, g.M);
+  b.setup(g.b, tile.n0, g.N);
+  a.load(g.a, tile.m0, g.M, first, end);
+  b.load(g.b, tile.n0, g.N, first, end);
   for (long k = first; k < end; k += kStep) {
     __syncthreads();
     a.store(sa);
     b.store(sb);
     __syncthreads();
-    a.load(g.a, m0, g.M, k + kStep, end);
-    b.load(g.b, n0, g.N, k + kStep, end);
-    uintx4 fb[PIECES][4];
+    if (k + kStep < end) {
+      a.load(g.a, tile.m0, g.M, k + kStep, end);
+      b.load(g.b, tile.n0, g.N, k + kStep, end);
+    }
+    uintx4 fb[PIECES][RN];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) fb[p][j] = Stage<T, BK>::fragment(sb + p * BYTES, wn + 16 * j);
+      for (int j = 0; j < RN; ++j) fb[p][j] = B::fragment(sb + p * B::pieceBytes, wn + 16 * j);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RM; ++i) {
       uintx4 fa[PIECES];
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) fa[p] = Stage<T, AK>::fragment(sa + p * BYTES, wm + 16 * i);
+      for (int p = 0; p < PIECES; ++p) fa[p] = A::fragment(sa + p * A::pieceBytes, wm + 16 * i);
       // the products of pieces p and q, the smallest first
 #pragma unroll
       for (int order = PIECES - 1; order >= 0; --order)
 #pragma unroll
         for (int p = 0; p <= order; ++p)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) sum[i][j] = multiply(fb[order - p][j], fa[p], sum[i][j], P());
+          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[order - p][j], fa[p], sum[i][j], P());
+    }
+  }
+  __syncthreads();
+  constexpr int FIT = SHARE / (WN * 64), TURN = FIT >= RM ? RM : FIT >= 2 ? 2 : 1;  // blocks of rows
+  static_assert(FIT > 0 && RM % TURN == 0, "a wave's share of LDS holds whole rows of blocks");
+  leave<T, RM, RN, TURN>(g, blockIdx.y, tile.m0 + wm, tile.n0 + wn, sum, space + wave * SHARE);
+}
+
+// ---- operands of 16 bits that go straight from memory to LDS ----
+
+typedef __attribute__((address_space(3))) void* LdsAddress;
+
+constexpr int kDeep = 64;  // k of a step
+
+// One step of an operand, ROWS rows by kDeep of k, in 16-byte words.  A wave's load fills 1024 neighbouring bytes of
+// LDS, so the words are permuted where they are read from memory.  KC: k is contiguous, a line is a row, of eight
+// words; else a line is a k, of ROWS / 8.
+template <int ROWS, bool KC, int WAVES>
+struct Direct {
+  static constexpr int words = kDeep * ROWS / 8, loads = words / 64 / WAVES, perLine = KC ? kDeep / 8 : ROWS / 8;
+  static constexpr int bytes = words * 16;
+  unsigned at[loads];  // of each load's word: bytes from the step's first
+  unsigned k[loads];   // its k (KC)
+
+  // which word lies where: KC: so that 16 rows of one k take all places of 256 bytes; else four k and two halves of
+  // a fragment do
+  static __device__ __forceinline__ int permuted(int line, int word) {
+    if (KC) return word ^ (line / 2 % 8);
+    return word ^ ((line % 4 + line / 8 % 2 * 4) * 2);
+  }
+
+  __device__ __forceinline__ void setup(long step) {
+#pragma unroll
+    for (int i = 0; i < loads; ++i) {
+      const int place = ((int)threadIdx.x / 64 * loads + i) * 64 + threadIdx.x % 64, line = place / perLine;
+      const int word = permuted(line, place % perLine);
+      at[i] = (unsigned)(line * step + word * 8) * 2;
+      k[i] = word * 8;
     }
   }
 
+  // base: the step's first element; left: rows and k from there that are inside
+  __device__ __forceinline__ void load(const void* base, long step, long rows, long left, char* space) const {
+    const long lines = KC ? min(rows, (long)ROWS) : min(left, (long)kDeep), line = KC ? min(left, (long)kDeep) : min(rows, (long)ROWS);
+    const unsigned size = (unsigned)(((lines - 1) * step + line) * 2);  // words behind it read as zeros
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, size, 0x00020000);
+    char* const to = space + threadIdx.x / 64 * (loads * 1024);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long m = m0 + wm + 16 * i + lane % 16;
-    if (m >= g.M) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const long n = n0 + wn + 16 * j + lane / 16 * 4 + v;
-        if (n >= g.N) continue;
-        if (g.e.parts)
-          g.e.parts[(blockIdx.z * g.M + m) * g.N + n] = sum[i][j][v];
-        else
-          finish<T>(g.e, m, n, sum[i][j][v]);
-      }
+    for (int i = 0; i < loads; ++i) {
+      // (within a line the end is not the buffer's)
+      const unsigned from = KC && k[i] >= left ? 0x80000000u : at[i];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsAddress)(to + i * 1024), 16, from, 0, 0, 0);
+    }
   }
+
+  // eight k from 32 h + 8 (lane / 16) of row `row` + lane % 16
+  static __device__ __forceinline__ uintx4 fragment(const char* space, int row, int h) {
+    const int lane = threadIdx.x % 64;
+    if (KC) {
+      const int line = row + lane % 16;
+      return *reinterpret_cast<const uintx4*>(space + line * (kDeep * 2) + permuted(line, h * 4 + lane / 16) * 16);
+    }
+    uintx4 f;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int line = h * 32 + lane / 16 * 8 + 4 * q + lane % 16 / 4, first = row + lane % 4 * 4;
+      const char* const from = space + line * (ROWS * 2) + permuted(line, first / 8) * 16 + first % 8 * 2;
+      const uintx2 u = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                      (__attribute__((address_space(3))) shortx4*)const_cast<char*>(from)));
+      f[2 * q] = u[0];
+      f[2 * q + 1] = u[1];
+    }
+    return f;
+  }
+};
+
+// A workgroup: BM x BN results over one range of k, a wave WM x WN of them; two steps' operands in LDS, one of which
+// is multiplied while the other arrives.
+template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(ProductArgs g) {
+  constexpr int WAVES = BM / WM * (BN / WN), RM = WM / 16, RN = WN / 16;
+  typedef Direct<BM, AK, WAVES> A;
+  typedef Direct<BN, BK, WAVES> B;
+  __shared__ __attribute__((aligned(1024))) char space[2][A::bytes + B::bytes];
+  const int wave = threadIdx.x / 64;
+  const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+  const Tile<BM, BN> tile(g.M, g.N);
+  if (!tile.any) return;
+  const long m0 = tile.m0, n0 = tile.n0, first = blockIdx.y * g.range, end = min(first + g.range, g.K);
+
+  const long stepA = AK ? g.a.row : g.a.col, stepB = BK ? g.b.row : g.b.col;
+  const T* const baseA = static_cast<const T*>(g.a.data) + m0 * g.a.row;
+  const T* const baseB = static_cast<const T*>(g.b.data) + n0 * g.b.row;
+  A a;
+  B b;
+  a.setup(stepA);
+  b.setup(stepB);
+  auto load = [&](long k, char* to) __attribute__((always_inline)) {
+    a.load(baseA + k * g.a.col, stepA, g.M - m0, end - k, to);
+    b.load(baseB + k * g.b.col, stepB, g.N - n0, end - k, to + A::bytes);
+  };
+
+  floatx4 sum[RM][RN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  load(first, space[0]);
+  int now = 0;
+  for (long k = first; k < end; k += kDeep, now ^= 1) {
+    __syncthreads();
+    if (k + kDeep < end) load(k + kDeep, space[now ^ 1]);
+    const char *const sa = space[now], *const sb = sa + A::bytes;
+#pragma unroll
+    for (int h = 0; h < kDeep / 32; ++h) {
+      uintx4 fb[RN];
+#pragma unroll
+      for (int j = 0; j < RN; ++j) fb[j] = B::fragment(sb, wn + 16 * j, h);
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        const uintx4 fa = A::fragment(sa, wm + 16 * i, h);
+#pragma unroll
+        for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[j], fa, sum[i][j], T());
+      }
+    }
+  }
+
+  __syncthreads();
+  constexpr int SHARE = 2 * (A::bytes + B::bytes) / WAVES, FIT = SHARE / (WN * 64);  // blocks of rows
+  constexpr int TURN = FIT >= RM ? RM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+  static_assert(FIT > 0 && RM % TURN == 0, "a wave's share of LDS holds whole rows of blocks");
+  leave<T, RM, RN, TURN>(g, blockIdx.y, m0 + wm, n0 + wn, sum, &space[0][0] + wave * SHARE);
 }
 
-// Results from the sums of `ranges` ranges of k, in their order.
+// Results from the sums of `ranges` ranges of k, in their order (of none: from 0).
 template <class T>
 __global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, int ranges) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= M * N) return;
-  float z = 0.f;
-  for (int r = 0; r < ranges; ++r) z += e.parts[(long)r * M * N + i];
-  finish<T>(e, i / N, i % N, z);
-}
-
-// Results without any k.
-template <class T>
-__global__ __launch_bounds__(256) void noProduct(Epilogue e, long M, long N) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i < M * N) finish<T>(e, i / N, i % N, 0.f);
+  const long words = (N + 7) / 8, i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= M * words) return;
+  const long m = i / words, n = i % words * 8;
+  const float* const from = e.parts + m * N + n;
+  finish<T>(
+      e, m, n, N - n,
+      [&](float(&z)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) z[q] = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < ranges; ++r) {
+          float v[8];
+          loadPack<float, 8>(from + r * M * N, v);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) z[q] += v[q];
+        }
+      },
+      [&](int v) __attribute__((always_inline)) {
+        float z = 0.f;
+        for (int r = 0; r < ranges; ++r) z += from[r * M * N + v];
+        return z;
+      });
 }
 
 constexpr int kBiasRows = 64;  // rows of dz that a workgroup sums
@@ -261,45 +509,119 @@ __global__ __launch_bounds__(256) void biasGradient(const float* parts, Line out
 long ceilDivLong(long a, long b) { return (a + b - 1) / b; }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// ranges of k: enough workgroups for two on each compute unit, at least 8 steps in a range
-long rangesOf(long M, long N, long K) {
-  const long tiles = ceilDivLong(M, kTile) * ceilDivLong(N, kTile);
-  return std::max(1L, std::min({512 / std::max(tiles, 1L), K / (8 * kStep), 64L}));
+// ---- what runs ----
+
+// The kernel of a product, the rows and columns of its tile and the ranges that k is cut into.
+struct ProductPlan {
+  enum Kind { Staged, Straight };
+  int kind, rows, cols;
+  long ranges, range;
+};
+
+bool contiguousK(const Matrix& m) { return m.col == 1 || m.row != 1; }
+
+// an operand of 16 bits whose 16-byte words can go straight to LDS: aligned, no word over the end of a line, a tile's
+// lines within 31 bits
+bool goesStraight(const Matrix& m, long rows, long K) {
+  const bool kc = contiguousK(m);
+  const long inner = kc ? m.col : m.row, step = kc ? m.row : m.col, line = kc ? K : rows;
+  return inner == 1 && line % 8 == 0 && step % 8 == 0 && step >= line && step < (1l << 21) && aligned(m.data, 16);
 }
 
-size_t partsBytes(long M, long N, long K) {
-  const long ranges = rangesOf(M, N, K);
+// The kernel with the least expected time, from what each takes for a step of k and for its results (us, measured on
+// products of 8192 x 8192 x 2048 and 4096 x 1024 x 4096: 256 x 256 tiles, one to a compute unit, 1.95 a step of 64; 128 x 128
+// ones 0.95 alone and 1.3 for two).  A range of k more costs its sums' way to memory and back.
+template <class T>
+ProductPlan planOf(long M, long N, long K, bool straight) {
+  struct Option {
+    int kind, rows, cols, step, together;  // together: workgroups that share a compute unit
+    double alone, shared, results;
+  };
+  static const Option wide[] = {{ProductPlan::Straight, 256, 256, 64, 1, 1.95, 1.95, 8}, {ProductPlan::Straight, 128, 128, 64, 2, 0.95, 1.3, 4}};
+  static const Option pieces[] = {{ProductPlan::Staged, 128, 128, 32, 2, 2.0, 2.6, 5}, {ProductPlan::Staged, 128, 64, 32, 3, 1.2, 2.0, 3},
+                                  {ProductPlan::Staged, 64, 64, 32, 4, 0.8, 1.6, 2}};
+  static const Option staged[] = {{ProductPlan::Staged, 128, 128, 32, 2, 0.9, 1.2, 5}, {ProductPlan::Staged, 128, 64, 32, 3, 0.7, 1.2, 3},
+                                  {ProductPlan::Staged, 64, 64, 32, 4, 0.5, 1.0, 2}};
+  const Option* const options = straight ? wide : sizeof(T) == 4 ? pieces : staged;
+  const int count = straight ? 2 : 3, units = computeUnits();
+  ProductPlan best{};
+  double least = 0;
+  for (int o = 0; o < count; ++o) {
+    const Option& a = options[o];
+    const long tiles = ceilDivLong(M, a.rows) * ceilDivLong(N, a.cols);
+    for (long ranges = 1; ranges <= 64; ranges *= 2) {
+      const long range = ceilDivLong(ceilDivLong(K, ranges), a.step) * a.step, used = ceilDivLong(K, range);
+      if (ranges > 1 && range < 2 * a.step) break;
+      const long groups = tiles * used, slots = (long)units * a.together;
+      const double step = groups <= units ? a.alone : a.shared;
+      const double rounds = groups <= slots ? 1.0 : std::max((double)groups / slots, groups < 4 * slots ? (double)ceilDivLong(groups, slots) : 1.0);
+      double time = rounds * (range / a.step * step + a.results);
+      if (used > 1) time += 4.0 + (double)M * N * used * 8 / 4e6;
+      if (least == 0 || time < least) {
+        least = time;
+        best = ProductPlan{a.kind, a.rows, a.cols, used, range};
+      }
+    }
+  }
+  return best;
+}
+
+size_t partsBytes(long M, long N, long K, int type) {
+  // (whichever way the operands lie)
+  const ProductPlan plans[] = {type == FBFFT_FLOAT32 ? planOf<float>(M, N, K, false) : planOf<half16>(M, N, K, true), planOf<half16>(M, N, K, false)};
+  long ranges = plans[0].ranges;
+  if (type != FBFFT_FLOAT32) ranges = std::max(ranges, plans[1].ranges);
   return ranges > 1 ? rounded((size_t)ranges * M * N * sizeof(float)) : 0;
+}
+
+template <class T, bool AK, bool BK>
+void launchProduct(const ProductPlan& plan, const ProductArgs& g, hipStream_t s) {
+  const long tiles = ceilDivLong(g.M, plan.rows) * ceilDivLong(g.N, plan.cols);
+  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)plan.ranges);
+  if constexpr (sizeof(T) == 2) {
+    if (plan.kind == ProductPlan::Straight) {
+      if (plan.rows == 256)
+        productDirect<T, AK, BK, 256, 256, 128, 64><<<grid, 512, 0, s>>>(g);
+      else
+        productDirect<T, AK, BK, 128, 128, 64, 32><<<grid, 512, 0, s>>>(g);
+      return;
+    }
+  }
+  if (plan.cols == 128)
+    product<T, AK, BK, 128, 128, 64, 64><<<grid, 256, 0, s>>>(g);
+  else if (plan.rows == 128)
+    product<T, AK, BK, 128, 64, 32, 64><<<grid, 256, 0, s>>>(g);
+  else
+    product<T, AK, BK, 64, 64, 32, 32><<<grid, 256, 0, s>>>(g);
 }
 
 template <class T>
 int multiplyAll(const Matrix& a, const Matrix& b, long M, long N, long K, Epilogue e, float* parts, hipStream_t s) {
-  const dim3 flat((unsigned)ceilDivLong(M * N, 256));
+  const dim3 flat((unsigned)ceilDivLong(M * ceilDivLong(N, 8), 256));
+  e.dense = e.out.col == 1 && (!e.residual.data || e.residual.col == 1) && (!e.z.data || e.z.col == 1);
   if (K == 0) {
-    noProduct<T><<<flat, 256, 0, s>>>(e, M, N);
+    joinRanges<T><<<flat, 256, 0, s>>>(e, M, N, 0);
     return launchStatus();
   }
-  ProductArgs g{a, b, M, N, K, K, e};
-  const long ranges = rangesOf(M, N, K);
-  g.range = ceilDivLong(ceilDivLong(K, ranges), kStep) * kStep;
-  if (ranges > 1) g.e.parts = parts;
-  const dim3 grid((unsigned)ceilDivLong(N, kTile), (unsigned)ceilDivLong(M, kTile), (unsigned)ranges);
-  const bool ak = a.col == 1 || a.row != 1, bk = b.col == 1 || b.row != 1;
+  const bool ak = contiguousK(a), bk = contiguousK(b);
+  const ProductPlan plan = planOf<T>(M, N, K, sizeof(T) == 2 && goesStraight(a, M, K) && goesStraight(b, N, K));
+  ProductArgs g{a, b, M, N, K, plan.range, e};
+  if (plan.ranges > 1) g.e.parts = parts;
   if (ak && bk)
-    product<T, true, true><<<grid, 256, 0, s>>>(g);
+    launchProduct<T, true, true>(plan, g, s);
   else if (ak)
-    product<T, true, false><<<grid, 256, 0, s>>>(g);
+    launchProduct<T, true, false>(plan, g, s);
   else if (bk)
-    product<T, false, true><<<grid, 256, 0, s>>>(g);
+    launchProduct<T, false, true>(plan, g, s);
   else
-    product<T, false, false><<<grid, 256, 0, s>>>(g);
-  if (ranges > 1) joinRanges<T><<<flat, 256, 0, s>>>(g.e, M, N, (int)ranges);
+    launchProduct<T, false, false>(plan, g, s);
+  if (plan.ranges > 1) joinRanges<T><<<flat, 256, 0, s>>>(g.e, M, N, (int)plan.ranges);
   return launchStatus();
 }
 
 template <class T>
 int forward(const LinearProblem& p, hipStream_t s) {
-  Epilogue e{p.y, p.residual, p.z, p.bias, p.activation, nullptr};
+  Epilogue e{p.y, p.residual, p.z, p.bias, p.activation, false, nullptr};
   return multiplyAll<T>(p.x, p.w, p.M, p.N, p.K, e, static_cast<float*>(p.workspace), s);
 }
 
@@ -324,20 +646,20 @@ int backward(const LinearProblem& p, hipStream_t s) {
     biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 256)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
   int rc = launchStatus();
   if (rc == FBFFT_SUCCESS && p.dx.data && p.M > 0 && p.K > 0)
-    rc = multiplyAll<T>(dz, Matrix{p.w.data, p.w.col, p.w.row}, p.M, p.K, p.N, Epilogue{p.dx, {}, {}, {}, 0, nullptr},
+    rc = multiplyAll<T>(dz, Matrix{p.w.data, p.w.col, p.w.row}, p.M, p.K, p.N, Epilogue{p.dx, {}, {}, {}, 0, false, nullptr},
                         reinterpret_cast<float*>(space), s);
   if (rc == FBFFT_SUCCESS && p.dw.data && p.N > 0 && p.K > 0)
     rc = multiplyAll<T>(Matrix{dz.data, dz.col, dz.row}, Matrix{p.x.data, p.x.col, p.x.row}, p.N, p.K, p.M,
-                        Epilogue{p.dw, {}, {}, {}, 0, nullptr}, reinterpret_cast<float*>(space), s);
+                        Epilogue{p.dw, {}, {}, {}, 0, false, nullptr}, reinterpret_cast<float*>(space), s);
   return rc;
 }
 
 }  // namespace
 
 size_t linearWorkspaceBytes(int pass, long M, long K, long N, int type) {
-  if (pass == 0) return partsBytes(M, N, K);
+  if (pass == 0) return K > 0 ? partsBytes(M, N, K, type) : 0;
   return rounded((size_t)ceilDivLong(M, kBiasRows) * N * sizeof(float)) +
-         rounded((size_t)M * N * (type == FBFFT_FLOAT32 ? 4 : 2)) + std::max(partsBytes(M, K, N), partsBytes(N, K, M));
+         rounded((size_t)M * N * (type == FBFFT_FLOAT32 ? 4 : 2)) + std::max(partsBytes(M, K, N, type), partsBytes(N, K, M, type));
 }
 
 int launchLinearForward(const LinearProblem& p, hipStream_t s) {
