@@ -331,61 +331,70 @@ __global__ __launch_bounds__(256) void product(ProductArgs g) {
 
 typedef __attribute__((address_space(3))) void* LdsAddress;
 
-constexpr int kDeep = 64;  // k of a step
-
-// One step of an operand, ROWS rows by kDeep of k, in 16-byte words.  A wave's load fills 1024 neighbouring bytes of
+// One step of an operand, ROWS rows by DEEP (32 or 64) of k, in 16-byte words.  A wave's load fills 1024 neighbouring bytes of
 // LDS, so the words are permuted where they are read from memory.  KC: k is contiguous, a line is a row, of eight
 // words; else a line is a k, of ROWS / 8.
-template <int ROWS, bool KC, int WAVES>
+template <int ROWS, int DEEP, bool KC, int WAVES>
 struct Direct {
-  static constexpr int words = kDeep * ROWS / 8, loads = words / 64 / WAVES, perLine = KC ? kDeep / 8 : ROWS / 8;
+  static constexpr int words = DEEP * ROWS / 8, loads = words / 64 / WAVES, perLine = KC ? DEEP / 8 : ROWS / 8;
   static constexpr int bytes = words * 16;
+  static_assert(loads * 64 * WAVES == words, "whole loads");
   unsigned at[loads];  // of each load's word: bytes from the step's first
-  unsigned k[loads];   // its k (KC)
+  int k[loads];        // its k
 
   // which word lies where: KC: so that 16 rows of one k take all places of 256 bytes; else four k and two halves of
   // a fragment do
   static __device__ __forceinline__ int permuted(int line, int word) {
-    if (KC) return word ^ (line / 2 % 8);
+    if (KC) return word ^ (DEEP == 64 ? line / 2 % 8 : line / 4 % 4);
     return word ^ ((line % 4 + line / 8 % 2 * 4) * 2);
   }
 
-  __device__ __forceinline__ void setup(long step) {
+  const char* base;  // the next step's first word
+  long advance;      // bytes from a step to the next
+  int size;          // of a step, from its first word to the end of its last
+
+  // rows: from the tile's first, inside
+  __device__ __forceinline__ void setup(const void* first, long step, long rows) {
 #pragma unroll
     for (int i = 0; i < loads; ++i) {
       const int place = ((int)threadIdx.x / 64 * loads + i) * 64 + threadIdx.x % 64, line = place / perLine;
       const int word = permuted(line, place % perLine);
       at[i] = (unsigned)(line * step + word * 8) * 2;
-      k[i] = word * 8;
+      k[i] = KC ? word * 8 : line;
     }
+    const long inside = min(rows, (long)ROWS);
+    base = static_cast<const char*>(first);
+    advance = KC ? DEEP * 2 : DEEP * 2 * step;
+    size = (int)((KC ? (inside - 1) * step + DEEP : (DEEP - 1) * step + inside) * 2);
   }
 
-  // base: the step's first element; left: rows and k from there that are inside
-  __device__ __forceinline__ void load(const void* base, long step, long rows, long left, char* space) const {
-    const long lines = KC ? min(rows, (long)ROWS) : min(left, (long)kDeep), line = KC ? min(left, (long)kDeep) : min(rows, (long)ROWS);
-    const unsigned size = (unsigned)(((lines - 1) * step + line) * 2);  // words behind it read as zeros
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, size, 0x00020000);
-    char* const to = space + threadIdx.x / 64 * (loads * 1024);
-#pragma unroll
-    for (int i = 0; i < loads; ++i) {
-      // (within a line the end is not the buffer's)
-      const unsigned from = KC && k[i] >= left ? 0x80000000u : at[i];
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsAddress)(to + i * 1024), 16, from, 0, 0, 0);
-    }
+  // Load i of the next step, of which `left` k are inside (perhaps none): words behind them, and rows behind the last,
+  // read as zeros.
+  __device__ __forceinline__ void load(int i, int left, char* space) const {
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, size, 0x00020000);
+    char* const to = space + (threadIdx.x / 64 * loads + i) * 1024;
+    const unsigned place = k[i] >= left ? 0x80000000u : at[i];
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsAddress)to, 16, place, 0, 0, 0);
   }
 
-  // eight k from 32 h + 8 (lane / 16) of row `row` + lane % 16
-  static __device__ __forceinline__ uintx4 fragment(const char* space, int row, int h) {
+  // Where this lane's part of the fragments from row `first` (a multiple of 16 times their number) lies in a step, and
+  // fragment i of half h: eight k from 32 h + 8 (lane / 16) of row first + 16 i + lane % 16.
+  static __device__ __forceinline__ int laneAt(int first) {
     const int lane = threadIdx.x % 64;
     if (KC) {
-      const int line = row + lane % 16;
-      return *reinterpret_cast<const uintx4*>(space + line * (kDeep * 2) + permuted(line, h * 4 + lane / 16) * 16);
+      const int line = first + lane % 16;
+      return line * (DEEP * 2) + permuted(line, lane / 16) * 16;
     }
+    const int line = lane / 16 * 8 + lane % 16 / 4, row = first + lane % 4 * 4;
+    return line * (ROWS * 2) + permuted(line, row / 8) * 16 + row % 8 * 2;
+  }
+  static __device__ __forceinline__ uintx4 fragment(const char* step, int lane, int h, int i) {
+    if (KC) return *reinterpret_cast<const uintx4*>(step + (lane ^ h * 64) + i * (16 * DEEP * 2));
     uintx4 f;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int line = h * 32 + lane / 16 * 8 + 4 * q + lane % 16 / 4, first = row + lane % 4 * 4;
-      const char* const from = space + line * (ROWS * 2) + permuted(line, first / 8) * 16 + first % 8 * 2;
+      // (four and 32 lines on, the words of a line are permuted the same way)
+      const char* const from = step + (lane ^ i * 32) + (32 * h + 4 * q) * (ROWS * 2);
       const uintx2 u = __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                                       (__attribute__((address_space(3))) shortx4*)const_cast<char*>(from)));
       f[2 * q] = u[0];
@@ -395,31 +404,37 @@ struct Direct {
   }
 };
 
-// A workgroup: BM x BN results over one range of k, a wave WM x WN of them; two steps' operands in LDS, one of which
-// is multiplied while the other arrives.
-template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN>
+// Waits until at most PENDING of this wave's loads are on their way, and its reads of LDS have arrived, then for the
+// workgroup's other waves.  (In instructions that the compiler counts with, so that it adds no waits of its own.)
+template <int PENDING>
+__device__ __forceinline__ void arrive() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(PENDING % 16 | 0x70 | PENDING / 16 << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A workgroup: BM x BN results over one range of k, a wave WM x WN of them.  LDS holds the operands of DEPTH steps of
+// DEEP k; the fragments of the next 32 k are on their way from LDS while a wave multiplies those of these, and waves
+// meet once a step.  Steps of 64 k take rows whose k are contiguous in whole lines of 128 bytes (8192 x 8192 x 2048, us:
+// 268, steps of 32: 307); where both operands' rows are contiguous instead, more and shorter steps are better (331 / 283).
+template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, int DEEP, int DEPTH>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(ProductArgs g) {
   constexpr int WAVES = BM / WM * (BN / WN), RM = WM / 16, RN = WN / 16;
-  typedef Direct<BM, AK, WAVES> A;
-  typedef Direct<BN, BK, WAVES> B;
-  __shared__ __attribute__((aligned(1024))) char space[2][A::bytes + B::bytes];
+  typedef Direct<BM, DEEP, AK, WAVES> A;
+  typedef Direct<BN, DEEP, BK, WAVES> B;
+  constexpr int STEP = A::bytes + B::bytes, LOADS = A::loads + B::loads;
+  __shared__ __attribute__((aligned(1024))) char space[DEPTH * STEP];
   const int wave = threadIdx.x / 64;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
   const Tile<BM, BN> tile(g.M, g.N);
   if (!tile.any) return;
   const long m0 = tile.m0, n0 = tile.n0, first = blockIdx.y * g.range, end = min(first + g.range, g.K);
 
-  const long stepA = AK ? g.a.row : g.a.col, stepB = BK ? g.b.row : g.b.col;
-  const T* const baseA = static_cast<const T*>(g.a.data) + m0 * g.a.row;
-  const T* const baseB = static_cast<const T*>(g.b.data) + n0 * g.b.row;
   A a;
   B b;
-  a.setup(stepA);
-  b.setup(stepB);
-  auto load = [&](long k, char* to) __attribute__((always_inline)) {
-    a.load(baseA + k * g.a.col, stepA, g.M - m0, end - k, to);
-    b.load(baseB + k * g.b.col, stepB, g.N - n0, end - k, to + A::bytes);
-  };
+  a.setup(static_cast<const T*>(g.a.data) + m0 * g.a.row + first * g.a.col, AK ? g.a.row : g.a.col, g.M - m0);
+  b.setup(static_cast<const T*>(g.b.data) + n0 * g.b.row + first * g.b.col, BK ? g.b.row : g.b.col, g.N - n0);
 
   floatx4 sum[RM][RN];
 #pragma unroll
@@ -427,31 +442,74 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(Produc
 #pragma unroll
     for (int j = 0; j < RN; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  load(first, space[0]);
-  int now = 0;
-  for (long k = first; k < end; k += kDeep, now ^= 1) {
-    __syncthreads();
-    if (k + kDeep < end) load(k + kDeep, space[now ^ 1]);
-    const char *const sa = space[now], *const sb = sa + A::bytes;
+  auto load = [&](int q, int left, char* to) __attribute__((always_inline)) {
+    if (q < A::loads)
+      a.load(q, left, to);
+    else
+      b.load(q - A::loads, left, to + A::bytes);
+  };
+  int left = (int)(end - first);  // k that are not on their way yet
+  auto loaded = [&]() __attribute__((always_inline)) {
+    a.base += a.advance;
+    b.base += b.advance;
+    left -= DEEP;
+  };
+  // (behind the last step too, without a word, so that as many loads are always on their way)
 #pragma unroll
-    for (int h = 0; h < kDeep / 32; ++h) {
-      uintx4 fb[RN];
+  for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
-      for (int j = 0; j < RN; ++j) fb[j] = B::fragment(sb, wn + 16 * j, h);
+    for (int q = 0; q < LOADS; ++q) load(q, left, space + d * STEP);
+    loaded();
+  }
+  const int laneA = A::laneAt(wm), laneB = B::laneAt(wn);
+  uintx4 fa[2][RM], fb[2][RN];
+  auto read = [&](int set, const char* from, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < RN; ++j) fb[set][j] = B::fragment(from + A::bytes, laneB, half, j);
+#pragma unroll
+    for (int i = 0; i < RM; ++i) fa[set][i] = A::fragment(from, laneA, half, i);
+  };
+  auto row = [&](int set, int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[set][j], fa[set][i], sum[i][j], T());
+  };
+  constexpr int HALVES = DEEP / 32;
+  static_assert(DEPTH * HALVES % 2 == 0, "two sets of fragments, in turn");
+  arrive<(DEPTH - 1) * LOADS>();
+  read(0, space, 0);
+  auto round = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int set = d * HALVES % 2, last = (set + HALVES - 1) % 2;
+      if constexpr (HALVES == 2) {
+        read(last, space + d * STEP, 1);
+#pragma unroll
+        for (int i = 0; i < RM; ++i) row(set, i);
+      }
+      // the next step's operands are there, and this one's place is free: every wave has its fragments
+      arrive<(DEPTH - 2) * LOADS>();
+      read(last ^ 1, space + (d + 1) % DEPTH * STEP, 0);
+      // (loads one at a time between matrix instructions: a wave waits where it issues them)
 #pragma unroll
       for (int i = 0; i < RM; ++i) {
-        const uintx4 fa = A::fragment(sa, wm + 16 * i, h);
+        row(last, i);
 #pragma unroll
-        for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[j], fa, sum[i][j], T());
+        for (int q = i * LOADS / RM; q < (i + 1) * LOADS / RM; ++q) load(q, left, space + d * STEP);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      loaded();
+      if (left <= -DEPTH * DEEP) return false;  // that was the last step
     }
+    return true;
+  };
+  while (round()) {
   }
 
   __syncthreads();
-  constexpr int SHARE = 2 * (A::bytes + B::bytes) / WAVES, FIT = SHARE / (WN * 64);  // blocks of rows
+  constexpr int SHARE = DEPTH * STEP / WAVES, FIT = SHARE / (WN * 64);  // of LDS, to a wave; blocks of rows
   constexpr int TURN = FIT >= RM ? RM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
   static_assert(FIT > 0 && RM % TURN == 0, "a wave's share of LDS holds whole rows of blocks");
-  leave<T, RM, RN, TURN>(g, blockIdx.y, m0 + wm, n0 + wn, sum, &space[0][0] + wave * SHARE);
+  leave<T, RM, RN, TURN>(g, blockIdx.y, m0 + wm, n0 + wn, sum, space + wave * SHARE);
 }
 
 // Results from the sums of `ranges` ranges of k, in their order (of none: from 0).
@@ -529,15 +587,16 @@ bool goesStraight(const Matrix& m, long rows, long K) {
 }
 
 // The kernel with the least expected time, from what each takes for a step of k and for its results (us, measured on
-// products of 8192 x 8192 x 2048 and 4096 x 1024 x 4096: 256 x 256 tiles, one to a compute unit, 1.95 a step of 64; 128 x 128
-// ones 0.95 alone and 1.3 for two).  A range of k more costs its sums' way to memory and back.
+// products of 8192 x 8192 x 2048, 4096 x 1024 x 4096 and single tiles: 256 x 256 tiles, one to a compute unit, 1.75 a step of
+// 64 and 12 for the results; 128 x 128 ones 0.85 alone and 1.1 for two).  A range of k more costs its sums' way to memory
+// and back.
 template <class T>
 ProductPlan planOf(long M, long N, long K, bool straight) {
   struct Option {
     int kind, rows, cols, step, together;  // together: workgroups that share a compute unit
     double alone, shared, results;
   };
-  static const Option wide[] = {{ProductPlan::Straight, 256, 256, 64, 1, 1.95, 1.95, 8}, {ProductPlan::Straight, 128, 128, 64, 2, 0.95, 1.3, 4}};
+  static const Option wide[] = {{ProductPlan::Straight, 256, 256, 64, 1, 1.75, 1.75, 12}, {ProductPlan::Straight, 128, 128, 64, 2, 0.85, 1.1, 5}};
   static const Option pieces[] = {{ProductPlan::Staged, 128, 128, 32, 2, 2.0, 2.6, 5}, {ProductPlan::Staged, 128, 64, 32, 3, 1.2, 2.0, 3},
                                   {ProductPlan::Staged, 64, 64, 32, 4, 0.8, 1.6, 2}};
   static const Option staged[] = {{ProductPlan::Staged, 128, 128, 32, 2, 0.9, 1.2, 5}, {ProductPlan::Staged, 128, 64, 32, 3, 0.7, 1.2, 3},
@@ -580,10 +639,11 @@ void launchProduct(const ProductPlan& plan, const ProductArgs& g, hipStream_t s)
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)plan.ranges);
   if constexpr (sizeof(T) == 2) {
     if (plan.kind == ProductPlan::Straight) {
+      constexpr int DEEP = AK || BK ? 64 : 32, DEPTH = 128 / DEEP;
       if (plan.rows == 256)
-        productDirect<T, AK, BK, 256, 256, 128, 64><<<grid, 512, 0, s>>>(g);
+        productDirect<T, AK, BK, 256, 256, 128, 64, DEEP, DEPTH><<<grid, 512, 0, s>>>(g);
       else
-        productDirect<T, AK, BK, 128, 128, 64, 32><<<grid, 512, 0, s>>>(g);
+        productDirect<T, AK, BK, 128, 128, 64, 32, DEEP, DEPTH><<<grid, 512, 0, s>>>(g);
       return;
     }
   }
