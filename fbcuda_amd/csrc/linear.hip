@@ -147,17 +147,14 @@ struct Stage {
   }
 };
 
-// v[0 ... 7] plus the biases from j
-__device__ __forceinline__ void addBias(const Line& bias, long j, float (&v)[8]) {
-  float b[8];
+// the biases from j
+__device__ __forceinline__ void loadBias(const Line& bias, long j, float (&b)[8]) {
   if (bias.stride == 1 && bias.type == FBFFT_FLOAT32) {
     loadPack<float, 8>(static_cast<const float*>(bias.data) + j, b);
   } else {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) b[q] = loadAny(bias.data, bias.type, (j + q) * bias.stride);
+    for (int q = 0; q < 8; ++q) b[q] = bias.data ? loadAny(bias.data, bias.type, (j + q) * bias.stride) : 0.f;
   }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) v[q] += b[q];
 }
 
 // Eight neighbouring results of row i, or the `count` of them that are inside, from their sums: all of them at once
@@ -170,7 +167,10 @@ __device__ __forceinline__ void finish(const Epilogue& e, long i, long j, long c
   if (e.dense && count >= 8) {
     float z[8];
     eight(z);
-    if (e.bias.data) addBias(e.bias, j, z);
+    float b[8];
+    loadBias(e.bias, j, b);
+#pragma unroll
+    for (int v = 0; v < 8; ++v) z[v] += b[v];
     if (e.z.data) storePack<T, 8>(kept, z);
     activateAll(z, e.activation);
     if (e.residual.data) {
@@ -210,35 +210,76 @@ __device__ __forceinline__ void leave(const ProductArgs& g, long range, long m0,
         *reinterpret_cast<floatx4*>(space + (row * WORDS + word) * 16) = sum[i0 + i][j];
       }
     waveExchange();
-#pragma unroll 1
-    for (int row = lane / LANES; row < 16 * TURN; row += 64 / LANES) {
-      const long m = m0 + 16 * i0 + row, n = n0 + lane % LANES * 8, count = g.N - n;
-      if (m >= g.M || count <= 0) continue;
+    const long n = n0 + lane % LANES * 8, count = g.N - n;
+    const int word = lane % LANES * 2;
+    auto eight = [&](int row, float(&v)[8]) __attribute__((always_inline)) {
       const char* const line = space + row * (WORDS * 16);
-      const int word = lane % LANES * 2;
-      auto eight = [&](float(&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const floatx4 q = *reinterpret_cast<const floatx4*>(line + ((word + h) ^ (row & MASK)) * 16);
+      for (int h = 0; h < 2; ++h) {
+        const floatx4 q = *reinterpret_cast<const floatx4*>(line + ((word + h) ^ (row & MASK)) * 16);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[4 * h + k] = q[k];
-        }
-      };
-      auto one = [&](int v) __attribute__((always_inline)) {
-        return *reinterpret_cast<const float*>(line + ((word + v / 4) ^ (row & MASK)) * 16 + v % 4 * 4);
-      };
-      if (!g.e.parts) {
-        finish<T>(g.e, m, n, count, eight, one);
-        continue;
+        for (int k = 0; k < 4; ++k) v[4 * h + k] = q[k];
       }
-      float* const to = g.e.parts + (range * g.M + m) * g.N + n;
-      if (count >= 8) {
-        float v[8];
-        eight(v);
-        storePack<float, 8>(to, v);
-      } else {
+    };
+    auto one = [&](int row, int v) __attribute__((always_inline)) {
+      return *reinterpret_cast<const float*>(space + row * (WORDS * 16) + ((word + v / 4) ^ (row & MASK)) * 16 + v % 4 * 4);
+    };
+    constexpr int ROWS = 64 / LANES, TIMES = 16 * TURN / ROWS, AT_ONCE = TIMES < 4 ? TIMES : 4;
+    const long m1 = m0 + 16 * i0;
+    if (g.e.parts) {
 #pragma unroll 1
-        for (int v = 0; v < count; ++v) to[v] = one(v);
+      for (int row = lane / LANES; row < 16 * TURN; row += ROWS) {
+        const long m = m1 + row;
+        if (m >= g.M || count <= 0) continue;
+        float* const to = g.e.parts + (range * g.M + m) * g.N + n;
+        if (count >= 8) {
+          float v[8];
+          eight(row, v);
+          storePack<float, 8>(to, v);
+        } else {
+#pragma unroll 1
+          for (int v = 0; v < count; ++v) to[v] = one(row, v);
+        }
+      }
+    } else if (g.e.dense && n0 + COLS <= g.N) {
+      // whole rows: a few rows' residuals on their way at once (one by one, each of them waits for memory: 8192 x 8192 x
+      // 2048 with residual and preactivation 333 us)
+      float bias[8];
+      loadBias(g.e.bias, n, bias);
+      const T* const residual = static_cast<const T*>(g.e.residual.data);
+#pragma unroll 1
+      for (int t = 0; t < TIMES; t += AT_ONCE) {
+        typename Pack<T, 8>::type r[AT_ONCE];
+        if (residual)
+#pragma unroll
+          for (int q = 0; q < AT_ONCE; ++q)
+            r[q] = *reinterpret_cast<const typename Pack<T, 8>::type*>(
+                residual + min(m1 + lane / LANES + (t + q) * ROWS, g.M - 1) * g.e.residual.row + n);
+#pragma unroll
+        for (int q = 0; q < AT_ONCE; ++q) {
+          const int row = lane / LANES + (t + q) * ROWS;
+          const long m = m1 + row;
+          if (m >= g.M) break;
+          float z[8];
+          eight(row, z);
+#pragma unroll
+          for (int v = 0; v < 8; ++v) z[v] += bias[v];
+          if (g.e.z.data) storePack<T, 8>(static_cast<T*>(g.e.z.data) + m * g.e.z.row + n, z);
+          activateAll(z, g.e.activation);
+          if (residual)
+#pragma unroll
+            for (int v = 0; v < 8; ++v) z[v] += (float)r[q][v];
+          storePack<T, 8>(static_cast<T*>(g.e.out.data) + m * g.e.out.row + n, z);
+        }
+      }
+    } else {
+#pragma unroll 1
+      for (int row = lane / LANES; row < 16 * TURN; row += ROWS) {
+        const long m = m1 + row;
+        if (m >= g.M || count <= 0) continue;
+        finish<T>(
+            g.e, m, n, count, [&](float(&v)[8]) __attribute__((always_inline)) { eight(row, v); },
+            [&](int v) __attribute__((always_inline)) { return one(row, v); });
       }
     }
   }
@@ -512,6 +553,88 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(Produc
   leave<T, RM, RN, TURN>(g, blockIdx.y, m0 + wm, n0 + wn, sum, space + wave * SHARE);
 }
 
+// ---- a few rows: as fast as the weights can be read ----
+
+constexpr int kFew = 16;
+
+// Eight neighbouring k of a row from memory to the matrix instructions, as pieces.
+template <class T>
+struct Slice {
+  static constexpr int PIECES = Pieces<T>::count;
+  typename Pack<T, 8>::type v;
+
+  __device__ __forceinline__ void load(const T* row, long k, long end) {
+    if (k + 8 <= end) {
+      v = *reinterpret_cast<const typename Pack<T, 8>::type*>(row + k);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = k + j < end ? row[k + j] : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ void pieces(uintx4 (&to)[PIECES]) const {
+    if constexpr (PIECES == 1) {
+      to[0] = __builtin_bit_cast(uintx4, v);
+    } else {
+      float r[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) r[j] = v[j];
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        to[p] = uintx4{leading(r[0], r[1]), leading(r[2], r[3]), leading(r[4], r[5]), leading(r[6], r[7])};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = withoutLeading(r[j]);
+      }
+    }
+  }
+};
+
+// Up to 16 rows of x.  A workgroup: 16 rows of w, its waves a range of k each, straight from memory to the matrix
+// instructions (rows of x behind the last are the last again, and nobody takes their results); their sums meet in LDS.
+template <class T, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void fewRows(ProductArgs g) {
+  typedef typename Pieces<T>::type P;
+  constexpr int PIECES = Pieces<T>::count, AHEAD = sizeof(T) == 2 ? 8 : 4;
+  __shared__ float sums[WAVES][256];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const long n0 = (long)blockIdx.x * 16;
+  const T* const w = static_cast<const T*>(g.b.data) + min(n0 + lane % 16, g.N - 1) * g.b.row;
+  const T* const x = static_cast<const T*>(g.a.data) + min((long)lane % 16, g.M - 1) * g.a.row;
+  const long share = (g.K + WAVES * 32 - 1) / (WAVES * 32) * 32, first = wave * share, end = min(first + share, g.K);
+  floatx4 sum{0.f, 0.f, 0.f, 0.f};
+  for (long k0 = first; k0 < end; k0 += AHEAD * 32) {
+    Slice<T> sw[AHEAD], sx[AHEAD];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      const long k = k0 + 32 * s + lane / 16 * 8;
+      sw[s].load(w, k, end);
+      sx[s].load(x, k, end);
+    }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      uintx4 pw[PIECES], px[PIECES];
+      sw[s].pieces(pw);
+      sx[s].pieces(px);
+#pragma unroll
+      for (int order = PIECES - 1; order >= 0; --order)
+#pragma unroll
+        for (int p = 0; p <= order; ++p) sum = multiply(pw[order - p], px[p], sum, P());
+    }
+  }
+  // (lane: row lane % 16 of x, four rows of w)
+#pragma unroll
+  for (int v = 0; v < 4; ++v) sums[wave][lane % 16 * 16 + lane / 16 * 4 + v] = sum[v];
+  __syncthreads();
+  const long m = threadIdx.x / 16, n = n0 + threadIdx.x % 16;
+  if (threadIdx.x >= 256 || m >= g.M || n >= g.N) return;
+  float z = lineOr(g.e.bias, n, 0.f);
+#pragma unroll
+  for (int q = 0; q < WAVES; ++q) z += sums[q][threadIdx.x];
+  if (g.e.z.data) static_cast<T*>(g.e.z.data)[m * g.e.z.row + n * g.e.z.col] = (T)z;
+  z = activate(z, g.e.activation);
+  if (g.e.residual.data) z += (float)static_cast<const T*>(g.e.residual.data)[m * g.e.residual.row + n * g.e.residual.col];
+  static_cast<T*>(g.e.out.data)[m * g.e.out.row + n * g.e.out.col] = (T)z;
+}
+
 // Results from the sums of `ranges` ranges of k, in their order (of none: from 0).
 template <class T>
 __global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, int ranges) {
@@ -541,27 +664,98 @@ __global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, in
 
 constexpr int kBiasRows = 64;  // rows of dz that a workgroup sums
 
-// dz = dy activation'(z), dense, and its columns' sums over kBiasRows rows each
-template <class T>
+// dz = dy activation'(z), dense, and its columns' sums over kBiasRows rows each.  A workgroup: 32 words of VEC columns,
+// eight rows of lanes.
+template <class T, int VEC>
 __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z, T* dz, float* parts, long M, long N, int activation) {
-  const long n = (long)blockIdx.x * 256 + threadIdx.x, m0 = (long)blockIdx.y * kBiasRows;
-  if (n >= N) return;
-  float sum = 0.f;
-  for (long m = m0; m < min(m0 + kBiasRows, M); ++m) {
-    float v = (float)static_cast<const T*>(dy.data)[m * dy.row + n * dy.col];
-    if (activation != FBFFT_ACTIVATION_NONE) v *= slope((float)static_cast<const T*>(z.data)[m * z.row + n * z.col], activation);
-    if (dz) dz[m * N + n] = (T)v;
-    sum += v;
+  typedef typename Pack<T, VEC>::type Word;
+  constexpr int AHEAD = 4;
+  __shared__ float sums[8][32 * VEC];
+  const int column = threadIdx.x % 32, r = threadIdx.x / 32;
+  const long n = ((long)blockIdx.x * 32 + column) * VEC, m0 = (long)blockIdx.y * kBiasRows, end = min(m0 + kBiasRows, M);
+  const bool whole = n + VEC <= N;
+  auto load = [&](const Matrix& from, long m) __attribute__((always_inline)) {
+    const T* const p = static_cast<const T*>(from.data) + min(m, end - 1) * from.row + n * from.col;
+    Word w{};
+    if constexpr (VEC == 1) {
+      if (whole) w = *p;
+    } else if (whole) {
+      w = *reinterpret_cast<const Word*>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (n + j < N) w[j] = p[j];
+    }
+    return w;
+  };
+  auto unpacked = [&](const Word& w, float(&v)[VEC]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      if constexpr (VEC == 1)
+        v[j] = (float)w;
+      else
+        v[j] = (float)w[j];
+    }
+  };
+  float sum[VEC] = {};
+  for (long m = m0 + r; m < end; m += 8 * AHEAD) {
+    Word wg[AHEAD], wz[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      wg[q] = load(dy, m + 8 * q);
+      if (activation != FBFFT_ACTIVATION_NONE) wz[q] = load(z, m + 8 * q);
+    }
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      if (m + 8 * q >= end) break;
+      float v[VEC], a[VEC];
+      unpacked(wg[q], v);
+      if (activation != FBFFT_ACTIVATION_NONE) {
+        unpacked(wz[q], a);
+        slopeAll(a, v, activation);
+      }
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum[j] += v[j];
+      if (!dz) continue;
+      T* const to = dz + (m + 8 * q) * N + n;
+      if (whole) {
+        storePack<T, VEC>(to, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (n + j < N) to[j] = (T)v[j];
+      }
+    }
   }
-  if (parts) parts[blockIdx.y * N + n] = sum;
+  if (!parts) return;
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) sums[r][column * VEC + j] = sum[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
+    const long at = (long)blockIdx.x * 32 * VEC + i;
+    float v = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += sums[q][i];
+    if (at < N) parts[blockIdx.y * N + at] = v;
+  }
 }
 
+// A workgroup: eight columns, 32 lanes to each.
 __global__ __launch_bounds__(256) void biasGradient(const float* parts, Line out, long N, long count) {
-  const long n = (long)blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
-  double sum = 0;
-  for (long r = 0; r < count; ++r) sum += parts[r * N + n];
-  storeAny(out.data, out.type, n * out.stride, (float)sum);
+  __shared__ float sums[32][8];
+  const int column = threadIdx.x % 8, slice = threadIdx.x / 8;
+  const long n = (long)blockIdx.x * 8 + column;
+  float sum = 0.f;
+  if (n < N)
+#pragma unroll 4
+    for (long r = slice; r < count; r += 32) sum += parts[r * N + n];
+  sums[slice][column] = sum;
+  __syncthreads();
+  if (slice > 0 || n >= N) return;
+  sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < 32; ++q) sum += sums[q][column];
+  storeAny(out.data, out.type, n * out.stride, sum);
 }
 
 long ceilDivLong(long a, long b) { return (a + b - 1) / b; }
@@ -615,7 +809,7 @@ ProductPlan planOf(long M, long N, long K, bool straight) {
       const double step = groups <= units ? a.alone : a.shared;
       const double rounds = groups <= slots ? 1.0 : std::max((double)groups / slots, groups < 4 * slots ? (double)ceilDivLong(groups, slots) : 1.0);
       double time = rounds * (range / a.step * step + a.results);
-      if (used > 1) time += 4.0 + (double)M * N * used * 8 / 4e6;
+      if (used > 1) time += 4.0 + (double)M * N * used * 8 / 6e6;
       if (least == 0 || time < least) {
         least = time;
         best = ProductPlan{a.kind, a.rows, a.cols, used, range};
@@ -664,6 +858,16 @@ int multiplyAll(const Matrix& a, const Matrix& b, long M, long N, long K, Epilog
     return launchStatus();
   }
   const bool ak = contiguousK(a), bk = contiguousK(b);
+  if (M <= kFew && a.col == 1 && b.col == 1) {
+    // (as many waves as there are steps of k for)
+    const ProductArgs g{a, b, M, N, K, K, e};
+    const dim3 tiles((unsigned)ceilDivLong(N, 16));
+    if (K <= 2048)
+      fewRows<T, 8><<<tiles, 512, 0, s>>>(g);
+    else
+      fewRows<T, 16><<<tiles, 1024, 0, s>>>(g);
+    return launchStatus();
+  }
   const ProductPlan plan = planOf<T>(M, N, K, sizeof(T) == 2 && goesStraight(a, M, K) && goesStraight(b, N, K));
   ProductArgs g{a, b, M, N, K, plan.range, e};
   if (plan.ranges > 1) g.e.parts = parts;
@@ -698,12 +902,18 @@ int backward(const LinearProblem& p, hipStream_t s) {
     space += rounded((size_t)p.M * p.N * sizeof(T));
   }
   if (p.M > 0 && p.N > 0 && (apart || p.gradBias.data)) {
-    const dim3 grid((unsigned)ceilDivLong(p.N, 256), (unsigned)chunks);
-    preactivationGradient<T><<<grid, 256, 0, s>>>(p.dy, p.z, apart ? static_cast<T*>(dz.data) : nullptr,
-                                                  p.gradBias.data ? parts : nullptr, p.M, p.N, p.activation);
+    constexpr int W = 16 / sizeof(T);
+    const bool words = p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
+    const dim3 grid((unsigned)ceilDivLong(p.N, 32 * (words ? W : 1)), (unsigned)chunks);
+    T* const to = apart ? static_cast<T*>(dz.data) : nullptr;
+    float* const sums = p.gradBias.data ? parts : nullptr;
+    if (words)
+      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, p.M, p.N, p.activation);
+    else
+      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, p.M, p.N, p.activation);
   }
   if (p.gradBias.data && p.N > 0)
-    biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 256)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
+    biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 8)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
   int rc = launchStatus();
   if (rc == FBFFT_SUCCESS && p.dx.data && p.M > 0 && p.K > 0)
     rc = multiplyAll<T>(dz, Matrix{p.w.data, p.w.col, p.w.row}, p.M, p.K, p.N, Epilogue{p.dx, {}, {}, {}, 0, false, nullptr},
