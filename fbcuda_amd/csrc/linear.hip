@@ -458,7 +458,7 @@ __device__ __forceinline__ void arrive() {
 // A workgroup: BM x BN results over one range of k, a wave WM x WN of them.  LDS holds the operands of DEPTH steps of
 // DEEP k; the fragments of the next 32 k are on their way from LDS while a wave multiplies those of these, and waves
 // meet once a step.  Steps of 64 k take rows whose k are contiguous in whole lines of 128 bytes (8192 x 8192 x 2048, us:
-// 268, steps of 32: 307); where both operands' rows are contiguous instead, more and shorter steps are better (331 / 283).
+// 268, steps of 32: 307); where rows are contiguous instead, more and shorter steps are better (both: 283, 331).
 template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN, int DEEP, int DEPTH>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(ProductArgs g) {
   constexpr int WAVES = BM / WM * (BN / WN), RM = WM / 16, RN = WN / 16;
@@ -504,35 +504,48 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(Produc
   }
   const int laneA = A::laneAt(wm), laneB = B::laneAt(wn);
   uintx4 fa[2][RM], fb[2][RN];
-  auto read = [&](int set, const char* from, int half) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < RN; ++j) fb[set][j] = B::fragment(from + A::bytes, laneB, half, j);
-#pragma unroll
-    for (int i = 0; i < RM; ++i) fa[set][i] = A::fragment(from, laneA, half, i);
+  constexpr int READS = RM + RN;
+  auto read = [&](int q, int set, const char* from, int half) __attribute__((always_inline)) {
+    if (q < RN)
+      fb[set][q] = B::fragment(from + A::bytes, laneB, half, q);
+    else
+      fa[set][q - RN] = A::fragment(from, laneA, half, q - RN);
   };
   auto row = [&](int set, int i) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[set][j], fa[set][i], sum[i][j], T());
   };
+  // Reads and loads go between matrix instructions a few at a time: a wave waits where it issues them (8192 x 8192 x
+  // 2048, us: 251, all reads first 268).  Not the transposing reads, which the compiler holds back until no load is on
+  // its way: all of them first (280, between matrix instructions 328).
+  constexpr bool SPREAD = AK && BK;
+  auto reads = [&](int i, int set, const char* from, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < READS; ++q)
+      if (SPREAD ? q >= i * READS / RM && q < (i + 1) * READS / RM : i == 0) read(q, set, from, half);
+  };
   constexpr int HALVES = DEEP / 32;
   static_assert(DEPTH * HALVES % 2 == 0, "two sets of fragments, in turn");
   arrive<(DEPTH - 1) * LOADS>();
-  read(0, space, 0);
+#pragma unroll
+  for (int q = 0; q < READS; ++q) read(q, 0, space, 0);
   auto round = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const int set = d * HALVES % 2, last = (set + HALVES - 1) % 2;
       if constexpr (HALVES == 2) {
-        read(last, space + d * STEP, 1);
 #pragma unroll
-        for (int i = 0; i < RM; ++i) row(set, i);
+        for (int i = 0; i < RM; ++i) {
+          reads(i, last, space + d * STEP, 1);
+          row(set, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       // the next step's operands are there, and this one's place is free: every wave has its fragments
       arrive<(DEPTH - 2) * LOADS>();
-      read(last ^ 1, space + (d + 1) % DEPTH * STEP, 0);
-      // (loads one at a time between matrix instructions: a wave waits where it issues them)
 #pragma unroll
       for (int i = 0; i < RM; ++i) {
+        reads(i, last ^ 1, space + (d + 1) % DEPTH * STEP, 0);
         row(last, i);
 #pragma unroll
         for (int q = i * LOADS / RM; q < (i + 1) * LOADS / RM; ++q) load(q, left, space + d * STEP);
@@ -833,7 +846,7 @@ void launchProduct(const ProductPlan& plan, const ProductArgs& g, hipStream_t s)
   const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)plan.ranges);
   if constexpr (sizeof(T) == 2) {
     if (plan.kind == ProductPlan::Straight) {
-      constexpr int DEEP = AK || BK ? 64 : 32, DEPTH = 128 / DEEP;
+      constexpr int DEEP = AK && BK ? 64 : 32, DEPTH = 128 / DEEP;
       if (plan.rows == 256)
         productDirect<T, AK, BK, 256, 256, 128, 64, DEEP, DEPTH><<<grid, 512, 0, s>>>(g);
       else
