@@ -45,7 +45,7 @@ __device__ __forceinline__ Words philox(unsigned long long block, unsigned long 
 }
 
 // A thread takes the eight elements of one counter.  DENSE: they are neighbours in every operand.
-template <class T, bool DENSE>
+template <class T, bool DENSE, bool STREAM>
 __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
   const long block = (long)blockIdx.x * 256 + threadIdx.x, first = block * 8;
   if (first >= g.total) return;
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
     if (residual) loadPack<T, 8>(residual + first, r);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = result(j, v[j], r[j]);
-    storePack<T, 8>(y + first, v);
+    leavePack<STREAM, T, 8>(y + first, v);
     return;
   }
   long at[FBFFT_MAX_DIM];
@@ -92,12 +92,14 @@ __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
 }
 
 template <class T>
-void launch(const DropoutArgs& g, bool dense, hipStream_t s) {
+void launch(const DropoutArgs& g, bool dense, bool stream, hipStream_t s) {
   const dim3 grid((unsigned)((g.total + 2047) / 2048));
-  if (dense)
-    dropout<T, true><<<grid, 256, 0, s>>>(g);
+  if (!dense)
+    dropout<T, false, false><<<grid, 256, 0, s>>>(g);
+  else if (stream)
+    dropout<T, true, true><<<grid, 256, 0, s>>>(g);
   else
-    dropout<T, false><<<grid, 256, 0, s>>>(g);
+    dropout<T, true, false><<<grid, 256, 0, s>>>(g);
 }
 
 }  // namespace
@@ -119,12 +121,13 @@ int launchDropout(const DropoutProblem& p, hipStream_t s) {
     if (g.size[d] != 1) dense = dense && g.xs[d] == run && g.ys[d] == run && (!g.residual || g.rs[d] == run);
     run *= g.size[d];
   }
+  const bool stream = streams((double)p.total, p.type);
   if (p.type == FBFFT_FLOAT32)
-    launch<float>(g, dense, s);
+    launch<float>(g, dense, stream, s);
   else if (p.type == FBFFT_FLOAT16)
-    launch<half16>(g, dense, s);
+    launch<half16>(g, dense, stream, s);
   else
-    launch<brain16>(g, dense, s);
+    launch<brain16>(g, dense, stream, s);
   return launchStatus();
 }
 

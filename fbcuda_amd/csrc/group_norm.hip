@@ -28,13 +28,13 @@ struct NormArgs {
   float *mean, *rstd;
   long meanB, meanG, rstdB, rstdG;
   long B, C, G, D, H, W, P;
-  Divisor byW, byP, byD, byLanes, byPieces, byBands;
+  Divisor byW, byP, byD, byLanes, byPieces, byCuts, byBands;
   double share;  // 1 / (D P)
   int activation;
   float eps;
   // channels-last plan: channels of a workgroup, rows of lanes and lanes of a row, pixels of a piece; planes: values of one
-  int band, rows, lanes, pieces;
-  long piece;
+  int band, rows, rowsSecond, lanes, pieces, cuts;
+  long piece, cut;  // of the first launch's pieces, and of the second one's
   double2* sums;     // forward: of x and x^2, [image][group][piece]
   float2* groups;    // backward: sums of w dz and w dz xh, [image][group][piece]
   float2* channels;  // backward: sums of dz and dz xh, [image][piece][channel]
@@ -107,8 +107,9 @@ __global__ __launch_bounds__(256) void normParameters(NormArgs a) {
 
 // ---- Last ----
 
-constexpr int kBand = 1024;  // channels of a workgroup at most
-constexpr int kAhead = 4;    // pixels whose loads a lane has in flight where it walks over a piece
+constexpr int kBand = 1024;   // channels of a workgroup at most
+constexpr int kFirst = 512;   // lanes of the first of two launches: few pieces, which every workgroup of the second one joins
+constexpr int kAhead = 4, kAheadTwo = 2;  // pixels of one and of each of two operands that a lane has on their way
 
 template <int NT, int VEC, class S>
 struct Columns {
@@ -171,13 +172,17 @@ struct Band {
   int b, piece, first, firstGroup;  // image, piece, channels and groups in front of the band
   int channels, lanes, groups;      // of the band; lanes: of a row, with channels
   int column, r;                    // of this lane: its place in a row of lanes, and the row
+  int rows, p, end;                 // rows of lanes; first pixel, and the one behind the last
   bool live;
 };
-template <int VEC>
+// (SECOND: of the second launch, of 256 lanes)
+template <int VEC, bool SECOND = false>
 __device__ __forceinline__ Band bandOf(const NormArgs& a, int index) {
   Band w;
-  const int row = quotient(index, a.byPieces);
-  w.piece = index - row * a.pieces;
+  const int row = quotient(index, SECOND ? a.byCuts : a.byPieces);
+  w.piece = index - row * (SECOND ? a.cuts : a.pieces);
+  w.p = w.piece * (int)(SECOND ? a.cut : a.piece);
+  w.end = (int)min(w.p + (SECOND ? a.cut : a.piece), a.P);
   w.b = quotient(row, a.byBands);
   w.first = (row - w.b * (int)a.byBands.value) * a.band;
   w.channels = min(a.band, (int)a.C - w.first);
@@ -186,7 +191,8 @@ __device__ __forceinline__ Band bandOf(const NormArgs& a, int index) {
   w.groups = quotient(w.channels, a.byD);
   w.r = quotient(threadIdx.x, a.byLanes);
   w.column = threadIdx.x - w.r * a.lanes;
-  w.live = w.r < a.rows && w.column < w.lanes;
+  w.rows = SECOND ? a.rowsSecond : a.rows;
+  w.live = w.r < w.rows && w.column < w.lanes;
   return w;
 }
 template <class T>
@@ -299,7 +305,7 @@ __device__ __forceinline__ int nearWork(int total) {
 }
 
 // All pixels of a band in registers: one read, one write.
-template <class T, int VEC, int NT, int ITEMS>
+template <class T, int VEC, int NT, int ITEMS, bool STREAM>
 __global__ __launch_bounds__(NT) void lastForward(NormArgs a, int total) {
   __shared__ Columns<NT, VEC, double> space;
   __shared__ double sums[kBand];
@@ -340,41 +346,63 @@ __global__ __launch_bounds__(NT) void lastForward(NormArgs a, int total) {
     unpack(raw[i], v);
     ch.template apply<T>(v);
     activateAll(v, a.activation);
-    storePack<T, VEC>(y + pixelAt(a, a.y, p), v);
+    leavePack<STREAM, T, VEC>(y + pixelAt(a, a.y, p), v);
   }
 }
+
+// Where a lane walks over the pixels of a piece: AHEAD of them are on their way from memory, requested before what has
+// to be known to use them, and in the loop before the ones in hand are used.
+template <class T, int VEC, int AHEAD>
+struct Walk {
+  typedef typename Pack<T, VEC>::type Word;
+  const T* from;
+  int p, end, rows;
+  Word coming[AHEAD], now[AHEAD];
+
+  __device__ __forceinline__ void request(const NormArgs& a, const Image& i) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) coming[k] = *reinterpret_cast<const Word*>(from + pixelAt(a, i, min(p + k * rows, end - 1)));
+  }
+  __device__ __forceinline__ Walk(const NormArgs& a, const Image& i, const Band& band)
+      : from(laneOf<const T>(a, i, band, VEC)), p(band.p + band.r), end(band.end), rows(band.rows) {
+    if (band.live && p < end) request(a, i);
+  }
+  __device__ __forceinline__ void next(const NormArgs& a, const Image& i) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) now[k] = coming[k];
+    p += AHEAD * rows;
+    if (p < end) request(a, i);
+  }
+};
 
 // The sums of a piece of each group.
 template <class T, int VEC>
-__global__ __launch_bounds__(256) void lastSums(NormArgs a) {
-  __shared__ Columns<256, VEC, double> space;
+__global__ __launch_bounds__(kFirst) void lastSums(NormArgs a) {
+  __shared__ Columns<kFirst, VEC, double> space;
   __shared__ double sums[kBand];
   const Band band = bandOf<VEC>(a, blockIdx.x);
-  const T* const x = laneOf<const T>(a, a.x, band, VEC);
-  const int end = (int)min((band.piece + 1) * a.piece, a.P);
+  Walk<T, VEC, kAhead> x(a, a.x, band);
   double s1[VEC] = {}, s2[VEC] = {};
-  if (band.live) {
-    for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
-      typename Pack<T, VEC>::type raw[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) raw[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, min(p + k * a.rows, end - 1)));
+  if (band.live)
+    for (int p = x.p; p < x.end; p += kAhead * x.rows) {
+      x.next(a, a.x);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
-        if (p + k * a.rows < end) {
+        if (p + k * x.rows < x.end) {
           float v[VEC];
-          unpack(raw[k], v);
+          unpack(x.now[k], v);
           moments(v, s1, s2);
         }
     }
-  }
-  joinMoments<256, VEC>(a, band, s1, s2, space, sums, nullptr, true);
+  joinMoments<kFirst, VEC>(a, band, s1, s2, space, sums, nullptr, true);
 }
 
-template <class T, int VEC>
-__global__ __launch_bounds__(256) void lastApply(NormArgs a) {
+template <class T, int VEC, bool STREAM>
+__global__ __launch_bounds__(kFirst) void lastApply(NormArgs a) {
   __shared__ Moments stats[256];
   __shared__ float2 params[kBand];
-  const Band band = bandOf<VEC>(a, gridDim.x - 1 - blockIdx.x);
+  const Band band = bandOf<VEC, true>(a, gridDim.x - 1 - blockIdx.x);
+  Walk<T, VEC, kAhead> x(a, a.x, band);
   bandParameters(a, band, params, 256);
   for (int g = threadIdx.x / 64; g < band.groups; g += 4) {
     const long group = band.firstGroup + g;
@@ -395,21 +423,17 @@ __global__ __launch_bounds__(256) void lastApply(NormArgs a) {
   if (!band.live) return;
   Channel<VEC> ch;
   ch.load(a, band, stats, params);
-  const T* const x = laneOf<const T>(a, a.x, band, VEC);
   T* const y = laneOf<T>(a, a.y, band, VEC);
-  const int end = (int)min((band.piece + 1) * a.piece, a.P);
-  for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
-    typename Pack<T, VEC>::type raw[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) raw[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, min(p + k * a.rows, end - 1)));
+  for (int p = x.p; p < x.end; p += kAhead * x.rows) {
+    x.next(a, a.x);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
-      if (p + k * a.rows < end) {
+      if (p + k * x.rows < x.end) {
         float v[VEC];
-        unpack(raw[k], v);
+        unpack(x.now[k], v);
         ch.template apply<T>(v);
         activateAll(v, a.activation);
-        storePack<T, VEC>(y + pixelAt(a, a.y, p + k * a.rows), v);
+        leavePack<STREAM, T, VEC>(y + pixelAt(a, a.y, p + k * x.rows), v);
       }
   }
 }
@@ -458,7 +482,7 @@ __device__ __forceinline__ void inputGradient(const Channel<VEC>& ch, const floa
 }
 
 // All pixels of a band of input and gradient in registers: two reads, one write.
-template <class T, int VEC, int NT, int ITEMS>
+template <class T, int VEC, int NT, int ITEMS, bool STREAM>
 __global__ __launch_bounds__(NT) void lastBackward(NormArgs a, int total) {
   __shared__ Columns<NT, VEC, float> space;
   __shared__ float sums[2][kBand];
@@ -523,40 +547,33 @@ __global__ __launch_bounds__(NT) void lastBackward(NormArgs a, int total) {
     ch.arguments(v, z);
     slopeAll(z, dz, a.activation);
     inputGradient(ch, m1, m2, v, dz);
-    storePack<T, VEC>(y + pixelAt(a, a.y, p), dz);
+    leavePack<STREAM, T, VEC>(y + pixelAt(a, a.y, p), dz);
   }
 }
 
 template <class T, int VEC>
-__global__ __launch_bounds__(256) void lastGradSums(NormArgs a) {
-  __shared__ Columns<256, VEC, float> space;
+__global__ __launch_bounds__(kFirst) void lastGradSums(NormArgs a) {
+  __shared__ Columns<kFirst, VEC, float> space;
   __shared__ float sums[2][kBand];
-  __shared__ Moments stats[256];
+  __shared__ Moments stats[kFirst];
   __shared__ float2 params[kBand];
   const Band band = bandOf<VEC>(a, blockIdx.x);
-  const T* const x = laneOf<const T>(a, a.x, band, VEC);
-  const T* const g = laneOf<const T>(a, a.g, band, VEC);
-  bandParameters(a, band, params, 256);
-  keptMoments(a, band, stats, 256);
+  Walk<T, VEC, kAheadTwo> x(a, a.x, band), g(a, a.g, band);
+  bandParameters(a, band, params, kFirst);
+  keptMoments(a, band, stats, kFirst);
   Channel<VEC> ch;
   ch.load(a, band, stats, params);
-  const int end = (int)min((band.piece + 1) * a.piece, a.P);
   float s1[VEC] = {}, s2[VEC] = {};
-  if (band.live) {
-    for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
-      typename Pack<T, VEC>::type rx[kAhead], rg[kAhead];
+  if (band.live)
+    for (int p = x.p; p < x.end; p += kAheadTwo * x.rows) {
+      x.next(a, a.x);
+      g.next(a, a.g);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int at = min(p + k * a.rows, end - 1);
-        rx[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, at));
-        rg[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(g + pixelAt(a, a.g, at));
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        if (p + k * a.rows < end) {
+      for (int k = 0; k < kAheadTwo; ++k)
+        if (p + k * x.rows < x.end) {
           float v[VEC], dz[VEC], z[VEC];
-          unpack(rx[k], v);
-          unpack(rg[k], dz);
+          unpack(x.now[k], v);
+          unpack(g.now[k], dz);
           ch.arguments(v, z);
           slopeAll(z, dz, a.activation);
 #pragma unroll
@@ -566,14 +583,13 @@ __global__ __launch_bounds__(256) void lastGradSums(NormArgs a) {
           }
         }
     }
-  }
-  joinGradients<256, VEC>(a, band, s1, s2, space, sums, params, [&](int k, float m1, float m2) {
+  joinGradients<kFirst, VEC>(a, band, s1, s2, space, sums, params, [&](int k, float m1, float m2) {
     a.groups[(band.b * a.G + band.firstGroup + k) * a.pieces + band.piece] = float2{m1, m2};
   });
 }
 
 // (The first `before` workgroups add up the gradients of weight and bias.)
-template <class T, int VEC>
+template <class T, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void lastGradApply(NormArgs a, int before) {
   __shared__ Moments stats[256], means[256];
   __shared__ union {
@@ -581,7 +597,8 @@ __global__ __launch_bounds__(256) void lastGradApply(NormArgs a, int before) {
   } space;
   if ((int)blockIdx.x < before) return parameterGradients(a, blockIdx.x, space.part);
   float2* const params = space.params;
-  const Band band = bandOf<VEC>(a, gridDim.x - 1 - blockIdx.x);
+  const Band band = bandOf<VEC, true>(a, gridDim.x - 1 - blockIdx.x);
+  Walk<T, VEC, kAheadTwo> x(a, a.x, band), g(a, a.g, band);
   bandParameters(a, band, params, 256);
   for (int k = threadIdx.x / 64; k < band.groups; k += 4) {
     float m1 = 0, m2 = 0;
@@ -596,8 +613,6 @@ __global__ __launch_bounds__(256) void lastGradApply(NormArgs a, int before) {
   }
   keptMoments(a, band, stats, 256);
   if (!band.live) return;
-  const T* const x = laneOf<const T>(a, a.x, band, VEC);
-  const T* const g = laneOf<const T>(a, a.g, band, VEC);
   T* const y = laneOf<T>(a, a.y, band, VEC);
   Channel<VEC> ch;
   ch.load(a, band, stats, params);
@@ -608,25 +623,19 @@ __global__ __launch_bounds__(256) void lastGradApply(NormArgs a, int before) {
     m1[j] = m.mean;
     m2[j] = m.rstd;
   }
-  const int end = (int)min((band.piece + 1) * a.piece, a.P);
-  for (int p = band.piece * (int)a.piece + band.r; p < end; p += kAhead * a.rows) {
-    typename Pack<T, VEC>::type rx[kAhead], rg[kAhead];
+  for (int p = x.p; p < x.end; p += kAheadTwo * x.rows) {
+    x.next(a, a.x);
+    g.next(a, a.g);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int at = min(p + k * a.rows, end - 1);
-      rx[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(x + pixelAt(a, a.x, at));
-      rg[k] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(g + pixelAt(a, a.g, at));
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (p + k * a.rows < end) {
+    for (int k = 0; k < kAheadTwo; ++k)
+      if (p + k * x.rows < x.end) {
         float v[VEC], dz[VEC], z[VEC];
-        unpack(rx[k], v);
-        unpack(rg[k], dz);
+        unpack(x.now[k], v);
+        unpack(g.now[k], dz);
         ch.arguments(v, z);
         slopeAll(z, dz, a.activation);
         inputGradient(ch, m1, m2, v, dz);
-        storePack<T, VEC>(y + pixelAt(a, a.y, p + k * a.rows), dz);
+        leavePack<STREAM, T, VEC>(y + pixelAt(a, a.y, p + k * x.rows), dz);
       }
   }
 }
@@ -652,11 +661,12 @@ struct Words {
       for (int j = 0; j < VEC; ++j) raw[j] = e + j < n ? base[e + j] : (T)0.f;
     }
   }
+  template <bool STREAM>
   static __device__ __forceinline__ void store(const NormArgs& a, const Image& i, T* base, int e, int n, const float (&v)[VEC]) {
     if constexpr (VEC == 1) {
       if (e < n) base[offset(a, i, e)] = (T)v[0];
     } else if (e + VEC <= n) {
-      storePack<T, VEC>(base + e, v);
+      leavePack<STREAM, T, VEC>(base + e, v);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j)
@@ -689,7 +699,7 @@ struct Along {
 };
 
 // A team of TEAM lanes holds a group in registers; teams of 64 share a workgroup of 256.
-template <class T, int VEC, int TEAM, int ITEMS>
+template <class T, int VEC, int TEAM, int ITEMS, bool STREAM>
 __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void planesForward(NormArgs a) {
   constexpr int TEAMS = TEAM < 256 ? 256 / TEAM : 1;
   __shared__ double space[TEAM / 64];
@@ -729,7 +739,7 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void planesForward(NormArg
 #pragma unroll
     for (int j = 0; j < VEC; ++j) out[j] = affine((out[j] - m.mean) * m.rstd, p.w[j], p.shift[j]);
     activateAll(out, a.activation);
-    Words<T, VEC>::store(a, a.y, y, e, n, out);
+    Words<T, VEC>::template store<STREAM>(a, a.y, y, e, n, out);
   }
 }
 
@@ -755,7 +765,7 @@ __global__ __launch_bounds__(256) void planesSums(NormArgs a) {
   if (threadIdx.x == 0) a.sums[index * a.pieces + piece] = double2{s1[0], s2[0]};
 }
 
-template <class T, int VEC>
+template <class T, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void planesApply(NormArgs a) {
   __shared__ double space[4];
   const long block = gridDim.x - 1 - blockIdx.x;
@@ -787,7 +797,7 @@ __global__ __launch_bounds__(256) void planesApply(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) out[j] = affine((out[j] - m.mean) * m.rstd, p.w[j], p.shift[j]);
     activateAll(out, a.activation);
-    Words<T, VEC>::store(a, a.y, y, (int)e, end, out);
+    Words<T, VEC>::template store<STREAM>(a, a.y, y, (int)e, end, out);
   }
 }
 
@@ -835,7 +845,7 @@ __global__ __launch_bounds__(256) void planesGradSums(NormArgs a) {
 
 // A workgroup: 256 VEC elements, times `each`, of a group.  The first `before` of them add up the gradients of weight
 // and bias.
-template <class T, int VEC>
+template <class T, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void planesGradApply(NormArgs a, long blocks, int each, int before) {
   __shared__ float space[4];
   __shared__ float2 sums[32][kParameters];
@@ -878,7 +888,135 @@ __global__ __launch_bounds__(256) void planesGradApply(NormArgs a, long blocks, 
     slopeAll(z, out, a.activation);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) out[j] = rstd * (out[j] * p.w[j] - m1 - fx[j] * m2);
-    Words<T, VEC>::store(a, a.y, y, e, n, out);
+    Words<T, VEC>::template store<STREAM>(a, a.y, y, e, n, out);
+  }
+}
+
+// Large planes: a workgroup to a piece of one plane, whose weight and bias it knows.  (The pieces and cuts are of a
+// plane here.)  What a lane has on its way: four words of one operand, two of each of two.
+template <class T, int VEC, int AHEAD>
+struct Run {
+  Words<T, VEC> coming[AHEAD], now[AHEAD];
+  const T* from;
+  int e, end;
+
+  __device__ __forceinline__ void request(const NormArgs& a, const Image& i) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (e + k * 256 * VEC < end) coming[k].load(a, i, from, e + k * 256 * VEC, end);
+  }
+  __device__ __forceinline__ Run(const NormArgs& a, const Image& i, long b, long c, long first, long size)
+      : from(static_cast<const T*>(i.data) + b * i.b + c * i.c), e((int)first + threadIdx.x * VEC), end((int)min(first + size, a.P)) {
+    request(a, i);
+  }
+  __device__ __forceinline__ void next(const NormArgs& a, const Image& i) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) now[k] = coming[k];
+    e += AHEAD * 256 * VEC;
+    request(a, i);
+  }
+};
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void planeSums(NormArgs a) {
+  __shared__ double space[4];
+  const int index = quotient(blockIdx.x, a.byPieces), piece = blockIdx.x - index * a.pieces;
+  const long b = index / (int)a.C, c = index % (int)a.C;
+  Run<T, VEC, kAhead> x(a, a.x, b, c, piece * a.piece, a.piece);
+  double s1[VEC] = {}, s2[VEC] = {};
+  for (int e = x.e; e < x.end; e += kAhead * 256 * VEC) {
+    x.next(a, a.x);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (e + k * 256 * VEC < x.end) {  // (zeros behind the end of a word)
+        float v[VEC];
+        unpack(x.now[k].raw, v);
+        moments(v, s1, s2);
+      }
+  }
+#pragma unroll
+  for (int j = 1; j < VEC; ++j) s1[0] += s1[j], s2[0] += s2[j];
+  s1[0] = teamSum<256>(s1[0], space);
+  s2[0] = teamSum<256>(s2[0], space);
+  if (threadIdx.x == 0) a.sums[(long)index * a.pieces + piece] = double2{s1[0], s2[0]};
+}
+
+template <class T, int VEC, bool STREAM>
+__global__ __launch_bounds__(256) void planeApply(NormArgs a) {
+  __shared__ double space[4];
+  const int block = gridDim.x - 1 - blockIdx.x, index = quotient(block, a.byCuts), cut = block - index * a.cuts;
+  const long b = index / (int)a.C, c = index % (int)a.C, g = quotient((int)c, a.byD);
+  Run<T, VEC, kAhead> x(a, a.x, b, c, cut * a.cut, a.cut);
+  const float w = lineOr(a.weight, c, 1.f), shift = lineOr(a.bias, c, 0.f);
+  const double2* const sums = a.sums + (b * a.C + g * a.D) * a.pieces;
+  double s1 = 0, s2 = 0;
+  for (long i = threadIdx.x; i < a.D * a.pieces; i += 256) {
+    s1 += sums[i].x;
+    s2 += sums[i].y;
+  }
+  s1 = teamSum<256>(s1, space);
+  s2 = teamSum<256>(s2, space);
+  const Moments m = momentsOf(a, s1, s2);
+  if (threadIdx.x == 0 && cut == 0 && c == g * a.D) {
+    if (a.mean) a.mean[b * a.meanB + g * a.meanG] = m.mean;
+    if (a.rstd) a.rstd[b * a.rstdB + g * a.rstdG] = m.rstd;
+  }
+  T* const y = static_cast<T*>(a.y.data) + b * a.y.b + c * a.y.c;
+  for (int e = x.e; e < x.end; e += kAhead * 256 * VEC) {
+    x.next(a, a.x);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (e + k * 256 * VEC < x.end) {
+        float v[VEC];
+        unpack(x.now[k].raw, v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = affine((v[j] - m.mean) * m.rstd, w, shift);
+        activateAll(v, a.activation);
+        Words<T, VEC>::template store<STREAM>(a, a.y, y, e + k * 256 * VEC, x.end, v);
+      }
+  }
+}
+
+template <class T, int VEC, bool STREAM>
+__global__ __launch_bounds__(256) void planeGradApply(NormArgs a, int before) {
+  __shared__ float space[4];
+  __shared__ float2 sums[32][kParameters];
+  if ((int)blockIdx.x < before) return parameterGradients(a, blockIdx.x, sums);
+  const int block = gridDim.x - 1 - blockIdx.x, index = quotient(block, a.byCuts), cut = block - index * a.cuts;
+  const long b = index / (int)a.C, c = index % (int)a.C, group = quotient((int)c, a.byD);
+  Run<T, VEC, kAheadTwo> x(a, a.x, b, c, cut * a.cut, a.cut), g(a, a.g, b, c, cut * a.cut, a.cut);
+  const float mean = a.mean[b * a.meanB + group * a.meanG], rstd = a.rstd[b * a.rstdB + group * a.rstdG];
+  const float w = lineOr(a.weight, c, 1.f), shift = lineOr(a.bias, c, 0.f);
+  float m1 = 0, m2 = 0;
+  for (long i = threadIdx.x; i < a.D * a.pieces; i += 256) {
+    const long other = group * a.D + i % a.D;
+    const float2 s = a.channels[(b * a.pieces + i / a.D) * a.C + other];
+    const float v = lineOr(a.weight, other, 1.f);
+    m1 += s.x * v;
+    m2 += s.y * v;
+  }
+  m1 = teamSum<256>(m1, space) * (float)a.share;
+  m2 = teamSum<256>(m2, space) * (float)a.share;
+  T* const y = static_cast<T*>(a.y.data) + b * a.y.b + c * a.y.c;
+  for (int e = x.e; e < x.end; e += kAheadTwo * 256 * VEC) {
+    x.next(a, a.x);
+    g.next(a, a.g);
+#pragma unroll
+    for (int k = 0; k < kAheadTwo; ++k)
+      if (e + k * 256 * VEC < x.end) {
+        float v[VEC], out[VEC], z[VEC];
+        unpack(x.now[k].raw, v);
+        unpack(g.now[k].raw, out);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          v[j] = (v[j] - mean) * rstd;
+          z[j] = affine(v[j], w, shift);
+        }
+        slopeAll(z, out, a.activation);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) out[j] = rstd * (out[j] * w - m1 - v[j] * m2);
+        Words<T, VEC>::template store<STREAM>(a, a.y, y, e + k * 256 * VEC, x.end, out);
+      }
   }
 }
 
@@ -969,7 +1107,8 @@ enum Family { Last, Planes, Any };
 struct NormPlan {
   Family family;
   int vec, threads, items, band, lanes, rows;
-  long pieces, piece;
+  bool large;  // Planes: a workgroup to a piece of one plane
+  long pieces, piece, cuts, cut;
 };
 
 struct Shape {
@@ -983,7 +1122,7 @@ bool wordsFit(const Image& i, long vec, size_t size) {
   return i.b % vec == 0 && i.h % vec == 0 && i.w % vec == 0 && aligned(i.data, vec * size);
 }
 
-constexpr long kMostPieces = 256;
+constexpr long kMostPieces = 64, kLargePlane = 2048;
 // (of each image's pixels, or of a group's values; the bound that the workspace is made for)
 long piecesOf(long units, long images) {
   return std::max(1L, std::min({kMostPieces, 1024 / std::max(1L, images), units}));
@@ -1006,19 +1145,26 @@ NormPlan planOf(const NormProblem& p, bool backward) {
   if (unit || (nearer && !channels)) {
     plan.family = Planes;
     plan.vec = unit && P >= most ? most : 1;
-    const long words = (n + plan.vec - 1) / plan.vec;
+    const long held = (n + plan.vec - 1) / plan.vec;
     if (!backward) {
-      plan.threads = words <= 64 * 4 ? 64 : words <= 256 * 4 ? 256 : 1024;
-      plan.items = words <= plan.threads * 4L ? 4 : words <= plan.threads * 8L ? 8 : 0;
-      if (plan.items == 0) {
+      plan.threads = held <= 64 * 4 ? 64 : held <= 256 * 4 ? 256 : 1024;
+      plan.items = held <= plan.threads * 4L ? 4 : held <= plan.threads * 8L ? 8 : 0;
+      plan.large = plan.items == 0 && P >= kLargePlane;
+      if (plan.items == 0 && !plan.large) {
         plan.pieces = piecesOf((n + 4095) / 4096, p.B * p.G);
         plan.piece = ((n + plan.pieces - 1) / plan.pieces + plan.vec - 1) / plan.vec * plan.vec;
+        return plan;
       }
     } else {
       plan.threads = P <= 64 * 4 * plan.vec ? 64 : 256;
-      plan.pieces = piecesOf((P + 4095) / 4096, p.B * p.C);
-      plan.piece = ((P + plan.pieces - 1) / plan.pieces + plan.vec - 1) / plan.vec * plan.vec;
+      plan.large = P >= kLargePlane;
     }
+    // (pieces and cuts begin with whole words)
+    const auto words = [&](long size) { return (size + plan.vec - 1) / plan.vec * plan.vec; };
+    plan.pieces = piecesOf((P + 4095) / 4096, p.B * p.C);
+    plan.piece = words((P + plan.pieces - 1) / plan.pieces);
+    plan.cuts = std::max(1L, std::min(2048 / (p.B * p.C), (P + 4095) / 4096));
+    plan.cut = words((P + plan.cuts - 1) / plan.cuts);
     return plan;
   }
   plan.family = Last;
@@ -1058,10 +1204,12 @@ NormPlan planOf(const NormProblem& p, bool backward) {
   while (band + least <= p.C && (band + least) / vec <= 256 && band + least <= kBand && (band + least) / D <= 256 &&
          (D % vec == 0 || band + least <= 256))
     band += least;
-  setBand(band, 256);
-  const long bands = (p.C + plan.band - 1) / plan.band;
-  plan.pieces = piecesOf((P + 4 * plan.rows - 1) / (4 * plan.rows), p.B * bands);
+  setBand(band, kFirst);
+  const long images = p.B * ((p.C + plan.band - 1) / plan.band), second = 256 / plan.lanes;
+  plan.pieces = piecesOf((P + 4 * plan.rows - 1) / (4 * plan.rows), images);
   plan.piece = (P + plan.pieces - 1) / plan.pieces;
+  plan.cuts = std::max(1L, std::min(2048 / images, (P + 4 * second - 1) / (4 * second)));
+  plan.cut = (P + plan.cuts - 1) / plan.cuts;
   return plan;
 }
 
@@ -1077,76 +1225,80 @@ NormArgs argsOf(const NormProblem& p, const NormPlan& plan, bool backward) {
   a.byW = divisorOf(a.W), a.byP = divisorOf(a.P), a.byD = divisorOf(a.D), a.byLanes = divisorOf(plan.lanes);
   a.byPieces = divisorOf(plan.pieces), a.byBands = divisorOf(plan.band ? (p.C + plan.band - 1) / plan.band : 1);
   a.band = plan.band, a.rows = plan.rows, a.lanes = plan.lanes, a.pieces = (int)plan.pieces, a.piece = plan.piece;
+  a.rowsSecond = plan.lanes ? 256 / plan.lanes : 0, a.cuts = (int)plan.cuts, a.cut = plan.cut, a.byCuts = divisorOf(plan.cuts);
   char* const space = static_cast<char*>(p.workspace);
   if (!backward) {
     a.sums = reinterpret_cast<double2*>(space);
   } else {
     a.groups = reinterpret_cast<float2*>(space);
-    a.channels = a.groups + (p.B * kMostPieces < 4096 ? p.B * kMostPieces : std::max(4096L, p.B)) * p.G;
+    a.channels = a.groups + (p.B * kMostPieces < 1024 ? p.B * kMostPieces : std::max(1024L, p.B)) * p.G;
   }
   return a;
 }
 
 unsigned blocksOf(const NormArgs& a) { return (unsigned)(a.B * ((a.C + a.band - 1) / a.band) * a.pieces); }
 
-template <class T, int VEC>
+template <class T, int VEC, bool S>
 int forwardLast(const NormPlan& plan, const NormArgs& a, hipStream_t s) {
   const int total = (int)blocksOf(a);
-  const dim3 grid((unsigned)total), dealt((unsigned)((total + 7) / 8 * 8));
+  const dim3 grid((unsigned)total), dealt((unsigned)((total + 7) / 8 * 8)), second((unsigned)(total / a.pieces * a.cuts));
   if (plan.items == 0) {
-    lastSums<T, VEC><<<grid, 256, 0, s>>>(a);
-    lastApply<T, VEC><<<grid, 256, 0, s>>>(a);
+    lastSums<T, VEC><<<grid, kFirst, 0, s>>>(a);
+    lastApply<T, VEC, S><<<second, 256, 0, s>>>(a);
   } else if (plan.items == 4) {
-    lastForward<T, VEC, 256, 4><<<dealt, 256, 0, s>>>(a, total);
+    lastForward<T, VEC, 256, 4, S><<<dealt, 256, 0, s>>>(a, total);
   } else if (plan.threads == 256) {
-    lastForward<T, VEC, 256, 8><<<dealt, 256, 0, s>>>(a, total);
+    lastForward<T, VEC, 256, 8, S><<<dealt, 256, 0, s>>>(a, total);
   } else if (plan.threads == 512) {
-    lastForward<T, VEC, 512, 8><<<dealt, 512, 0, s>>>(a, total);
+    lastForward<T, VEC, 512, 8, S><<<dealt, 512, 0, s>>>(a, total);
   } else {
-    lastForward<T, VEC, 1024, 8><<<dealt, 1024, 0, s>>>(a, total);
+    lastForward<T, VEC, 1024, 8, S><<<dealt, 1024, 0, s>>>(a, total);
   }
   return launchStatus();
 }
 
-template <class T, int VEC>
+template <class T, int VEC, bool S>
 int forwardPlanes(const NormPlan& plan, const NormArgs& a, hipStream_t s) {
   const long groups = a.B * a.G;
-  if (plan.items == 0) {
+  if (plan.large) {
+    planeSums<T, VEC><<<dim3((unsigned)(a.B * a.C * a.pieces)), 256, 0, s>>>(a);
+    planeApply<T, VEC, S><<<dim3((unsigned)(a.B * a.C * a.cuts)), 256, 0, s>>>(a);
+  } else if (plan.items == 0) {
     planesSums<T, VEC><<<dim3((unsigned)(groups * a.pieces)), 256, 0, s>>>(a);
-    planesApply<T, VEC><<<dim3((unsigned)(groups * a.pieces)), 256, 0, s>>>(a);
+    planesApply<T, VEC, S><<<dim3((unsigned)(groups * a.pieces)), 256, 0, s>>>(a);
   } else if (plan.threads == 64) {
-    planesForward<T, VEC, 64, 4><<<dim3((unsigned)((groups + 3) / 4)), 256, 0, s>>>(a);
+    planesForward<T, VEC, 64, 4, S><<<dim3((unsigned)((groups + 3) / 4)), 256, 0, s>>>(a);
   } else if (plan.threads == 256) {
-    planesForward<T, VEC, 256, 4><<<dim3((unsigned)groups), 256, 0, s>>>(a);
+    planesForward<T, VEC, 256, 4, S><<<dim3((unsigned)groups), 256, 0, s>>>(a);
   } else if (plan.items == 4) {
-    planesForward<T, VEC, 1024, 4><<<dim3((unsigned)groups), 1024, 0, s>>>(a);
+    planesForward<T, VEC, 1024, 4, S><<<dim3((unsigned)groups), 1024, 0, s>>>(a);
   } else {
-    planesForward<T, VEC, 1024, 8><<<dim3((unsigned)groups), 1024, 0, s>>>(a);
+    planesForward<T, VEC, 1024, 8, S><<<dim3((unsigned)groups), 1024, 0, s>>>(a);
   }
   return launchStatus();
 }
 
 // (both: whether the gradients of weight and bias are done, by `before` workgroups)
-template <class T, int VEC>
+template <class T, int VEC, bool S>
 bool backwardLast(const NormPlan& plan, const NormArgs& a, int before, hipStream_t s) {
   const int total = (int)blocksOf(a);
-  const dim3 grid((unsigned)total), dealt((unsigned)((total + 7) / 8 * 8));
+  const dim3 grid((unsigned)total), dealt((unsigned)((total + 7) / 8 * 8)), second((unsigned)(total / a.pieces * a.cuts));
   if (plan.items == 0) {
-    lastGradSums<T, VEC><<<grid, 256, 0, s>>>(a);
+    lastGradSums<T, VEC><<<grid, kFirst, 0, s>>>(a);
     if (!a.y.data) return false;
-    lastGradApply<T, VEC><<<dim3((unsigned)(total + before)), 256, 0, s>>>(a, before);
+    lastGradApply<T, VEC, S><<<dim3(second.x + (unsigned)before), 256, 0, s>>>(a, before);
     return true;
   }
   if (plan.items == 4)
-    lastBackward<T, VEC, 256, 4><<<dealt, 256, 0, s>>>(a, total);
+    lastBackward<T, VEC, 256, 4, S><<<dealt, 256, 0, s>>>(a, total);
   else if (plan.threads == 256)
-    lastBackward<T, VEC, 256, 8><<<dealt, 256, 0, s>>>(a, total);
+    lastBackward<T, VEC, 256, 8, S><<<dealt, 256, 0, s>>>(a, total);
   else
-    lastBackward<T, VEC, 512, 8><<<dealt, 512, 0, s>>>(a, total);
+    lastBackward<T, VEC, 512, 8, S><<<dealt, 512, 0, s>>>(a, total);
   return false;
 }
 
-template <class T, int VEC>
+template <class T, int VEC, bool S>
 bool backwardPlanes(const NormPlan& plan, const NormArgs& a, int before, hipStream_t s) {
   const long planes = a.B * a.C * a.pieces;
   if (plan.threads == 64)
@@ -1154,9 +1306,13 @@ bool backwardPlanes(const NormPlan& plan, const NormArgs& a, int before, hipStre
   else
     planesGradSums<T, VEC, 256><<<dim3((unsigned)planes), 256, 0, s>>>(a);
   if (!a.y.data) return false;
+  if (plan.large) {
+    planeGradApply<T, VEC, S><<<dim3((unsigned)(a.B * a.C * a.cuts + before)), 256, 0, s>>>(a, before);
+    return true;
+  }
   const long words = (a.D * a.P + VEC - 1) / VEC, each = std::max(1L, std::min(8L, words * a.B * a.G / (256 * 4096)));
   const long blocks = (words + 256 * each - 1) / (256 * each);
-  planesGradApply<T, VEC><<<dim3((unsigned)(a.B * a.G * blocks + before)), 256, 0, s>>>(a, blocks, (int)each, before);
+  planesGradApply<T, VEC, S><<<dim3((unsigned)(a.B * a.G * blocks + before)), 256, 0, s>>>(a, blocks, (int)each, before);
   return true;
 }
 
@@ -1165,11 +1321,16 @@ int forward(const NormProblem& p, hipStream_t s) {
   constexpr int W = 16 / sizeof(T);
   const NormPlan plan = planOf(p, false);
   const NormArgs a = argsOf(p, plan, false);
-  if (plan.family == Planes) return plan.vec == W ? forwardPlanes<T, W>(plan, a, s) : forwardPlanes<T, 1>(plan, a, s);
-  if (plan.family == Last)
-    return plan.vec == W   ? forwardLast<T, W>(plan, a, s)
-           : plan.vec == 2 ? forwardLast<T, 2>(plan, a, s)
-                           : forwardLast<T, 1>(plan, a, s);
+  const bool stream = streams((double)p.B * p.C * a.P, p.type);
+  if (plan.family == Planes) {
+    if (plan.vec == 1) return forwardPlanes<T, 1, false>(plan, a, s);
+    return stream ? forwardPlanes<T, W, true>(plan, a, s) : forwardPlanes<T, W, false>(plan, a, s);
+  }
+  if (plan.family == Last) {
+    if (plan.vec == 1) return forwardLast<T, 1, false>(plan, a, s);
+    if (plan.vec == 2) return forwardLast<T, 2, false>(plan, a, s);
+    return stream ? forwardLast<T, W, true>(plan, a, s) : forwardLast<T, W, false>(plan, a, s);
+  }
   normAny<T><<<dim3((unsigned)(a.B * a.G)), 256, 0, s>>>(a);
   return launchStatus();
 }
@@ -1186,12 +1347,19 @@ int backward(const NormProblem& p, hipStream_t s) {
   } else {
     plan = planOf(p, true);
     a = argsOf(p, plan, true);
+    const bool stream = streams((double)p.B * p.C * a.P, p.type);
     if (plan.family == Planes) {
-      done |= plan.vec == W ? backwardPlanes<T, W>(plan, a, parameters, s) : backwardPlanes<T, 1>(plan, a, parameters, s);
+      if (plan.vec == 1)
+        done |= backwardPlanes<T, 1, false>(plan, a, parameters, s);
+      else
+        done |= stream ? backwardPlanes<T, W, true>(plan, a, parameters, s) : backwardPlanes<T, W, false>(plan, a, parameters, s);
     } else if (plan.family == Last) {
-      done |= plan.vec == W   ? backwardLast<T, W>(plan, a, parameters, s)
-              : plan.vec == 2 ? backwardLast<T, 2>(plan, a, parameters, s)
-                              : backwardLast<T, 1>(plan, a, parameters, s);
+      if (plan.vec == 1)
+        done |= backwardLast<T, 1, false>(plan, a, parameters, s);
+      else if (plan.vec == 2)
+        done |= backwardLast<T, 2, false>(plan, a, parameters, s);
+      else
+        done |= stream ? backwardLast<T, W, true>(plan, a, parameters, s) : backwardLast<T, W, false>(plan, a, parameters, s);
     } else {
       normSumsAny<T><<<dim3((unsigned)(a.B * a.C)), 256, 0, s>>>(a);
       if (a.y.data) normGradAny<T><<<dim3((unsigned)(a.B * a.G)), 256, 0, s>>>(a);
@@ -1205,8 +1373,8 @@ int backward(const NormProblem& p, hipStream_t s) {
 
 size_t normWorkspaceBytes(int pass, long B, long C, long P, long G) {
   // images times pieces: of any plan
-  const long rows = B * kMostPieces < 4096 ? B * kMostPieces : std::max(4096L, B);
-  if (pass == 0) return (size_t)rows * G * sizeof(double2);
+  const long rows = B * kMostPieces < 1024 ? B * kMostPieces : std::max(1024L, B);
+  if (pass == 0) return (size_t)(rows * G + std::max(B * C, 1024L)) * sizeof(double2);
   return (size_t)rows * (G + C) * sizeof(float2);
 }
 

@@ -41,6 +41,25 @@ __device__ __forceinline__ void storePack(T* p, const float (&v)[N]) {
   }
 }
 
+// storePack, STREAM: of results that are not read again soon, past the caches.  (A choice at run time would not do: the
+// compiler makes one plain store of the two.)
+template <bool STREAM, class T, int N>
+__device__ __forceinline__ void leavePack(T* p, const float (&v)[N]) {
+  if constexpr (!STREAM || N == 1) {
+    storePack<T, N>(p, v);
+  } else {
+    typename Pack<T, N>::type w;
+#pragma unroll
+    for (int j = 0; j < N; ++j) w[j] = (T)v[j];
+    __builtin_nontemporal_store(w, reinterpret_cast<typename Pack<T, N>::type*>(p));
+  }
+}
+
+// Results of 48 MiB and more are such (us, past the caches / through them: group norm of 16 x 32 x 256 x 256 bf16
+// 43.9 / 48.9 forward and 74.5 / 78.8 backward, of 128 x 192 x 23 x 23 fp32 22.3 / 26.1; dropout of 67 MB 36.9 / 38.4);
+// smaller ones are likely read from there next (32 x 192 x 23 x 23 fp32 13.5 / 9.7, dropout of 19 MB 11.0 / 10.7).
+inline bool streams(double elements, int type) { return elements * (type == FBFFT_FLOAT32 ? 4 : 2) >= (double)(48 << 20); }
+
 // element i of an array of a type that is known at run time
 __device__ __forceinline__ float loadAny(const void* p, int type, long i) {
   if (type == FBFFT_FLOAT32) return static_cast<const float*>(p)[i];
