@@ -1111,10 +1111,6 @@ struct NormPlan {
   long pieces, piece, cuts, cut;
 };
 
-struct Shape {
-  int threads, items;
-};
-
 bool unitPixels(const Image& i, long C, long H, long W) {
   return (W == 1 || i.w == 1) && (H == 1 || i.h == W) && (C == 1 || i.c == H * W);
 }
@@ -1185,20 +1181,27 @@ NormPlan planOf(const NormProblem& p, bool backward) {
     plan.band = (int)std::min(band, p.C), plan.threads = threads;
     plan.lanes = (int)(plan.band / vec), plan.rows = threads / plan.lanes;
   };
-  // a band of 128 bytes of neighbouring channels or more where this leaves a workgroup for each compute unit, or of 64,
-  // or of whatever a group has
+  // A group in registers: workgroups of 256 lanes, several to a compute unit, before larger ones (128 x 192 x 23 x 23 bf16,
+  // us: 20.0 and 32.5, backward 36.5 and 40), and of the bands of channels that fit them the widest that leaves a
+  // workgroup for each unit.  16-bit types go down to bands of 32 bytes before larger workgroups, float32 does not (the
+  // same shape, backward: 83 and 58); whatever a group has comes last.
+  struct Choice {
+    int threads, items, bytes;
+  };
+  const bool narrow = size == 2;
+  const Choice choices[] = {{256, 4, 128}, {256, 8, 128}, {256, 4, 64},  {256, 8, 64},  {256, 4, narrow ? 32 : 0}, {256, 8, narrow ? 32 : 0},
+                            {512, 8, 128}, {512, 8, 64},  {1024, 8, 64}, {256, 4, 1},   {256, 8, 1},               {512, 8, 1},
+                            {1024, 8, 1}};
   const long bytes = least * (long)size;
-  for (long want : {128L, 64L, 1L}) {
-    const long band = std::min(p.C, (want + bytes - 1) / bytes * least), lanes = band / vec, bands = (p.C + band - 1) / band;
-    if (want > 1 && p.B * bands < 256 && band > least) continue;
-    for (const auto& shape : {Shape{256, 4}, Shape{256, 8}, Shape{512, 8}, Shape{1024, 8}}) {
-      if (backward && shape.threads == 1024) break;  // (input, gradient and a lane's sums would not fit its registers)
-      if (lanes > shape.threads || band / D > shape.threads || band > kBand || P > shape.threads / lanes * (long)shape.items) continue;
-      setBand(band, shape.threads);
-      plan.items = shape.items;
-      plan.pieces = 1, plan.piece = P;
-      return plan;
-    }
+  for (const Choice& c : choices) {
+    if (c.bytes == 0 || (backward && c.threads == 1024)) continue;  // (two operands of 1024 lanes would not fit their registers)
+    const long band = std::min(p.C, (c.bytes + bytes - 1) / bytes * least), lanes = band / vec, bands = (p.C + band - 1) / band;
+    if (c.bytes > 1 && p.B * bands < 256 && band > least) continue;
+    if (lanes > c.threads || band / D > c.threads || band > kBand || P > c.threads / lanes * (long)c.items) continue;
+    setBand(band, c.threads);
+    plan.items = c.items;
+    plan.pieces = 1, plan.piece = P;
+    return plan;
   }
   long band = least;
   while (band + least <= p.C && (band + least) / vec <= 256 && band + least <= kBand && (band + least) / D <= 256 &&

@@ -308,7 +308,7 @@ struct Tile {
 // matrix instruction, so that a lane ends with four neighbouring results of one row.  The next step's words are in
 // registers while this one's pieces are multiplied.
 template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(256) void product(ProductArgs g) {
+__global__ __launch_bounds__(256, BM * BN == 8192 ? 3 : 1) void product(ProductArgs g) {
   typedef typename Pieces<T>::type P;
   typedef Stage<T, AK, BM> A;
   typedef Stage<T, BK, BN> B;
@@ -675,17 +675,20 @@ __global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, in
       });
 }
 
-constexpr int kBiasRows = 64;  // rows of dz that a workgroup sums
+// Rows of dz that a workgroup sums: all of a few, whose sums are then the bias's gradient.
+constexpr long kBiasRows = 64, kBiasFew = 128;
+inline long biasRows(long M) { return M <= kBiasFew ? std::max(M, 1L) : kBiasRows; }
 
-// dz = dy activation'(z), dense, and its columns' sums over kBiasRows rows each.  A workgroup: 32 words of VEC columns,
-// eight rows of lanes.
+// dz = dy activation'(z), dense, and its columns' sums over `rows` rows each, or, of all rows, the bias's gradient.  A
+// workgroup: 32 words of VEC columns, eight rows of lanes.
 template <class T, int VEC>
-__global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z, T* dz, float* parts, long M, long N, int activation) {
+__global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z, T* dz, float* parts, Line bias, long M, long N,
+                                                             int activation, long rows) {
   typedef typename Pack<T, VEC>::type Word;
   constexpr int AHEAD = 4;
   __shared__ float sums[8][32 * VEC];
   const int column = threadIdx.x % 32, r = threadIdx.x / 32;
-  const long n = ((long)blockIdx.x * 32 + column) * VEC, m0 = (long)blockIdx.y * kBiasRows, end = min(m0 + kBiasRows, M);
+  const long n = ((long)blockIdx.x * 32 + column) * VEC, m0 = blockIdx.y * rows, end = min(m0 + rows, M);
   const bool whole = n + VEC <= N;
   auto load = [&](const Matrix& from, long m) __attribute__((always_inline)) {
     const T* const p = static_cast<const T*>(from.data) + min(m, end - 1) * from.row + n * from.col;
@@ -740,7 +743,7 @@ __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z
       }
     }
   }
-  if (!parts) return;
+  if (!parts && !bias.data) return;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sums[r][column * VEC + j] = sum[j];
   __syncthreads();
@@ -749,7 +752,11 @@ __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) v += sums[q][i];
-    if (at < N) parts[blockIdx.y * N + at] = v;
+    if (at >= N) continue;
+    if (parts)
+      parts[blockIdx.y * N + at] = v;
+    else
+      storeAny(bias.data, bias.type, at * bias.stride, v);
   }
 }
 
@@ -906,7 +913,7 @@ template <class T>
 int backward(const LinearProblem& p, hipStream_t s) {
   char* space = static_cast<char*>(p.workspace);
   Matrix dz = p.dy;
-  const long chunks = ceilDivLong(p.M, kBiasRows);
+  const long chunks = ceilDivLong(p.M, biasRows(p.M));
   float* const parts = reinterpret_cast<float*>(space);
   space += rounded((size_t)chunks * p.N * sizeof(float));
   const bool products = p.dx.data || p.dw.data, apart = products && p.activation != FBFFT_ACTIVATION_NONE;
@@ -919,13 +926,14 @@ int backward(const LinearProblem& p, hipStream_t s) {
     const bool words = p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
     const dim3 grid((unsigned)ceilDivLong(p.N, 32 * (words ? W : 1)), (unsigned)chunks);
     T* const to = apart ? static_cast<T*>(dz.data) : nullptr;
-    float* const sums = p.gradBias.data ? parts : nullptr;
+    float* const sums = p.gradBias.data && chunks > 1 ? parts : nullptr;
+    const Line bias = chunks > 1 ? Line{} : p.gradBias;
     if (words)
-      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, p.M, p.N, p.activation);
+      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M));
     else
-      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, p.M, p.N, p.activation);
+      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M));
   }
-  if (p.gradBias.data && p.N > 0)
+  if (p.gradBias.data && p.N > 0 && chunks != 1)
     biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 8)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
   int rc = launchStatus();
   if (rc == FBFFT_SUCCESS && p.dx.data && p.M > 0 && p.K > 0)
@@ -941,7 +949,7 @@ int backward(const LinearProblem& p, hipStream_t s) {
 
 size_t linearWorkspaceBytes(int pass, long M, long K, long N, int type) {
   if (pass == 0) return K > 0 ? partsBytes(M, N, K, type) : 0;
-  return rounded((size_t)ceilDivLong(M, kBiasRows) * N * sizeof(float)) +
+  return rounded((size_t)ceilDivLong(M, biasRows(M)) * N * sizeof(float)) +
          rounded((size_t)M * N * (type == FBFFT_FLOAT32 ? 4 : 2)) + std::max(partsBytes(M, K, N, type), partsBytes(N, K, M, type));
 }
 
