@@ -648,31 +648,69 @@ __global__ __launch_bounds__(WAVES * 64) void fewRows(ProductArgs g) {
   static_cast<T*>(g.e.out.data)[m * g.e.out.row + n * g.e.out.col] = (T)z;
 }
 
-// Results from the sums of `ranges` ranges of k, in their order (of none: from 0).
+// Results from the sums of `ranges` ranges of k, in their order (of none: from 0).  A lane: eight neighbours.
 template <class T>
-__global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, int ranges) {
-  const long words = (N + 7) / 8, i = (long)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void joinWords(Epilogue e, long M, long N, int ranges) {
+  const long words = N / 8, i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= M * words) return;
   const long m = i / words, n = i % words * 8;
   const float* const from = e.parts + m * N + n;
-  finish<T>(
-      e, m, n, N - n,
-      [&](float(&z)[8]) __attribute__((always_inline)) {
+  auto eight = [&](float(&z)[8]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) z[q] = 0.f;
+    for (int q = 0; q < 8; ++q) z[q] = 0.f;
 #pragma unroll 4
-        for (int r = 0; r < ranges; ++r) {
-          float v[8];
-          loadPack<float, 8>(from + r * M * N, v);
+    for (int r = 0; r < ranges; ++r) {
+      float v[8];
+      loadPack<float, 8>(from + r * M * N, v);
 #pragma unroll
-          for (int q = 0; q < 8; ++q) z[q] += v[q];
-        }
-      },
-      [&](int v) __attribute__((always_inline)) {
-        float z = 0.f;
-        for (int r = 0; r < ranges; ++r) z += from[r * M * N + v];
-        return z;
-      });
+      for (int q = 0; q < 8; ++q) z[q] += v[q];
+    }
+  };
+  auto one = [&](int v) __attribute__((always_inline)) {
+    float z = 0.f;
+    for (int r = 0; r < ranges; ++r) z += from[r * M * N + v];
+    return z;
+  };
+  finish<T>(e, m, n, 8, eight, one);
+}
+
+// The same, a result to a lane, or to GROUPS of them that take the ranges in turn: for few results, or rows that no
+// words fit.
+template <class T, int GROUPS>
+__global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, int ranges) {
+  constexpr int SIDE = 256 / GROUPS;
+  __shared__ float sums[256];
+  const int group = threadIdx.x / SIDE;
+  const long i = (long)blockIdx.x * SIDE + threadIdx.x % SIDE;
+  float z = 0.f;
+  if (i < M * N)
+#pragma unroll 8
+    for (int r = group; r < ranges; r += GROUPS) z += e.parts[r * M * N + i];
+  if (GROUPS > 1) {
+    sums[threadIdx.x] = z;
+    __syncthreads();
+    if (group > 0) return;
+    z = 0.f;
+#pragma unroll
+    for (int q = 0; q < GROUPS; ++q) z += sums[q * SIDE + threadIdx.x];
+  }
+  if (i >= M * N) return;
+  const long m = i / N, n = i - m * N;
+  z += lineOr(e.bias, n, 0.f);
+  if (e.z.data) static_cast<T*>(e.z.data)[m * e.z.row + n * e.z.col] = (T)z;
+  z = activate(z, e.activation);
+  if (e.residual.data) z += (float)static_cast<const T*>(e.residual.data)[m * e.residual.row + n * e.residual.col];
+  static_cast<T*>(e.out.data)[m * e.out.row + n * e.out.col] = (T)z;
+}
+
+template <class T>
+void launchJoin(const Epilogue& e, long M, long N, int ranges, hipStream_t s) {
+  if (N % 8 == 0 && e.dense && M * N >= 1 << 18)
+    joinWords<T><<<dim3((unsigned)((M * (N / 8) + 255) / 256)), 256, 0, s>>>(e, M, N, ranges);
+  else if (ranges < 8)
+    joinRanges<T, 1><<<dim3((unsigned)((M * N + 255) / 256)), 256, 0, s>>>(e, M, N, ranges);
+  else
+    joinRanges<T, 8><<<dim3((unsigned)((M * N + 31) / 32)), 256, 0, s>>>(e, M, N, ranges);
 }
 
 // Rows of dz that a workgroup sums: all of a few, whose sums are then the bias's gradient.
@@ -688,21 +726,12 @@ __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z
   constexpr int AHEAD = 4;
   __shared__ float sums[8][32 * VEC];
   const int column = threadIdx.x % 32, r = threadIdx.x / 32;
-  const long n = ((long)blockIdx.x * 32 + column) * VEC, m0 = blockIdx.y * rows, end = min(m0 + rows, M);
-  const bool whole = n + VEC <= N;
+  const long first = ((long)blockIdx.x * 32 + column) * VEC, m0 = blockIdx.y * rows, end = min(m0 + rows, M);
+  // (the last word of a row ends with it, and repeats what the one before it has: N is no less than a word)
+  const long n = min(first, N - VEC);
+  const int repeats = (int)min(first - n, (long)VEC);
   auto load = [&](const Matrix& from, long m) __attribute__((always_inline)) {
-    const T* const p = static_cast<const T*>(from.data) + min(m, end - 1) * from.row + n * from.col;
-    Word w{};
-    if constexpr (VEC == 1) {
-      if (whole) w = *p;
-    } else if (whole) {
-      w = *reinterpret_cast<const Word*>(p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (n + j < N) w[j] = p[j];
-    }
-    return w;
+    return *reinterpret_cast<const Word*>(static_cast<const T*>(from.data) + min(m, end - 1) * from.row + n * from.col);
   };
   auto unpacked = [&](const Word& w, float(&v)[VEC]) __attribute__((always_inline)) {
 #pragma unroll
@@ -714,45 +743,39 @@ __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z
     }
   };
   float sum[VEC] = {};
-  for (long m = m0 + r; m < end; m += 8 * AHEAD) {
-    Word wg[AHEAD], wz[AHEAD];
+  if (repeats < VEC)
+    for (long m = m0 + r; m < end; m += 8 * AHEAD) {
+      Word wg[AHEAD], wz[AHEAD];
 #pragma unroll
-    for (int q = 0; q < AHEAD; ++q) {
-      wg[q] = load(dy, m + 8 * q);
-      if (activation != FBFFT_ACTIVATION_NONE) wz[q] = load(z, m + 8 * q);
-    }
-#pragma unroll
-    for (int q = 0; q < AHEAD; ++q) {
-      if (m + 8 * q >= end) break;
-      float v[VEC], a[VEC];
-      unpacked(wg[q], v);
-      if (activation != FBFFT_ACTIVATION_NONE) {
-        unpacked(wz[q], a);
-        slopeAll(a, v, activation);
+      for (int q = 0; q < AHEAD; ++q) {
+        wg[q] = load(dy, m + 8 * q);
+        if (activation != FBFFT_ACTIVATION_NONE) wz[q] = load(z, m + 8 * q);
       }
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[j] += v[j];
-      if (!dz) continue;
-      T* const to = dz + (m + 8 * q) * N + n;
-      if (whole) {
-        storePack<T, VEC>(to, v);
-      } else {
+      for (int q = 0; q < AHEAD; ++q) {
+        if (m + 8 * q >= end) break;
+        float v[VEC], a[VEC];
+        unpacked(wg[q], v);
+        if (activation != FBFFT_ACTIVATION_NONE) {
+          unpacked(wz[q], a);
+          slopeAll(a, v, activation);
+        }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          if (n + j < N) to[j] = (T)v[j];
+        for (int j = 0; j < VEC; ++j) sum[j] += v[j];
+        if (dz) storePack<T, VEC>(dz + (m + 8 * q) * N + n, v);
       }
     }
-  }
   if (!parts && !bias.data) return;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) sums[r][column * VEC + j] = sum[j];
+  for (int j = 0; j < VEC; ++j)
+    if (j >= repeats) sums[r][column * VEC + j - repeats] = sum[j];
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
     const long at = (long)blockIdx.x * 32 * VEC + i;
+    if (at >= N) continue;
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) v += sums[q][i];
-    if (at >= N) continue;
     if (parts)
       parts[blockIdx.y * N + at] = v;
     else
@@ -829,7 +852,7 @@ ProductPlan planOf(long M, long N, long K, bool straight) {
       const double step = groups <= units ? a.alone : a.shared;
       const double rounds = groups <= slots ? 1.0 : std::max((double)groups / slots, groups < 4 * slots ? (double)ceilDivLong(groups, slots) : 1.0);
       double time = rounds * (range / a.step * step + a.results);
-      if (used > 1) time += 4.0 + (double)M * N * used * 8 / 6e6;
+      if (used > 1) time += 4.0 + 0.15 * used + (double)M * N * used * 8 / 6e6;
       if (least == 0 || time < least) {
         least = time;
         best = ProductPlan{a.kind, a.rows, a.cols, used, range};
@@ -871,10 +894,9 @@ void launchProduct(const ProductPlan& plan, const ProductArgs& g, hipStream_t s)
 
 template <class T>
 int multiplyAll(const Matrix& a, const Matrix& b, long M, long N, long K, Epilogue e, float* parts, hipStream_t s) {
-  const dim3 flat((unsigned)ceilDivLong(M * ceilDivLong(N, 8), 256));
   e.dense = e.out.col == 1 && (!e.residual.data || e.residual.col == 1) && (!e.z.data || e.z.col == 1);
   if (K == 0) {
-    joinRanges<T><<<flat, 256, 0, s>>>(e, M, N, 0);
+    launchJoin<T>(e, M, N, 0, s);
     return launchStatus();
   }
   const bool ak = contiguousK(a), bk = contiguousK(b);
@@ -899,7 +921,7 @@ int multiplyAll(const Matrix& a, const Matrix& b, long M, long N, long K, Epilog
     launchProduct<T, false, true>(plan, g, s);
   else
     launchProduct<T, false, false>(plan, g, s);
-  if (plan.ranges > 1) joinRanges<T><<<flat, 256, 0, s>>>(g.e, M, N, (int)plan.ranges);
+  if (plan.ranges > 1) launchJoin<T>(g.e, M, N, (int)plan.ranges, s);
   return launchStatus();
 }
 
@@ -923,7 +945,7 @@ int backward(const LinearProblem& p, hipStream_t s) {
   }
   if (p.M > 0 && p.N > 0 && (apart || p.gradBias.data)) {
     constexpr int W = 16 / sizeof(T);
-    const bool words = p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
+    const bool words = p.N >= W && p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
     const dim3 grid((unsigned)ceilDivLong(p.N, 32 * (words ? W : 1)), (unsigned)chunks);
     T* const to = apart ? static_cast<T*>(dz.data) : nullptr;
     float* const sums = p.gradBias.data && chunks > 1 ? parts : nullptr;
