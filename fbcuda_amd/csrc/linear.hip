@@ -714,7 +714,7 @@ void launchJoin(const Epilogue& e, long M, long N, int ranges, hipStream_t s) {
 }
 
 // Rows of dz that a workgroup sums: all of a few, whose sums are then the bias's gradient.
-constexpr long kBiasRows = 64, kBiasFew = 128;
+constexpr long kBiasRows = 64, kBiasFew = 64;
 inline long biasRows(long M) { return M <= kBiasFew ? std::max(M, 1L) : kBiasRows; }
 
 // dz = dy activation'(z), dense, and its columns' sums over `rows` rows each, or, of all rows, the bias's gradient.  A
