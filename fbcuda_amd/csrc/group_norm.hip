@@ -75,6 +75,19 @@ __device__ __forceinline__ S teamSum(S v, S* space) {
   return v;
 }
 
+// A workgroup's lanes shared out among its groups, up to NT of them: neighbours, as many to each, a power of two up to a
+// wave, as there are and as have a term to add, so that all groups are summed at once (a wave to one group after the
+// other: 4 x 64 x 199 x 199 f16, 32 groups of 64 pieces, 30 us instead of 21.6; 80 x 32 x 107 x 106, 60 and 45).
+struct Share {
+  int lanes, group, place;
+};
+template <int NT>
+__device__ __forceinline__ Share shareOf(int groups, int terms) {
+  int lanes = 64;
+  while (lanes > 1 && (lanes * groups > NT || lanes / 2 >= terms)) lanes /= 2;
+  return {lanes, (int)threadIdx.x / lanes, (int)threadIdx.x & (lanes - 1)};
+}
+
 // The gradients of weight and bias: the sums over images and pieces.  256 lanes: eight channels, 32 lanes to each.
 constexpr int kParameters = 8;
 __device__ __forceinline__ void parameterGradients(const NormArgs& a, int block, float2 (&part)[32][kParameters]) {
@@ -243,25 +256,22 @@ struct Channel {
 template <int NT, int VEC>
 __device__ __forceinline__ void joinMoments(const NormArgs& a, const Band& band, double (&s1)[VEC], double (&s2)[VEC],
                                             Columns<NT, VEC, double>& space, double* sums, Moments* stats, bool raw) {
-  const int D = (int)a.D, t = threadIdx.x;
+  const int D = (int)a.D;
   // a lane's channels of one group, where groups and words start together
   const int step = D % VEC == 0 ? VEC : VEC % D == 0 ? D : 1, wide = D / step;
+  const Share share = shareOf<NT>(band.groups, wide);
   auto one = [&](double(&s)[VEC]) __attribute__((always_inline)) {
     joinRows<NT, VEC>(a, band.lanes, band.column, band.r, step, s, space, sums);
     __syncthreads();
-    // a wave to a group (as many as a wave has lanes, or fewer, to each: NT groups at most)
-    double kept = 0;
-    for (int g = t / 64, k = 0; g < band.groups; g += NT / 64, ++k) {
-      double v = 0;
-      for (int i = t % 64; i < wide; i += 64) v += sums[g * wide + i];
-      v = waveSum(v);
-      if (t % 64 == k) kept = v;
-    }
-    return kept;
+    double v = 0;
+    if (share.group < band.groups)
+#pragma unroll 4
+      for (int i = share.place; i < wide; i += share.lanes) v += sums[share.group * wide + i];
+    return waveSumOf(v, share.lanes);
   };
   const double first = one(s1), second = one(s2);
-  const int g = t / 64 + t % 64 * (NT / 64);
-  if (g < band.groups) {
+  const int g = share.group;
+  if (g < band.groups && share.place == 0) {
     const long group = band.firstGroup + g;
     if (raw) {
       a.sums[(band.b * a.G + group) * a.pieces + band.piece] = double2{first, second};
@@ -404,20 +414,23 @@ __global__ __launch_bounds__(kFirst) void lastApply(NormArgs a) {
   const Band band = bandOf<VEC, true>(a, gridDim.x - 1 - blockIdx.x);
   Walk<T, VEC, kAhead> x(a, a.x, band);
   bandParameters(a, band, params, 256);
-  for (int g = threadIdx.x / 64; g < band.groups; g += 4) {
-    const long group = band.firstGroup + g;
-    double s1 = 0, s2 = 0;
-    for (int i = threadIdx.x % 64; i < a.pieces; i += 64) {
+  const Share share = shareOf<256>(band.groups, a.pieces);
+  const long group = band.firstGroup + share.group;
+  double s1 = 0, s2 = 0;
+  if (share.group < band.groups)
+#pragma unroll 4
+    for (int i = share.place; i < a.pieces; i += share.lanes) {
       const double2 s = a.sums[(band.b * a.G + group) * a.pieces + i];
       s1 += s.x;
       s2 += s.y;
     }
-    const Moments m = momentsOf(a, waveSum(s1), waveSum(s2));
-    if (threadIdx.x % 64 == 0) {
-      stats[g] = m;
-      if (band.piece == 0 && a.mean) a.mean[band.b * a.meanB + group * a.meanG] = m.mean;
-      if (band.piece == 0 && a.rstd) a.rstd[band.b * a.rstdB + group * a.rstdG] = m.rstd;
-    }
+  s1 = waveSumOf(s1, share.lanes);
+  s2 = waveSumOf(s2, share.lanes);
+  if (share.group < band.groups && share.place == 0) {
+    const Moments m = momentsOf(a, s1, s2);
+    stats[share.group] = m;
+    if (band.piece == 0 && a.mean) a.mean[band.b * a.meanB + group * a.meanG] = m.mean;
+    if (band.piece == 0 && a.rstd) a.rstd[band.b * a.rstdB + group * a.rstdG] = m.rstd;
   }
   __syncthreads();
   if (!band.live) return;
@@ -464,13 +477,17 @@ __device__ __forceinline__ void joinGradients(const NormArgs& a, const Band& ban
   }
   __syncthreads();
   const int D = (int)a.D;
-  for (int g = threadIdx.x / 64; g < band.groups; g += NT / 64) {
-    float m1 = 0, m2 = 0;
-    for (int i = threadIdx.x % 64; i < D; i += 64) m1 += sums[0][g * D + i], m2 += sums[1][g * D + i];
-    m1 = waveSum(m1);
-    m2 = waveSum(m2);
-    if (threadIdx.x % 64 == 0) done(g, m1, m2);
-  }
+  const Share share = shareOf<NT>(band.groups, D);
+  float m1 = 0, m2 = 0;
+  if (share.group < band.groups)
+#pragma unroll 4
+    for (int i = share.place; i < D; i += share.lanes) {
+      m1 += sums[0][share.group * D + i];
+      m2 += sums[1][share.group * D + i];
+    }
+  m1 = waveSumOf(m1, share.lanes);
+  m2 = waveSumOf(m2, share.lanes);
+  if (share.group < band.groups && share.place == 0) done(share.group, m1, m2);
 }
 
 // dx in the place of dz, from xh
@@ -600,17 +617,18 @@ __global__ __launch_bounds__(256) void lastGradApply(NormArgs a, int before) {
   const Band band = bandOf<VEC, true>(a, gridDim.x - 1 - blockIdx.x);
   Walk<T, VEC, kAheadTwo> x(a, a.x, band), g(a, a.g, band);
   bandParameters(a, band, params, 256);
-  for (int k = threadIdx.x / 64; k < band.groups; k += 4) {
-    float m1 = 0, m2 = 0;
-    for (int i = threadIdx.x % 64; i < a.pieces; i += 64) {
-      const float2 s = a.groups[(band.b * a.G + band.firstGroup + k) * a.pieces + i];
-      m1 += s.x;
-      m2 += s.y;
+  const Share share = shareOf<256>(band.groups, a.pieces);
+  float f1 = 0, f2 = 0;
+  if (share.group < band.groups)
+#pragma unroll 4
+    for (int i = share.place; i < a.pieces; i += share.lanes) {
+      const float2 s = a.groups[(band.b * a.G + band.firstGroup + share.group) * a.pieces + i];
+      f1 += s.x;
+      f2 += s.y;
     }
-    m1 = waveSum(m1);
-    m2 = waveSum(m2);
-    if (threadIdx.x % 64 == 0) means[k] = Moments{m1 * (float)a.share, m2 * (float)a.share};
-  }
+  f1 = waveSumOf(f1, share.lanes);
+  f2 = waveSumOf(f2, share.lanes);
+  if (share.group < band.groups && share.place == 0) means[share.group] = Moments{f1 * (float)a.share, f2 * (float)a.share};
   keptMoments(a, band, stats, 256);
   if (!band.live) return;
   T* const y = laneOf<T>(a, a.y, band, VEC);
@@ -1203,6 +1221,8 @@ NormPlan planOf(const NormProblem& p, bool backward) {
     plan.pieces = 1, plan.piece = P;
     return plan;
   }
+  // two launches: bands as wide as they may be, of which a pixel's values fill whole lines (69 x 160 x 66 x 69 f16, 63 us;
+  // bands of 256 and 128 bytes: 93 and 133)
   long band = least;
   while (band + least <= p.C && (band + least) / vec <= 256 && band + least <= kBand && (band + least) / D <= 256 &&
          (D % vec == 0 || band + least <= 256))

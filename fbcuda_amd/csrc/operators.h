@@ -142,6 +142,17 @@ __device__ __forceinline__ S waveSumEvery(S v, int period) {
   return swappedSum<true>(v);
 }
 
+// The same over `lanes` neighbours, a power of two up to 64.
+template <class S>
+__device__ __forceinline__ S waveSumOf(S v, int lanes) {
+  if (lanes > 1) v += moved<0xB1>(v);
+  if (lanes > 2) v += moved<0x4E>(v);
+  if (lanes > 4) v += moved<0x141>(v);
+  if (lanes > 8) v += moved<0x140>(v);
+  if (lanes > 16) v = swappedSum<false>(v);
+  return lanes > 32 ? swappedSum<true>(v) : v;
+}
+
 // a vector of parameters, or nothing
 struct Line {
   void* data;
