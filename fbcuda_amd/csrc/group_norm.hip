@@ -411,7 +411,7 @@ __global__ __launch_bounds__(kFirst) void lastSums(NormArgs a) {
 
 // 16 x 32 x 256 x 256 bf16, GELU: 26 us for 134 MB, 5.1 TB/s (half of it still in the last-level cache).
 template <class T, int VEC, bool STREAM>
-__global__ __launch_bounds__(kFirst) void lastApply(NormArgs a) {
+__global__ __launch_bounds__(256) void lastApply(NormArgs a) {
   __shared__ Moments stats[256];
   __shared__ float2 params[kBand];
   const Band band = bandOf<VEC, true>(a, gridDim.x - 1 - blockIdx.x);

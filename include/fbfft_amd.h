@@ -384,7 +384,7 @@ int fbfft_group_norm_bprop(const fbfft_array* input, const fbfft_array* weight, 
  * type.  bias, residual: NULL for none.  preactivation: z, rounded, for the backward pass, or NULL; output is
  * computed from z before that rounding.  residual may be output itself; no other operand may overlap it.
  * K = 0 gives activation(bias) + residual.  float32 operands are multiplied as three bf16 pieces each,
- * in six products that leave out terms below 2^-24 of a product; a value that is not finite reaches every
+ * in six products that leave out less than 2^-21 of a product, 2^-24 on average; a value that is not finite reaches every
  * result that it is a factor of, as infinity or NaN.
  * workspace: fbfft_linear_workspace(0, ...) bytes, 256-byte aligned, NULL where that is 0. */
 size_t fbfft_linear_workspace(int pass, long long M, long long K, long long N, int type);
