@@ -18,6 +18,9 @@ struct DropoutArgs {
   const void *x, *residual;
   void* y;
   long size[FBFFT_MAX_DIM], xs[FBFFT_MAX_DIM], rs[FBFFT_MAX_DIM], ys[FBFFT_MAX_DIM];
+  // from an element to the next one, which lies in the next place of dimension d and the first of those after it
+  long xn[FBFFT_MAX_DIM], rn[FBFFT_MAX_DIM], yn[FBFFT_MAX_DIM];
+  int outer;  // the first dimension of more than one
   long total;
   Divisor byInner;  // the innermost extent, where places are counted in 31 bits
   bool counted, words;  // whether they are; whether neighbours of a row are neighbours in every operand
@@ -49,8 +52,9 @@ __device__ __forceinline__ Words philox(unsigned long long block, unsigned long 
 
 // A thread takes the eight elements of one counter.  DENSE: they are neighbours in every operand.  Otherwise they still
 // move as words where they lie in one row of neighbours: 8192 rows of 2048 fp32 with 8 more between the rows, with a
-// residual, 152 -> 39.5 us (5.1 TB/s), 9403 of 2087 bf16 with 5 more 55 -> 34.9 us, element by element at the
-// rows' ends only.
+// residual, 152 us element by element, 39 as words (5.2 TB/s).  What lies across the end of a row goes by steps from place to
+// place, all reads before the writes: 9403 rows of 2087 bf16 with 5 between them 24 us, 9683847 of 3 f16 with 5 148 us (each
+// place computed from its index, one element after the other: 35 and 446).
 template <class T, bool DENSE, bool STREAM>
 __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
   const long block = (long)blockIdx.x * 256 + threadIdx.x, first = block * 8;
@@ -63,7 +67,13 @@ __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
     const unsigned u = j % 2 ? words.w[j / 2] >> 16 : words.w[j / 2] & 0xFFFFu;
     return (u >= g.threshold ? v * g.factor : 0.f) + r;
   };
-  if (DENSE && first + 8 <= g.total) {
+  if (DENSE) {
+    if (first + 8 > g.total) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (first + j < g.total) y[first + j] = (T)result(j, (float)x[first + j], residual ? (float)residual[first + j] : 0.f);
+      return;
+    }
     float v[8], r[8] = {};
     loadPack<T, 8>(x + first, v);
     if (residual) loadPack<T, 8>(residual + first, r);
@@ -78,15 +88,15 @@ __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
   at[INNER] = first - rest * g.size[INNER];
 #pragma unroll
   for (int d = INNER - 1; d > 0; --d) {
-    const long next = g.size[d] == 1 ? rest : rest / g.size[d];
+    const long next = d <= g.outer ? 0 : rest / g.size[d];
     at[d] = rest - next * g.size[d];
     rest = next;
   }
   at[0] = rest;
-  if (g.words && at[INNER] + 8 <= g.size[INNER]) {
-    long xo = at[INNER], ro = at[INNER], yo = at[INNER];
+  long xo = 0, ro = 0, yo = 0;
 #pragma unroll
-    for (int d = 0; d < INNER; ++d) xo += at[d] * g.xs[d], ro += at[d] * g.rs[d], yo += at[d] * g.ys[d];
+  for (int d = 0; d <= INNER; ++d) xo += at[d] * g.xs[d], ro += at[d] * g.rs[d], yo += at[d] * g.ys[d];
+  if (g.words && at[INNER] + 8 <= g.size[INNER]) {
     float v[8], r[8] = {};
     loadPack<T, 8>(x + xo, v);
     if (residual) loadPack<T, 8>(residual + ro, r);
@@ -95,21 +105,32 @@ __global__ __launch_bounds__(256) void dropout(DropoutArgs g) {
     storePack<T, 8>(y + yo, v);
     return;
   }
+  const int count = (int)min(8l, g.total - first);
+  long from[8], by[8], to[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    if (first + j >= g.total) break;
-    long xo = 0, ro = 0, yo = 0;
+    from[j] = xo, by[j] = ro, to[j] = yo;
+    bool carry = j + 1 < count;  // (behind the last element the places stay those of the last)
 #pragma unroll
-    for (int d = 0; d < FBFFT_MAX_DIM; ++d) xo += at[d] * g.xs[d], ro += at[d] * g.rs[d], yo += at[d] * g.ys[d];
-    y[yo] = (T)result(j, (float)x[xo], residual ? (float)residual[ro] : 0.f);
-    bool carry = true;
-#pragma unroll
-    for (int d = FBFFT_MAX_DIM - 1; d >= 0; --d) {
-      at[d] += carry;
-      carry = carry && at[d] == g.size[d];
-      if (carry) at[d] = 0;
+    for (int d = INNER; d >= 0; --d) {
+      if (!carry) continue;
+      carry = ++at[d] == g.size[d];
+      if (carry)
+        at[d] = 0;
+      else
+        xo += g.xn[d], ro += g.rn[d], yo += g.yn[d];
     }
   }
+  // (all reads before the first write, for which nobody then waits)
+  float v[8], r[8] = {};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (float)x[from[j]];
+  if (residual)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (float)residual[by[j]];
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < count) y[to[j]] = (T)result(j, v[j], r[j]);
 }
 
 template <class T>
@@ -150,6 +171,15 @@ int launchDropout(const DropoutProblem& p, hipStream_t s) {
     }
   }
   for (int d = 0; d < last; ++d) g.size[d] = 1;
+  g.outer = last;
+  for (int d = 0; d < FBFFT_MAX_DIM; ++d) {
+    g.xn[d] = g.xs[d], g.rn[d] = g.rs[d], g.yn[d] = g.ys[d];
+    for (int e = d + 1; e < FBFFT_MAX_DIM; ++e) {
+      g.xn[d] -= (g.size[e] - 1) * g.xs[e];
+      g.rn[d] -= (g.size[e] - 1) * g.rs[e];
+      g.yn[d] -= (g.size[e] - 1) * g.ys[e];
+    }
+  }
   g.words = g.xs[FBFFT_MAX_DIM - 1] == 1 && g.ys[FBFFT_MAX_DIM - 1] == 1 && (!g.residual || g.rs[FBFFT_MAX_DIM - 1] == 1);
   g.words = g.words || g.total == 1;
   const bool dense = g.words && last == FBFFT_MAX_DIM - 1;
