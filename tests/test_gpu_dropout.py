@@ -62,6 +62,20 @@ def test_rows_apart(rows, cols, pitch, dtype):
     assert bool((y[:, cols:] == 7.0).all())
 
 
+@pytest.mark.parametrize("shape", [(301, 2, 3), (7, 5, 3, 2), (11, 9, 13), (2, 3, 1, 5, 7), (5, 1, 1, 17)], ids=str)
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+def test_gaps_after_every_dimension(shape, dtype):
+    """A thread's eight elements cross the ends of rows, planes and images, each followed by a gap of its own."""
+    gen = torch.Generator().manual_seed(7)
+    wide = [n + d for d, n in enumerate(shape)]
+    inner = tuple(slice(0, n) for n in shape)
+    x, r = (randn(gen, *wide).to(dtype).to(dev())[inner] for _ in range(2))
+    y = torch.full(wide, 7.0, dtype=dtype, device=dev())
+    check(x, r, 0.25, 3, 4, y[inner])
+    assert int((y == 7.0).sum()) >= y.numel() - x.numel()
+    check(x, r.permute(*reversed(range(r.dim()))).contiguous().permute(*reversed(range(r.dim()))), 0.25, 3, 4, y[inner])
+
+
 def test_published_numbers():
     """Philox4x32-10's known answer for a counter and key of zeros, 6627e8d5 e169c58d bc57ac4c 9b00dbd8: element j is
     kept for a threshold of its own number and dropped for one more."""

@@ -112,6 +112,16 @@ def test_without_parameters_and_in_place(layout, shape):
     within(gy, wx, rounded(wx, x.dtype) + bx)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(3, 2602, 3, 5, 2), (2, 96, 70, 71, 48), (3, 130, 80, 33, 130), (1, 512, 40, 40, 64)], ids=str)
+@pytest.mark.parametrize("layout", ["last", "slice"])
+def test_many_channels_and_many_groups(layout, shape, dtype):
+    """Groups wider than a row of lanes, several of them and images; and bands of 2, 1 and 8 channels to a group."""
+    x, weight, bias, gy = make(shape[:4], shape[4], dtype, layout, 9)
+    mean, rstd = check_forward(x, weight, bias, shape[4], "silu", layout)
+    check_backward(x, weight, bias, gy, mean, rstd, shape[4], "silu", layout)
+
+
 @pytest.mark.parametrize("layout", ["last", "planes"])
 @pytest.mark.parametrize("side", [16, 160])
 def test_variance_far_below_the_squared_mean(layout, side):
