@@ -833,8 +833,8 @@ bool goesStraight(const Matrix& m, long rows, long K) {
 
 // The kernel with the least expected time, from what each takes for a step of k and for its results (us, measured on
 // products of 8192 x 8192 x 2048, 4096 x 1024 x 4096 and single tiles: 256 x 256 tiles, one to a compute unit, 1.75 a step of
-// 64 and 12 for the results; 128 x 128 ones 0.85 alone and 1.1 for two; the staged tiles' are estimates).  A range of k more costs its sums' way to memory
-// and back.
+// 64 and 12 for the results; 128 x 128 ones 0.85 alone and 1.1 for two; the staged ones' are estimates).  A range of k more
+// costs its sums' way to memory and back.
 template <class T>
 ProductPlan planOf(long M, long N, long K, bool straight) {
   struct Option {
