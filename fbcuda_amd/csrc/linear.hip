@@ -7,6 +7,7 @@
 // 16-bit matrix instructions with fp32 sums.  float32 operands are cut into three bf16 pieces of 8 bits each (exactly:
 // the pieces are the leading, middle and last bits), of whose nine products the six largest are summed; what is left
 // out is below 2^-21 of a product (the second piece is below 2^-7 of a value, the third below 2^-15), 2^-24 on average.
+#include "linear_step.h"
 #include "operators.h"
 
 #include <algorithm>
@@ -375,49 +376,30 @@ __global__ __launch_bounds__(256, BM * BN == 8192 ? 3 : 1) void product(ProductA
 
 typedef __attribute__((address_space(3))) void* LdsAddress;
 
-// One step of an operand, ROWS rows by DEEP (32 or 64) of k, in 16-byte words.  A wave's load fills 1024 neighbouring bytes of
-// LDS, so the words are permuted where they are read from memory.  KC: k is contiguous, a line is a row, of eight
-// words; else a line is a k, of ROWS / 8.
+// One step of an operand on its way to LDS, in the words of linear_step.h.  The buffer's own bounds are of no use for what
+// lies behind an operand (they hold for one length only, while lines of a step end in different places): a word is read
+// where its row and its k are inside.
 template <int ROWS, int DEEP, bool KC, int WAVES>
-struct Direct {
-  static constexpr int words = DEEP * ROWS / 8, loads = words / 64 / WAVES, perLine = KC ? DEEP / 8 : ROWS / 8;
-  static constexpr int bytes = words * 16;
-  static_assert(loads * 64 * WAVES == words, "whole loads");
-  unsigned at[loads];  // of each load's word: bytes from the step's first
-  int k[loads];        // its k
-
-  // which word lies where: KC: so that 16 rows of one k take all places of 256 bytes; else four k and two halves of
-  // a fragment do
-  static __device__ __forceinline__ int permuted(int line, int word) {
-    if (KC) return word ^ (DEEP == 64 ? line / 2 % 8 : line / 4 % 4);
-    return word ^ ((line % 4 + line / 8 % 2 * 4) * 2);
-  }
-
-  const char* base;  // the next step's first word
-  long advance;      // bytes from a step to the next
-  int size;          // of a step, from its first word to the end of its last
+struct Direct : StepWords<ROWS, DEEP, KC, WAVES> {
+  typedef StepWords<ROWS, DEEP, KC, WAVES> Places;
+  using Places::loads, Places::permuted;
+  typename Places::Word word[loads];  // of each load
+  const char* base;                   // the next step's first word
+  long advance;                       // bytes from a step to the next
 
   // rows: from the tile's first, inside
   __device__ __forceinline__ void setup(const void* first, long step, long rows) {
 #pragma unroll
-    for (int i = 0; i < loads; ++i) {
-      const int place = ((int)threadIdx.x / 64 * loads + i) * 64 + threadIdx.x % 64, line = place / perLine;
-      const int word = permuted(line, place % perLine);
-      at[i] = (unsigned)(line * step + word * 8) * 2;
-      k[i] = KC ? word * 8 : line;
-    }
-    const long inside = min(rows, (long)ROWS);
+    for (int i = 0; i < loads; ++i) word[i] = Places::wordOf(threadIdx.x, i, step, rows);
     base = static_cast<const char*>(first);
     advance = KC ? DEEP * 2 : DEEP * 2 * step;
-    size = (int)((KC ? (inside - 1) * step + DEEP : (DEEP - 1) * step + inside) * 2);
   }
 
-  // Load i of the next step, of which `left` k are inside (perhaps none): words behind them, and rows behind the last,
-  // read as zeros.
+  // Load i of the next step, of which `left` k are inside (perhaps none): what is not inside reads as zeros.
   __device__ __forceinline__ void load(int i, int left, char* space) const {
-    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, size, 0x00020000);
+    const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, kReach, 0x00020000);
     char* const to = space + (threadIdx.x / 64 * loads + i) * 1024;
-    const unsigned place = k[i] >= left ? 0x80000000u : at[i];
+    const unsigned place = Places::placeOf(word[i], left);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsAddress)to, 16, place, 0, 0, 0);
   }
 

@@ -156,3 +156,14 @@ def test_python_wrappers_refuse():
         F.array(torch.zeros((1,) * 6))
     with pytest.raises(TypeError):
         F.linear_workspace(0, 1, 1, 1, torch.float64)
+
+
+def test_words_that_products_read_lie_in_their_operands():
+    """tests/cpp/linear_check.cpp: every word that a product of 16-bit operands moves straight to LDS
+    (fbcuda_amd/csrc/linear_step.h) over ragged rows and k, both layouts and ranges of k."""
+    import os
+    import subprocess
+    at = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
+    subprocess.check_call(["make", "-C", at, "-B", "linear_check"], stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    out = subprocess.run([os.path.join(at, "linear_check")], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.strip() == "OK", out.stdout
