@@ -708,15 +708,16 @@ constexpr long kBiasRows = 32, kBiasFew = 64;
 inline long biasRows(long M) { return M <= kBiasFew ? std::max(M, 1L) : kBiasRows; }
 
 // dz = dy activation'(z), dense, and its columns' sums over `rows` rows each, or, of all rows, the bias's gradient.  A
-// workgroup: 32 words of VEC columns, eight rows of lanes.
+// workgroup: 32 words of VEC columns, eight rows of lanes.  (All workgroups along x, `across` of them to a part of the
+// rows: the other axes count to 65535 only, which parts of 32 rows pass at 2097121 rows.)
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z, T* dz, float* parts, Line bias, long M, long N,
-                                                             int activation, long rows) {
+                                                             int activation, long rows, int across) {
   typedef typename Pack<T, VEC>::type Word;
   constexpr int AHEAD = 4;
   __shared__ float sums[8][32 * VEC];
-  const int column = threadIdx.x % 32, r = threadIdx.x / 32;
-  const long first = ((long)blockIdx.x * 32 + column) * VEC, m0 = blockIdx.y * rows, end = min(m0 + rows, M);
+  const int column = threadIdx.x % 32, r = threadIdx.x / 32, part = blockIdx.x / across, block = blockIdx.x - part * across;
+  const long first = ((long)block * 32 + column) * VEC, m0 = part * rows, end = min(m0 + rows, M);
   // (the last word of a row ends with it, and repeats what the one before it has: N is no less than a word)
   const long n = min(first, N - VEC);
   const int repeats = (int)min(first - n, (long)VEC);
@@ -761,13 +762,13 @@ __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z
     if (j >= repeats) sums[r][column * VEC + j - repeats] = sum[j];
   __syncthreads();
   for (int i = threadIdx.x; i < 32 * VEC; i += 256) {
-    const long at = (long)blockIdx.x * 32 * VEC + i;
+    const long at = (long)block * 32 * VEC + i;
     if (at >= N) continue;
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) v += sums[q][i];
     if (parts)
-      parts[blockIdx.y * N + at] = v;
+      parts[part * N + at] = v;
     else
       storeAny(bias.data, bias.type, at * bias.stride, v);
   }
@@ -936,14 +937,15 @@ int backward(const LinearProblem& p, hipStream_t s) {
   if (p.M > 0 && p.N > 0 && (apart || p.gradBias.data)) {
     constexpr int W = 16 / sizeof(T);
     const bool words = p.N >= W && p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
-    const dim3 grid((unsigned)ceilDivLong(p.N, 32 * (words ? W : 1)), (unsigned)chunks);
+    const int across = (int)ceilDivLong(p.N, 32 * (words ? W : 1));
+    const dim3 grid((unsigned)(across * chunks));
     T* const to = apart ? static_cast<T*>(dz.data) : nullptr;
     float* const sums = p.gradBias.data && chunks > 1 ? parts : nullptr;
     const Line bias = chunks > 1 ? Line{} : p.gradBias;
     if (words)
-      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M));
+      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), across);
     else
-      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M));
+      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), across);
   }
   if (p.gradBias.data && p.N > 0 && chunks != 1)
     biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 8)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);

@@ -229,3 +229,11 @@ def test_offsets_past_32_bits():
     x.copy_(randn(gen, 40, 64).to(dev()))
     check_forward(x, w, None, None, "none")
     del store
+
+
+@pytest.mark.parametrize("name", ["none", "silu"])
+@pytest.mark.parametrize("m", [65535 * 32, 65535 * 32 + 1])
+def test_backward_of_many_rows(m, name):
+    """Parts of 32 rows, as many as 16 bits count and one more: the pixels of 32 images of 256 x 256 are that many rows."""
+    x, w, bias, r, gy = make(m, 8, 16, torch.bfloat16, 11)
+    check_backward(x, w, gy, r, name)
