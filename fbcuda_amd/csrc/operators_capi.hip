@@ -170,6 +170,9 @@ extern "C" int fbfft_linear_bprop(const fbfft_array* input, const fbfft_array* w
   if (preactivation && !okMatrix(preactivation, M, N, type)) return FBFFT_UNSUPPORTED_DIMENSION;
   if (!okLine(gradBias, N)) return FBFFT_UNSUPPORTED_DIMENSION;
   if (!okLinearSize(M) || !okLinearSize(N) || !okLinearSize(K)) return FBFFT_UNSUPPORTED_SIZE;
+  // (an operand that is not given has not been checked, and no size of a workspace stands for such products: 0 is that of
+  // calls that need none)
+  if (M * K > kMost || N * K > kMost) return FBFFT_UNSUPPORTED_SIZE;
   if (!okWorkspace(workspace, workspaceBytes, fbfft_linear_workspace(1, M, K, N, type))) return FBFFT_UNSUPPORTED_DIMENSION;
   LinearProblem p{};
   p.x = matrixOf(input), p.w = matrixOf(weight), p.dy = matrixOf(gradOutput), p.z = matrixOf(preactivation);

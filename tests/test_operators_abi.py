@@ -103,6 +103,15 @@ def test_linear_backward_refuses(change, code):
     assert linear_back(**change) == code
 
 
+@pytest.mark.parametrize("change", [
+    dict(x=None, w=arr(1, 4000000), g=arr(4000000, 1), gx=None, gw=None, gb=arr(1)),
+    dict(x=arr(100, 4000000), w=None, g=arr(100, 400000), gx=None, gw=None, gb=arr(400000))])
+def test_linear_backward_refuses_products_that_no_workspace_is_made_for(change):
+    """gradBias alone: M K or N K, of an operand that is not given, above 2^40.  The workspace's size is 0 there, and a call
+    without one would take address 0 for it."""
+    assert linear_back(ws=None, size=0, **change) == 1
+
+
 def test_linear_of_nothing():
     assert linear(x=arr(0, 6), y=arr(0, 5), ws=None, size=0) == 0
     assert linear(w=arr(0, 6), y=arr(4, 0), ws=None, size=0) == 0
