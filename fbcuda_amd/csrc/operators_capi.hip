@@ -129,8 +129,8 @@ extern "C" size_t fbfft_linear_workspace(int pass, long long M, long long K, lon
 }
 
 namespace {
-// tiles are counted in 16 bits along the rows of a result and in 31 bits along its columns
-bool okLinearSize(long long n) { return n <= 65535ll * 64; }
+// (rows and columns by their number; what a launch can hold of their product is checked with the launch)
+bool okLinearSize(long long n) { return n < 1ll << 23; }
 }  // namespace
 
 extern "C" int fbfft_linear_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,

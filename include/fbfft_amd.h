@@ -383,6 +383,7 @@ int fbfft_group_norm_bprop(const fbfft_array* input, const fbfft_array* weight, 
  * input [M][K], weight [N][K], residual, preactivation, output [M][N], all of one type; bias [N] of any
  * type.  bias, residual: NULL for none.  preactivation: z, rounded, for the backward pass, or NULL; output is
  * computed from z before that rounding.  residual may be output itself; no other operand may overlap it.
+ * M and N are below 2^23 (8388608, 128 images of 256 x 256 pixels as rows).
  * K = 0 gives activation(bias) + residual.  float32 operands are multiplied as three bf16 pieces each,
  * in six products that leave out less than 2^-21 of a product, 2^-24 on average; a value that is not finite reaches every
  * result that it is a factor of, as infinity or NaN.
@@ -397,7 +398,8 @@ int fbfft_linear_fprop(const fbfft_array* input, const fbfft_array* weight, cons
  * preactivation: NULL where activation is none.  Any of the three gradients is NULL where it is not wanted, and
  * weight without gradInput and input without gradWeight may be NULL; all are overwritten.  Between dz and the two
  * products stands one rounding to the operands' type, which the matrix instructions take; gradBias sums dz before
- * it.  Reproducible bit for bit.  workspace: fbfft_linear_workspace(1, ...). */
+ * it.  M, N and K are below 2^23, M K and N K at most 2^40.  Reproducible bit for bit.  workspace:
+ * fbfft_linear_workspace(1, ...). */
 int fbfft_linear_bprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* gradOutput,
                        const fbfft_array* preactivation, const fbfft_array* gradInput, const fbfft_array* gradWeight,
                        const fbfft_array* gradBias, int activation, void* workspace, size_t workspaceBytes,

@@ -231,6 +231,13 @@ def test_offsets_past_32_bits():
     del store
 
 
+def test_rows_of_64_images_of_256_by_256():
+    m, k, n = 1 << 22, 16, 16
+    x, w, bias, r, gy = make(m, k, n, torch.bfloat16, 12)
+    check_forward(x, w, bias, None, "relu")
+    check_backward(x, w, gy, r, "relu")
+
+
 @pytest.mark.parametrize("name", ["none", "silu"])
 @pytest.mark.parametrize("m", [65535 * 32, 65535 * 32 + 1])
 def test_backward_of_many_rows(m, name):
