@@ -691,14 +691,25 @@ __global__ __launch_bounds__(256) void joinRanges(Epilogue e, long M, long N, in
   static_cast<T*>(e.out.data)[m * e.out.row + n * e.out.col] = (T)z;
 }
 
+// How the sums of `ranges` ranges become results: words of eight, or a lane or eight to a result.
+struct JoinPlan {
+  int kind;  // 0: words; 1, 8: joinRanges' groups
+  long blocks;
+};
+JoinPlan joinOf(bool dense, long M, long N, long ranges) {
+  if (N % 8 == 0 && dense && M * N >= 1 << 18) return {0, (M * (N / 8) + 255) / 256};
+  return ranges < 8 ? JoinPlan{1, (M * N + 255) / 256} : JoinPlan{8, (M * N + 31) / 32};
+}
+
 template <class T>
-void launchJoin(const Epilogue& e, long M, long N, int ranges, hipStream_t s) {
-  if (N % 8 == 0 && e.dense && M * N >= 1 << 18)
-    joinWords<T><<<dim3((unsigned)((M * (N / 8) + 255) / 256)), 256, 0, s>>>(e, M, N, ranges);
-  else if (ranges < 8)
-    joinRanges<T, 1><<<dim3((unsigned)((M * N + 255) / 256)), 256, 0, s>>>(e, M, N, ranges);
+void launchJoin(const JoinPlan& plan, const Epilogue& e, long M, long N, int ranges, hipStream_t s) {
+  const dim3 grid((unsigned)plan.blocks);
+  if (plan.kind == 0)
+    joinWords<T><<<grid, 256, 0, s>>>(e, M, N, ranges);
+  else if (plan.kind == 1)
+    joinRanges<T, 1><<<grid, 256, 0, s>>>(e, M, N, ranges);
   else
-    joinRanges<T, 8><<<dim3((unsigned)((M * N + 31) / 32)), 256, 0, s>>>(e, M, N, ranges);
+    joinRanges<T, 8><<<grid, 256, 0, s>>>(e, M, N, ranges);
 }
 
 // Rows of dz that a workgroup sums: all of a few, whose sums are then the bias's gradient (60 x 64 x 128 f32: all three
@@ -862,9 +873,8 @@ size_t partsBytes(long M, long N, long K, int type) {
 }
 
 template <class T, bool AK, bool BK>
-void launchProduct(const ProductPlan& plan, const ProductArgs& g, hipStream_t s) {
-  const long tiles = ceilDivLong(g.M, plan.rows) * ceilDivLong(g.N, plan.cols);
-  const dim3 grid((unsigned)((tiles + 7) / 8 * 8), (unsigned)plan.ranges);
+void launchProduct(const ProductPlan& plan, long blocks, const ProductArgs& g, hipStream_t s) {
+  const dim3 grid((unsigned)blocks, (unsigned)plan.ranges);
   if constexpr (sizeof(T) == 2) {
     if (plan.kind == ProductPlan::Straight) {
       constexpr int DEEP = AK && BK ? 64 : 32, DEPTH = 128 / DEEP;
@@ -883,43 +893,68 @@ void launchProduct(const ProductPlan& plan, const ProductArgs& g, hipStream_t s)
     product<T, AK, BK, 64, 64, 32, 32><<<grid, 256, 0, s>>>(g);
 }
 
+// A product and the launches that it takes, known before anything is enqueued.
 template <class T>
-int multiplyAll(const Matrix& a, const Matrix& b, long M, long N, long K, Epilogue e, float* parts, hipStream_t s) {
-  e.dense = e.out.col == 1 && (!e.residual.data || e.residual.col == 1) && (!e.z.data || e.z.col == 1);
-  if (K == 0) {
-    launchJoin<T>(e, M, N, 0, s);
+struct Product {
+  Matrix a, b;
+  long M, N, K;
+  Epilogue e;
+  bool few;          // few rows, straight from memory
+  ProductPlan plan;  // else (K = 0: of no ranges)
+  JoinPlan join;
+  long blocks;
+
+  Product(const Matrix& a, const Matrix& b, long M, long N, long K, const Epilogue& epilogue)
+      : a(a), b(b), M(M), N(N), K(K), e(epilogue), few(false), plan{}, join{}, blocks(0) {
+    e.dense = e.out.col == 1 && (!e.residual.data || e.residual.col == 1) && (!e.z.data || e.z.col == 1);
+    few = K > 0 && M <= kFew && a.col == 1 && b.col == 1;
+    if (few) {
+      blocks = ceilDivLong(N, 16);
+      return;
+    }
+    if (K > 0) {
+      plan = planOf<T>(M, N, K, sizeof(T) == 2 && goesStraight(a, M, K) && goesStraight(b, N, K));
+      blocks = (ceilDivLong(M, plan.rows) * ceilDivLong(N, plan.cols) + 7) / 8 * 8;
+    }
+    if (plan.ranges != 1) join = joinOf(e.dense, M, N, plan.ranges);
+  }
+
+  // (as many waves as there are steps of k for)
+  int fewLanes() const { return K <= 2048 ? 512 : 1024; }
+  bool fits() const {
+    return launches(blocks, few ? fewLanes() : plan.kind == ProductPlan::Straight ? 512 : 256) && launches(join.blocks, 256);
+  }
+
+  int run(float* parts, hipStream_t s) const {
+    ProductArgs g{a, b, M, N, K, few ? K : plan.range, e};
+    if (few) {
+      if (K <= 2048)
+        fewRows<T, 8><<<dim3((unsigned)blocks), 512, 0, s>>>(g);
+      else
+        fewRows<T, 16><<<dim3((unsigned)blocks), 1024, 0, s>>>(g);
+      return launchStatus();
+    }
+    if (plan.ranges > 1) g.e.parts = parts;
+    if (K > 0) {
+      const bool ak = contiguousK(a), bk = contiguousK(b);
+      if (ak && bk)
+        launchProduct<T, true, true>(plan, blocks, g, s);
+      else if (ak)
+        launchProduct<T, true, false>(plan, blocks, g, s);
+      else if (bk)
+        launchProduct<T, false, true>(plan, blocks, g, s);
+      else
+        launchProduct<T, false, false>(plan, blocks, g, s);
+    }
+    if (plan.ranges != 1) launchJoin<T>(join, g.e, M, N, (int)plan.ranges, s);
     return launchStatus();
   }
-  const bool ak = contiguousK(a), bk = contiguousK(b);
-  if (M <= kFew && a.col == 1 && b.col == 1) {
-    // (as many waves as there are steps of k for)
-    const ProductArgs g{a, b, M, N, K, K, e};
-    const dim3 tiles((unsigned)ceilDivLong(N, 16));
-    if (K <= 2048)
-      fewRows<T, 8><<<tiles, 512, 0, s>>>(g);
-    else
-      fewRows<T, 16><<<tiles, 1024, 0, s>>>(g);
-    return launchStatus();
-  }
-  const ProductPlan plan = planOf<T>(M, N, K, sizeof(T) == 2 && goesStraight(a, M, K) && goesStraight(b, N, K));
-  ProductArgs g{a, b, M, N, K, plan.range, e};
-  if (plan.ranges > 1) g.e.parts = parts;
-  if (ak && bk)
-    launchProduct<T, true, true>(plan, g, s);
-  else if (ak)
-    launchProduct<T, true, false>(plan, g, s);
-  else if (bk)
-    launchProduct<T, false, true>(plan, g, s);
-  else
-    launchProduct<T, false, false>(plan, g, s);
-  if (plan.ranges > 1) launchJoin<T>(g.e, M, N, (int)plan.ranges, s);
-  return launchStatus();
-}
+};
 
 template <class T>
 int forward(const LinearProblem& p, hipStream_t s) {
-  Epilogue e{p.y, p.residual, p.z, p.bias, p.activation, false, nullptr};
-  return multiplyAll<T>(p.x, p.w, p.M, p.N, p.K, e, static_cast<float*>(p.workspace), s);
+  const Product<T> y(p.x, p.w, p.M, p.N, p.K, Epilogue{p.y, p.residual, p.z, p.bias, p.activation, false, nullptr});
+  return y.fits() ? y.run(static_cast<float*>(p.workspace), s) : FBFFT_UNSUPPORTED_SIZE;
 }
 
 template <class T>
@@ -934,28 +969,31 @@ int backward(const LinearProblem& p, hipStream_t s) {
     if (apart) dz = Matrix{space, p.N, 1};
     space += rounded((size_t)p.M * p.N * sizeof(T));
   }
-  if (p.M > 0 && p.N > 0 && (apart || p.gradBias.data)) {
-    constexpr int W = 16 / sizeof(T);
-    const bool words = p.N >= W && p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
-    const int across = (int)ceilDivLong(p.N, 32 * (words ? W : 1));
+  constexpr int W = 16 / sizeof(T);
+  const bool words = p.N >= W && p.dy.col == 1 && (p.activation == FBFFT_ACTIVATION_NONE || p.z.col == 1);
+  const long across = ceilDivLong(p.N, 32 * (words ? W : 1));
+  const bool first = p.M > 0 && p.N > 0 && (apart || p.gradBias.data), hasX = p.dx.data && p.M > 0 && p.K > 0;
+  const bool hasW = p.dw.data && p.N > 0 && p.K > 0, hasBias = p.gradBias.data && p.N > 0 && chunks != 1;
+  const Product<T> dx(dz, Matrix{p.w.data, p.w.col, p.w.row}, p.M, p.K, p.N, Epilogue{p.dx, {}, {}, {}, 0, false, nullptr});
+  const Product<T> dw(Matrix{dz.data, dz.col, dz.row}, Matrix{p.x.data, p.x.col, p.x.row}, p.N, p.K, p.M,
+                      Epilogue{p.dw, {}, {}, {}, 0, false, nullptr});
+  if ((first && !launches(across * chunks, 256)) || (hasBias && !launches(ceilDivLong(p.N, 8), 256)) || (hasX && !dx.fits()) ||
+      (hasW && !dw.fits()))
+    return FBFFT_UNSUPPORTED_SIZE;
+  if (first) {
     const dim3 grid((unsigned)(across * chunks));
     T* const to = apart ? static_cast<T*>(dz.data) : nullptr;
     float* const sums = p.gradBias.data && chunks > 1 ? parts : nullptr;
     const Line bias = chunks > 1 ? Line{} : p.gradBias;
     if (words)
-      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), across);
+      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), (int)across);
     else
-      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), across);
+      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), (int)across);
   }
-  if (p.gradBias.data && p.N > 0 && chunks != 1)
-    biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 8)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
+  if (hasBias) biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 8)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
   int rc = launchStatus();
-  if (rc == FBFFT_SUCCESS && p.dx.data && p.M > 0 && p.K > 0)
-    rc = multiplyAll<T>(dz, Matrix{p.w.data, p.w.col, p.w.row}, p.M, p.K, p.N, Epilogue{p.dx, {}, {}, {}, 0, false, nullptr},
-                        reinterpret_cast<float*>(space), s);
-  if (rc == FBFFT_SUCCESS && p.dw.data && p.N > 0 && p.K > 0)
-    rc = multiplyAll<T>(Matrix{dz.data, dz.col, dz.row}, Matrix{p.x.data, p.x.col, p.x.row}, p.N, p.K, p.M,
-                        Epilogue{p.dw, {}, {}, {}, 0, false, nullptr}, reinterpret_cast<float*>(space), s);
+  if (rc == FBFFT_SUCCESS && hasX) rc = dx.run(reinterpret_cast<float*>(space), s);
+  if (rc == FBFFT_SUCCESS && hasW) rc = dw.run(reinterpret_cast<float*>(space), s);
   return rc;
 }
 

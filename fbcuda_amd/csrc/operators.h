@@ -60,6 +60,9 @@ __device__ __forceinline__ void leavePack(T* p, const float (&v)[N]) {
 // smaller ones are likely read from there next (32 x 192 x 23 x 23 fp32 13.5 / 9.7, dropout of 19 MB 11.0 / 10.7).
 inline bool streams(double elements, int type) { return elements * (type == FBFFT_FLOAT32 ? 4 : 2) >= (double)(48 << 20); }
 
+// Whether one launch holds so many workgroups: it counts its lanes in 32 bits.
+inline bool launches(double blocks, int lanes) { return blocks * lanes < 4294967296.0; }
+
 // element i of an array of a type that is known at run time
 __device__ __forceinline__ float loadAny(const void* p, int type, long i) {
   if (type == FBFFT_FLOAT32) return static_cast<const float*>(p)[i];

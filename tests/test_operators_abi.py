@@ -112,6 +112,19 @@ def test_linear_backward_refuses_products_that_no_workspace_is_made_for(change):
     assert linear_back(ws=None, size=0, **change) == 1
 
 
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+def test_linear_refuses_what_no_launch_holds(kind):
+    """2^32 lanes and more, known before anything is enqueued (without a GPU, a launch is another error)."""
+    n, most = 1 << 20, 1 << 50  # bytes of a workspace
+    a = lambda *size: arr(*size, kind=kind)  # noqa: E731
+    assert linear(x=a(n, 0), w=a(n, 0), y=a(n, n), size=most) == 1  # results that are the bias's activation
+    assert linear(x=a(n, 1), w=a(n, 1), y=a(n, n), size=most) == 1
+    assert linear(x=a(1 << 19, 4), w=a(n, 4), y=arr(1 << 19, n, kind=kind, stride=(1, 1 << 19)), size=most) == 1
+    assert linear_back(x=None, w=None, g=a(n, n), gx=None, gw=None, gb=arr(n), size=most) == 1
+    assert linear_back(x=None, w=a(1, n), g=a(n, 1), gx=a(n, n), gw=None, gb=None, size=most) == 1
+    assert linear_back(x=a(1, n), w=None, g=a(1, n), gx=None, gw=a(n, n), gb=None, size=most) == 1
+
+
 def test_linear_of_nothing():
     assert linear(x=arr(0, 6), y=arr(0, 5), ws=None, size=0) == 0
     assert linear(w=arr(0, 6), y=arr(4, 0), ws=None, size=0) == 0
