@@ -1291,7 +1291,56 @@ NormArgs argsOf(const NormProblem& p, const NormPlan& plan, bool backward) {
   return a;
 }
 
-unsigned blocksOf(const NormArgs& a) { return (unsigned)(a.B * ((a.C + a.band - 1) / a.band) * a.pieces); }
+long blocksOf(const NormArgs& a) { return a.B * ((a.C + a.band - 1) / a.band) * a.pieces; }
+
+// the parts that planesGradApply cuts a group into, and the words of a lane of each
+struct Parts {
+  long blocks, each;
+};
+Parts partsOf(const NormPlan& plan, const NormArgs& a) {
+  const long words = (a.D * a.P + plan.vec - 1) / plan.vec, each = std::max(1L, std::min(8L, words * a.B * a.G / (256 * 4096)));
+  return {(words + 256 * each - 1) / (256 * each), each};
+}
+
+// Whether each launch of a pass holds its lanes (`before`: workgroups that add up the gradients of weight and bias).
+bool fits(const NormPlan& plan, const NormArgs& a, bool backward, long before) {
+  const double groups = (double)a.B * a.G, planes = (double)a.B * a.C;
+  if (plan.family == Last) {
+    const double total = (double)blocksOf(a);
+    if (plan.items > 0) return launches(total + 8, plan.threads);
+    return launches(total, kFirst) && launches(total / a.pieces * a.cuts + before, 256);
+  }
+  if (plan.family == Any) return launches(groups, kAny) && (!backward || launches((double)a.B * ((a.C + 63) / 64), 256));
+  if (plan.large) return launches(planes * a.pieces, 256) && launches(planes * a.cuts + before, 256);
+  if (backward)
+    return launches(plan.threads == 64 ? (planes * a.pieces + 3) / 4 : planes * a.pieces, 256) &&
+           launches(groups * partsOf(plan, a).blocks + before, 256);
+  if (plan.items == 0) return launches(groups * a.pieces, 256);
+  return plan.threads == 64 ? launches((groups + 3) / 4, 256) : launches(groups, plan.threads);
+}
+
+// images `first` ... `first` + count - 1 of a problem
+NormProblem imagesOf(NormProblem p, long first, long count) {
+  const long size = p.type == FBFFT_FLOAT32 ? 4 : 2;
+  for (Image* i : {&p.x, &p.y, &p.g})
+    if (i->data) i->data = static_cast<char*>(i->data) + first * i->b * size;
+  if (p.mean) p.mean += first * p.meanB;
+  if (p.rstd) p.rstd += first * p.rstdB;
+  p.B = count;
+  return p;
+}
+
+// How many images go into one set of launches where all of them do not: of 2^22 and more planes or groups, whose lanes pass
+// what a launch holds.  0: not even one.
+long imagesAtOnce(const NormProblem& p, bool backward, long before) {
+  for (long images = p.B; images > 1;) {
+    images = (images + 1) / 2;
+    const NormProblem q = imagesOf(p, 0, images);
+    const NormPlan plan = planOf(q, backward);
+    if (fits(plan, argsOf(q, plan, backward), backward, before)) return images;
+  }
+  return 0;
+}
 
 template <class T, int VEC, bool S>
 int forwardLast(const NormPlan& plan, const NormArgs& a, hipStream_t s) {
@@ -1365,18 +1414,14 @@ bool backwardPlanes(const NormPlan& plan, const NormArgs& a, int before, hipStre
     planeGradApply<T, VEC, S><<<dim3((unsigned)(a.B * a.C * a.cuts + before)), 256, 0, s>>>(a, before);
     return true;
   }
-  const long words = (a.D * a.P + VEC - 1) / VEC, each = std::max(1L, std::min(8L, words * a.B * a.G / (256 * 4096)));
-  const long blocks = (words + 256 * each - 1) / (256 * each);
-  planesGradApply<T, VEC, S><<<dim3((unsigned)(a.B * a.G * blocks + before)), 256, 0, s>>>(a, blocks, (int)each, before);
+  const Parts parts = partsOf(plan, a);
+  planesGradApply<T, VEC, S><<<dim3((unsigned)(a.B * a.G * parts.blocks + before)), 256, 0, s>>>(a, parts.blocks, (int)parts.each, before);
   return true;
 }
 
 template <class T>
-int forward(const NormProblem& p, hipStream_t s) {
+int forwardImages(const NormPlan& plan, const NormArgs& a, bool stream, hipStream_t s) {
   constexpr int W = 16 / sizeof(T);
-  const NormPlan plan = planOf(p, false);
-  const NormArgs a = argsOf(p, plan, false);
-  const bool stream = streams((double)p.B * p.C * a.P, p.type);
   if (plan.family == Planes) {
     if (plan.vec == 1) return forwardPlanes<T, 1, false>(plan, a, s);
     return stream ? forwardPlanes<T, W, true>(plan, a, s) : forwardPlanes<T, W, false>(plan, a, s);
@@ -1391,11 +1436,47 @@ int forward(const NormProblem& p, hipStream_t s) {
 }
 
 template <class T>
-int backward(const NormProblem& p, hipStream_t s) {
+int forward(const NormProblem& p, hipStream_t s) {
+  const NormPlan plan = planOf(p, false);
+  const NormArgs a = argsOf(p, plan, false);
+  const bool stream = streams((double)p.B * p.C * a.P, p.type);
+  if (fits(plan, a, false, 0)) return forwardImages<T>(plan, a, stream, s);
+  const long images = imagesAtOnce(p, false, 0);
+  if (images == 0) return FBFFT_UNSUPPORTED_SIZE;
+  int rc = FBFFT_SUCCESS;
+  for (long first = 0; first < p.B && rc == FBFFT_SUCCESS; first += images) {
+    const NormProblem q = imagesOf(p, first, std::min(images, p.B - first));
+    const NormPlan part = planOf(q, false);
+    rc = forwardImages<T>(part, argsOf(q, part, false), stream, s);
+  }
+  return rc;
+}
+
+// (whether the gradients of weight and bias are done, by `before` workgroups)
+template <class T>
+bool backwardImages(const NormPlan& plan, const NormArgs& a, int before, bool stream, hipStream_t s) {
   constexpr int W = 16 / sizeof(T);
+  if (plan.family == Planes) {
+    if (plan.vec == 1) return backwardPlanes<T, 1, false>(plan, a, before, s);
+    return stream ? backwardPlanes<T, W, true>(plan, a, before, s) : backwardPlanes<T, W, false>(plan, a, before, s);
+  }
+  if (plan.family == Last) {
+    if (plan.vec == 1) return backwardLast<T, 1, false>(plan, a, before, s);
+    if (plan.vec == 2) return backwardLast<T, 2, false>(plan, a, before, s);
+    return stream ? backwardLast<T, W, true>(plan, a, before, s) : backwardLast<T, W, false>(plan, a, before, s);
+  }
+  const long blocks = (a.C + 63) / 64;
+  normSumsAny<T><<<dim3((unsigned)(a.B * blocks)), 256, 0, s>>>(a, (int)blocks);
+  if (a.y.data) normGradAny<T><<<dim3((unsigned)(a.B * a.G)), kAny, 0, s>>>(a);
+  return false;
+}
+
+template <class T>
+int backward(const NormProblem& p, hipStream_t s) {
   NormPlan plan{Any};
   NormArgs a = argsOf(p, plan, true);
-  const int parameters = a.gradWeight.data || a.gradBias.data ? (int)((a.C + kParameters - 1) / kParameters) : 0;
+  const long parameters = a.gradWeight.data || a.gradBias.data ? (a.C + kParameters - 1) / kParameters : 0;
+  if (!launches(parameters, 256)) return FBFFT_UNSUPPORTED_SIZE;
   bool done = parameters == 0;
   if (a.B == 0 || a.P == 0) {
     a.B = 0;  // the gradients of weight and bias are sums of nothing
@@ -1403,22 +1484,20 @@ int backward(const NormProblem& p, hipStream_t s) {
     plan = planOf(p, true);
     a = argsOf(p, plan, true);
     const bool stream = streams((double)p.B * p.C * a.P, p.type);
-    if (plan.family == Planes) {
-      if (plan.vec == 1)
-        done |= backwardPlanes<T, 1, false>(plan, a, parameters, s);
-      else
-        done |= stream ? backwardPlanes<T, W, true>(plan, a, parameters, s) : backwardPlanes<T, W, false>(plan, a, parameters, s);
-    } else if (plan.family == Last) {
-      if (plan.vec == 1)
-        done |= backwardLast<T, 1, false>(plan, a, parameters, s);
-      else if (plan.vec == 2)
-        done |= backwardLast<T, 2, false>(plan, a, parameters, s);
-      else
-        done |= stream ? backwardLast<T, W, true>(plan, a, parameters, s) : backwardLast<T, W, false>(plan, a, parameters, s);
+    if (fits(plan, a, true, parameters)) {
+      done |= backwardImages<T>(plan, a, (int)parameters, stream, s);
     } else {
-      const long blocks = (a.C + 63) / 64;
-      normSumsAny<T><<<dim3((unsigned)(a.B * blocks)), 256, 0, s>>>(a, (int)blocks);
-      if (a.y.data) normGradAny<T><<<dim3((unsigned)(a.B * a.G)), kAny, 0, s>>>(a);
+      const long images = imagesAtOnce(p, true, 0);
+      if (images == 0) return FBFFT_UNSUPPORTED_SIZE;
+      a.pieces = 1;  // the channels' sums of one image after the other
+      for (long first = 0; first < p.B; first += images) {
+        const NormProblem q = imagesOf(p, first, std::min(images, p.B - first));
+        NormPlan part = planOf(q, true);
+        part.pieces = 1, part.piece = a.P;
+        NormArgs some = argsOf(q, part, true);
+        some.channels = a.channels + first * a.C;
+        backwardImages<T>(part, some, 0, stream, s);
+      }
     }
   }
   if (!done) normParameters<<<dim3((unsigned)parameters), 256, 0, s>>>(a);

@@ -231,3 +231,61 @@ def test_offsets_past_32_bits():
     x.copy_(v.to(dev()))
     check_forward(x, None, None, 2, "silu", "planes")
     del store
+
+
+def test_forward_of_more_lanes_than_a_launch_holds():
+    """2^24 images whose channels a workgroup takes, and 2^26 groups of a wave each: both pass 2^32 lanes, and go in several
+    launches.  Images do not depend on each other: they have the bits that they have in smaller batches."""
+    for shape, groups, layout in (((1 << 24, 8, 1, 2), 1, "last"), ((1 << 26, 2, 1, 1), 1, "planes")):
+        n = shape[0]
+        gen = torch.Generator(device=dev()).manual_seed(12)
+        dense = torch.randn(n, 1, 2, 8, generator=gen, device=dev(), dtype=torch.float16) if layout == "last" else None
+        x = dense.permute(0, 3, 1, 2) if layout == "last" else torch.randn(shape, generator=gen, device=dev(), dtype=torch.float16)
+        assert x.shape == shape
+        w, b = torch.randn(shape[1], generator=gen, device=dev()), torch.randn(shape[1], generator=gen, device=dev())
+        y, part = torch.full_like(x, 7.0), torch.empty_like(x[:n // 16])
+        stats = [torch.full((n, groups), 7.0, device=dev()) for _ in range(2)]
+        assert F.group_norm_fprop(x, w, b, y, groups, space(0, x, groups), activation="silu", mean=stats[0],
+                                  rstd=stats[1]) == F.Success
+        for k in range(16):
+            inside = slice(k * (n // 16), (k + 1) * (n // 16))
+            few = [torch.empty((n // 16, groups), device=dev()) for _ in range(2)]
+            assert F.group_norm_fprop(x[inside], w, b, part, groups, space(0, part, groups), activation="silu", mean=few[0],
+                                      rstd=few[1]) == F.Success
+            assert torch.equal(y[inside], part)
+            assert torch.equal(stats[0][inside], few[0]) and torch.equal(stats[1][inside], few[1])
+        want, _, _, bound = norm(x[-3:], w, b, groups, 1e-5, "silu")
+        within(y[-3:], want, rounded(want, x.dtype) + bound)
+
+
+@pytest.mark.parametrize("layout", ["planes", "last"])
+def test_backward_of_more_lanes_than_a_launch_holds(layout):
+    """[65536][1024][1][1], a wave to each of 2^26 planes, and 2^24 images of two pixels, channels last: gradInput as in
+    smaller batches, the parameters' gradients from 64-bit sums."""
+    b, c, h, w, groups = (65536, 1024, 1, 1, 8) if layout == "planes" else (1 << 24, 4, 1, 2, 1)
+    gen = torch.Generator(device=dev()).manual_seed(13)
+    x, gy = (torch.randn(b, h, w, c, generator=gen, device=dev(), dtype=torch.float16).permute(0, 3, 1, 2) for _ in range(2))
+    weight, bias = torch.randn(c, generator=gen, device=dev()), torch.randn(c, generator=gen, device=dev())
+    mean, rstd = torch.randn(b, groups, generator=gen, device=dev()), torch.rand(b, groups, generator=gen, device=dev()) + 0.5
+    gx, gw, gb = torch.full_like(x, 7.0), torch.full_like(weight, 7.0), torch.full_like(weight, 7.0)
+    args = (weight, bias, mean, rstd)
+    assert F.group_norm_bprop(x, *args, gy, gx, gw, gb, groups, space(1, x, groups)) == F.Success
+    want, n = torch.zeros(4, c, dtype=torch.float64), b // 16
+    for k in range(16):
+        inside = slice(k * n, (k + 1) * n)
+        part = torch.empty_like(x[inside])
+        assert F.group_norm_bprop(x[inside], weight, bias, mean[inside], rstd[inside], gy[inside], part, None, None, groups,
+                                  space(1, part, groups)) == F.Success
+        assert torch.equal(gx[inside], part)
+        each = lambda v: v[inside].repeat_interleave(c // groups, 1)[:, :, None, None].double()  # noqa: E731
+        dz, xh = gy[inside].double(), (x[inside].double() - each(mean)) * each(rstd)
+        size = gy[inside].double().abs() * (1 + (x[inside].double().abs() + each(mean).abs()) * each(rstd))
+        for i, v in enumerate((dz, dz * xh, dz.abs(), size)):
+            want[i] += v.sum((0, 2, 3)).cpu()
+    # roundings of the terms, and of sums over b h w values in 32 bits: a random walk's share of their number
+    chain = R * (16 + 2 * (b * h * w) ** 0.5)
+    within(gb, want[0], rounded(want[0], torch.float32) + chain * want[2])
+    within(gw, want[1], rounded(want[1], torch.float32) + chain * want[3])
+    one = slice(b - 2, b)
+    (wx, bx), _, _ = norm_grads(x[one], weight, bias, mean[one], rstd[one], gy[one], groups, "none")
+    within(gx[one], wx, rounded(wx, x.dtype) + bx)

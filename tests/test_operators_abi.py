@@ -70,6 +70,15 @@ def test_group_norm_backward_refuses(change, code):
     assert norm_back(**change) == code
 
 
+def test_group_norm_refuses_what_no_launch_holds():
+    """One image of 2^32 lanes and more, known before anything is enqueued (without a GPU, a launch is another error)."""
+    c, most = 1 << 28, 1 << 50
+    x = arr(1, c, 1, 1, kind=F16)
+    assert norm(input=x, output=x, groups=c, size=most) == 1
+    stats = arr(1, c // 2)
+    assert norm_back(input=x, g=x, gi=x, mean=stats, rstd=stats, groups=c // 2, size=most) == 1
+
+
 def test_group_norm_of_nothing():
     assert norm(input=arr(0, 8, 3, 3, data=None), output=arr(0, 8, 3, 3, data=None), ws=None, size=0) == 0
     assert norm(input=arr(2, 8, 0, 3), output=arr(2, 8, 0, 3), ws=None, size=0) == 0
