@@ -147,6 +147,7 @@ void launch(const DropoutArgs& g, bool dense, bool stream, hipStream_t s) {
 }  // namespace
 
 int launchDropout(const DropoutProblem& p, hipStream_t s) {
+  if (!launches((double)((p.total + 2047) / 2048), 256)) return FBFFT_UNSUPPORTED_SIZE;
   DropoutArgs g{};
   g.x = p.x, g.residual = p.residual, g.y = p.y, g.total = p.total;
   std::copy(p.size, p.size + FBFFT_MAX_DIM, g.size);

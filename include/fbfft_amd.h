@@ -413,7 +413,8 @@ int fbfft_linear_bprop(const fbfft_array* input, const fbfft_array* weight, cons
  * whose high 64 bits are offset + (step ? *step : 0); the key is seed.  So the element is kept with the probability
  * 1 - T / 65536 that its factor makes up for.  A dropped element is 0 whatever it holds.  input, residual
  * (or NULL), output: rank 1 to 5, of one type and one shape; output may be either of the others.  step: a device
- * address, or NULL: a captured graph that adds to it draws another mask with every replay.  0 <= p <= 1. */
+ * address, or NULL: a captured graph that adds to it draws another mask with every replay.  0 <= p <= 1.  At most
+ * 2^35 - 2048 elements. */
 int fbfft_dropout_fprop(const fbfft_array* input, const fbfft_array* residual, const fbfft_array* output, double p,
                         unsigned long long seed, unsigned long long offset, const unsigned long long* step,
                         fbfft_stream_t stream);

@@ -156,6 +156,13 @@ def test_dropout_refuses(change, code):
         assert F.lib().fbfft_dropout_bprop(args["x"], args["y"], args["p"], 1, 2, args["step"], None) == code
 
 
+def test_dropout_refuses_what_no_launch_holds():
+    for kind in (F32, F16, BF16):
+        for n in (1 << 35, 1 << 40):
+            assert drop(x=arr(n, kind=kind), y=arr(n, kind=kind)) == 1
+            assert F.lib().fbfft_dropout_bprop(arr(n, kind=kind), arr(n, kind=kind), 0.5, 1, 2, None, None) == 1
+
+
 def test_dropout_of_nothing():
     assert drop(x=arr(0, data=None), y=arr(0, data=None)) == 0
     assert drop(x=arr(3, 0, 2), y=arr(3, 0, 2), p=1.0) == 0
