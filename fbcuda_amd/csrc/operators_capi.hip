@@ -8,6 +8,7 @@ using namespace fbfft_amd;
 namespace {
 
 constexpr long long kMost = 1ll << 40;  // elements of one array
+constexpr long long kMostGroup = (1ll << 31) - (1 << 16);  // values of a group of group norm
 
 bool okArray(const fbfft_array* a, int dim) {
   if (!a || a->dim != dim || a->type < FBFFT_FLOAT32 || a->type > FBFFT_BFLOAT16) return false;
@@ -56,8 +57,9 @@ int checkNorm(const fbfft_array* input, const fbfft_array* weight, const fbfft_a
   const long long C = input->size[1];
   if (groups < 1 || C % groups != 0) return FBFFT_UNSUPPORTED_SIZE;
   if (!okLine(weight, C) || !okLine(bias, C)) return FBFFT_UNSUPPORTED_DIMENSION;
-  // (workgroups count images times channels, and lanes the values of a group in 31 bits)
-  if (input->size[0] * C > 0x7fffffff || C / groups * input->size[2] * input->size[3] > 0x7ffff000) return FBFFT_UNSUPPORTED_SIZE;
+  // (workgroups count images times channels, and lanes the values of a group in 31 bits.  A lane's place runs past a
+  // group's end by less than 2^16: pieces rounded up to words add 2^14, words on their way 14336, rows of lanes 3584)
+  if (input->size[0] * C > 0x7fffffff || C / groups * input->size[2] * input->size[3] > kMostGroup) return FBFFT_UNSUPPORTED_SIZE;
   return FBFFT_SUCCESS;
 }
 

@@ -357,9 +357,10 @@ typedef struct fbfft_array {
  *   mean, var: over the n = D H W values of image b and group g (var divides by n)
  *   z = (input - mean) / sqrt(var + eps) * weight[c] + bias[c],  output = activation(z)
  * weight, bias: [C] of any type, or NULL for 1 and 0.  mean, rstd (= 1 / sqrt(var + eps)): float32
- * [B][groups], written for the backward pass, or NULL.  output may be input itself (same address and
- * strides); any other overlap is not defined.  workspace: fbfft_group_norm_workspace(0, ...) bytes,
- * 256-byte aligned, NULL where that is 0; its contents need not survive. */
+ * [B][groups], written for the backward pass, or NULL.  B C is below 2^31, n at most 2^31 - 2^16.
+ * output may be input itself (same address and strides); any other overlap is not defined.
+ * workspace: fbfft_group_norm_workspace(0, ...) bytes, 256-byte aligned, NULL where that is 0; its
+ * contents need not survive. */
 size_t fbfft_group_norm_workspace(int pass, long long batch, long long channels, long long pixels, long long groups);
 int fbfft_group_norm_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
                            const fbfft_array* output, const fbfft_array* mean, const fbfft_array* rstd,

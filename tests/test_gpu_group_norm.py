@@ -289,3 +289,34 @@ def test_backward_of_more_lanes_than_a_launch_holds(layout):
     one = slice(b - 2, b)
     (wx, bx), _, _ = norm_grads(x[one], weight, bias, mean[one], rstd[one], gy[one], groups, "none")
     within(gx[one], wx, rounded(wx, x.dtype) + bx)
+
+
+def test_the_largest_group():
+    """2^31 - 2^16 values, one plane: places that run past its end stay 31-bit numbers.  The sums of its parts in 64 bits."""
+    n, piece = (1 << 31) - (1 << 16), 1 << 26
+    gen = torch.Generator(device=dev()).manual_seed(14)
+    x, gy = (torch.randn(1, 1, 1, n, generator=gen, device=dev(), dtype=torch.float16) for _ in range(2))
+    w, b = torch.tensor([1.25], device=dev()), torch.tensor([0.5], device=dev())
+    y, mean, rstd = torch.full_like(x, 7.0), torch.empty((1, 1), device=dev()), torch.empty((1, 1), device=dev())
+    assert F.group_norm_fprop(x, w, b, y, 1, space(0, x, 1), mean=mean, rstd=rstd) == F.Success
+    pieces = [slice(k, min(k + piece, n)) for k in range(0, n, piece)]
+    s1 = sum(x[0, 0, 0, p].double().sum() for p in pieces)
+    s2 = sum(x[0, 0, 0, p].double().square().sum() for p in pieces)
+    centre = s1 / n
+    scale = 1 / torch.sqrt(s2 / n - centre ** 2 + 1e-5)
+    within(mean, centre.view(1, 1).cpu(), 4 * R * centre.abs().cpu() + 1e-12)
+    within(rstd, scale.view(1, 1).cpu(), 8 * R * scale.cpu())
+    gx, gw, gb = gy.clone(), torch.empty_like(w), torch.empty_like(b)
+    assert F.group_norm_bprop(x, w, b, mean, rstd, gx, gx, gw, gb, 1, space(1, x, 1)) == F.Success
+    m, r = mean.double().item(), rstd.double().item()
+    of = lambda p: (gy[0, 0, 0, p].double(), (x[0, 0, 0, p].double() - m) * r)  # noqa: E731
+    total = [sum(float(v.sum()) for v in parts) for parts in zip(*((g, g * xh, g.abs(), (g * xh).abs()) for g, xh in map(of, pieces)))]
+    chain = R * (16 + 2 * n ** 0.5)
+    within(gb, torch.tensor([total[0]]), torch.tensor([chain * total[2]]))
+    within(gw, torch.tensor([total[1]]), torch.tensor([chain * total[3]]))
+    for p in (slice(0, 1 << 16), slice(n // 2, n // 2 + (1 << 16)), slice(n - (1 << 16), n)):
+        g, xh = of(p)
+        want = (x[0, 0, 0, p].double() - centre) * scale * 1.25 + 0.5
+        within(y[0, 0, 0, p], want.cpu(), (rounded(want, x.dtype) + 16 * R * (want.abs() + 1)).cpu())
+        want = r * 1.25 * (g - total[0] / n - xh * total[1] / n)
+        within(gx[0, 0, 0, p], want.cpu(), (rounded(want, x.dtype) + 32 * R * (g.abs() + xh.abs() + 1)).cpu())

@@ -79,6 +79,15 @@ def test_group_norm_refuses_what_no_launch_holds():
     assert norm_back(input=x, g=x, gi=x, mean=stats, rstd=stats, groups=c // 2, size=most) == 1
 
 
+@pytest.mark.parametrize("size", [(1, 1, 1, 0x7fff0001), (1, 1, 1, 0x7ffff000), (1, 3, 1, 0x7ffffff // 3 * 16)])
+def test_group_norm_refuses_groups_whose_ends_31_bits_do_not_pass(size):
+    """A lane steps past the end of its group by up to 14336 values and more before it compares: of a group of 2^31 - 4096
+    its 32-bit place would come out negative, in front of the group."""
+    x, most = arr(*size, kind=F16), 1 << 50
+    assert norm(input=x, output=x, groups=1, size=most) == 1
+    assert norm_back(input=x, g=x, gi=x, mean=arr(1, 1), rstd=arr(1, 1), groups=1, size=most) == 1
+
+
 def test_group_norm_of_nothing():
     assert norm(input=arr(0, 8, 3, 3, data=None), output=arr(0, 8, 3, 3, data=None), ws=None, size=0) == 0
     assert norm(input=arr(2, 8, 0, 3), output=arr(2, 8, 0, 3), ws=None, size=0) == 0
