@@ -235,12 +235,11 @@ struct Channel {
       shift[j] = p.y;
     }
   }
-  // The activation's arguments in the place of x.  16-bit results take one multiply-add: what it loses to the mean's
-  // size, 2^-24 mean / deviation, is below their rounding (and that of x, whose bits the mean's size takes, too).
-  template <class T>
+  // The activation's arguments in the place of x.  (One multiply-add of x by rstd w would round at the size of mean rstd w,
+  // which in a group of nearly constant values is far above the result: 0.5 at 30000.)
   __device__ __forceinline__ void apply(float (&x)[VEC]) const {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = sizeof(T) == 4 ? affine((x[j] - mean[j]) * rstd[j], w[j], shift[j]) : __builtin_fmaf(x[j], rstd[j] * w[j], __builtin_fmaf(-mean[j], rstd[j] * w[j], shift[j]));
+    for (int j = 0; j < VEC; ++j) x[j] = affine((x[j] - mean[j]) * rstd[j], w[j], shift[j]);
   }
   // x is replaced by the normalised values, z by the activation's arguments
   __device__ __forceinline__ void arguments(float (&x)[VEC], float (&z)[VEC]) const {
@@ -355,7 +354,7 @@ __global__ __launch_bounds__(NT) void lastForward(NormArgs a, int total) {
     if (p >= P) break;
     float v[VEC];
     unpack(raw[i], v);
-    ch.template apply<T>(v);
+    ch.apply(v);
     activateAll(v, a.activation);
     leavePack<STREAM, T, VEC>(y + pixelAt(a, a.y, p), v);
   }
@@ -447,7 +446,7 @@ __global__ __launch_bounds__(256) void lastApply(NormArgs a) {
       if (p + k * x.rows < x.end) {
         float v[VEC];
         unpack(x.now[k], v);
-        ch.template apply<T>(v);
+        ch.apply(v);
         activateAll(v, a.activation);
         leavePack<STREAM, T, VEC>(y + pixelAt(a, a.y, p + k * x.rows), v);
       }

@@ -4,7 +4,7 @@ import torch
 
 import fbcuda_amd as F
 from gpu_util import dev
-from operators_util import ACTS, NAMES, R, TYPES, norm, norm_grads, randn, rounded, within
+from operators_util import ACTS, NAMES, R, TYPES, act, norm, norm_grads, randn, rounded, within
 
 pytestmark = pytest.mark.gpu
 
@@ -320,3 +320,54 @@ def test_the_largest_group():
         within(y[0, 0, 0, p], want.cpu(), (rounded(want, x.dtype) + 16 * R * (want.abs() + 1)).cpu())
         want = r * 1.25 * (g - total[0] / n - xh * total[1] / n)
         within(gx[0, 0, 0, p], want.cpu(), (rounded(want, x.dtype) + 32 * R * (g.abs() + xh.abs() + 1)).cpu())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("layout", ["last", "planes", "slice"])
+@pytest.mark.parametrize("side", [4, 180])
+def test_constant_groups_are_the_biases_activation(layout, side, dtype):
+    """x - mean is 0 whatever the values' size and the deviation's (1 / sqrt(eps) = 316 stands for it): nothing of the mean is
+    left, in any type, on the path in registers and in two launches.  And both passes agree on what a ReLU lets through."""
+    gen = torch.Generator().manual_seed(15)
+    v = torch.empty(4, 16, side, side, dtype=torch.float64)
+    for image, values in enumerate([(3.0, -7.0), (100.0, 0.25), (1000.0, 1008.0), (30000.0, -512.0)]):
+        v[image, :8], v[image, 8:] = values
+    x = images(v, dtype, layout)
+    assert torch.equal(x.cpu().double(), v.to(dtype).double())
+    weight, bias = randn(gen, 16, std=0.3, mean=1.0), randn(gen, 16, std=0.3)
+    bias[::3] = 0.0
+    weight, bias = weight.float().to(dev()), bias.float().to(dev())
+    ones = images(torch.ones_like(v), dtype, layout)
+    for name in ACTS:
+        y, mean, rstd = torch.full_like(x, 7.0), torch.empty((4, 2), device=dev()), torch.empty((4, 2), device=dev())
+        assert F.group_norm_fprop(x, weight, bias, y, 2, space(0, x, 2), activation=name, mean=mean, rstd=rstd) == F.Success
+        z = bias.cpu().double()[None, :, None, None].expand_as(v)
+        want = act(z, name)
+        within(y, want, rounded(want, dtype) + 8 * R * (1 + z.abs()) * (name != "none"))
+        if name == "relu":
+            gx, gw, gb = torch.empty_like(x), torch.empty_like(weight), torch.empty_like(bias)
+            assert F.group_norm_bprop(x, weight, bias, mean, rstd, ones, gx, gw, gb, 2, space(1, x, 2),
+                                      activation=name) == F.Success
+            assert torch.equal(gb.cpu(), (y > 0).sum((0, 2, 3)).float().cpu())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("layout", ["last", "planes"])
+@pytest.mark.parametrize("side", [12, 160])
+def test_means_far_above_the_deviation(layout, side, dtype):
+    """Values of a few neighbouring numbers of their type around 1000 and -30000: what the mean's own rounding costs, and no
+    more than that, is allowed."""
+    gen = torch.Generator().manual_seed(16)
+    step = 1000 * torch.finfo(dtype).eps
+    v = randn(gen, 2, 16, side, side, std=2 * step, mean=1000.0)
+    v[1] = v[1] * -30
+    x = images(v, dtype, layout)
+    weight, bias = randn(gen, 16, std=0.3, mean=1.0).float().to(dev()), randn(gen, 16, std=0.3).float().to(dev())
+    y = torch.full_like(x, 7.0)
+    assert F.group_norm_fprop(x, weight, bias, y, 4, space(0, x, 4)) == F.Success
+    want, mean, rstd, _ = norm(x, weight, bias, 4, 1e-5, "none")
+    each = lambda t: t.repeat_interleave(4, 1)[:, :, None, None]  # noqa: E731
+    w = weight.cpu().double()[None, :, None, None].abs()
+    # half a unit of the mean, and three roundings of products and sums
+    bound = R * each(mean.abs() * rstd) * w + 4 * R * ((want - bias.cpu().double()[None, :, None, None]).abs() + want.abs())
+    within(y, want, rounded(want, dtype) + bound + 16 * R * want.abs())
