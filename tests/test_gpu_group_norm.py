@@ -371,3 +371,19 @@ def test_means_far_above_the_deviation(layout, side, dtype):
     # half a unit of the mean, and three roundings of products and sums
     bound = R * each(mean.abs() * rstd) * w + 4 * R * ((want - bias.cpu().double()[None, :, None, None]).abs() + want.abs())
     within(y, want, rounded(want, dtype) + bound + 16 * R * want.abs())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(2, 64, 27, 27, 8), (4, 192, 23, 23, 32), (3, 30, 5, 7, 5), (1, 16, 90, 91, 2), (2, 600, 6, 5, 2)],
+                         ids=str)
+@pytest.mark.parametrize("inner,outer", [("planes", "last"), ("last", "planes"), ("planes", "crop"), ("slice", "planes")])
+def test_layouts_that_differ(inner, outer, shape, dtype):
+    """What a convolution leaves as planes and a linear layer takes as rows of channels, and other pairs: the output and its
+    gradient in one layout, the input and its gradient in another; then each gradient in the other's."""
+    groups = shape[4]
+    x, weight, bias, gy = make(shape[:4], groups, dtype, inner, 17)
+    gy = images(gy.cpu().double(), dtype, outer)
+    y = images(torch.full(x.shape, 7.0, dtype=torch.float64), dtype, outer)
+    mean, rstd = check_forward(x, weight, bias, groups, "silu", outer, out=y)
+    check_backward(x, weight, bias, gy, mean, rstd, groups, "silu", inner)
+    check_backward(x, weight, bias, images(gy.cpu().double(), dtype, inner), mean, rstd, groups, "silu", outer)
