@@ -545,7 +545,8 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(Produc
   while (round()) {
   }
 
-  __syncthreads();
+  // (the loads requested behind the last step write zeros to LDS, which the results now go through)
+  arrive<0>();
   constexpr int SHARE = DEPTH * STEP / WAVES, FIT = SHARE / (WN * 64);  // of LDS, to a wave; blocks of rows
   constexpr int TURN = FIT >= RM ? RM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
   static_assert(FIT > 0 && RM % TURN == 0, "a wave's share of LDS holds whole rows of blocks");
