@@ -721,14 +721,15 @@ inline long biasRows(long M) { return M <= kBiasFew ? std::max(M, 1L) : kBiasRow
 
 // dz = dy activation'(z), dense, and its columns' sums over `rows` rows each, or, of all rows, the bias's gradient.  A
 // workgroup: 32 words of VEC columns, eight rows of lanes.  (All workgroups along x, `across` of them to a part of the
-// rows: the other axes count to 65535 only, which parts of 32 rows pass at 2097121 rows.)
+// rows: the other axes count to 65535 only, fewer than the parts of 32 rows from 2097121 rows on.)
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z, T* dz, float* parts, Line bias, long M, long N,
-                                                             int activation, long rows, int across) {
+                                                             int activation, long rows, Divisor across) {
   typedef typename Pack<T, VEC>::type Word;
   constexpr int AHEAD = 4;
   __shared__ float sums[8][32 * VEC];
-  const int column = threadIdx.x % 32, r = threadIdx.x / 32, part = blockIdx.x / across, block = blockIdx.x - part * across;
+  const int column = threadIdx.x % 32, r = threadIdx.x / 32, part = quotient(blockIdx.x, across);
+  const int block = blockIdx.x - part * (int)across.value;
   const long first = ((long)block * 32 + column) * VEC, m0 = part * rows, end = min(m0 + rows, M);
   // (the last word of a row ends with it, and repeats what the one before it has: N is no less than a word)
   const long n = min(first, N - VEC);
@@ -987,9 +988,9 @@ int backward(const LinearProblem& p, hipStream_t s) {
     float* const sums = p.gradBias.data && chunks > 1 ? parts : nullptr;
     const Line bias = chunks > 1 ? Line{} : p.gradBias;
     if (words)
-      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), (int)across);
+      preactivationGradient<T, W><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), divisorOf(across));
     else
-      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), (int)across);
+      preactivationGradient<T, 1><<<grid, 256, 0, s>>>(p.dy, p.z, to, sums, bias, p.M, p.N, p.activation, biasRows(p.M), divisorOf(across));
   }
   if (hasBias) biasGradient<<<dim3((unsigned)ceilDivLong(p.N, 8)), 256, 0, s>>>(parts, p.gradBias, p.N, p.M > 0 ? chunks : 0);
   int rc = launchStatus();
