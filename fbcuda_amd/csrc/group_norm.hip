@@ -408,7 +408,8 @@ __global__ __launch_bounds__(kFirst) void lastSums(NormArgs a) {
   joinMoments<kFirst, VEC>(a, band, s1, s2, space, sums, nullptr, true);
 }
 
-// 16 x 32 x 256 x 256 bf16, GELU: 26 us for 134 MB, 5.1 TB/s (half of it still in the last-level cache).
+// 16 x 32 x 256 x 256 bf16, GELU: 28 us for 134 MB, 4.8 TB/s (half of it still in the last-level cache; one multiply-add a value
+// in place of affine(): 26).
 template <class T, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void lastApply(NormArgs a) {
   __shared__ Moments stats[256];
@@ -501,8 +502,9 @@ __device__ __forceinline__ void inputGradient(const Channel<VEC>& ch, const floa
 }
 
 // All pixels of a band of input and gradient in registers: two reads, one write.  128 x 192 x 23 x 23 bf16, groups of six:
-// 33 us for 78 MB, 2.4 TB/s; the registers of two operands leave two workgroups to a compute unit, whose reads, joins and
-// writes hardly meet (capped at 128 registers they spill: 58 us).
+// 32-34 us for 78 MB, 2.4 TB/s.  164 registers leave three workgroups to a compute unit; the 1024 of this shape are four to each,
+// so a round of three and one of one, and a workgroup's read, join and write do not overlap (capped at 128 registers
+// they spill: 58 us).
 template <class T, int VEC, int NT, int ITEMS, bool STREAM>
 __global__ __launch_bounds__(NT) void lastBackward(NormArgs a, int total) {
   __shared__ Columns<NT, VEC, float> space;

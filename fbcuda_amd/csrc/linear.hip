@@ -310,7 +310,8 @@ struct Tile {
 // registers while this one's pieces are multiplied.  67712 x 192 x 64 fp32 with GELU, residual and preactivation: 30 us for
 // 104 MB, 3.5 TB/s, where cutting operands into pieces, LDS and memory take turns; 5330 x 1920 x 208: 43 us, 98 TFLOP/s of
 // fp32, six times that in matrix instructions (two steps ahead in registers: 34 and more us instead of 30; rows of x straight
-// from memory: 36.5).
+// from memory: 36.5).  The bound of three workgroups to a compute unit leaves the float32 kernels of 128 x 64 168 registers, and
+// 12 to 24 values of a lane in scratch memory.
 template <class T, bool AK, bool BK, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(256, BM * BN == 8192 ? 3 : 1) void product(ProductArgs g) {
   typedef typename Pieces<T>::type P;
@@ -502,8 +503,9 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void productDirect(Produc
     for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[set][j], fa[set][i], sum[i][j], T());
   };
   // Reads and loads go between matrix instructions a few at a time: a wave waits where it issues them (8192 x 8192 x
-  // 2048, us: 251, all reads first 268).  Not the transposing reads, which the compiler holds back until no load is on
-  // its way: all of them first (280, between matrix instructions 328).
+  // 2048, us: 251, all reads first 268).  Not the transposing reads, which the compiler holds back until none of the wave's loads
+  // is on its way: all of them first (280, between matrix instructions 328).  Behind every barrier of those forms stands
+  // that wait, so of their four steps in LDS no more than one is in flight while a wave reads.
   constexpr bool SPREAD = AK && BK;
   auto reads = [&](int i, int set, const char* from, int half) __attribute__((always_inline)) {
 #pragma unroll
@@ -721,7 +723,10 @@ inline long biasRows(long M) { return M <= kBiasFew ? std::max(M, 1L) : kBiasRow
 
 // dz = dy activation'(z), dense, and its columns' sums over `rows` rows each, or, of all rows, the bias's gradient.  A
 // workgroup: 32 words of VEC columns, eight rows of lanes.  (All workgroups along x, `across` of them to a part of the
-// rows: the other axes count to 65535 only, fewer than the parts of 32 rows from 2097121 rows on.)
+// rows: the other axes count to 65535 only, fewer than the parts of 32 rows from 2097121 rows on.)  dz is rounded to the
+// operands' type, which the matrix instructions take, after its sum: what a program does whose activation returns a gradient of
+// that type.  It costs gradients half again of what rounding them costs (4096 x 1024 x 4096 bf16: 2.35e-3 from the sums in 64 bits
+// instead of 1.66e-3); two pieces of dz would keep it and double both products.
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void preactivationGradient(Matrix dy, Matrix z, T* dz, float* parts, Line bias, long M, long N,
                                                              int activation, long rows, Divisor across) {
@@ -830,7 +835,13 @@ bool goesStraight(const Matrix& m, long rows, long K) {
 // The kernel with the least expected time, from what each takes for a step of k and for its results (us, measured on
 // products of 8192 x 8192 x 2048, 4096 x 1024 x 4096 and single tiles: 256 x 256 tiles, one to a compute unit, 1.75 a step of
 // 64 and 12 for the results; 128 x 128 ones 0.85 alone and 1.1 for two; the staged ones' are estimates).  A range of k more
-// costs its sums' way to memory and back.
+// costs its sums' way to memory and back.  (`together` is a number of the model, no occupancy: registers leave a compute unit
+// three float32 workgroups of 64 x 64, or four where k is contiguous in neither operand, and two of 128 x 128, or one where it
+// is in one of them only: 128 to 140 registers, 256 to 272.)
+// What the estimates cost, on random products timed with every staged tile and 1 to 64 ranges, in times of the fastest's
+// (geometric mean of 25 to 30, greatest): float32 x w^T 1.02, 1.26, of odd sizes 1.00, 1.29, dz w 1.05, 1.36, dz^T x 1.06,
+// 1.34; 16 bits of odd sizes 0.99, 1.25 and 1.00, 1.25 and 1.04, 1.36 (below 1 by chance).  Farthest off are mostly products that
+// tiles of 64 x 64 would serve better.
 template <class T>
 ProductPlan planOf(long M, long N, long K, bool straight) {
   struct Option {
