@@ -47,6 +47,12 @@ class Array(ctypes.Structure):
                 ("size", ctypes.c_longlong * MAX_DIM), ("dim", ctypes.c_int), ("type", ctypes.c_int)]
 
 
+class Mx4(ctypes.Structure):
+    """fbfft_mx4 of include/fbfft_amd.h."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("rows", ctypes.c_longlong),
+                ("blocks", ctypes.c_longlong), ("codeStride", ctypes.c_longlong), ("scaleStride", ctypes.c_longlong)]
+
+
 assert ctypes.sizeof(Tile) == 48
 assert ctypes.sizeof(Array) == 96
 
@@ -66,6 +72,9 @@ EXPORTS = (
     "fbfft_group_norm_workspace", "fbfft_group_norm_fprop", "fbfft_group_norm_bprop",
     "fbfft_linear_workspace", "fbfft_linear_fprop", "fbfft_linear_bprop",
     "fbfft_dropout_fprop", "fbfft_dropout_bprop",
+    "fbfft_layer_norm_workspace", "fbfft_layer_norm_fprop", "fbfft_layer_norm_bprop",
+    "fbfft_orthogonalize_workspace", "fbfft_orthogonalize",
+    "fbfft_mx4_quantize", "fbfft_mx4_dequantize", "fbfft_linear_mx4_workspace", "fbfft_linear_mx4_fprop",
 )
 
 # enum fbfft_activation of include/fbfft_amd.h
@@ -131,6 +140,19 @@ def lib():
         L.fbfft_linear_bprop.argtypes = [ap] * 7 + [i32, vp, size, vp]
         L.fbfft_dropout_fprop.argtypes = [ap] * 3 + [ctypes.c_double, ull, ull, vp, vp]
         L.fbfft_dropout_bprop.argtypes = [ap] * 2 + [ctypes.c_double, ull, ull, vp, vp]
+        f32, mp = ctypes.c_float, ctypes.POINTER(Mx4)
+        L.fbfft_layer_norm_workspace.argtypes = [i32] + [ll] * 2
+        L.fbfft_layer_norm_workspace.restype = size
+        L.fbfft_layer_norm_fprop.argtypes = [ap] * 6 + [f32, vp, size, vp]
+        L.fbfft_layer_norm_bprop.argtypes = [ap] * 8 + [vp, size, vp]
+        L.fbfft_orthogonalize_workspace.argtypes = [ll] * 3
+        L.fbfft_orthogonalize_workspace.restype = size
+        L.fbfft_orthogonalize.argtypes = [ap] * 2 + [ctypes.POINTER(f32), i32, f32, f32, vp, size, vp]
+        L.fbfft_mx4_quantize.argtypes = [ap, mp, vp]
+        L.fbfft_mx4_dequantize.argtypes = [mp, ap, vp]
+        L.fbfft_linear_mx4_workspace.argtypes = [ll] * 3
+        L.fbfft_linear_mx4_workspace.restype = size
+        L.fbfft_linear_mx4_fprop.argtypes = [ap, mp, mp] + [ap] * 3 + [i32, vp, size, vp]
         L.fbfft_bench_copy.argtypes = [vp, vp, ctypes.c_size_t, vp]
         L.fbfft_error_string.argtypes = [ctypes.c_int]
         L.fbfft_error_string.restype = ctypes.c_char_p
@@ -648,6 +670,128 @@ def dropout_bprop(gradOutput, gradInput, p, seed, offset, step=None, stream=None
             return rc
     return lib().fbfft_dropout_bprop(*_given(gradOutput, gradInput), float(p), _word(seed), _word(offset), _step(step),
                                      _stream(stream))
+
+
+# ---- around a linear layer: layer norm, orthogonalised updates, 4-bit weights ----
+
+def layer_norm_workspace(pass_, rows, cols):
+    """Workspace bytes of layer_norm_fprop (pass 0) or layer_norm_bprop (1) on input [rows][cols]."""
+    return lib().fbfft_layer_norm_workspace(int(pass_), rows, cols)
+
+
+def layer_norm_fprop(input, weight, bias, output, workspace, eps=1e-5, mean=None, rstd=None, stream=None):
+    """output = (input - mean) * rstd * weight + bias, mean and rstd = 1 / sqrt(var + eps) over each row.
+
+    input, output: [M][N] of one type, any strides.  weight, bias: [N] of any type, or None.  mean, rstd: float32 [M], written
+    for layer_norm_bprop, or None.  output may be input."""
+    if stream is None:
+        rc = (_native or _load_native()).layer_norm_fprop(input, weight, bias, output, mean, rstd, float(eps), workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_layer_norm_fprop(*_given(input, weight, bias, output, mean, rstd), float(eps), *_space(workspace),
+                                        _stream(stream))
+
+
+def layer_norm_bprop(input, weight, mean, rstd, gradOutput, gradInput, gradWeight, gradBias, workspace, stream=None):
+    """The gradients of layer_norm_fprop from its input, mean and rstd.  gradInput, gradWeight, gradBias: any of them None
+    where it is not wanted; gradInput may be gradOutput or input."""
+    if stream is None:
+        rc = (_native or _load_native()).layer_norm_bprop(input, weight, mean, rstd, gradOutput, gradInput, gradWeight, gradBias,
+                                                          workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_layer_norm_bprop(*_given(input, weight, mean, rstd, gradOutput, gradInput, gradWeight, gradBias),
+                                        *_space(workspace), _stream(stream))
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # singular values from 0.003 to 1 come out between 0.68 and 1.21 after five steps
+
+
+def orthogonalize_workspace(batch, rows, cols):
+    """Workspace bytes of orthogonalize on `batch` matrices [rows][cols]."""
+    return lib().fbfft_orthogonalize_workspace(batch, rows, cols)
+
+
+def orthogonalize(input, output, workspace, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, scale=1.0, stream=None):
+    """output = scale times what `steps` Newton-Schulz products make of X = input / (|input| + eps):
+    A = X X^T, X = a X + (b A + c A A) X, which brings all singular values near one.
+
+    input, output: [rows][cols] or [batch][rows][cols] of one type, any strides; each matrix by itself, with |input| the root
+    of its squares' sum.  coefficients: (a, b, c) for all steps, or a triple for each."""
+    triples = [coefficients] * steps if len(coefficients) == 3 and not hasattr(coefficients[0], "__len__") else list(coefficients)
+    if len(triples) != steps or any(len(t) != 3 for t in triples):
+        raise ValueError("coefficients are one triple, or one for each of %d steps" % steps)
+    flat = tuple(float(v) for t in triples for v in t)
+    if stream is None:
+        rc = (_native or _load_native()).orthogonalize(input, output, flat, float(eps), float(scale), workspace)
+        if rc is not NotImplemented:
+            return rc
+    return lib().fbfft_orthogonalize(*_given(input, output), (ctypes.c_float * len(flat))(*flat), steps, float(eps),
+                                     float(scale), *_space(workspace), _stream(stream))
+
+
+def packed_rows(codes, scales):
+    """fbfft_mx4 describing uint8 tensors codes [rows][16 blocks] and scales [rows][blocks]; None for None."""
+    import torch
+    if codes is None:
+        return None
+    if codes.dtype != torch.uint8 or scales is None or scales.dtype != torch.uint8:
+        raise TypeError("codes and scales are uint8")
+    if codes.dim() != 2 or scales.dim() != 2 or codes.size(0) != scales.size(0) or codes.size(1) != 16 * scales.size(1):
+        raise ValueError("codes are [rows][16 blocks], scales [rows][blocks]")
+    if (codes.size(1) > 1 and codes.stride(1) != 1) or (scales.size(1) > 1 and scales.stride(1) != 1):
+        raise ValueError("bytes of a row are neighbours")
+    return Mx4(codes.data_ptr(), scales.data_ptr(), scales.size(0), scales.size(1), codes.stride(0), scales.stride(0))
+
+
+def mx4_quantize(input, codes, scales, stream=None):
+    """Rows as 4-bit numbers (E2M1) that share a scale, a power of two, with the 31 others of their block (MXFP4).
+
+    input [M][K], any of the three types, any strides.  codes: uint8 [M][16 blocks], two numbers to a byte, 16-byte aligned
+    rows; scales: uint8 [M][blocks], exponents + 127; blocks = ceil(K / 32)."""
+    if stream is None:
+        rc = (_native or _load_native()).mx4_quantize(input, codes, scales)
+        if rc is not NotImplemented:
+            return rc
+    _on_gpu(input, codes, scales)
+    return lib().fbfft_mx4_quantize(array(input), packed_rows(codes, scales), _stream(stream))
+
+
+def mx4_dequantize(codes, scales, output, stream=None):
+    """output [M][K] = what the rows of mx4_quantize stand for, in output's type."""
+    if stream is None:
+        rc = (_native or _load_native()).mx4_dequantize(codes, scales, output)
+        if rc is not NotImplemented:
+            return rc
+    _on_gpu(codes, scales, output)
+    return lib().fbfft_mx4_dequantize(packed_rows(codes, scales), array(output), _stream(stream))
+
+
+def linear_mx4_workspace(rows, inputs, outputs):
+    """Workspace bytes of linear_mx4_fprop on rows [rows][inputs] and a weight [outputs][inputs]."""
+    return lib().fbfft_linear_mx4_workspace(rows, inputs, outputs)
+
+
+def linear_mx4_fprop(input, weight, weightScales, bias, output, workspace, activation="none", residual=None, inputScales=None,
+                     stream=None):
+    """output = activation(x w^T + bias) + residual, w held in 4 bits (weight, weightScales of mx4_quantize), x quantised on
+    the way.
+
+    input [M][K]: of output's type, any strides; or the codes of rows that are quantised already, with inputScales.
+    residual, output [M][N] of one type, any strides; bias [N] of any type.  bias, residual: or None; residual may be output."""
+    act = _activation(activation)
+    if stream is None:
+        rc = (_native or _load_native()).linear_mx4_fprop(input, inputScales, weight, weightScales, bias, residual, output, act,
+                                                          workspace)
+        if rc is not NotImplemented:
+            return rc
+    _on_gpu(input, weight, weightScales)
+    ready = inputScales is not None
+    if ready:
+        _on_gpu(inputScales)
+    return lib().fbfft_linear_mx4_fprop(None if ready else array(input), packed_rows(input, inputScales) if ready else None,
+                                        packed_rows(weight, weightScales), *_given(bias, residual, output), act,
+                                        *_space(workspace), _stream(stream))
 
 
 def _word(v):

@@ -299,6 +299,114 @@ PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- operators around a linear layer ----
+
+// (input, weight, bias, output, mean, rstd, eps, workspace)
+PyObject* layerNormForward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 8, [&]() -> PyObject* {
+    Arrays x;
+    float eps;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 6, &x) || !real(a[6], &eps) || !space(a[7], &ws, &bytes)) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_layer_norm_fprop(x.at[0], x.at[1], x.at[2], x.at[3], x.at[4], x.at[5], eps, ws, bytes, (fbfft_stream_t)s);
+    });
+  });
+}
+
+// (input, weight, mean, rstd, gradOutput, gradInput, gradWeight, gradBias, workspace)
+PyObject* layerNormBackward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    Arrays x;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 8, &x) || !space(a[8], &ws, &bytes)) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_layer_norm_bprop(x.at[0], x.at[1], x.at[2], x.at[3], x.at[4], x.at[5], x.at[6], x.at[7], ws, bytes,
+                                    (fbfft_stream_t)s);
+    });
+  });
+}
+
+// (input, output, coefficients, eps, scale, workspace); coefficients: a tuple of floats, three for each step
+PyObject* orthogonalize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 6, [&]() -> PyObject* {
+    constexpr Py_ssize_t most = 96;
+    Arrays x;
+    float coefficients[most], eps, scale;
+    void* ws;
+    size_t bytes;
+    if (!arraysOf(a, 2, &x) || !PyTuple_CheckExact(a[2]) || !real(a[3], &eps) || !real(a[4], &scale) || !space(a[5], &ws, &bytes))
+      Py_RETURN_NOTIMPLEMENTED;
+    const Py_ssize_t count = PyTuple_GET_SIZE(a[2]);
+    if (count > most || count % 3 != 0) Py_RETURN_NOTIMPLEMENTED;
+    for (Py_ssize_t i = 0; i < count; ++i)
+      if (!real(PyTuple_GET_ITEM(a[2], i), &coefficients[i])) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_orthogonalize(x.at[0], x.at[1], coefficients, (int)(count / 3), eps, scale, ws, bytes, (fbfft_stream_t)s);
+    });
+  });
+}
+
+// a matrix of bytes whose rows' bytes are neighbours
+bool bytesOf(PyObject* o, void** data, int64_t* rows, int64_t* cols, long long* stride) {
+  if (!THPVariable_CheckExact(o)) return false;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.scalar_type() != at::kByte || t.dim() != 2) return false;
+  if (t.size(1) > 1 && t.stride(1) != 1) return false;
+  *data = t.data_ptr();
+  *rows = t.size(0), *cols = t.size(1), *stride = t.stride(0);
+  return true;
+}
+
+bool packedOf(PyObject* codes, PyObject* scales, fbfft_mx4* to) {
+  int64_t rows, bytes, scaleRows, blocks;
+  if (!bytesOf(codes, &to->codes, &rows, &bytes, &to->codeStride) || !bytesOf(scales, &to->scales, &scaleRows, &blocks, &to->scaleStride))
+    return false;
+  to->rows = rows, to->blocks = blocks;
+  return rows == scaleRows && bytes == 16 * blocks;
+}
+
+// (input, codes, scales)
+PyObject* mx4Quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    Arrays x;
+    fbfft_mx4 q;
+    if (!arraysOf(a, 1, &x) || !packedOf(a[1], a[2], &q)) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) { return fbfft_mx4_quantize(x.at[0], &q, (fbfft_stream_t)s); });
+  });
+}
+
+// (codes, scales, output)
+PyObject* mx4Dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 3, [&]() -> PyObject* {
+    Arrays x;
+    fbfft_mx4 q;
+    if (!packedOf(a[0], a[1], &q) || !arraysOf(a + 2, 1, &x)) Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) { return fbfft_mx4_dequantize(&q, x.at[0], (fbfft_stream_t)s); });
+  });
+}
+
+// (input, inputScales or None, weight, weightScales, bias, residual, output, activation, workspace)
+PyObject* linearMx4Forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    Arrays x, rows;
+    fbfft_mx4 q, w;
+    int activation;
+    void* ws;
+    size_t bytes;
+    const bool ready = a[1] != Py_None;
+    if (!(ready ? packedOf(a[0], a[1], &q) : a[0] != Py_None && arraysOf(a, 1, &rows)) || !packedOf(a[2], a[3], &w) ||
+        !arraysOf(a + 4, 3, &x) || !integer(a[7], &activation) || !space(a[8], &ws, &bytes))
+      Py_RETURN_NOTIMPLEMENTED;
+    return call([&](void* s) {
+      return fbfft_linear_mx4_fprop(ready ? nullptr : rows.at[0], ready ? &q : nullptr, &w, x.at[0], x.at[1], x.at[2], activation,
+                                    ws, bytes, (fbfft_stream_t)s);
+    });
+  });
+}
+
 // (getDevice, rawStream): how torch names the current stream; kept for the life of the process
 PyObject* setup(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2) {
@@ -330,6 +438,12 @@ PyMethodDef methods[] = {
     FBFFT_METHOD("linear_fprop", linearForward),
     FBFFT_METHOD("linear_bprop", linearBackward),
     FBFFT_METHOD("dropout", dropout),
+    FBFFT_METHOD("layer_norm_fprop", layerNormForward),
+    FBFFT_METHOD("layer_norm_bprop", layerNormBackward),
+    FBFFT_METHOD("orthogonalize", orthogonalize),
+    FBFFT_METHOD("mx4_quantize", mx4Quantize),
+    FBFFT_METHOD("mx4_dequantize", mx4Dequantize),
+    FBFFT_METHOD("linear_mx4_fprop", linearMx4Forward),
     {nullptr, nullptr, 0, nullptr}};
 #undef FBFFT_METHOD
 

@@ -1,4 +1,5 @@
-// Shared by the operators around a convolution layer: group norm, products with an epilogue, dropout.
+// Shared by the operators around convolution and linear layers: group and layer norm, products with an epilogue, dropout,
+// orthogonalised updates, 4-bit rows.
 #pragma once
 
 #include "common.h"
@@ -310,5 +311,53 @@ struct DropoutProblem {
   const unsigned long long* step;
 };
 int launchDropout(const DropoutProblem& p, hipStream_t s);
+
+// rows of a matrix: 2-d operands of layer norm
+struct LayerNormProblem {
+  Matrix x, y, g;  // forward: x, y.  backward: x, g (gradOutput), y (gradInput; data may be null)
+  Line weight, bias, gradWeight, gradBias;
+  float *mean, *rstd;
+  long meanStride, rstdStride;
+  long M, N;
+  int type;
+  float eps;
+  void* workspace;
+};
+size_t layerNormWorkspaceBytes(int pass, long M, long N);
+int launchLayerNormForward(const LayerNormProblem& p, hipStream_t s);
+int launchLayerNormBackward(const LayerNormProblem& p, hipStream_t s);
+
+struct OrthogonalProblem {
+  Matrix x, y;  // of the first matrix
+  long xBatch, yBatch;
+  long batch, rows, cols;
+  int type;
+  const float* coefficients;
+  int steps;
+  float eps, scale;
+  void* workspace;
+};
+size_t orthogonalWorkspaceBytes(long batch, long rows, long cols);
+int launchOrthogonalize(const OrthogonalProblem& p, hipStream_t s);
+
+// rows in the 4-bit format
+struct Mx4 {
+  unsigned char *codes, *scales;
+  long codeStride, scaleStride;
+};
+int launchMx4Quantize(const Matrix& x, int type, long M, long K, const Mx4& to, hipStream_t s);
+int launchMx4Dequantize(const Mx4& from, const Matrix& y, int type, long M, long K, hipStream_t s);
+
+struct LinearMx4Problem {
+  Matrix x;  // data null: xq instead
+  Mx4 xq, w;
+  Matrix residual, y;
+  Line bias;
+  long M, K, blocks, N;
+  int type, activation;
+  void* workspace;
+};
+size_t linearMx4WorkspaceBytes(long M, long blocks, long N);
+int launchLinearMx4(const LinearMx4Problem& p, hipStream_t s);
 
 }  // namespace fbfft_amd

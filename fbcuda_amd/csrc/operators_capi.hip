@@ -1,4 +1,4 @@
-// C ABI of the operators around a convolution layer: argument validation and dispatch.
+// C ABI of the operators around convolution and linear layers: argument validation and dispatch.
 #include "operators.h"
 
 #include <cmath>
@@ -222,4 +222,200 @@ extern "C" int fbfft_dropout_bprop(const fbfft_array* gradOutput, const fbfft_ar
                                    unsigned long long seed, unsigned long long offset, const unsigned long long* step,
                                    fbfft_stream_t stream) {
   return dropoutOf(gradOutput, nullptr, gradInput, p, seed, offset, step, stream);
+}
+
+extern "C" size_t fbfft_layer_norm_workspace(int pass, long long rows, long long cols) {
+  if (pass < 0 || pass > 1 || rows <= 0 || cols <= 0 || rows > 0x7fffffff || cols > 0x7fffffff || rows > kMost / cols) return 0;
+  return layerNormWorkspaceBytes(pass, rows, cols);
+}
+
+namespace {
+
+bool okRowStatistics(const fbfft_array* a, long long rows) {
+  return okArray(a, 1) && a->type == FBFFT_FLOAT32 && a->size[0] == rows;
+}
+
+// What both passes of layer norm share; 0 or an error.
+int checkLayerNorm(const fbfft_array* input, const fbfft_array* weight) {
+  if (!okArray(input, 2) || !okLine(weight, input->size[1])) return FBFFT_UNSUPPORTED_DIMENSION;
+  return input->size[0] > 0x7fffffff || input->size[1] > 0x7fffffff ? FBFFT_UNSUPPORTED_SIZE : FBFFT_SUCCESS;
+}
+
+LayerNormProblem layerNormOf(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* mean,
+                             const fbfft_array* rstd, void* workspace) {
+  LayerNormProblem p{};
+  p.x = matrixOf(input), p.weight = lineOf(weight);
+  if (mean) p.mean = static_cast<float*>(mean->data), p.meanStride = mean->stride[0];
+  if (rstd) p.rstd = static_cast<float*>(rstd->data), p.rstdStride = rstd->stride[0];
+  p.M = input->size[0], p.N = input->size[1], p.type = input->type, p.workspace = workspace;
+  return p;
+}
+
+}  // namespace
+
+extern "C" int fbfft_layer_norm_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
+                                      const fbfft_array* output, const fbfft_array* mean, const fbfft_array* rstd, float eps,
+                                      void* workspace, size_t workspaceBytes, fbfft_stream_t stream) {
+  const int rc = checkLayerNorm(input, weight);
+  if (rc != FBFFT_SUCCESS) return rc;
+  const long long M = input->size[0], N = input->size[1];
+  if (!okMatrix(output, M, N, input->type) || !okLine(bias, N)) return FBFFT_UNSUPPORTED_DIMENSION;
+  if ((mean && !okRowStatistics(mean, M)) || (rstd && !okRowStatistics(rstd, M))) return FBFFT_UNSUPPORTED_DIMENSION;
+  if (!(eps >= 0.f) || std::isinf(eps)) return FBFFT_UNSUPPORTED_SIZE;
+  if (M * N == 0) return FBFFT_SUCCESS;
+  if (!okWorkspace(workspace, workspaceBytes, fbfft_layer_norm_workspace(0, M, N))) return FBFFT_UNSUPPORTED_DIMENSION;
+  LayerNormProblem p = layerNormOf(input, weight, mean, rstd, workspace);
+  p.y = matrixOf(output), p.bias = lineOf(bias), p.eps = eps;
+  return launchLayerNormForward(p, stream);
+}
+
+extern "C" int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* mean,
+                                      const fbfft_array* rstd, const fbfft_array* gradOutput, const fbfft_array* gradInput,
+                                      const fbfft_array* gradWeight, const fbfft_array* gradBias, void* workspace,
+                                      size_t workspaceBytes, fbfft_stream_t stream) {
+  const int rc = checkLayerNorm(input, weight);
+  if (rc != FBFFT_SUCCESS) return rc;
+  const long long M = input->size[0], N = input->size[1];
+  if (!okMatrix(gradOutput, M, N, input->type) || (gradInput && !okMatrix(gradInput, M, N, input->type)))
+    return FBFFT_UNSUPPORTED_DIMENSION;
+  if (!okLine(gradWeight, N) || !okLine(gradBias, N)) return FBFFT_UNSUPPORTED_DIMENSION;
+  if (!okRowStatistics(mean, M) || !okRowStatistics(rstd, M)) return FBFFT_UNSUPPORTED_DIMENSION;
+  if (N == 0 || (!gradInput && !gradWeight && !gradBias)) return FBFFT_SUCCESS;
+  if (!okWorkspace(workspace, workspaceBytes, fbfft_layer_norm_workspace(1, M, N))) return FBFFT_UNSUPPORTED_DIMENSION;
+  LayerNormProblem p = layerNormOf(input, weight, mean, rstd, workspace);
+  p.g = matrixOf(gradOutput), p.y = matrixOf(gradInput);
+  p.gradWeight = lineOf(gradWeight), p.gradBias = lineOf(gradBias);
+  return launchLayerNormBackward(p, stream);
+}
+
+namespace {
+
+constexpr long long kMostSide = 65536;  // of a matrix that is orthogonalised
+constexpr double kMostSingular = 32;    // of what its products meet: pieces hold numbers below 64
+
+// Whether singular values that start in [0, 1] and what the products make of them stay within kMostSingular under these
+// polynomials: the greatest magnitude of each over the interval so far, at its ends and where its derivative is 0.
+bool staysInside(const float* coefficients, int steps) {
+  double most = 1;
+  for (int i = 0; i < steps; ++i) {
+    const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+    double next = 0, inner = 0;
+    auto at = [&](double u) {  // u: the singular value's square
+      if (!(u >= 0 && u <= most * most)) return;
+      next = std::fmax(next, std::fabs(std::sqrt(u) * (a + u * (b + u * c))));
+      inner = std::fmax(inner, std::fabs(u * (b + u * c)));
+    };
+    at(most * most);
+    if (c != 0) at(-b / (2 * c));
+    // a + 3 b u + 5 c u^2 = 0
+    const double d = 9 * b * b - 20 * a * c;
+    if (c == 0) {
+      if (b != 0) at(-a / (3 * b));
+    } else if (d >= 0) {
+      at((-3 * b + std::sqrt(d)) / (10 * c));
+      at((-3 * b - std::sqrt(d)) / (10 * c));
+    }
+    if (!(next <= kMostSingular && inner <= kMostSingular && most * most <= kMostSingular)) return false;
+    most = next;
+  }
+  return true;
+}
+
+}  // namespace
+
+extern "C" size_t fbfft_orthogonalize_workspace(long long batch, long long rows, long long cols) {
+  if (batch <= 0 || rows <= 0 || cols <= 0 || rows > kMostSide || cols > kMostSide || batch > kMost / (rows * cols)) return 0;
+  return orthogonalWorkspaceBytes(batch, rows, cols);
+}
+
+extern "C" int fbfft_orthogonalize(const fbfft_array* input, const fbfft_array* output, const float* coefficients, int steps,
+                                   float eps, float scale, void* workspace, size_t workspaceBytes, fbfft_stream_t stream) {
+  const int dim = input ? input->dim : 0;
+  if ((dim != 2 && dim != 3) || !okArray(input, dim) || !okArray(output, dim) || !sameShape(input, output) || !coefficients)
+    return FBFFT_UNSUPPORTED_DIMENSION;
+  const long long batch = dim == 3 ? input->size[0] : 1, rows = input->size[dim - 2], cols = input->size[dim - 1];
+  if (steps < 1 || steps > 32 || !(eps >= 0.f) || std::isinf(eps) || !std::isfinite(scale)) return FBFFT_UNSUPPORTED_SIZE;
+  if (!staysInside(coefficients, steps)) return FBFFT_UNSUPPORTED_SIZE;
+  if (batch * rows * cols == 0) return FBFFT_SUCCESS;
+  if (rows > kMostSide || cols > kMostSide) return FBFFT_UNSUPPORTED_SIZE;
+  if (!okWorkspace(workspace, workspaceBytes, fbfft_orthogonalize_workspace(batch, rows, cols))) return FBFFT_UNSUPPORTED_DIMENSION;
+  OrthogonalProblem p{};
+  p.x = Matrix{input->data, (long)input->stride[dim - 2], (long)input->stride[dim - 1]};
+  p.y = Matrix{output->data, (long)output->stride[dim - 2], (long)output->stride[dim - 1]};
+  if (dim == 3) p.xBatch = input->stride[0], p.yBatch = output->stride[0];
+  p.batch = batch, p.rows = rows, p.cols = cols, p.type = input->type;
+  p.coefficients = coefficients, p.steps = steps, p.eps = eps, p.scale = scale, p.workspace = workspace;
+  return launchOrthogonalize(p, stream);
+}
+
+namespace {
+
+constexpr long long kMostBlocks = 1 << 17;      // of a row in the 4-bit format
+constexpr long long kMostCodeStride = 1 << 22;  // 256 of them are far inside 31 bits
+
+bool okMx4(const fbfft_mx4* a) {
+  if (!a || a->rows < 0 || a->blocks < 0 || a->rows > kMost || a->blocks > kMost) return false;
+  if (a->rows == 0 || a->blocks == 0) return true;
+  if (!a->codes || !a->scales || !aligned(a->codes, 16)) return false;
+  return a->rows == 1 || (a->codeStride % 16 == 0 && a->codeStride >= 16 * a->blocks && a->scaleStride >= a->blocks);
+}
+bool okMx4Size(const fbfft_mx4* a) {
+  return a->blocks <= kMostBlocks && (a->rows <= 1 || (a->codeStride <= kMostCodeStride && a->scaleStride <= kMostCodeStride));
+}
+Mx4 mx4Of(const fbfft_mx4* a) {
+  if (!a) return Mx4{};
+  const bool one = a->rows <= 1;  // (whose strides say nothing)
+  return Mx4{static_cast<unsigned char*>(a->codes), static_cast<unsigned char*>(a->scales), (long)(one ? 16 * a->blocks : a->codeStride),
+             (long)(one ? a->blocks : a->scaleStride)};
+}
+
+// whether `array` is rows that `packed` holds or is to hold
+bool okPacked(const fbfft_array* array, const fbfft_mx4* packed) {
+  return okArray(array, 2) && okMx4(packed) && packed->rows == array->size[0] && packed->blocks == (array->size[1] + 31) / 32;
+}
+
+}  // namespace
+
+extern "C" int fbfft_mx4_quantize(const fbfft_array* input, const fbfft_mx4* output, fbfft_stream_t stream) {
+  if (!okPacked(input, output)) return FBFFT_UNSUPPORTED_DIMENSION;
+  const long long M = input->size[0], K = input->size[1];
+  if (M > 0x7fffffff || !okMx4Size(output)) return FBFFT_UNSUPPORTED_SIZE;
+  if (M * K == 0) return FBFFT_SUCCESS;
+  return launchMx4Quantize(matrixOf(input), input->type, M, K, mx4Of(output), stream);
+}
+
+extern "C" int fbfft_mx4_dequantize(const fbfft_mx4* input, const fbfft_array* output, fbfft_stream_t stream) {
+  if (!okPacked(output, input)) return FBFFT_UNSUPPORTED_DIMENSION;
+  const long long M = output->size[0], K = output->size[1];
+  if (M > 0x7fffffff || !okMx4Size(input)) return FBFFT_UNSUPPORTED_SIZE;
+  if (M * K == 0) return FBFFT_SUCCESS;
+  return launchMx4Dequantize(mx4Of(input), matrixOf(output), output->type, M, K, stream);
+}
+
+extern "C" size_t fbfft_linear_mx4_workspace(long long M, long long K, long long N) {
+  if (M <= 0 || K < 0 || N <= 0 || !okLinearSize(M) || !okLinearSize(N) || K > kMostBlocks * 32) return 0;
+  return linearMx4WorkspaceBytes(M, (K + 31) / 32, N);
+}
+
+extern "C" int fbfft_linear_mx4_fprop(const fbfft_array* input, const fbfft_mx4* quantized, const fbfft_mx4* weight,
+                                      const fbfft_array* bias, const fbfft_array* residual, const fbfft_array* output,
+                                      int activation, void* workspace, size_t workspaceBytes, fbfft_stream_t stream) {
+  if (!okArray(output, 2) || !okMx4(weight) || !okActivation(activation) || !input == !quantized) return FBFFT_UNSUPPORTED_DIMENSION;
+  const long long M = output->size[0], N = output->size[1], blocks = weight->blocks;
+  const int type = output->type;
+  if (weight->rows != N || !okLine(bias, N) || (residual && !okMatrix(residual, M, N, type))) return FBFFT_UNSUPPORTED_DIMENSION;
+  if (input ? !okArray(input, 2) || input->type != type || input->size[0] != M || (input->size[1] + 31) / 32 != blocks
+            : !okMx4(quantized) || quantized->rows != M || quantized->blocks != blocks)
+    return FBFFT_UNSUPPORTED_DIMENSION;
+  if (!okLinearSize(M) || !okLinearSize(N) || !okMx4Size(weight) || (quantized && !okMx4Size(quantized)))
+    return FBFFT_UNSUPPORTED_SIZE;
+  if (M == 0 || N == 0) return FBFFT_SUCCESS;
+  if (!okWorkspace(workspace, workspaceBytes, fbfft_linear_mx4_workspace(M, 32 * blocks, N))) return FBFFT_UNSUPPORTED_DIMENSION;
+  LinearMx4Problem p{};
+  p.x = matrixOf(input), p.xq = mx4Of(quantized), p.w = mx4Of(weight);
+  p.residual = matrixOf(residual), p.y = matrixOf(output), p.bias = lineOf(bias);
+  p.M = M, p.K = input ? input->size[1] : 32 * blocks, p.blocks = blocks, p.N = N;
+  p.type = type, p.activation = activation, p.workspace = workspace;
+  return launchLinearMx4(p, stream);
 }

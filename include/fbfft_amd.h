@@ -424,6 +424,84 @@ int fbfft_dropout_fprop(const fbfft_array* input, const fbfft_array* residual, c
 int fbfft_dropout_bprop(const fbfft_array* gradOutput, const fbfft_array* gradInput, double p, unsigned long long seed,
                         unsigned long long offset, const unsigned long long* step, fbfft_stream_t stream);
 
+/* ---- Around a linear layer: layer norm, orthogonalised updates, 4-bit weights ---- */
+
+/* Layer norm of rows.  input, output [M][N] of one type, any strides:
+ *   mean, var: over the N values of a row (var divides by N)
+ *   output = (input - mean) / sqrt(var + eps) * weight[n] + bias[n]
+ * weight, bias: [N] of any type, or NULL for 1 and 0.  mean, rstd (= 1 / sqrt(var + eps)): float32 [M], written for the
+ * backward pass, or NULL.  M and N are below 2^31.  output may be input itself (same address and strides); any other
+ * overlap is not defined.  workspace: fbfft_layer_norm_workspace(0, ...) bytes, 256-byte aligned, NULL where that is 0;
+ * its contents need not survive. */
+size_t fbfft_layer_norm_workspace(int pass, long long rows, long long cols);
+int fbfft_layer_norm_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
+                           const fbfft_array* output, const fbfft_array* mean, const fbfft_array* rstd, float eps,
+                           void* workspace, size_t workspaceBytes, fbfft_stream_t stream);
+
+/* Its gradients, from the input and the mean and rstd that the forward pass wrote (xh = (input - mean) rstd):
+ *   gradBias[n] = sum_m gradOutput,  gradWeight[n] = sum_m gradOutput xh
+ *   gradInput = rstd (weight gradOutput - sum_n(weight gradOutput) / N - xh sum_n(weight gradOutput xh) / N)
+ * gradInput, gradWeight, gradBias: any of them NULL where it is not wanted; the latter two are overwritten.  gradInput
+ * may be gradOutput or input itself.  Reproducible bit for bit.  workspace: fbfft_layer_norm_workspace(1, ...). */
+int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* mean,
+                           const fbfft_array* rstd, const fbfft_array* gradOutput, const fbfft_array* gradInput,
+                           const fbfft_array* gradWeight, const fbfft_array* gradBias, void* workspace,
+                           size_t workspaceBytes, fbfft_stream_t stream);
+
+/* A matrix made nearly orthogonal by Newton-Schulz products, as an optimiser does with a weight's gradient:
+ *   X = input / (|input| + eps),  |input|: the root of the sum of all squares
+ *   for each of `steps` triples (a, b, c) of coefficients:  A = X X^T,  X = a X + (b A + c A A) X
+ *   output = scale X
+ * (of a matrix with more rows than columns: of its transpose, the same by the formula).  Every singular value of
+ * input / |input| goes through the polynomials a s + b s^3 + c s^5 one after the other.
+ * input, output: [rows][cols] or [batch][rows][cols] of one type, any strides, not overlapping; each matrix of a batch
+ * by itself.  coefficients: 3 steps numbers in host memory, read during the call.  Products are summed in 32 bits;
+ * between them X, A and b A + c A A are held as two 16-bit pieces of a value, 22 bits of it together, and products
+ * leave out that of the second pieces: about what 32-bit arithmetic gives.  A matrix of zeros gives zeros where
+ * eps > 0; values that are not finite make all of their matrix NaN.
+ * steps from 1 to 32; eps and scale finite, eps >= 0; coefficients under which a singular value in [0, 1] or what the
+ * products make of it could pass 32 are refused (UnsupportedSize): the pieces end at 64.  rows, cols up to 65536.
+ * workspace: fbfft_orthogonalize_workspace bytes, 256-byte aligned.  Reproducible bit for bit. */
+size_t fbfft_orthogonalize_workspace(long long batch, long long rows, long long cols);
+int fbfft_orthogonalize(const fbfft_array* input, const fbfft_array* output, const float* coefficients, int steps,
+                        float eps, float scale, void* workspace, size_t workspaceBytes, fbfft_stream_t stream);
+
+/* Rows in microscaled 4-bit floating point (MXFP4 of the OCP Microscaling Formats specification): 32 neighbours of a row
+ * share a scale, a power of two; each is a 4-bit number of sign, two bits of exponent and one of mantissa:
+ *   0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives (codes 0 ... 7, 8 ... 15)
+ * codes: [rows][16 blocks] bytes, element 2 i of a row in the lower half of byte i; 16-byte aligned, rows codeStride bytes
+ * apart, a multiple of 16.  scales: [rows][blocks] bytes, exponent + 127; 255 stands for NaN; rows scaleStride bytes apart.
+ * Rows do not overlap and lie up to 2^22 bytes apart; of a single row the strides are not read.  A row of K values, up to
+ * 2^22, takes ceil(K / 32) blocks, whose last is filled up with zeros. */
+typedef struct fbfft_mx4 {
+  void* codes;
+  void* scales;
+  long long rows, blocks;
+  long long codeStride, scaleStride;
+} fbfft_mx4;
+
+/* output = input [M][K] of any of the three types, any strides, in that format:
+ *   scale = 2^e, e = floor(log2 of the block's largest magnitude) - 2, at least -127
+ *   code: the nearest to value / scale, ties to the even code, magnitudes over 6 to 6
+ * A block of zeros has the scale 2^-127; one that holds NaN or an infinity has the scale NaN. */
+int fbfft_mx4_quantize(const fbfft_array* input, const fbfft_mx4* output, fbfft_stream_t stream);
+
+/* output [M][K] = what the format stands for, rounded to output's type (bfloat16 and float32 hold it exactly). */
+int fbfft_mx4_dequantize(const fbfft_mx4* input, const fbfft_array* output, fbfft_stream_t stream);
+
+/* Rows times a weight matrix held in that format, for serving:
+ *   output[m][n] = activation(sum_k x[m][k] w[n][k] + bias[n]) + residual[m][n]
+ * w: weight, N rows.  x: input [M][K], any of the three types and any strides, quantised on the way as
+ * fbfft_mx4_quantize does, or, where input is NULL, quantized, M rows of the same number of blocks.  bias [N] of any type
+ * or NULL; residual, output [M][N] of one type (input's, where it is given); residual may be NULL or output itself, no
+ * other operand may overlap output.  Products of quantised values are exact and summed in 32 bits.
+ * M and N below 2^23, K up to 2^22.  workspace: fbfft_linear_mx4_workspace(M, K, N) bytes (K: 32 blocks where it is not
+ * known), 256-byte aligned, NULL where that is 0; its contents need not survive. */
+size_t fbfft_linear_mx4_workspace(long long M, long long K, long long N);
+int fbfft_linear_mx4_fprop(const fbfft_array* input, const fbfft_mx4* quantized, const fbfft_mx4* weight,
+                           const fbfft_array* bias, const fbfft_array* residual, const fbfft_array* output,
+                           int activation, void* workspace, size_t workspaceBytes, fbfft_stream_t stream);
+
 /* Measurement aid with no counterpart in the reference: a plain device-to-device copy
  * of `bytes` (a multiple of 16, both pointers 16-byte aligned) on `stream`, in the
  * shape that moves a batch the size of a transform's operands fastest from HBM to HBM.
