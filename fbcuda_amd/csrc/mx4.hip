@@ -2,40 +2,92 @@
 //
 //   a block of 32 neighbours v of a row:  e = floor(log2(max |v|)) - 2, at least -127;  code = nearest of v / 2^e, ties to even
 //   product                               y = activation(sum_k x w + bias) + residual
-#include "operators.h"
+//
+// The scaled matrix instruction takes 128 k of 16 rows of both operands: a lane a whole block, 16 bytes, and the byte of its scale.
+#include "product.h"
 
 #include <algorithm>
 
 namespace fbfft_amd {
 namespace {
 
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 typedef int intx8 __attribute__((ext_vector_type(8)));
 
-// The scale's byte of a block from the bits of its largest magnitude (as numbers without sign, which order like the values),
-// 255 for what is not finite.  floor(log2) is the exponent's field; numbers without one have their leading bit looked up, but
-// all of them are below 2^-125 and take the least scale.
+// The scale's byte of a block from the bits of its largest magnitude as float32 (numbers without sign, which order like the
+// values), 255 for what is not finite.  floor(log2) is the exponent's field; numbers without one are below 2^-125, as
+// are all that take the least scale.
 __device__ __forceinline__ int scaleOf(unsigned most) {
   const int exponent = (int)(most >> 23);
   return exponent == 255 ? 255 : max(exponent - 2, 0);
 }
 
-// Eight values, of a block with this scale, as codes.  (v / 2^e is a product with 2^-e, which is exact: a finite value's scale
-// is at most 252, so 2^-e a normal number.)
-__device__ __forceinline__ unsigned codesOf(const float (&v)[8], int scale) {
-  if (scale == 255) return 0;
-  const float by = __builtin_bit_cast(float, (unsigned)(254 - scale) << 23);
-  unsigned codes = 0;
+// N neighbours of a row, N a multiple of eight; behind `left` of them zeros.
+template <class T, int N>
+struct Values {
+  static constexpr int per = 16 / sizeof(T), words = N / per;
+  typename Pack<T, per>::type v[words];
+
+  __device__ __forceinline__ void load(const T* from, long left) {
+    if (left >= N) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float a = __builtin_fabsf(v[j] * by);
-    // ties to the even code
-    const unsigned code = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
-    codes |= (code | (__builtin_bit_cast(unsigned, v[j]) >> 28 & 8u)) << 4 * j;
+      for (int i = 0; i < words; ++i) v[i] = *reinterpret_cast<const typename Pack<T, per>::type*>(from + i * per);
+    } else {
+#pragma unroll
+      for (int i = 0; i < words; ++i)
+#pragma unroll
+        for (int j = 0; j < per; ++j) v[i][j] = i * per + j < left ? from[i * per + j] : (T)0.f;
+    }
   }
-  return codes;
-}
+  __device__ __forceinline__ void gather(const T* from, long stride, long left) {
+#pragma unroll
+    for (int i = 0; i < words; ++i)
+#pragma unroll
+      for (int j = 0; j < per; ++j) v[i][j] = i * per + j < left ? from[(i * per + j) * stride] : (T)0.f;
+  }
+
+  // the bits of the largest magnitude, as float32
+  __device__ __forceinline__ unsigned most() const {
+    if constexpr (sizeof(T) == 4) {
+      unsigned m = 0;
+#pragma unroll
+      for (int i = 0; i < words; ++i)
+#pragma unroll
+        for (int j = 0; j < per; ++j) m = max(m, __builtin_bit_cast(unsigned, (float)v[i][j]) & 0x7fffffffu);
+      return m;
+    } else {
+      typedef unsigned short __attribute__((ext_vector_type(8))) Bits;
+      Bits m = __builtin_bit_cast(Bits, v[0]) & (unsigned short)0x7fff;
+#pragma unroll
+      for (int i = 1; i < words; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(Bits, v[i]) & (unsigned short)0x7fff);
+      unsigned short one = m[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) one = max(one, m[j]);
+      return __builtin_bit_cast(unsigned, (float)__builtin_bit_cast(T, one));
+    }
+  }
+
+  // The codes of eight of them from 8 q.  The instruction takes the scale as the exponent of a float32 and divides exactly,
+  // rounds to the nearest, ties to even, and saturates; a block whose scale is NaN has codes of zeros.
+  __device__ __forceinline__ unsigned codes(int q, int scale) const {
+    const float by = __builtin_bit_cast(float, (unsigned)scale << 23);
+    unsigned c = 0;
+#define FBFFT_PAIR(J, BYTE)                                                                                                       \
+  if constexpr (sizeof(T) == 4) {                                                                                                 \
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2 * q + J / 4][J % 4], v[2 * q + J / 4][J % 4 + 1], by, BYTE);              \
+  } else if constexpr (__is_same(T, half16)) {                                                                                    \
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(c, Two{v[q][J % per], v[q][J % per + 1]}, by, BYTE);                             \
+  } else {                                                                                                                        \
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, Two{v[q][J % per], v[q][J % per + 1]}, by, BYTE);                            \
+  }
+    typedef T __attribute__((ext_vector_type(2))) Two;
+    FBFFT_PAIR(0, 0)
+    FBFFT_PAIR(2, 1)
+    FBFFT_PAIR(4, 2)
+    FBFFT_PAIR(6, 3)
+#undef FBFFT_PAIR
+    return scale == 255 ? 0 : c;
+  }
+};
 
 __device__ __forceinline__ float powerOf(int scale) {  // 2^(scale - 127); NaN for 255
   return __builtin_bit_cast(float, scale == 255 ? 0x7fc00000u : scale == 0 ? 0x00400000u : (unsigned)scale << 23);
@@ -53,28 +105,19 @@ __device__ __forceinline__ unsigned mostOfFour(unsigned v) {
   return max(v, (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, 0x4E, 0xF, 0xF, false));
 }
 
-template <class T>
-__device__ __forceinline__ void loadEight(const T* row, long stride, long k, long K, float (&v)[8]) {
-  if (stride == 1 && k + 8 <= K) {
-    loadPack<T, 8>(row + k, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? (float)row[(k + j) * stride] : 0.f;
-  }
-}
-
 // Eight values to a lane, a block to four neighbouring lanes.
 template <class T>
 __global__ __launch_bounds__(256) void quantize(Matrix x, long M, long K, Mx4 to, Divisor perRow) {
   const int i = blockIdx.x * 256 + threadIdx.x, m = quotient(i, perRow), word = i - m * (int)perRow.value;
   if (m >= M) return;  // (a block's four lanes together)
-  float v[8];
-  loadEight(static_cast<const T*>(x.data) + m * x.row, x.col, 8l * word, K, v);
-  unsigned most = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) most = max(most, __builtin_bit_cast(unsigned, v[j]) & 0x7fffffffu);
-  const int scale = scaleOf(mostOfFour(most));
-  *reinterpret_cast<unsigned*>(to.codes + m * to.codeStride + 4l * word) = codesOf(v, scale);
+  Values<T, 8> v;
+  const T* const from = static_cast<const T*>(x.data) + m * x.row + 8l * word * x.col;
+  if (x.col == 1)
+    v.load(from, K - 8l * word);
+  else
+    v.gather(from, x.col, K - 8l * word);
+  const int scale = scaleOf(mostOfFour(v.most()));
+  *reinterpret_cast<unsigned*>(to.codes + m * to.codeStride + 4l * word) = v.codes(0, scale);
   if (word % 4 == 0) to.scales[m * to.scaleStride + word / 4] = (unsigned char)scale;
 }
 
@@ -109,56 +152,302 @@ int inLaunches(long M, long blocks, F f) {
   return launchStatus();
 }
 
+// ---- products ----
+
+struct Mx4Args {
+  Mx4 x, w;
+  long M, N, blocks, range;  // blocks per range of k
+  Epilogue e;
+};
+
+// c + a b^T, with bytes OA and OB of the scales
+template <int OA, int OB>
 __device__ __forceinline__ floatx4 multiply(uintx4 a, int scaleA, uintx4 b, int scaleB, floatx4 c) {
   const intx8 x{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, y{(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, 0, scaleA, 0, scaleB);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 4, 4, OA, scaleA, OB, scaleB);
+}
+// bytes 2 a + H and 2 b + H, a and b 0 or 1 and known where this is compiled
+template <int H>
+__device__ __forceinline__ floatx4 multiplyAt(int a, int b, uintx4 fa, int scaleA, uintx4 fb, int scaleB, floatx4 c) {
+  if (a) return b ? multiply<2 + H, 2 + H>(fa, scaleA, fb, scaleB, c) : multiply<2 + H, H>(fa, scaleA, fb, scaleB, c);
+  return b ? multiply<H, 2 + H>(fa, scaleA, fb, scaleB, c) : multiply<H, H>(fa, scaleA, fb, scaleB, c);
 }
 
-// A wave: 16 x 16 results, straight from memory to the matrix instructions: lane l has block l / 16 of four of row l % 16.
-template <class T>
-__global__ __launch_bounds__(256) void product(LinearMx4Problem p) {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const long down = (p.M + 15) / 16, tile = blockIdx.x * 4l + wave, m0 = tile % down * 16, n0 = tile / down * 16;
-  if (n0 >= p.N) return;
-  const long xm = min(m0 + lane % 16, p.M - 1), wn = min(n0 + lane % 16, p.N - 1);
-  const unsigned char *const x = p.xq.codes + xm * p.xq.codeStride, *const w = p.w.codes + wn * p.w.codeStride;
-  const unsigned char *const xs = p.xq.scales + xm * p.xq.scaleStride, *const ws = p.w.scales + wn * p.w.scaleStride;
-  floatx4 sum{0.f, 0.f, 0.f, 0.f};
-  for (long b0 = 0; b0 < p.blocks; b0 += 4) {
-    const long b = b0 + lane / 16;
-    uintx4 a{}, c{};
-    int sa = 0, sc = 0;  // (a block behind the last: zeros times 2^-127)
-    if (b < p.blocks) {
-      a = *reinterpret_cast<const uintx4*>(w + 16 * b), c = *reinterpret_cast<const uintx4*>(x + 16 * b);
-      sa = ws[b], sc = xs[b];
+// One step of an operand: eight blocks of each row, lines of 128 bytes.  A lane takes two neighbouring blocks of its row in
+// two instructions, so that their scales are two neighbouring bytes.
+template <int ROWS, int WAVES>
+struct Packed : Direct<ROWS, 64, true, WAVES> {
+  static __device__ __forceinline__ int laneAt(int first) {
+    const int lane = threadIdx.x % 64, line = first + lane % 16;
+    return line * 128 + Packed::permuted(line, lane / 16 * 2) * 16;
+  }
+  static __device__ __forceinline__ uintx4 fragment(const char* step, int lane, int h, int i) {
+    return *reinterpret_cast<const uintx4*>(step + (lane ^ h * 16) + i * (16 * 128));
+  }
+};
+
+// A workgroup: BM x BN results over one range of k, a wave WM x WN of them.  LDS holds the operands of two steps of 256 k; a
+// thread moves the eight scales of one row of one operand through its registers.  In LDS the scales of rows r and r + 16 lie
+// side by side for each pair of blocks: a lane's scales of two fragments in both instructions are one word.
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
+  constexpr int WAVES = BM / WM * (BN / WN), RM = WM / 16, RN = WN / 16;
+  typedef Packed<BM, WAVES> A;
+  typedef Packed<BN, WAVES> B;
+  constexpr int SCALES = (BM + BN) * 8, STEP = A::bytes + B::bytes, LOADS = A::loads + B::loads;
+  static_assert(BM + BN == WAVES * 64 && BM % 32 == 0 && WM % 32 == 0 && WN % 32 == 0, "a row's scales to a thread");
+  __shared__ __attribute__((aligned(1024))) char space[2 * STEP];
+  __shared__ __attribute__((aligned(16))) char scales[2][SCALES];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+  const Tile<BM, BN> tile(g.M, g.N);
+  if (!tile.any) return;
+  const long m0 = tile.m0, n0 = tile.n0, first = blockIdx.y * g.range, end = min(first + g.range, g.blocks);
+
+  A a;
+  B b;
+  a.setup(g.x.codes + m0 * g.x.codeStride + 16 * first, g.x.codeStride / 2, g.M - m0);
+  b.setup(g.w.codes + n0 * g.w.codeStride + 16 * first, g.w.codeStride / 2, g.N - n0);
+
+  // this thread's row of scales: of A, then of B (behind the last: the last again, whose results nobody takes)
+  const bool ofA = threadIdx.x < BM;
+  const int row = ofA ? threadIdx.x : threadIdx.x - BM;
+  const unsigned char* from = ofA ? g.x.scales + min(m0 + row, g.M - 1) * g.x.scaleStride + first
+                                  : g.w.scales + min(n0 + row, g.N - 1) * g.w.scaleStride + first;
+  const int place = (ofA ? 0 : BM * 8) + row / 32 * 256 + row % 16 * 4 + row / 16 % 2 * 2;
+  int ahead = (int)(end - first);  // blocks whose scales are not loaded yet
+  typedef unsigned long __attribute__((aligned(1))) Eight;
+  // (blocks behind the last: 2^-127, their codes are zeros)
+  auto loadScales = [&]() __attribute__((always_inline)) {
+    unsigned long v = 0;
+    if (ahead >= 8) {
+      v = *reinterpret_cast<const Eight*>(from);
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < ahead; ++j) v |= (unsigned long)from[j] << 8 * j;
     }
-    sum = multiply(a, sa, c, sc, sum);
-  }
-  const long m = m0 + lane % 16;
-  if (m >= p.M) return;
+    from += 8;
+    ahead -= 8;
+    return v;
+  };
+  auto storeScales = [&](unsigned long v, int to) __attribute__((always_inline)) {
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
-    const long n = n0 + lane / 16 * 4 + v;
-    if (n >= p.N) break;
-    float z = activate(sum[v] + lineOr(p.bias, n, 0.f), p.activation);
-    if (p.residual.data) z += (float)static_cast<const T*>(p.residual.data)[m * p.residual.row + n * p.residual.col];
-    static_cast<T*>(p.y.data)[m * p.y.row + n * p.y.col] = (T)z;
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<unsigned short*>(scales[to] + place + q * 64) = (unsigned short)(v >> 16 * q);
+  };
+
+  floatx4 sum[RM][RN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  int left = (int)(end - first) * 8;  // 16-bit words of a row that are not on their way yet
+  auto load = [&](int q, char* to) __attribute__((always_inline)) {
+    if (q < A::loads)
+      a.load(q, left, to);
+    else
+      b.load(q - A::loads, left, to + A::bytes);
+  };
+  auto loaded = [&]() __attribute__((always_inline)) {
+    a.base += a.advance;
+    b.base += b.advance;
+    left -= 64;
+  };
+#pragma unroll
+  for (int q = 0; q < LOADS; ++q) load(q, space);
+  loaded();
+  const unsigned long scales0 = loadScales();
+#pragma unroll
+  for (int q = 0; q < LOADS; ++q) load(q, space + STEP);
+  loaded();
+  unsigned long coming = loadScales();  // of the step after the one that is multiplied
+  storeScales(scales0, 0);
+
+  const int laneA = A::laneAt(wm), laneB = B::laneAt(wn);
+  const int scaleA = wm / 32 * 256 + lane / 16 * 64 + lane % 16 * 4, scaleB = BM * 8 + wn / 32 * 256 + lane / 16 * 64 + lane % 16 * 4;
+  uintx4 fa[2][RM], fb[2][RN];
+  int sa[2][RM / 2], sb[2][RN / 2];
+  constexpr int READS = RM + RN;
+  auto read = [&](int q, int d, int h) __attribute__((always_inline)) {
+    const char* const at = space + d * STEP;
+    if (q < RN)
+      fb[h][q] = B::fragment(at + A::bytes, laneB, h, q);
+    else
+      fa[h][q - RN] = A::fragment(at, laneA, h, q - RN);
+  };
+  auto readScales = [&](int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < RM / 2; ++i) sa[d][i] = *reinterpret_cast<const int*>(scales[d] + scaleA + i * 256);
+#pragma unroll
+    for (int j = 0; j < RN / 2; ++j) sb[d][j] = *reinterpret_cast<const int*>(scales[d] + scaleB + j * 256);
+  };
+  // (the first step's words are there; at most the second's are on their way)
+  arrive<LOADS>();
+  readScales(0);
+#pragma unroll
+  for (int q = 0; q < READS; ++q) read(q, 0, 0);
+  auto round = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+#pragma unroll
+        for (int q = i * READS / RM; q < (i + 1) * READS / RM; ++q) read(q, d, 1);
+#pragma unroll
+        for (int j = 0; j < RN; ++j) sum[i][j] = multiplyAt<0>(j % 2, i % 2, fb[0][j], sb[d][j / 2], fa[0][i], sa[d][i / 2], sum[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      storeScales(coming, d ^ 1);
+      // the next step's operands are there, and this one's place is free: every wave has its fragments
+      arrive<0>();
+      readScales(d ^ 1);
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+#pragma unroll
+        for (int q = i * READS / RM; q < (i + 1) * READS / RM; ++q) read(q, d ^ 1, 0);
+#pragma unroll
+        for (int j = 0; j < RN; ++j) sum[i][j] = multiplyAt<1>(j % 2, i % 2, fb[1][j], sb[d][j / 2], fa[1][i], sa[d][i / 2], sum[i][j]);
+#pragma unroll
+        for (int q = i * LOADS / RM; q < (i + 1) * LOADS / RM; ++q) load(q, space + d * STEP);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      coming = loadScales();
+      loaded();
+      if (left <= -128) return false;  // that was the last step
+    }
+    return true;
+  };
+  while (round()) {
+  }
+
+  // (the loads requested behind the last step write zeros to LDS, which the results now go through)
+  arrive<0>();
+  constexpr int SHARE = 2 * STEP / WAVES, FIT = SHARE / (WN * 64);  // of LDS, to a wave; blocks of rows
+  constexpr int TURN = FIT >= RM ? RM : FIT >= 4 ? 4 : FIT >= 2 ? 2 : 1;
+  static_assert(FIT > 0 && RM % TURN == 0, "a wave's share of LDS holds whole rows of blocks");
+  leave<T, RM, RN, TURN>(g, blockIdx.y, m0 + wm, n0 + wn, sum, space + wave * SHARE);
+}
+
+// Few rows.  A workgroup: 16 rows of w and 16 RB of x, its waves a range of k each, straight from memory to the matrix
+// instructions (rows behind the last are the last again, and nobody takes their results); their sums meet in LDS.  READY: x
+// is quantised; else (RB = 1) a lane quantises the block that it hands to the instruction.
+template <class T, bool READY, int RB, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void fewRows(Mx4Args g, Matrix xv, long K, Divisor across) {
+  static_assert(READY || RB == 1, "quantised on the way: one fragment of rows");
+  constexpr int AHEAD = READY ? 4 : sizeof(T) == 2 ? 4 : 2;
+  __shared__ float sums[WAVES][RB * 256];
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int band = quotient(blockIdx.x, across);
+  const long n0 = (long)(blockIdx.x - band * across.value) * 16, m0 = (long)band * (16 * RB);
+  const long n = min(n0 + lane % 16, g.N - 1);
+  const unsigned char *const w = g.w.codes + n * g.w.codeStride, *const ws = g.w.scales + n * g.w.scaleStride;
+  const long share = (g.blocks + WAVES * 4 - 1) / (WAVES * 4) * 4, first = wave * share, end = min(first + share, g.blocks);
+  floatx4 sum[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) sum[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (long b0 = first; b0 < end; b0 += 4 * AHEAD) {
+    uintx4 cw[AHEAD], cx[AHEAD][RB];
+    int sw[AHEAD], sx[AHEAD][RB];
+    Values<T, 32> v[READY ? 1 : AHEAD];
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      const long b = b0 + 4 * s + lane / 16;
+      const bool there = b < end;  // (else zeros times 2^-127)
+      cw[s] = there ? *reinterpret_cast<const uintx4*>(w + 16 * b) : uintx4{0, 0, 0, 0};
+      sw[s] = there ? ws[b] : 0;
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const long m = min(m0 + 16 * i + lane % 16, g.M - 1);
+        if constexpr (READY) {
+          cx[s][i] = there ? *reinterpret_cast<const uintx4*>(g.x.codes + m * g.x.codeStride + 16 * b) : uintx4{0, 0, 0, 0};
+          sx[s][i] = there ? g.x.scales[m * g.x.scaleStride + b] : 0;
+        } else {
+          v[s].load(static_cast<const T*>(xv.data) + m * xv.row + 32 * b, there ? K - 32 * b : 0);
+        }
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      if constexpr (!READY) {
+        sx[s][0] = scaleOf(v[s].most());
+#pragma unroll
+        for (int q = 0; q < 4; ++q) cx[s][0][q] = v[s].codes(q, sx[s][0]);
+      }
+#pragma unroll
+      for (int i = 0; i < RB; ++i) sum[i] = multiply<0, 0>(cw[s], sw[s], cx[s][i], sx[s][i], sum[i]);
+    }
+  }
+  // (lane: row lane % 16 of x, four rows of w)
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sums[wave][(16 * i + lane % 16) * 16 + lane / 16 * 4 + q] = sum[i][q];
+  __syncthreads();
+  for (int at = threadIdx.x; at < RB * 256; at += WAVES * 64) {
+    const long m = m0 + at / 16, o = n0 + at % 16;
+    if (m >= g.M || o >= g.N) continue;
+    float z = lineOr(g.e.bias, o, 0.f);
+#pragma unroll
+    for (int q = 0; q < WAVES; ++q) z += sums[q][at];
+    z = activate(z, g.e.activation);
+    if (g.e.residual.data) z += (float)static_cast<const T*>(g.e.residual.data)[m * g.e.residual.row + o * g.e.residual.col];
+    static_cast<T*>(g.e.out.data)[m * g.e.out.row + o * g.e.out.col] = (T)z;
   }
 }
 
-size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+// ---- what runs ----
+
+struct Mx4Plan {
+  enum Kind { Few, Tiles } kind;
+  long ranges, range;  // of k, in blocks
+};
+
+Mx4Plan planOf(long M, long blocks, long N) {
+  if (M <= 64 || blocks == 0) return {Mx4Plan::Few, 1, blocks};
+  const long tiles = ceilDivLong(M, 128) * ceilDivLong(N, 128), slots = 2l * computeUnits();
+  long ranges = 1;
+  while (tiles * ranges * 2 <= slots && blocks / (ranges * 2) >= 16) ranges *= 2;
+  const long range = ceilDivLong(ceilDivLong(blocks, ranges), 8) * 8;
+  return {Mx4Plan::Tiles, ceilDivLong(blocks, range), range};
+}
+
+// whether x, of neighbouring values, is quantised by the product itself
+bool onTheWay(long M) { return M <= 16; }
 
 template <class T>
-int run(LinearMx4Problem p, hipStream_t s) {
-  const double groups = (double)((p.M + 15) / 16) * ((p.N + 15) / 16) / 4 + 1;
-  if (!launches(groups, 256)) return FBFFT_UNSUPPORTED_SIZE;
-  if (p.x.data && p.blocks > 0) {
-    p.xq = Mx4{static_cast<unsigned char*>(p.workspace), static_cast<unsigned char*>(p.workspace) + rounded((size_t)p.M * p.blocks * 16),
-               16 * p.blocks, p.blocks};
-    const int rc = launchMx4Quantize(p.x, p.type, p.M, p.K, p.xq, s);
+int run(const LinearMx4Problem& p, hipStream_t s) {
+  const Mx4Plan plan = planOf(p.M, p.blocks, p.N);
+  Mx4Args g{p.xq, p.w, p.M, p.N, p.blocks, plan.range, Epilogue{p.y, p.residual, {}, p.bias, p.activation, false, nullptr}};
+  g.e.dense = p.y.col == 1 && (!p.residual.data || p.residual.col == 1);
+  char* space = static_cast<char*>(p.workspace);
+  const bool few = plan.kind == Mx4Plan::Few, quantizes = p.x.data && p.blocks > 0 && !(few && onTheWay(p.M) && p.x.col == 1);
+  const long across = ceilDivLong(p.N, 16), down = ceilDivLong(p.M, p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64);
+  const long groups = few ? across * down : (ceilDivLong(p.M, 128) * ceilDivLong(p.N, 128) + 7) / 8 * 8;
+  const JoinPlan join = plan.ranges > 1 ? joinOf(g.e.dense, p.M, p.N, plan.ranges) : JoinPlan{};
+  if (!launches((double)groups * plan.ranges, few ? 512 : 256) || !launches(join.blocks, 256)) return FBFFT_UNSUPPORTED_SIZE;
+  if (quantizes) {
+    g.x = Mx4{reinterpret_cast<unsigned char*>(space), reinterpret_cast<unsigned char*>(space) + rounded((size_t)p.M * p.blocks * 16),
+              16 * p.blocks, p.blocks};
+    space += rounded((size_t)p.M * p.blocks * 16) + rounded((size_t)p.M * p.blocks);
+    const int rc = launchMx4Quantize(p.x, p.type, p.M, p.K, g.x, s);
     if (rc != FBFFT_SUCCESS) return rc;
   }
-  product<T><<<dim3((unsigned)groups), 256, 0, s>>>(p);
+  if (few) {
+    const dim3 grid((unsigned)groups);
+    const Divisor d = divisorOf(across);
+    if (p.x.data && !quantizes)
+      fewRows<T, false, 1, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
+    else if (p.M <= 16)
+      fewRows<T, true, 1, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
+    else if (p.M <= 32)
+      fewRows<T, true, 2, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
+    else
+      fewRows<T, true, 4, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
+    return launchStatus();
+  }
+  if (plan.ranges > 1) g.e.parts = reinterpret_cast<float*>(space);
+  product<T, 128, 128, 64, 64><<<dim3((unsigned)groups, (unsigned)plan.ranges), 256, 0, s>>>(g);
+  if (plan.ranges > 1) launchJoin<T>(join, g.e, p.M, p.N, (int)plan.ranges, s);
   return launchStatus();
 }
 
@@ -192,7 +481,11 @@ int launchMx4Dequantize(const Mx4& from, const Matrix& y, int type, long M, long
   });
 }
 
-size_t linearMx4WorkspaceBytes(long M, long blocks, long) { return rounded((size_t)M * blocks * 16) + rounded((size_t)M * blocks); }
+size_t linearMx4WorkspaceBytes(long M, long blocks, long N) {
+  const Mx4Plan plan = planOf(M, blocks, N);
+  const size_t rows = rounded((size_t)M * blocks * 16) + rounded((size_t)M * blocks);  // (x, where it is not on the way)
+  return rows + (plan.ranges > 1 ? rounded((size_t)plan.ranges * M * N * sizeof(float)) : 0);
+}
 
 int launchLinearMx4(const LinearMx4Problem& p, hipStream_t s) {
   if (p.type == FBFFT_FLOAT32) return run<float>(p, s);
