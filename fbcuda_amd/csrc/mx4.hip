@@ -196,8 +196,9 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
   typedef Packed<BN, WAVES> B;
   constexpr int SCALES = (BM + BN) * 8, STEP = A::bytes + B::bytes, LOADS = A::loads + B::loads;
   static_assert(BM + BN == WAVES * 64 && BM % 32 == 0 && WM % 32 == 0 && WN % 32 == 0, "a row's scales to a thread");
-  __shared__ __attribute__((aligned(1024))) char space[2 * STEP];
-  __shared__ __attribute__((aligned(16))) char scales[2][SCALES];
+  // (one array: of two, the compiler makes every read of LDS wait for the loads on their way to it)
+  __shared__ __attribute__((aligned(1024))) char space[2 * STEP + 2 * SCALES];
+  char* const scales = space + 2 * STEP;
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
   const Tile<BM, BN> tile(g.M, g.N);
@@ -217,8 +218,10 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
   const int place = (ofA ? 0 : BM * 8) + row / 32 * 256 + row % 16 * 4 + row / 16 % 2 * 2;
   int ahead = (int)(end - first);  // blocks whose scales are not loaded yet
   typedef unsigned long __attribute__((aligned(1))) Eight;
-  // (blocks behind the last: 2^-127, their codes are zeros)
-  auto loadScales = [&]() __attribute__((always_inline)) {
+  // The next eight scales; behind the last block 2^-127 (whose codes are zeros).  Of the first step there may be fewer than eight;
+  // later ones, if there is anything left, have eight in front of the end.  (Without a branch, which the order of the loop's
+  // instructions would not outlive: what is not wanted is read from the codes.)
+  auto firstScales = [&]() __attribute__((always_inline)) {
     unsigned long v = 0;
     if (ahead >= 8) {
       v = *reinterpret_cast<const Eight*>(from);
@@ -230,9 +233,17 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
     ahead -= 8;
     return v;
   };
+  unsigned long coming;  // scales of the step after the one that is multiplied, so many of them behind the end
+  int behind;
+  auto nextScales = [&]() __attribute__((always_inline)) {
+    behind = min(max(8 - ahead, 0), 7);
+    coming = *reinterpret_cast<const Eight*>(ahead > 0 ? from - behind : g.x.codes);
+    from += 8;
+    ahead -= 8;
+  };
   auto storeScales = [&](unsigned long v, int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) *reinterpret_cast<unsigned short*>(scales[to] + place + q * 64) = (unsigned short)(v >> 16 * q);
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<unsigned short*>(scales + to * SCALES + place + q * 64) = (unsigned short)(v >> 16 * q);
   };
 
   floatx4 sum[RM][RN];
@@ -256,62 +267,70 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
 #pragma unroll
   for (int q = 0; q < LOADS; ++q) load(q, space);
   loaded();
-  const unsigned long scales0 = loadScales();
+  const unsigned long scales0 = firstScales();
 #pragma unroll
   for (int q = 0; q < LOADS; ++q) load(q, space + STEP);
   loaded();
-  unsigned long coming = loadScales();  // of the step after the one that is multiplied
+  nextScales();
   storeScales(scales0, 0);
 
   const int laneA = A::laneAt(wm), laneB = B::laneAt(wn);
   const int scaleA = wm / 32 * 256 + lane / 16 * 64 + lane % 16 * 4, scaleB = BM * 8 + wn / 32 * 256 + lane / 16 * 64 + lane % 16 * 4;
-  uintx4 fa[2][RM], fb[2][RN];
+  // A step is 2 RM groups of RN matrix instructions, of one fragment of x each, which is read two groups ahead
+  constexpr int GROUPS = 2 * RM, AHEAD = 2, RING = 4;
+  static_assert(GROUPS % RING == 0 && RN <= RM && RN % AHEAD == 0 && LOADS % AHEAD == 0, "whole turns");
+  uintx4 fa[RING], fb[2][RN];
   int sa[2][RM / 2], sb[2][RN / 2];
-  constexpr int READS = RM + RN;
-  auto read = [&](int q, int d, int h) __attribute__((always_inline)) {
-    const char* const at = space + d * STEP;
-    if (q < RN)
-      fb[h][q] = B::fragment(at + A::bytes, laneB, h, q);
-    else
-      fa[h][q - RN] = A::fragment(at, laneA, h, q - RN);
-  };
+  auto readA = [&](int t, int d) __attribute__((always_inline)) { fa[t % RING] = A::fragment(space + d * STEP, laneA, t / RM, t % RM); };
+  auto readB = [&](int j, int h, int d) __attribute__((always_inline)) { fb[h][j] = B::fragment(space + d * STEP + A::bytes, laneB, h, j); };
   auto readScales = [&](int d) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < RM / 2; ++i) sa[d][i] = *reinterpret_cast<const int*>(scales[d] + scaleA + i * 256);
+    for (int i = 0; i < RM / 2; ++i) sa[d][i] = *reinterpret_cast<const int*>(scales + d * SCALES + scaleA + i * 256);
 #pragma unroll
-    for (int j = 0; j < RN / 2; ++j) sb[d][j] = *reinterpret_cast<const int*>(scales[d] + scaleB + j * 256);
+    for (int j = 0; j < RN / 2; ++j) sb[d][j] = *reinterpret_cast<const int*>(scales + d * SCALES + scaleB + j * 256);
   };
   // (the first step's words are there; at most the second's are on their way)
   arrive<LOADS>();
   readScales(0);
 #pragma unroll
-  for (int q = 0; q < READS; ++q) read(q, 0, 0);
+  for (int j = 0; j < RN; ++j) readB(j, 0, 0);
+#pragma unroll
+  for (int t = 0; t < AHEAD; ++t) readA(t, 0);
   auto round = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
 #pragma unroll
-      for (int i = 0; i < RM; ++i) {
+      for (int t = 0; t < GROUPS; ++t) {
+        const int last = t - (GROUPS - AHEAD);  // of the step's last groups
+        if (last == 0) {
+          // every wave has this step's fragments, so that its place is free, and the next step's operands are there
+          storeScales(coming >> 8 * behind, d ^ 1);
+          arrive<0>();
+          readScales(d ^ 1);
+        }
+        if (last < 0) {
+          readA(t + AHEAD, d);
+          if (t < RN) readB(t, 1, d);
+        } else {
+          readA(last, d ^ 1);
 #pragma unroll
-        for (int q = i * READS / RM; q < (i + 1) * READS / RM; ++q) read(q, d, 1);
+          for (int j = last * (RN / AHEAD); j < (last + 1) * (RN / AHEAD); ++j) readB(j, 0, d ^ 1);
+        }
 #pragma unroll
-        for (int j = 0; j < RN; ++j) sum[i][j] = multiplyAt<0>(j % 2, i % 2, fb[0][j], sb[d][j / 2], fa[0][i], sa[d][i / 2], sum[i][j]);
+        for (int j = 0; j < RN; ++j) {
+          const int i = t % RM;
+          if (t < RM)
+            sum[i][j] = multiplyAt<0>(j % 2, i % 2, fb[0][j], sb[d][j / 2], fa[t % RING], sa[d][i / 2], sum[i][j]);
+          else
+            sum[i][j] = multiplyAt<1>(j % 2, i % 2, fb[1][j], sb[d][j / 2], fa[t % RING], sa[d][i / 2], sum[i][j]);
+        }
+        if (last >= 0) {
+#pragma unroll
+          for (int q = last * (LOADS / AHEAD); q < (last + 1) * (LOADS / AHEAD); ++q) load(q, space + d * STEP);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
-      storeScales(coming, d ^ 1);
-      // the next step's operands are there, and this one's place is free: every wave has its fragments
-      arrive<0>();
-      readScales(d ^ 1);
-#pragma unroll
-      for (int i = 0; i < RM; ++i) {
-#pragma unroll
-        for (int q = i * READS / RM; q < (i + 1) * READS / RM; ++q) read(q, d ^ 1, 0);
-#pragma unroll
-        for (int j = 0; j < RN; ++j) sum[i][j] = multiplyAt<1>(j % 2, i % 2, fb[1][j], sb[d][j / 2], fa[1][i], sa[d][i / 2], sum[i][j]);
-#pragma unroll
-        for (int q = i * LOADS / RM; q < (i + 1) * LOADS / RM; ++q) load(q, space + d * STEP);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      coming = loadScales();
+      nextScales();
       loaded();
       if (left <= -128) return false;  // that was the last step
     }
@@ -328,125 +347,227 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
   leave<T, RM, RN, TURN>(g, blockIdx.y, m0 + wm, n0 + wn, sum, space + wave * SHARE);
 }
 
-// Few rows.  A workgroup: 16 rows of w and 16 RB of x, its waves a range of k each, straight from memory to the matrix
-// instructions (rows behind the last are the last again, and nobody takes their results); their sums meet in LDS.  READY: x
-// is quantised; else (RB = 1) a lane quantises the block that it hands to the instruction.
-template <class T, bool READY, int RB, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void fewRows(Mx4Args g, Matrix xv, long K, Divisor across) {
-  static_assert(READY || RB == 1, "quantised on the way: one fragment of rows");
-  constexpr int AHEAD = READY ? 4 : sizeof(T) == 2 ? 4 : 2;
-  __shared__ float sums[WAVES][RB * 256];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int band = quotient(blockIdx.x, across);
-  const long n0 = (long)(blockIdx.x - band * across.value) * 16, m0 = (long)band * (16 * RB);
-  const long n = min(n0 + lane % 16, g.N - 1);
-  const unsigned char *const w = g.w.codes + n * g.w.codeStride, *const ws = g.w.scales + n * g.w.scaleStride;
-  const long share = (g.blocks + WAVES * 4 - 1) / (WAVES * 4) * 4, first = wave * share, end = min(first + share, g.blocks);
-  floatx4 sum[RB];
+// Few rows.  A workgroup: 16 NB rows of w and 16 RB of x, its waves a range of k each, w straight from memory to the matrix
+// instructions (rows behind the last are the last again, and nobody takes their results); their sums meet in LDS.  WAY (RB =
+// 1): the workgroup quantises x to LDS by itself, while the first of w are on their way; else x is quantised already.
+constexpr int kFewWaves = 8;
+
+struct FewArgs {
+  Mx4Args g;
+  Matrix x;
+  long K;
+  Divisor across, words;  // workgroups to a band of rows; of eight values to a row of x
+  int pitch, scales;      // of x in LDS: bytes from a row to the next, and in front of the scales
+};
+
+template <class T, bool WAY, int RB, int NB, int AHEAD>
+__global__ __launch_bounds__(kFewWaves * 64) void fewRows(FewArgs f) {
+  static_assert(!WAY || RB == 1, "quantised on the way: 16 rows at most");
+  extern __shared__ __attribute__((aligned(16))) char space[];  // x, then the sums
+  const Mx4Args& g = f.g;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, band = quotient(blockIdx.x, f.across);
+  const long n0 = (long)(blockIdx.x - band * f.across.value) * (16 * NB), m0 = (long)band * (16 * RB);
+  const unsigned char *w[NB], *ws[NB], *x[RB], *xs[RB];
 #pragma unroll
-  for (int i = 0; i < RB; ++i) sum[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (long b0 = first; b0 < end; b0 += 4 * AHEAD) {
-    uintx4 cw[AHEAD], cx[AHEAD][RB];
-    int sw[AHEAD], sx[AHEAD][RB];
-    Values<T, 32> v[READY ? 1 : AHEAD];
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) {
-      const long b = b0 + 4 * s + lane / 16;
-      const bool there = b < end;  // (else zeros times 2^-127)
-      cw[s] = there ? *reinterpret_cast<const uintx4*>(w + 16 * b) : uintx4{0, 0, 0, 0};
-      sw[s] = there ? ws[b] : 0;
-#pragma unroll
-      for (int i = 0; i < RB; ++i) {
-        const long m = min(m0 + 16 * i + lane % 16, g.M - 1);
-        if constexpr (READY) {
-          cx[s][i] = there ? *reinterpret_cast<const uintx4*>(g.x.codes + m * g.x.codeStride + 16 * b) : uintx4{0, 0, 0, 0};
-          sx[s][i] = there ? g.x.scales[m * g.x.scaleStride + b] : 0;
-        } else {
-          v[s].load(static_cast<const T*>(xv.data) + m * xv.row + 32 * b, there ? K - 32 * b : 0);
-        }
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s) {
-      if constexpr (!READY) {
-        sx[s][0] = scaleOf(v[s].most());
-#pragma unroll
-        for (int q = 0; q < 4; ++q) cx[s][0][q] = v[s].codes(q, sx[s][0]);
-      }
-#pragma unroll
-      for (int i = 0; i < RB; ++i) sum[i] = multiply<0, 0>(cw[s], sw[s], cx[s][i], sx[s][i], sum[i]);
-    }
+  for (int j = 0; j < NB; ++j) {
+    const long n = min(n0 + 16 * j + lane % 16, g.N - 1);
+    w[j] = g.w.codes + n * g.w.codeStride, ws[j] = g.w.scales + n * g.w.scaleStride;
   }
-  // (lane: row lane % 16 of x, four rows of w)
+  const int share = (int)((g.blocks + kFewWaves * 4 - 1) / (kFewWaves * 4) * 4), first = wave * share, end = min(first + share, (int)g.blocks);
+  uintx4 cw[AHEAD][NB];
+  int sw[AHEAD][NB];
+  // (blocks behind the last: the last again, and then zeros times 2^-127)
+  auto load = [&](int b0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      const int b = min(b0 + 4 * s + lane / 16, end - 1);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        cw[s][j] = *reinterpret_cast<const uintx4*>(w[j] + 16 * b);
+        sw[s][j] = ws[j][b];
+      }
+    }
+  };
+  if (first < end) load(first);
+  if constexpr (WAY) {
+    const int words = (int)(g.M - m0 < 16 ? g.M - m0 : 16) * (int)f.words.value;
+    for (int i = threadIdx.x; i < words; i += kFewWaves * 64) {  // (a block's four lanes together: f.words is a multiple of four)
+      const int m = quotient(i, f.words), word = i - m * (int)f.words.value;
+      Values<T, 8> v;
+      v.load(static_cast<const T*>(f.x.data) + (m0 + m) * f.x.row + 8l * word, f.K - 8l * word);
+      const int scale = scaleOf(mostOfFour(v.most()));
+      *reinterpret_cast<unsigned*>(space + m * f.pitch + 4 * word) = v.codes(0, scale);
+      if (word % 4 == 0) space[f.scales + m * (f.pitch / 16) + word / 4] = (char)scale;
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const long m = min(m0 + 16 * i + lane % 16, g.M - 1);
+    x[i] = WAY ? reinterpret_cast<unsigned char*>(space) + (m - m0) * f.pitch : g.x.codes + m * g.x.codeStride;
+    xs[i] = WAY ? reinterpret_cast<unsigned char*>(space) + f.scales + (m - m0) * (f.pitch / 16) : g.x.scales + m * g.x.scaleStride;
+  }
+  floatx4 sum[RB][NB];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sums[wave][(16 * i + lane % 16) * 16 + lane / 16 * 4 + q] = sum[i][q];
-  __syncthreads();
-  for (int at = threadIdx.x; at < RB * 256; at += WAVES * 64) {
-    const long m = m0 + at / 16, o = n0 + at % 16;
-    if (m >= g.M || o >= g.N) continue;
-    float z = lineOr(g.e.bias, o, 0.f);
+    for (int j = 0; j < NB; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int b0 = first; b0 < end;) {
 #pragma unroll
-    for (int q = 0; q < WAVES; ++q) z += sums[q][at];
-    z = activate(z, g.e.activation);
-    if (g.e.residual.data) z += (float)static_cast<const T*>(g.e.residual.data)[m * g.e.residual.row + o * g.e.residual.col];
-    static_cast<T*>(g.e.out.data)[m * g.e.out.row + o * g.e.out.col] = (T)z;
+    for (int s = 0; s < AHEAD; ++s) {
+      const int at = b0 + 4 * s + lane / 16, b = min(at, end - 1);
+      const bool there = at < end;
+#pragma unroll
+      for (int i = 0; i < RB; ++i) {
+        const uintx4 c = *reinterpret_cast<const uintx4*>(x[i] + 16 * b);
+        const int sx = there ? xs[i][b] : 0;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+          sum[i][j] = multiply<0, 0>(there ? cw[s][j] : uintx4{0, 0, 0, 0}, there ? sw[s][j] : 0, c, sx, sum[i][j]);
+      }
+    }
+    b0 += 4 * AHEAD;
+    if (b0 < end) load(b0);
   }
+  if (WAY) __syncthreads();
+  // (lane: row lane % 16 of x, four rows of w)
+  float* const sums = reinterpret_cast<float*>(space);
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sums[wave * (RB * NB * 256) + (16 * i + lane % 16) * (16 * NB) + 16 * j + lane / 16 * 4 + q] = sum[i][j][q];
+  __syncthreads();
+  for (int at = threadIdx.x; at < RB * NB * 256; at += kFewWaves * 64) {
+    const long m = m0 + at / (16 * NB), n = n0 + at % (16 * NB);
+    if (m >= g.M || n >= g.N) continue;
+    float z = lineOr(g.e.bias, n, 0.f);
+#pragma unroll
+    for (int q = 0; q < kFewWaves; ++q) z += sums[q * (RB * NB * 256) + at];
+    z = activate(z, g.e.activation);
+    if (g.e.residual.data) z += (float)static_cast<const T*>(g.e.residual.data)[m * g.e.residual.row + n * g.e.residual.col];
+    static_cast<T*>(g.e.out.data)[m * g.e.out.row + n * g.e.out.col] = (T)z;
+  }
+}
+
+// of x in LDS: rows of codes 16 bytes apart, and their scales
+size_t fewBytes(long M, long blocks) { return std::min(M, 16l) * 17 * (blocks + 1); }
+
+template <class T, bool WAY, int RB, int NB>
+void launchFew(FewArgs f, hipStream_t s) {
+  const long across = ceilDivLong(f.g.N, 16 * NB);
+  f.across = divisorOf(across), f.words = divisorOf(4 * f.g.blocks);
+  f.pitch = (int)(16 * f.g.blocks + 16), f.scales = (int)std::min(f.g.M, 16l) * f.pitch;
+  const size_t rows = WAY ? fewBytes(f.g.M, f.g.blocks) : 0, bytes = std::max(rows, sizeof(float) * kFewWaves * RB * NB * 256);
+  const dim3 grid((unsigned)(across * ceilDivLong(f.g.M, 16 * RB)));
+  constexpr int most = RB * NB > 2 ? 2 : 4;
+  const int steps = (int)ceilDivLong(f.g.blocks, 4 * kFewWaves);
+  if (steps <= 1)
+    fewRows<T, WAY, RB, NB, 1><<<grid, kFewWaves * 64, bytes, s>>>(f);
+  else if (steps <= 2)
+    fewRows<T, WAY, RB, NB, 2><<<grid, kFewWaves * 64, bytes, s>>>(f);
+  else
+    fewRows<T, WAY, RB, NB, most><<<grid, kFewWaves * 64, bytes, s>>>(f);
 }
 
 // ---- what runs ----
 
+// The kernel of a product: its tile, or its fragments of x and w, and the ranges that k is cut into.
 struct Mx4Plan {
-  enum Kind { Few, Tiles } kind;
-  long ranges, range;  // of k, in blocks
+  enum Kind { Way, Few, Tiles };
+  int kind, rows, cols;  // Way, Few: RB and NB; Tiles: of a tile
+  long ranges, range;    // blocks
 };
 
-Mx4Plan planOf(long M, long blocks, long N) {
-  if (M <= 64 || blocks == 0) return {Mx4Plan::Few, 1, blocks};
-  const long tiles = ceilDivLong(M, 128) * ceilDivLong(N, 128), slots = 2l * computeUnits();
-  long ranges = 1;
-  while (tiles * ranges * 2 <= slots && blocks / (ranges * 2) >= 16) ranges *= 2;
-  const long range = ceilDivLong(ceilDivLong(blocks, ranges), 8) * 8;
-  return {Mx4Plan::Tiles, ceilDivLong(blocks, range), range};
-}
+constexpr size_t kWayMost = 64 << 10;  // of LDS, for x that a workgroup quantises
 
-// whether x, of neighbouring values, is quantised by the product itself
-bool onTheWay(long M) { return M <= 16; }
+// The kernel with the least expected time, in us, from what each takes for a block of k and for the rest: few rows 3.3 and a
+// launch more where x is quantised in front of it, and for each block and workgroup the numbers below, but no less than 230
+// workgroups' (fewer leave compute units idle); tiles for each step of eight blocks alone or shared with another workgroup, and
+// for their results.  (`way`: whether the workgroups may quantise x, which rows one by one are read for: 0.07 ns of a
+// block at one row, 0.144 at 16.)  Measured on rows from 1 to 1024 and weights of 256 x 256 to 8192 x 8192, each kernel with
+// each number of ranges: 1 x 2048 x 8192 5.5 us on the way and 7.2 in two launches, 128 x 1151 x 1000 6.0 and 7.0, tiles 11.6;
+// 32 x 8192 x 8192 21.8 and tiles in four ranges 19.6; 8192 x 8192 x 8192 in tiles of 256 282, of 128 377.
+Mx4Plan planOf(long M, long blocks, long N, bool way) {
+  if (blocks == 0) return {Mx4Plan::Few, 1, 1, 1, 0};
+  Mx4Plan best{};
+  double least = 0;
+  auto offer = [&](const Mx4Plan& plan, double time) {
+    if (least == 0 || time < least) least = time, best = plan;
+  };
+  auto few = [&](int kind, int rows, int cols, double base, double each) {
+    const double groups = (double)ceilDivLong(M, 16 * rows) * ceilDivLong(N, 16 * cols);
+    offer({kind, rows, cols, 1, blocks}, base + std::max(groups, 230.0) * blocks * each);
+  };
+  const double x = (double)std::min(M, 16l);
+  if (way && fewBytes(M, blocks) <= kWayMost) {
+    few(Mx4Plan::Way, 1, 1, 3.3, (0.068 + 0.0047 * x) / 1e3);
+    few(Mx4Plan::Way, 1, 2, 3.3, (0.15 + 0.0046 * x) / 1e3);
+  }
+  static const double each[3][2] = {{0.106, 0.157}, {0.157, 0.226}, {0.32, 0.42}};
+  for (int r = 0; r < 3; ++r)
+    for (int c = 0; c < 2; ++c) few(Mx4Plan::Few, 1 << r, 1 << c, 5.7, each[r][c] / 1e3);
+  struct Option {
+    int side, together;  // together: workgroups that share a compute unit
+    double alone, shared, results;
+  };
+  static const Option options[] = {{128, 2, 1.0, 1.34, 4.4}, {256, 1, 1.9, 1.9, 8}};
+  const int units = computeUnits();
+  for (const Option& a : options) {
+    const long tiles = ceilDivLong(M, a.side) * ceilDivLong(N, a.side);
+    for (long ranges = 1; ranges <= 32; ranges *= 2) {
+      const long range = ceilDivLong(ceilDivLong(blocks, ranges), 8) * 8, used = ceilDivLong(blocks, range);
+      if (ranges > 1 && range < 16) break;
+      const long groups = tiles * used, slots = (long)units * a.together;
+      const double step = groups <= units ? a.alone : a.shared;
+      const double rounds = groups <= slots ? 1.0 : std::max((double)groups / slots, groups < 4 * slots ? (double)ceilDivLong(groups, slots) : 1.0);
+      double time = 6.5 + rounds * (range / 8 * step + a.results);
+      if (used > 1) time += 2.5 + (double)M * N * used * 4 / 4e6;
+      offer({Mx4Plan::Tiles, a.side, a.side, used, range}, time);
+    }
+  }
+  return best;
+}
 
 template <class T>
 int run(const LinearMx4Problem& p, hipStream_t s) {
-  const Mx4Plan plan = planOf(p.M, p.blocks, p.N);
+  const Mx4Plan plan = planOf(p.M, p.blocks, p.N, p.x.data && p.x.col == 1);
   Mx4Args g{p.xq, p.w, p.M, p.N, p.blocks, plan.range, Epilogue{p.y, p.residual, {}, p.bias, p.activation, false, nullptr}};
   g.e.dense = p.y.col == 1 && (!p.residual.data || p.residual.col == 1);
   char* space = static_cast<char*>(p.workspace);
-  const bool few = plan.kind == Mx4Plan::Few, quantizes = p.x.data && p.blocks > 0 && !(few && onTheWay(p.M) && p.x.col == 1);
-  const long across = ceilDivLong(p.N, 16), down = ceilDivLong(p.M, p.M <= 16 ? 16 : p.M <= 32 ? 32 : 64);
-  const long groups = few ? across * down : (ceilDivLong(p.M, 128) * ceilDivLong(p.N, 128) + 7) / 8 * 8;
+  const bool tiles = plan.kind == Mx4Plan::Tiles;
+  const long rows = tiles ? plan.rows : 16 * plan.rows, cols = tiles ? plan.cols : 16 * plan.cols;
+  const long groups = ceilDivLong(p.M, rows) * ceilDivLong(p.N, cols) + (tiles ? 7 : 0), blocks = tiles ? groups / 8 * 8 : groups;
   const JoinPlan join = plan.ranges > 1 ? joinOf(g.e.dense, p.M, p.N, plan.ranges) : JoinPlan{};
-  if (!launches((double)groups * plan.ranges, few ? 512 : 256) || !launches(join.blocks, 256)) return FBFFT_UNSUPPORTED_SIZE;
-  if (quantizes) {
+  const int lanes = tiles ? plan.rows * 2 : kFewWaves * 64;
+  if (!launches((double)blocks * plan.ranges, lanes) || !launches(join.blocks, 256)) return FBFFT_UNSUPPORTED_SIZE;
+  if (p.x.data && p.blocks > 0 && plan.kind != Mx4Plan::Way) {
     g.x = Mx4{reinterpret_cast<unsigned char*>(space), reinterpret_cast<unsigned char*>(space) + rounded((size_t)p.M * p.blocks * 16),
               16 * p.blocks, p.blocks};
     space += rounded((size_t)p.M * p.blocks * 16) + rounded((size_t)p.M * p.blocks);
     const int rc = launchMx4Quantize(p.x, p.type, p.M, p.K, g.x, s);
     if (rc != FBFFT_SUCCESS) return rc;
   }
-  if (few) {
-    const dim3 grid((unsigned)groups);
-    const Divisor d = divisorOf(across);
-    if (p.x.data && !quantizes)
-      fewRows<T, false, 1, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
-    else if (p.M <= 16)
-      fewRows<T, true, 1, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
-    else if (p.M <= 32)
-      fewRows<T, true, 2, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
+  if (!tiles) {
+    const FewArgs f{g, p.x, p.K, {}, {}, 0, 0};
+    const bool two = plan.cols == 2;
+    if (plan.kind == Mx4Plan::Way)
+      two ? launchFew<T, true, 1, 2>(f, s) : launchFew<T, true, 1, 1>(f, s);
+    else if (plan.rows == 1)
+      two ? launchFew<T, false, 1, 2>(f, s) : launchFew<T, false, 1, 1>(f, s);
+    else if (plan.rows == 2)
+      two ? launchFew<T, false, 2, 2>(f, s) : launchFew<T, false, 2, 1>(f, s);
     else
-      fewRows<T, true, 4, 8><<<grid, 512, 0, s>>>(g, p.x, p.K, d);
+      two ? launchFew<T, false, 4, 2>(f, s) : launchFew<T, false, 4, 1>(f, s);
     return launchStatus();
   }
   if (plan.ranges > 1) g.e.parts = reinterpret_cast<float*>(space);
-  product<T, 128, 128, 64, 64><<<dim3((unsigned)groups, (unsigned)plan.ranges), 256, 0, s>>>(g);
+  const dim3 grid((unsigned)blocks, (unsigned)plan.ranges);
+  if (plan.rows == 256)
+    product<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(g);
+  else
+    product<T, 128, 128, 64, 64><<<grid, 256, 0, s>>>(g);
   if (plan.ranges > 1) launchJoin<T>(join, g.e, p.M, p.N, (int)plan.ranges, s);
   return launchStatus();
 }
@@ -482,9 +603,9 @@ int launchMx4Dequantize(const Mx4& from, const Matrix& y, int type, long M, long
 }
 
 size_t linearMx4WorkspaceBytes(long M, long blocks, long N) {
-  const Mx4Plan plan = planOf(M, blocks, N);
-  const size_t rows = rounded((size_t)M * blocks * 16) + rounded((size_t)M * blocks);  // (x, where it is not on the way)
-  return rows + (plan.ranges > 1 ? rounded((size_t)plan.ranges * M * N * sizeof(float)) : 0);
+  // (x, quantised in front of the product, and ranges' sums, whichever way x comes)
+  const long ranges = std::max(planOf(M, blocks, N, true).ranges, planOf(M, blocks, N, false).ranges);
+  return rounded((size_t)M * blocks * 16) + rounded((size_t)M * blocks) + (ranges > 1 ? rounded((size_t)ranges * M * N * sizeof(float)) : 0);
 }
 
 int launchLinearMx4(const LinearMx4Problem& p, hipStream_t s) {
