@@ -12,15 +12,16 @@
 //
 // A pair matrix has rows of a multiple of 32 columns, 32 leading pieces and then their 32 second pieces, 128 bytes: what a
 // matrix instruction takes of a row.  Rows and columns are filled up with zeros.
-#include "operators.h"
+#include "product.h"
 
 #include <algorithm>
+#include <cstdlib>
+#include <type_traits>
 
 namespace fbfft_amd {
 namespace {
 
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef half16 halfx8 __attribute__((ext_vector_type(8)));
+typedef half16 halfx4 __attribute__((ext_vector_type(4)));
 
 constexpr float kUnit = 1024.f;  // what stands for 1 in pieces
 
@@ -31,15 +32,13 @@ struct Pairs {
 };
 
 __device__ __forceinline__ long placeOf(const Pairs& m, long i, long j) { return 2 * (i * m.cols + j / 32 * 32) + j % 32; }
-__device__ __forceinline__ void storePair(const Pairs& m, long i, long j, float v) {
-  half16* const to = m.data + placeOf(m, i, j);
-  const half16 lead = (half16)v;
-  to[0] = lead;
-  to[32] = (half16)(v - (float)lead);
-}
-__device__ __forceinline__ float loadPair(const Pairs& m, long i, long j) {
-  const half16* const from = m.data + placeOf(m, i, j);
-  return (float)from[0] + (float)from[32];
+// eight values as their leading and second pieces
+__device__ __forceinline__ void splitEight(const float (&z)[8], halfx8& lead, halfx8& rest) {
+#pragma unroll
+  for (int v = 0; v < 8; ++v) {
+    lead[v] = (half16)z[v];
+    rest[v] = (half16)(z[v] - (float)lead[v]);
+  }
 }
 
 template <class T>
@@ -57,115 +56,614 @@ __device__ __forceinline__ double groupSum(double v, double* space) {
   return space[0] + space[1] + space[2] + space[3];
 }
 
-// Squares are summed in 64 bits: those of float32 values pass its range.
+// Eight neighbours of a line of `count` elements, from element j: zeros behind the last.
 template <class T>
-__global__ __launch_bounds__(256) void squares(Given<const T> g, long rows, long cols, double* sums) {
+__device__ __forceinline__ void loadEight(const T* line, long stride, long j, long count, float (&v)[8]) {
+  if (stride == 1 && j + 8 <= count) {
+    loadPack<T, 8>(line + j, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = j + q < count ? (float)line[(j + q) * stride] : 0.f;
+  }
+}
+
+// Squares are summed in 64 bits: those of float32 values pass its range.  (Lines are rows or columns, whichever elements are
+// neighbours; words: of eight elements to a line.)
+template <class T>
+__global__ __launch_bounds__(256) void squares(Given<const T> g, long lines, long count, Divisor words, double* sums) {
   __shared__ double space[4];
   const T* const from = g.data + blockIdx.y * g.batch;
+  const int total = (int)(lines * words.value);
   double sum = 0;
-  for (long i = blockIdx.x; i < rows; i += kShares)
-    for (long j = threadIdx.x; j < cols; j += 256) {
-      const double v = (double)(float)from[i * g.row + j * g.col];
-      sum += v * v;
-    }
+#pragma unroll 2
+  for (int at = (int)blockIdx.x * 256 + threadIdx.x; at < total; at += kShares * 256) {
+    const int i = quotient(at, words);
+    float v[8];
+    loadEight(from + i * g.row, g.col, 8l * (at - i * (int)words.value), count, v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) sum += (double)v[q] * (double)v[q];
+  }
   sum = groupSum(sum, space);
   if (threadIdx.x == 0) sums[blockIdx.y * kShares + blockIdx.x] = sum;
 }
 
-// X and its transpose from G: rows <= cols of them, up to the padded sizes.
-template <class T>
-__global__ __launch_bounds__(256) void begin(Given<const T> g, long rows, long cols, const double* sums, float eps, Pairs x, Pairs xt) {
+// X and its transpose from G, as pairs of a power of two times G; factors: what that leaves to 1 / (|G| + eps), from 1 to 2.  (So
+// the leading pieces hold 16-bit values by themselves.)  A workgroup: 64 x 64 elements, through LDS; LINES: columns are the
+// lines of neighbours.
+template <class T, bool LINES>
+__global__ __launch_bounds__(256) void begin(Given<const T> g, long rows, long cols, const double* sums, float eps, Pairs x, Pairs xt,
+                                             float* factors) {
+  constexpr int PITCH = 68;
   __shared__ double space[4];
-  const double norm = __builtin_sqrt(groupSum(sums[blockIdx.y * kShares + threadIdx.x], space));
-  const double by = (double)kUnit / (norm + (double)eps);
+  __shared__ __attribute__((aligned(16))) float tile[64 * PITCH];
+  const double by = (double)kUnit / (__builtin_sqrt(groupSum(sums[blockIdx.y * kShares + threadIdx.x], space)) + (double)eps);
+  // (0 and what is not finite leave no exponent: they go with the factor)
+  const bool normal = by > 0x1p-1000 && by < 0x1p1000;
+  const double power = normal ? __builtin_bit_cast(double, __builtin_bit_cast(unsigned long, by) & 0x7ff0000000000000ul) : 1.0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) factors[blockIdx.y] = (float)(by / power);
+  const int across = (int)((x.cols + 63) / 64), down = (int)blockIdx.x / across;
+  const long i0 = 64l * down, j0 = 64l * ((int)blockIdx.x - down * across);
+  const T* const from = g.data + blockIdx.y * g.batch;
+#pragma unroll
+  for (int at = threadIdx.x; at < 512; at += 256) {
+    const int line = at / 8, in = at % 8 * 8;
+    float v[8];
+    if (LINES) {
+      const long j = min(j0 + line, cols - 1);
+      loadEight(from + j * g.col, g.row, i0 + in, rows, v);
+    } else {
+      const long i = min(i0 + line, rows - 1);
+      loadEight(from + i * g.row, g.col, j0 + in, cols, v);
+    }
+    const bool there = LINES ? j0 + line < cols : i0 + line < rows;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) tile[LINES ? (in + q) * PITCH + line : line * PITCH + in + q] = there ? (float)((double)v[q] * power) : 0.f;
+  }
+  __syncthreads();
   x.data += blockIdx.y * x.batch, xt.data += blockIdx.y * xt.batch;
-  const long tall = xt.cols;  // rows of x
-  for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < tall * x.cols; at += (long)gridDim.x * 256) {
-    const long i = at / x.cols, j = at - i * x.cols;
-    const float v = i < rows && j < cols ? (float)((double)(float)g.data[blockIdx.y * g.batch + i * g.row + j * g.col] * by) : 0.f;
-    storePair(x, i, j, v);
-    storePair(xt, j, i, v);
+#pragma unroll
+  for (int at = threadIdx.x; at < 512; at += 256) {
+    const int line = at / 8, in = at % 8 * 8;
+    halfx8 lead, rest;
+    float z[8];
+    if (i0 + line < xt.cols && j0 + in < x.cols) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) z[q] = tile[line * PITCH + in + q];
+      splitEight(z, lead, rest);
+      half16* const to = x.data + placeOf(x, i0 + line, j0 + in);
+      *reinterpret_cast<halfx8*>(to) = lead;
+      *reinterpret_cast<halfx8*>(to + 32) = rest;
+    }
+    if (j0 + line < x.cols && i0 + in < xt.cols) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) z[q] = tile[(in + q) * PITCH + line];
+      splitEight(z, lead, rest);
+      half16* const to = xt.data + placeOf(xt, j0 + line, i0 + in);
+      *reinterpret_cast<halfx8*>(to) = lead;
+      *reinterpret_cast<halfx8*>(to + 32) = rest;
+    }
   }
 }
 
-__device__ __forceinline__ floatx4 multiply(halfx8 a, halfx8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void storeFour(half16* to, const float (&z)[4]) {
+  halfx4 lead, rest;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    lead[v] = (half16)z[v];
+    rest[v] = (half16)(z[v] - (float)lead[v]);
+  }
+  *reinterpret_cast<halfx4*>(to) = lead;
+  *reinterpret_cast<halfx4*>(to + 32) = rest;
+}
 
-struct PairProduct {
-  Pairs a, b;       // rows of both, k contiguous: a b^T
-  long M, N, K;     // padded
-  float by, beta;   // result: by (sum in units of 2^20) + beta old
+// ---- products ----
+
+__device__ __forceinline__ floatx4 multiply(uintx4 a, uintx4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+
+// a b^T of two pair matrices, and what becomes of it: z = by sum + beta old, to out, and to turned the other way round.
+struct PairArgs {
+  Pairs a, b;
+  long M, N, K, range;  // multiples of 32; k per range
+  float by, beta;
+  const float* factors;  // not null: of each matrix; `power` times in by, once in beta
+  int power;
   Pairs old, out, turned;  // old, turned: data may be null
+  bool symmetric;          // out is: tiles below the diagonal, and their mirror images
+  float* parts;            // not null: sums of each range, [matrix][range][tile][BM][BN], in place of results
 };
 
-// A wave: 32 x 32 results, straight from memory to the matrix instructions.  LAST: the result goes to the caller's matrix.
-template <class T, bool LAST>
-__global__ __launch_bounds__(256) void product(PairProduct p, Given<T> y, long rows, long cols, float scale) {
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const long across = p.N / 32, tile = blockIdx.x * 4l + wave, m0 = tile / across * 32, n0 = tile % across * 32;
-  if (m0 >= p.M) return;
-  const half16 *const a = p.a.data + blockIdx.y * p.a.batch, *const b = p.b.data + blockIdx.y * p.b.batch;
-  floatx4 sum[2][2] = {};
-  for (long k = 0; k < p.K; k += 32) {
-    halfx8 fa[2][2], fb[2][2];  // [block of rows][piece]
+// where the last product leaves its results, times a factor
+template <class T>
+struct Result {
+  Given<T> y;
+  long rows, cols;
+  float scale;
+};
+struct Nothing {};
+
+// 32 rows by COLS (64) columns of results from row m0 and column n0, both multiples of 32, by one wave: eight(row, column, v)
+// gives eight neighbouring sums.  Results that go the other way round meet in LDS, 32 x (COLS + 4) numbers.
+template <int COLS, class RESULT, class EIGHT>
+__device__ __forceinline__ void leavePairs(const PairArgs& g, const RESULT& result, long matrix, long m0, long n0, bool mirror,
+                                           float* space, EIGHT eight) {
+  constexpr int LANES = COLS / 8, ROWS = 64 / LANES, PITCH = COLS + 4;
+  constexpr bool LAST = !__is_same(RESULT, Nothing);
+  const int lane = threadIdx.x % 64, c = lane % LANES * 8;
+  bool turns = mirror;
+  if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1;
+  const bool inside = n0 + c < g.N;  // (N is a multiple of 32)
+  const float factor = g.factors ? g.factors[matrix] : 1.f, by = g.by * factor * (g.power == 2 ? factor : 1.f), beta = g.beta * factor;
+#pragma unroll 1
+  for (int row = lane / LANES; row < 32; row += ROWS) {
+    const long m = m0 + row, n = n0 + c;
+    float z[8];
+    eight(row, c, z);
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int v = 0; v < 8; ++v) z[v] *= by;
+    if (inside && m < g.M) {
+      if (g.old.data) {
+        const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m, n);
+        const halfx8 lead = *reinterpret_cast<const halfx8*>(from), rest = *reinterpret_cast<const halfx8*>(from + 32);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const long in = 2 * k + 32 * q + lane / 16 * 8;
-        fa[i][q] = *reinterpret_cast<const halfx8*>(a + 2 * (m0 + 16 * i + lane % 16) * p.a.cols + in);
-        fb[i][q] = *reinterpret_cast<const halfx8*>(b + 2 * (n0 + 16 * i + lane % 16) * p.b.cols + in);
+        for (int v = 0; v < 8; ++v) z[v] += beta * ((float)lead[v] + (float)rest[v]);
       }
+      if constexpr (LAST) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int v = 0; v < 8; ++v) z[v] *= result.scale;
+        auto* const to = result.y.data + matrix * result.y.batch + m * result.y.row + n * result.y.col;
+        if (!turns && m < result.rows) {
+          if (result.y.col == 1 && n + 8 <= result.cols) {
+            storePack(to, z);
+          } else {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        sum[i][j] = multiply(fb[j][1], fa[i][0], sum[i][j]);
-        sum[i][j] = multiply(fb[j][0], fa[i][1], sum[i][j]);
-        sum[i][j] = multiply(fb[j][0], fa[i][0], sum[i][j]);
+            for (int v = 0; v < 8; ++v)
+              if (n + v < result.cols) storePack(to + v * result.y.col, {z[v]});
+          }
+        }
+      } else {
+        halfx8 lead, rest;
+        splitEight(z, lead, rest);
+        half16* const to = g.out.data + matrix * g.out.batch + placeOf(g.out, m, n);
+        *reinterpret_cast<halfx8*>(to) = lead;
+        *reinterpret_cast<halfx8*>(to + 32) = rest;
       }
+    }
+    if (turns) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<floatx4*>(space + row * PITCH + c + 4 * h) = floatx4{z[4 * h], z[4 * h + 1], z[4 * h + 2], z[4 * h + 3]};
+    }
   }
-  Pairs old = p.old, out = p.out, turned = p.turned;
-  old.data += blockIdx.y * old.batch, out.data += blockIdx.y * out.batch, turned.data += blockIdx.y * turned.batch;
+  if (!turns) return;
+  waveExchange();
+  for (int column = lane; column < COLS; column += 64) {
+    const long n = n0 + column;
+    if (n >= g.N || m0 >= g.M) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float z[8];
+#pragma unroll
+      for (int v = 0; v < 8; ++v) z[v] = space[(8 * q + v) * PITCH + column];
+      if constexpr (LAST) {
+        auto* const to = result.y.data + matrix * result.y.batch + n * result.y.col + m0 + 8 * q;
+        if (n < result.cols) {
+          if (m0 + 8 * q + 8 <= result.rows) {
+            storePack(to, z);
+          } else {
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              if (m0 + 8 * q + v < result.rows) storePack(to + v, {z[v]});
+          }
+        }
+      } else {
+        halfx8 lead, rest;
+        splitEight(z, lead, rest);
+        half16* const to = g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n, m0) + 8 * q;
+        *reinterpret_cast<halfx8*>(to) = lead;
+        *reinterpret_cast<halfx8*>(to + 32) = rest;
+      }
+    }
+  }
+}
+
+// Tile `tile` of those on and below the diagonal, row after row.
+__device__ __forceinline__ void belowDiagonal(int tile, int& i, int& j) {
+  i = (int)((__builtin_sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+  while (i * (i + 1) / 2 > tile) --i;
+  while ((i + 1) * (i + 2) / 2 <= tile) ++i;
+  j = tile - i * (i + 1) / 2;
+}
+
+template <int BM, int BN>
+struct PairTile {
+  long m0, n0;
+  int index;  // among all tiles
+  bool any, mirror;
+
+  __device__ __forceinline__ PairTile(const PairArgs& g) {
+    if (g.symmetric) {
+      const int side = (int)((g.M + BM - 1) / BM), total = side * (side + 1) / 2, per = (total + 7) / 8;
+      index = (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
+      any = (int)blockIdx.x / 8 < per && index < total;
+      int i, j;
+      belowDiagonal(any ? index : 0, i, j);
+      m0 = (long)i * BM, n0 = (long)j * BN;
+      mirror = i != j;
+    } else {
+      const Tile<BM, BN> t(g.M, g.N);
+      m0 = t.m0, n0 = t.n0, any = t.any;
+      index = (int)(m0 / BM * ((g.N + BN - 1) / BN) + n0 / BN);
+      mirror = g.turned.data != nullptr;
+    }
+  }
+};
+
+// A workgroup: BM x BN results over one range of k, a wave WM x WN of them.  ONE: operands (1: b, 3: both) whose second pieces
+// are all zeros.  LDS holds the operands of two steps of 32 k, lines
+// of 128 bytes with both pieces.  A step is RM groups of 3 RN matrix instructions: the smaller products first.
+template <class RESULT, int ONE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, RESULT result) {
+  constexpr int WAVES = BM / WM * (BN / WN), RM = WM / 16, RN = WN / 16;
+  typedef Direct<BM, 64, true, WAVES> A;
+  typedef Direct<BN, 64, true, WAVES> B;
+  constexpr int STEP = A::bytes + B::bytes, LOADS = A::loads + B::loads;
+  __shared__ __attribute__((aligned(1024))) char space[2 * STEP];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+  const PairTile<BM, BN> tile(g);
+  if (!tile.any) return;
+  const long m0 = tile.m0, n0 = tile.n0, first = blockIdx.y * g.range, end = min(first + g.range, g.K), matrix = blockIdx.z;
+
+  A a;
+  B b;
+  a.setup(g.a.data + matrix * g.a.batch + 2 * (m0 * g.a.cols + first), 2 * g.a.cols, g.M - m0);
+  b.setup(g.b.data + matrix * g.b.batch + 2 * (n0 * g.b.cols + first), 2 * g.b.cols, g.N - n0);
+  floatx4 sum[RM][RN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < RN; ++j) sum[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+  int left = (int)(end - first) * 2;  // pieces of a row that are not on their way yet
+  auto load = [&](int q, char* to) __attribute__((always_inline)) {
+    if (q < A::loads)
+      a.load(q, left, to);
+    else
+      b.load(q - A::loads, left, to + A::bytes);
+  };
+  auto loaded = [&]() __attribute__((always_inline)) {
+    a.base += a.advance;
+    b.base += b.advance;
+    left -= 64;
+  };
+  // (behind the last step too, without a word, so that as many loads are always on their way)
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+#pragma unroll
+    for (int q = 0; q < LOADS; ++q) load(q, space + d * STEP);
+    loaded();
+  }
+  const int laneA = A::laneAt(wm), laneB = B::laneAt(wn);
+  uintx4 fa[2][2], fb[2][2][RN];  // [turn][piece]
+  auto readA = [&](int turn, int i, int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < (ONE == 3 ? 1 : 2); ++p) fa[turn][p] = A::fragment(space + d * STEP, laneA, p, i);
+  };
+  auto readB = [&](int d) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < (ONE ? 1 : 2); ++p)
+#pragma unroll
+      for (int j = 0; j < RN; ++j) fb[d][p][j] = B::fragment(space + d * STEP + A::bytes, laneB, p, j);
+  };
+  static_assert(RM % 2 == 0, "two turns of fragments");
+  arrive<LOADS>();
+  readB(0);
+  readA(0, 0, 0);
+  auto round = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        const int turn = i % 2;
+        if (i + 1 < RM) {
+          readA(turn ^ 1, i + 1, d);
+        } else {
+          // every wave has this step's fragments, so that its place is free, and the next step's operands are there
+          arrive<0>();
+          readB(d ^ 1);
+          readA(turn ^ 1, 0, d ^ 1);
+        }
+        if (!ONE) {
+#pragma unroll
+          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d][1][j], fa[turn][0], sum[i][j]);
+        }
+        if (ONE != 3) {
+#pragma unroll
+          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d][0][j], fa[turn][1], sum[i][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d][0][j], fa[turn][0], sum[i][j]);
+        if (i + 1 == RM) {
+#pragma unroll
+          for (int q = 0; q < LOADS; ++q) load(q, space + d * STEP);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      loaded();
+      if (left <= -128) return false;  // that was the last step
+    }
+    return true;
+  };
+  while (round()) {
+  }
+
+  // (the loads requested behind the last step write zeros to LDS, which the results now go through)
+  arrive<0>();
+  constexpr int PITCH = WN + 4;
+  static_assert(32 * PITCH * 4 <= 2 * STEP / WAVES, "a wave's share of LDS holds 32 rows");
+  float* const mine = reinterpret_cast<float*>(space + wave * (2 * STEP / WAVES));
+  auto eight = [&](int row, int c, float(&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const floatx4 q = *reinterpret_cast<const floatx4*>(mine + row * PITCH + c + 4 * h);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[4 * h + k] = q[k];
+    }
+  };
+#pragma unroll
+  for (int i0 = 0; i0 < RM; i0 += 2) {
+    waveExchange();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < RN; ++j) *reinterpret_cast<floatx4*>(mine + (16 * i + lane % 16) * PITCH + 16 * j + lane / 16 * 4) = sum[i0 + i][j];
+    waveExchange();
+    const int row0 = wm + 16 * i0;
+    if (g.parts) {
+      const long tiles = gridDim.x;
+      float* const to = g.parts + (((matrix * gridDim.y + blockIdx.y) * tiles + tile.index) * BM + row0) * BN + wn;
+#pragma unroll 1
+      for (int row = lane / (WN / 8); row < 32; row += 512 / WN) {
+        float v[8];
+        eight(row, lane % (WN / 8) * 8, v);
+        storePack(to + row * BN + lane % (WN / 8) * 8, v);
+      }
+    } else {
+      leavePairs<WN>(g, result, matrix, m0 + row0, n0 + wn, tile.mirror, mine, eight);
+    }
+  }
+}
+
+// Results from the sums of `ranges` ranges of k, in their order.  A wave: 32 rows of 64 columns of a tile.
+template <class RESULT, int BM, int BN>
+__global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int ranges, int tiles, int count) {
+  constexpr int ACROSS = BN / 64, BLOCKS = BM / 32 * ACROSS;  // of a tile
+  __shared__ float space[4][32 * 68];
+  const int wave = threadIdx.x / 64, at = (int)blockIdx.x * 4 + wave, index = at / BLOCKS, block = at % BLOCKS;
+  if (index >= count) return;
+  const long matrix = blockIdx.z;
+  int i, j;
+  if (g.symmetric) {
+    belowDiagonal(index, i, j);
+  } else {
+    const int across = (int)((g.N + BN - 1) / BN);
+    i = index / across, j = index % across;
+  }
+  const int row0 = block / ACROSS * 32, col0 = block % ACROSS * 64;
+  const long m0 = (long)i * BM + row0, n0 = (long)j * BN + col0;
+  if (m0 >= g.M || n0 >= g.N) return;
+  const long far = (long)tiles * BM * BN;  // from a range to the next
+  const float* const from = g.parts + matrix * ranges * far + ((long)index * BM + row0) * BN + col0;
+  leavePairs<64>(g, result, matrix, m0, n0, g.symmetric ? i != j : g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = 0.f;
+    for (int r = 0; r < ranges; ++r) {
+      float u[8];
+      loadPack<float, 8>(from + r * far + row * BN + c, u);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += u[q];
+    }
+  });
+}
+
+// Small products.  A workgroup: 32 x 32 results, its waves a range of k each, straight from memory to the matrix instructions;
+// their sums meet in LDS.
+template <class RESULT, int WAVES, int AHEAD>
+__global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
+  constexpr int PITCH = 36;
+  constexpr bool LAST = !__is_same(RESULT, Nothing);
+  __shared__ __attribute__((aligned(16))) float sums[WAVES][32 * PITCH];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+  const PairTile<32, 32> tile(g);
+  if (!tile.any) return;
+  const long m0 = tile.m0, n0 = tile.n0, matrix = blockIdx.z;
+  const long share = (g.K / 32 + WAVES - 1) / WAVES * 32, first = wave * share, end = min(first + share, g.K);
+  const half16* a[2];
+  const half16* b[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    a[i] = g.a.data + matrix * g.a.batch + 2 * (m0 + 16 * i + lane % 16) * g.a.cols + lane / 16 * 8;
+    b[i] = g.b.data + matrix * g.b.batch + 2 * (n0 + 16 * i + lane % 16) * g.b.cols + lane / 16 * 8;
+  }
+  floatx4 sum[2][2] = {};
+  for (long k0 = first; k0 < end; k0 += 32 * AHEAD) {
+    uintx4 fa[AHEAD][2][2], fb[AHEAD][2][2];  // [step][rows][piece]
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      const long k = min(k0 + 32 * s, end - 32);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          fa[s][i][p] = *reinterpret_cast<const uintx4*>(a[i] + 2 * k + 32 * p);
+          fb[s][i][p] = *reinterpret_cast<const uintx4*>(b[i] + 2 * k + 32 * p);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) {
+      if (k0 + 32 * s >= end) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sum[i][j] = multiply(fb[s][j][1], fa[s][i][0], sum[i][j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sum[i][j] = multiply(fb[s][j][0], fa[s][i][1], sum[i][j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) sum[i][j] = multiply(fb[s][j][0], fa[s][i][0], sum[i][j]);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
+      *reinterpret_cast<floatx4*>(&sums[wave][(16 * i + lane % 16) * PITCH + 16 * j + lane / 16 * 4]) = sum[i][j];
+  __syncthreads();
+  // four neighbours to a lane of the first 256
+  const int row = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
+  const long m = m0 + row, n = n0 + c;
+  bool turns = tile.mirror;
+  if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1;
+  float z[4] = {};
+  if (row < 32) {
+    const float factor = g.factors ? g.factors[matrix] : 1.f, by = g.by * factor * (g.power == 2 ? factor : 1.f), beta = g.beta * factor;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const floatx4 q = *reinterpret_cast<const floatx4*>(&sums[w][row * PITCH + c]);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) z[v] += q[v];
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) z[v] *= by;
+    if (g.old.data) {
+      const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m, n);
+      const halfx4 lead = *reinterpret_cast<const halfx4*>(from), rest = *reinterpret_cast<const halfx4*>(from + 32);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) z[v] += beta * ((float)lead[v] + (float)rest[v]);
+    }
+    if constexpr (LAST) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const long m = m0 + 16 * i + lane % 16, n = n0 + 16 * j + lane / 16 * 4 + v;
-        float z = sum[i][j][v] * p.by;
-        if (p.old.data) z += p.beta * loadPair(old, m, n);
-        if (LAST) {
-          if (m < rows && n < cols) y.data[blockIdx.y * y.batch + m * y.row + n * y.col] = (T)(z * scale);
-        } else {
-          storePair(out, m, n, z);
-          if (p.turned.data) storePair(turned, n, m, z);
-        }
+        z[v] *= result.scale;
+        if (!turns && m < result.rows && n + v < result.cols)
+          storePack(result.y.data + matrix * result.y.batch + m * result.y.row + (n + v) * result.y.col, {z[v]});
       }
+    } else {
+      storeFour(g.out.data + matrix * g.out.batch + placeOf(g.out, m, n), z);
+    }
+    if (turns) *reinterpret_cast<floatx4*>(&sums[0][row * PITCH + c]) = floatx4{z[0], z[1], z[2], z[3]};
+  }
+  if (!turns) return;
+  __syncthreads();
+  if (row < 32) {
+    // now a column, four of its rows
+#pragma unroll
+    for (int v = 0; v < 4; ++v) z[v] = sums[0][(c + v) * PITCH + row];
+    if constexpr (LAST) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (n0 + row < result.cols && m0 + c + v < result.rows)
+          storePack(result.y.data + matrix * result.y.batch + (n0 + row) * result.y.col + (m0 + c + v) * result.y.row, {z[v]});
+    } else {
+      storeFour(g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n0 + row, m0 + c), z);
+    }
+  }
 }
 
 long padded(long n) { return (n + 31) / 32 * 32; }
-size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 // What lies in the workspace, for so many matrices of P x Q.
 struct Space {
   double* sums;
+  float* factors;
   Pairs x, xt[2], gram, poly;
+  float* parts;
   size_t bytes;
 
   Space(void* workspace, long batch, long P, long Q) {
     char* at = static_cast<char*>(workspace);
     sums = reinterpret_cast<double*>(at);
     at += rounded((size_t)batch * kShares * sizeof(double));
+    factors = reinterpret_cast<float*>(at);
+    at += rounded((size_t)batch * sizeof(float));
     auto pairs = [&](long rows, long cols) {
       const Pairs m{reinterpret_cast<half16*>(at), cols, 2 * rows * cols};
       at += rounded((size_t)batch * 2 * rows * cols * sizeof(half16));
       return m;
     };
     x = pairs(P, Q), xt[0] = pairs(Q, P), xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
+    parts = reinterpret_cast<float*>(at);
+    at += (size_t)batch * 17 * ((P + 255) / 256 + 8) * 256 * ((Q + 255) / 256) * 256 * 4;
     bytes = at - static_cast<char*>(workspace);
   }
 };
+
+// The kernel of a product, and the ranges that its k is cut into.
+struct PairPlan {
+  int side;  // of a tile
+  long tiles, ranges, range;
+};
+
+static long forced(const char* k) { const char* f = getenv(k); return f ? atol(f) : 0; }
+
+PairPlan planOf(int which, long M, long N, long K) {
+  const char* sides[] = {"S0", "S1", "S2"}; const char* rs[] = {"R0", "R1", "R2"};
+  const bool symmetric = which < 2;
+  PairPlan p;
+  p.side = forced(sides[which]) ? (int)forced(sides[which]) : M >= 1024 ? 128 : 32;
+  const long down = ceilDivLong(M, p.side), across = ceilDivLong(N, p.side);
+  p.tiles = ((symmetric ? down * (down + 1) / 2 : down * across) + 7) / 8 * 8;
+  p.ranges = p.side == 32 ? 1 : forced(rs[which]) ? forced(rs[which]) : 1;
+  p.range = ceilDivLong(K / 32, p.ranges) * 32;
+  p.ranges = ceilDivLong(K, p.range);
+  return p;
+}
+
+// one: see product's ONE
+template <class RESULT>
+void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int one, float* parts, unsigned batch, hipStream_t s) {
+  const dim3 grid((unsigned)plan.tiles, (unsigned)plan.ranges, batch);
+  g.range = plan.range;
+  if (plan.ranges > 1) g.parts = parts;
+  if (plan.side == 32) {
+    if (g.K <= 256)
+      small<RESULT, 4, 2><<<grid, 256, 0, s>>>(g, result);
+    else if (g.K <= 512)
+      small<RESULT, 8, 2><<<grid, 512, 0, s>>>(g, result);
+    else
+      small<RESULT, 8, 4><<<grid, 512, 0, s>>>(g, result);
+    return;
+  }
+  auto tiles = [&](auto pieces) {
+    constexpr int ONE = decltype(pieces)::value;
+    if (plan.side == 64)
+      product<RESULT, ONE, 64, 64, 32, 32><<<grid, 256, 0, s>>>(g, result);
+    else if (plan.side == 128)
+      product<RESULT, ONE, 128, 128, 64, 64><<<grid, 256, 0, s>>>(g, result);
+    else
+      product<RESULT, ONE, 256, 256, 128, 64><<<grid, 512, 0, s>>>(g, result);
+  };
+  if (one == 3)
+    tiles(std::integral_constant<int, 3>());
+  else if (one == 1)
+    tiles(std::integral_constant<int, 1>());
+  else
+    tiles(std::integral_constant<int, 0>());
+  if (plan.ranges > 1) {
+    const long down = ceilDivLong(g.M, plan.side), count = g.symmetric ? down * (down + 1) / 2 : down * ceilDivLong(g.N, plan.side);
+    const dim3 blocks((unsigned)ceilDivLong(count * (plan.side / 32) * (plan.side / 64), 4), 1, batch);
+    if (plan.side == 64)
+      join<RESULT, 64, 64><<<blocks, 256, 0, s>>>(g, result, (int)plan.ranges, (int)plan.tiles, (int)count);
+    else if (plan.side == 128)
+      join<RESULT, 128, 128><<<blocks, 256, 0, s>>>(g, result, (int)plan.ranges, (int)plan.tiles, (int)count);
+    else
+      join<RESULT, 256, 256><<<blocks, 256, 0, s>>>(g, result, (int)plan.ranges, (int)plan.tiles, (int)count);
+  }
+}
 
 template <class T>
 int run(const OrthogonalProblem& p, hipStream_t s) {
@@ -175,23 +673,35 @@ int run(const OrthogonalProblem& p, hipStream_t s) {
   const Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
   const Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
   Space w(p.workspace, p.batch, P, Q);
-  const long most = 65535;
-  if (p.batch > most || !launches((double)p.batch * (P / 32 * (Q / 32) / 4 + 1), 256)) return FBFFT_UNSUPPORTED_SIZE;
+  const PairPlan gram = planOf(0, P, P, Q), poly = planOf(1, P, P, P), last = planOf(2, P, Q, P);
+  if (p.batch > 65535) return FBFFT_UNSUPPORTED_SIZE;
   const unsigned batch = (unsigned)p.batch;
-  auto blocks = [&](long M, long N) { return dim3((unsigned)((M / 32 * (N / 32) + 3) / 4), batch); };
-  squares<T><<<dim3(kShares, batch), 256, 0, s>>>(g, rows, cols, w.sums);
-  begin<T><<<dim3((unsigned)std::min((P * Q + 255) / 256, 4096l), batch), 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0]);
+  // lines of neighbours, for the squares
+  const bool lines = g.row == 1 && g.col != 1;
+  const Given<const T> by{g.data, lines ? g.col : g.row, lines ? g.row : g.col, g.batch};
+  const long count = lines ? rows : cols;
+  squares<T><<<dim3(kShares, batch), 256, 0, s>>>(by, lines ? cols : rows, count, divisorOf(ceilDivLong(count, 8)), w.sums);
+  const dim3 grid((unsigned)(ceilDivLong(P, 64) * ceilDivLong(Q, 64)), batch);
+  if (lines)
+    begin<T, true><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
+  else
+    begin<T, false><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
+  constexpr bool SHORT = sizeof(T) == 2;
   const float one = 1.f / kUnit;
   for (int i = 0; i < p.steps; ++i) {
     const float a = p.coefficients[3 * i], b = p.coefficients[3 * i + 1], c = p.coefficients[3 * i + 2];
     const Pairs from = w.xt[i % 2], to = w.xt[(i + 1) % 2], none{};
-    product<T, false><<<blocks(P, P), 256, 0, s>>>(PairProduct{w.x, w.x, P, P, Q, one, 0.f, none, w.gram, none}, y, 0, 0, 0.f);
-    product<T, false><<<blocks(P, P), 256, 0, s>>>(PairProduct{w.gram, w.gram, P, P, P, c * one, b, w.gram, w.poly, none}, y, 0, 0, 0.f);
-    const PairProduct last{w.poly, from, P, Q, P, one, a, w.x, w.x, to};
+    const float* const factors = i == 0 ? w.factors : nullptr;
+    const bool shorter = SHORT && i == 0;
+    launchProduct(PairArgs{w.x, w.x, P, P, Q, 0, one, 0.f, factors, 2, none, w.gram, w.gram, true, nullptr}, Nothing{}, gram,
+                  shorter ? 3 : 0, w.parts, batch, s);
+    launchProduct(PairArgs{w.gram, w.gram, P, P, P, 0, c * one, b, nullptr, 0, w.gram, w.poly, w.poly, true, nullptr}, Nothing{}, poly, 0,
+                  w.parts, batch, s);
+    const PairArgs x{w.poly, from, P, Q, P, 0, one, a, factors, 1, w.x, w.x, to, false, nullptr};
     if (i + 1 < p.steps)
-      product<T, false><<<blocks(P, Q), 256, 0, s>>>(last, y, 0, 0, 0.f);
+      launchProduct(x, Nothing{}, last, shorter ? 1 : 0, w.parts, batch, s);
     else
-      product<T, true><<<blocks(P, Q), 256, 0, s>>>(last, y, rows, cols, p.scale / kUnit);
+      launchProduct(x, Result<T>{y, rows, cols, p.scale / kUnit}, last, shorter ? 1 : 0, w.parts, batch, s);
   }
   return launchStatus();
 }
