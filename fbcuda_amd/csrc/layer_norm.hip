@@ -87,22 +87,324 @@ __global__ __launch_bounds__(kLanes) void anyParameters(LayerNormProblem p, floa
   parts[(2 * band + 1) * p.N + j] = b;
 }
 
-__global__ __launch_bounds__(kLanes) void joinParameters(LayerNormProblem p, const float* parts, long bands) {
-  const long j = (long)blockIdx.x * kLanes + threadIdx.x;
-  if (j >= p.N) return;
-  float w = 0.f, b = 0.f;
-  for (long i = 0; i < bands; ++i) {
-    w += parts[2 * i * p.N + j];
-    b += parts[(2 * i + 1) * p.N + j];
+// ---- rows of neighbours that lanes hold in registers ----
+
+// A row's words of VEC values, WORDS to a lane, LANES lanes to a row.
+template <class T, int VEC, int LANES, int WORDS>
+struct Row {
+  typename Pack<T, VEC>::type v[WORDS];
+
+  static __device__ __forceinline__ long at(int w) { return (long)(w * LANES + threadIdx.x % LANES) * VEC; }
+  __device__ __forceinline__ void load(const Matrix& m, long i, long N) {
+    const T* const from = static_cast<const T*>(m.data) + i * m.row;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const long j = at(w);
+      if (j + VEC <= N) {
+        v[w] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(from + j);
+      } else {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) v[w][q] = j + q < N ? from[j + q] : (T)0.f;
+      }
+    }
   }
-  if (p.gradWeight.data) storeAny(p.gradWeight.data, p.gradWeight.type, j * p.gradWeight.stride, w);
-  if (p.gradBias.data) storeAny(p.gradBias.data, p.gradBias.type, j * p.gradBias.stride, b);
+};
+
+template <bool STREAM, class T, int VEC>
+__device__ __forceinline__ void leaveWord(T* to, long j, long N, const float (&v)[VEC]) {
+  if (j + VEC <= N) {
+    leavePack<STREAM, T, VEC>(to + j, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q)
+      if (j + q < N) to[j + q] = (T)v[q];
+  }
 }
 
-long bandsOf(long M) { return std::min(M, 256L); }
+// VEC parameters from j
+template <int VEC>
+__device__ __forceinline__ void loadLine(const Line& l, long j, long N, float otherwise, float (&v)[VEC]) {
+  if (l.data && l.type == FBFFT_FLOAT32 && l.stride == 1 && j + VEC <= N) {
+    loadPack<float, VEC>(static_cast<const float*>(l.data) + j, v);
+  } else {
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) v[q] = j + q < N ? lineOr(l, j + q, otherwise) : 0.f;
+  }
+}
+
+// The same number, from which the compiler computes nothing in front of a loop: the addresses of all words' parameters, of three
+// types, take hundreds of registers there.
+__device__ __forceinline__ long hidden(long j) {
+  asm volatile("" : "+v"(j));
+  return j;
+}
+
+// The sums of two values over the lanes of a row, in every lane.  Rows of more than a wave meet in LDS, `turn` in turn two parts
+// of it, so that one barrier is enough.
+template <int LANES, int THREADS>
+__device__ __forceinline__ void rowSums(float& s1, float& s2, float (*space)[THREADS / 64][2], int turn) {
+  if constexpr (LANES <= 64) {
+    s1 = waveSumOf(s1, LANES);
+    s2 = waveSumOf(s2, LANES);
+  } else {
+    s1 = waveSum(s1);
+    s2 = waveSum(s2);
+    if (threadIdx.x % 64 == 0) space[turn][threadIdx.x / 64][0] = s1, space[turn][threadIdx.x / 64][1] = s2;
+    __syncthreads();
+    s1 = s2 = 0.f;
+    const int first = threadIdx.x / LANES * (LANES / 64);
+#pragma unroll
+    for (int q = 0; q < LANES / 64; ++q) {
+      s1 += space[turn][first + q][0];
+      s2 += space[turn][first + q][1];
+    }
+  }
+}
+
+// A workgroup takes THREADS / LANES rows at a time, the next ones on their way.  The variance is that of the values in registers
+// around their mean: nothing cancels.
+template <class T, int VEC, int LANES, int WORDS, int THREADS, bool STREAM>
+__global__ __launch_bounds__(THREADS) void rowsForward(LayerNormProblem p) {
+  constexpr int GROUPS = THREADS / LANES;
+  constexpr bool HOLDS = WORDS * VEC <= 16;  // the parameters, and the next row
+  __shared__ float space[2][THREADS / 64][2];
+  typedef Row<T, VEC, LANES, WORDS> R;
+  float weight[HOLDS ? WORDS : 1][VEC], bias[HOLDS ? WORDS : 1][VEC];
+  if constexpr (HOLDS) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      loadLine(p.weight, R::at(w), p.N, 1.f, weight[w]);
+      loadLine(p.bias, R::at(w), p.N, 0.f, bias[w]);
+    }
+  }
+  const long step = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  const float each = 1.f / (float)p.N;
+  R next;
+  if constexpr (HOLDS) next.load(p.x, min(first, p.M - 1), p.N);
+  for (long i = first; i - threadIdx.x / LANES < p.M; i += step) {  // (as often for all rows of a workgroup)
+    R x;
+    if constexpr (HOLDS) {
+      x = next;
+      if (i - threadIdx.x / LANES + step < p.M) next.load(p.x, min(i + step, p.M - 1), p.N);
+    } else {
+      x.load(p.x, min(i, p.M - 1), p.N);
+    }
+    float sum = 0.f, none = 0.f;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) sum += (float)x.v[w][q];
+    rowSums<LANES, THREADS>(sum, none, space, 0);
+    const float mean = sum * each;
+    sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) {
+        const float d = R::at(w) + q < p.N ? (float)x.v[w][q] - mean : 0.f;
+        sum = __builtin_fmaf(d, d, sum);
+      }
+    rowSums<LANES, THREADS>(sum, none, space, 1);
+    const float rstd = 1.f / __builtin_sqrtf(sum * each + p.eps);
+    if (i < p.M) {
+      T* const to = static_cast<T*>(p.y.data) + i * p.y.row;
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        float y[VEC];
+        if constexpr (!HOLDS) {
+          const long j = hidden(R::at(w));
+          loadLine(p.weight, j, p.N, 1.f, weight[0]);
+          loadLine(p.bias, j, p.N, 0.f, bias[0]);
+        }
+        constexpr int last = HOLDS ? WORDS - 1 : 0;
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) y[q] = __builtin_fmaf(((float)x.v[w][q] - mean) * rstd, weight[min(w, last)][q], bias[min(w, last)][q]);
+        leaveWord<STREAM, T, VEC>(to, R::at(w), p.N, y);
+      }
+      if (threadIdx.x % LANES == 0) {
+        if (p.mean) p.mean[i * p.meanStride] = mean;
+        if (p.rstd) p.rstd[i * p.rstdStride] = rstd;
+      }
+    }
+  }
+}
+
+// Rows as above, 1024 lanes to a workgroup; the columns' sums of its rows stay in registers, meet in LDS and go to parts
+// [workgroup][2][N].
+template <class T, int VEC, int LANES, int WORDS, bool STREAM>
+__global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* parts) {
+  constexpr int GROUPS = 1024 / LANES;
+  __shared__ float space[2][16][2];
+  typedef Row<T, VEC, LANES, WORDS> R;
+  constexpr bool HOLDS = WORDS == 1;  // the parameters, and the next row
+  float weight[VEC], sumW[WORDS][VEC] = {}, sumB[WORDS][VEC] = {};
+  if constexpr (HOLDS) loadLine(p.weight, R::at(0), p.N, 1.f, weight);
+  const long step = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  const float each = 1.f / (float)p.N;
+  R nextX, nextG;
+  float nextMean, nextRstd;
+  auto load = [&](long row) __attribute__((always_inline)) {
+    const long i = min(row, p.M - 1);
+    nextX.load(p.x, i, p.N);
+    nextG.load(p.g, i, p.N);
+    nextMean = p.mean[i * p.meanStride], nextRstd = p.rstd[i * p.rstdStride];
+  };
+  if constexpr (HOLDS) load(first);
+  int turn = 0;
+  for (long i = first; i - threadIdx.x / LANES < p.M; i += step) {
+    if constexpr (!HOLDS) load(i);
+    const R x = nextX, g = nextG;
+    const float mean = nextMean, rstd = nextRstd;
+    if (HOLDS && i - threadIdx.x / LANES + step < p.M) load(i + step);
+    float s1 = 0.f, s2 = 0.f;
+    if (i < p.M) {
+#pragma unroll
+      for (int w = 0; w < WORDS; ++w) {
+        if constexpr (!HOLDS) {
+          loadLine(p.weight, hidden(R::at(w)), p.N, 1.f, weight);
+        }
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          const float dy = (float)g.v[w][q], xh = ((float)x.v[w][q] - mean) * rstd, h = dy * weight[q];
+          s1 += h;
+          s2 = __builtin_fmaf(h, xh, s2);
+          sumB[w][q] += dy;
+          sumW[w][q] = __builtin_fmaf(dy, xh, sumW[w][q]);
+        }
+      }
+    }
+    if (p.y.data) {
+      rowSums<LANES, 1024>(s1, s2, space, turn);
+      s1 *= each;
+      s2 *= each;
+      if (i < p.M) {
+        T* const to = static_cast<T*>(p.y.data) + i * p.y.row;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) {
+          float d[VEC];
+          if constexpr (!HOLDS) {
+            loadLine(p.weight, hidden(R::at(w)), p.N, 1.f, weight);
+          }
+#pragma unroll
+          for (int q = 0; q < VEC; ++q) {
+            const float xh = ((float)x.v[w][q] - mean) * rstd, h = (float)g.v[w][q] * weight[q];
+            d[q] = rstd * (h - s1 - xh * s2);
+          }
+          leaveWord<STREAM, T, VEC>(to, R::at(w), p.N, d);
+        }
+      }
+    }
+    turn ^= 1;
+  }
+  if (!parts) return;
+  float* const to = parts + (long)blockIdx.x * 2 * p.N;
+  if constexpr (GROUPS == 1) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      leaveWord<false, float, VEC>(to, R::at(w), p.N, sumW[w]);
+      leaveWord<false, float, VEC>(to + p.N, R::at(w), p.N, sumB[w]);
+    }
+  } else {
+    static_assert(WORDS == 1, "a word to a lane");
+    __shared__ __attribute__((aligned(16))) float sums[GROUPS][LANES * VEC];
+    const int group = threadIdx.x / LANES, column = threadIdx.x % LANES * VEC;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) sums[group][column + q] = part ? sumB[0][q] : sumW[0][q];
+      __syncthreads();
+      for (int j = threadIdx.x; j < LANES * VEC && j < p.N; j += 1024) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < GROUPS; ++q) v += sums[q][j];
+        to[part * p.N + j] = v;
+      }
+    }
+  }
+}
+
+// The workgroups' sums, joined in their order: 16 columns of [2][N] to a workgroup, 64 lanes to each.
+__global__ __launch_bounds__(1024) void joinRows(LayerNormProblem p, const float* parts, int bands) {
+  __shared__ float sums[64][17];
+  const int column = threadIdx.x % 16, slice = threadIdx.x / 16;
+  const long j = (long)blockIdx.x * 16 + column;
+  float sum = 0.f;
+  if (j < 2 * p.N)
+#pragma unroll 8
+    for (int r = slice; r < bands; r += 64) sum += parts[r * 2 * p.N + j];
+  sums[slice][column] = sum;
+  __syncthreads();
+  if (slice > 0 || j >= 2 * p.N) return;
+  sum = 0.f;
+#pragma unroll
+  for (int q = 0; q < 64; ++q) sum += sums[q][column];
+  const Line& to = j < p.N ? p.gradWeight : p.gradBias;
+  if (to.data) storeAny(to.data, to.type, (j < p.N ? j : j - p.N) * to.stride, sum);
+}
+
+// Parts of the rows whose columns' sums are joined.
+long bandsOf(long M, long N) { return std::min(M, N < 4096 ? 512L : 256L); }
+
+// Lanes to a row: as many as it has words, so that a lane holds one; wider rows take more words to a lane.
+template <class T, bool STREAM>
+bool launchRows(const LayerNormProblem& p, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const long words = (p.N + V - 1) / V;
+  const unsigned most = 2048;
+  auto grid = [&](int groups) { return dim3((unsigned)std::min((p.M + groups - 1) / groups, (long)most)); };
+#define FBFFT_ROWS(LANES, WORDS, THREADS)                                                        \
+  if (words <= LANES * WORDS) {                                                                  \
+    rowsForward<T, V, LANES, WORDS, THREADS, STREAM><<<grid(THREADS / LANES), THREADS, 0, s>>>(p); \
+    return true;                                                                                 \
+  }
+  FBFFT_ROWS(8, 1, 256)
+  FBFFT_ROWS(16, 1, 256)
+  FBFFT_ROWS(32, 1, 256)
+  FBFFT_ROWS(64, 1, 256)
+  if (p.M >= 4 * computeUnits()) {
+    FBFFT_ROWS(64, 2, 256)
+    FBFFT_ROWS(64, 4, 256)
+  }
+  FBFFT_ROWS(256, 1, 256)
+  FBFFT_ROWS(256, 2, 256)
+  FBFFT_ROWS(256, 4, 256)
+  FBFFT_ROWS(1024, 2, 1024)
+  FBFFT_ROWS(1024, 4, 1024)
+  if constexpr (sizeof(T) == 4) {
+    FBFFT_ROWS(1024, 8, 1024)
+  }
+#undef FBFFT_ROWS
+  return false;
+}
+
+template <class T, bool STREAM>
+int launchRowsBack(const LayerNormProblem& p, float* parts, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const long words = (p.N + V - 1) / V, bands = bandsOf(p.M, p.N);
+#define FBFFT_ROWS(LANES, WORDS)                                                        \
+  if (words <= LANES * WORDS) {                                                         \
+    const long groups = std::min(bands, (p.M + 1024 / LANES - 1) / (1024 / LANES));     \
+    rowsBackward<T, V, LANES, WORDS, STREAM><<<dim3((unsigned)groups), 1024, 0, s>>>(p, parts); \
+    return (int)groups;                                                                 \
+  }
+  FBFFT_ROWS(8, 1)
+  FBFFT_ROWS(16, 1)
+  FBFFT_ROWS(32, 1)
+  FBFFT_ROWS(64, 1)
+  FBFFT_ROWS(128, 1)
+  FBFFT_ROWS(256, 1)
+  FBFFT_ROWS(512, 1)
+  FBFFT_ROWS(1024, 1)
+  FBFFT_ROWS(1024, 2)
+#undef FBFFT_ROWS
+  return 0;
+}
 
 template <class T>
 int forward(const LayerNormProblem& p, hipStream_t s) {
+  if (p.x.col == 1 && p.y.col == 1 && (streams((double)p.M * p.N, p.type) ? launchRows<T, true>(p, s) : launchRows<T, false>(p, s)))
+    return launchStatus();
   anyForward<T><<<dim3((unsigned)std::min(p.M, 1L << 20)), kLanes, 0, s>>>(p);
   return launchStatus();
 }
@@ -110,20 +412,26 @@ int forward(const LayerNormProblem& p, hipStream_t s) {
 template <class T>
 int backward(const LayerNormProblem& p, hipStream_t s) {
   float* const parts = static_cast<float*>(p.workspace);
-  const long bands = p.M > 0 ? bandsOf(p.M) : 0, across = (p.N + kLanes - 1) / kLanes;
-  // (before gradInput, which may be one of the operands)
-  if (p.gradWeight.data || p.gradBias.data) {
-    if (!launches((double)across * std::max(bands, 1L), kLanes)) return FBFFT_UNSUPPORTED_SIZE;
-    if (bands > 0) anyParameters<T><<<dim3((unsigned)(across * bands)), kLanes, 0, s>>>(p, parts, bands);
-    joinParameters<<<dim3((unsigned)across), kLanes, 0, s>>>(p, parts, bands);
+  const bool sums = p.gradWeight.data || p.gradBias.data;
+  const long across = (p.N + kLanes - 1) / kLanes;
+  long bands = p.M > 0 ? bandsOf(p.M, p.N) : 0;
+  if (sums && (!launches((double)across * std::max(bands, 1L), kLanes) || !launches((2.0 * p.N + 15) / 16, 1024))) return FBFFT_UNSUPPORTED_SIZE;
+  bool done = p.M == 0;
+  if (!done && p.x.col == 1 && p.g.col == 1 && (!p.y.data || p.y.col == 1)) {
+    float* const to = sums ? parts : nullptr;
+    const int groups = streams((double)p.M * p.N, p.type) ? launchRowsBack<T, true>(p, to, s) : launchRowsBack<T, false>(p, to, s);
+    if (groups) done = true, bands = groups;
   }
-  if (p.y.data && p.M > 0) anyBackward<T><<<dim3((unsigned)std::min(p.M, 1L << 20)), kLanes, 0, s>>>(p);
+  // (before gradInput, which may be one of the operands)
+  if (!done && sums) anyParameters<T><<<dim3((unsigned)(across * bands)), kLanes, 0, s>>>(p, parts, bands);
+  if (!done && p.y.data) anyBackward<T><<<dim3((unsigned)std::min(p.M, 1L << 20)), kLanes, 0, s>>>(p);
+  if (sums) joinRows<<<dim3((unsigned)((2 * p.N + 15) / 16)), 1024, 0, s>>>(p, parts, (int)bands);
   return launchStatus();
 }
 
 }  // namespace
 
-size_t layerNormWorkspaceBytes(int pass, long M, long N) { return pass == 0 ? 0 : (size_t)bandsOf(M) * 2 * N * sizeof(float); }
+size_t layerNormWorkspaceBytes(int pass, long M, long N) { return pass == 0 ? 0 : (size_t)bandsOf(M, N) * 2 * N * sizeof(float); }
 
 int launchLayerNormForward(const LayerNormProblem& p, hipStream_t s) {
   if (p.type == FBFFT_FLOAT32) return forward<float>(p, s);
