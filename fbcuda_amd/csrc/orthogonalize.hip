@@ -15,7 +15,7 @@
 #include "product.h"
 
 #include <algorithm>
-#include <cstdlib>
+#include <cmath>
 #include <type_traits>
 
 namespace fbfft_amd {
@@ -268,12 +268,24 @@ __device__ __forceinline__ void leavePairs(const PairArgs& g, const RESULT& resu
   }
 }
 
-// Tile `tile` of those on and below the diagonal, row after row.
-__device__ __forceinline__ void belowDiagonal(int tile, int& i, int& j) {
-  i = (int)((__builtin_sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-  while (i * (i + 1) / 2 > tile) --i;
-  while ((i + 1) * (i + 2) / 2 <= tile) ++i;
-  j = tile - i * (i + 1) / 2;
+// Tile `tile` of those on and below the diagonal of `down` rows of tiles: in strips of four rows, column after column, so that
+// those that run together share lines of both operands.
+__device__ __forceinline__ void belowDiagonal(int tile, int down, int& i, int& j) {
+  // (strip s begins with tile 8 s^2 + 2 s)
+  int s = (int)((__builtin_sqrtf(32.f * tile + 4.f) - 2.f) * 0.0625f);
+  while (s > 0 && 8 * s * s + 2 * s > tile) --s;
+  while (8 * (s + 1) * (s + 1) + 2 * (s + 1) <= tile) ++s;
+  tile -= 8 * s * s + 2 * s;
+  const int height = min(4, down - 4 * s);
+  if (tile < 4 * s * height) {
+    i = 4 * s + tile % height;
+    j = tile / height;
+    return;
+  }
+  tile -= 4 * s * height;
+  i = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3;
+  j = 4 * s + tile - i * (i + 1) / 2;
+  i += 4 * s;
 }
 
 template <int BM, int BN>
@@ -288,7 +300,7 @@ struct PairTile {
       index = (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
       any = (int)blockIdx.x / 8 < per && index < total;
       int i, j;
-      belowDiagonal(any ? index : 0, i, j);
+      belowDiagonal(any ? index : 0, side, i, j);
       m0 = (long)i * BM, n0 = (long)j * BN;
       mirror = i != j;
     } else {
@@ -301,15 +313,15 @@ struct PairTile {
 };
 
 // A workgroup: BM x BN results over one range of k, a wave WM x WN of them.  ONE: operands (1: b, 3: both) whose second pieces
-// are all zeros.  LDS holds the operands of two steps of 32 k, lines
-// of 128 bytes with both pieces.  A step is RM groups of 3 RN matrix instructions: the smaller products first.
-template <class RESULT, int ONE, int BM, int BN, int WM, int WN>
+// are all zeros.  LDS holds the operands of DEPTH steps of 32 k,
+// lines of 128 bytes with both pieces.  A step is RM groups of 3 RN matrix instructions: the smaller products first.
+template <class RESULT, int ONE, int BM, int BN, int WM, int WN, int DEPTH>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, RESULT result) {
   constexpr int WAVES = BM / WM * (BN / WN), RM = WM / 16, RN = WN / 16;
   typedef Direct<BM, 64, true, WAVES> A;
   typedef Direct<BN, 64, true, WAVES> B;
   constexpr int STEP = A::bytes + B::bytes, LOADS = A::loads + B::loads;
-  __shared__ __attribute__((aligned(1024))) char space[2 * STEP];
+  __shared__ __attribute__((aligned(1024))) char space[DEPTH * STEP];
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
   const PairTile<BM, BN> tile(g);
@@ -339,7 +351,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
   };
   // (behind the last step too, without a word, so that as many loads are always on their way)
 #pragma unroll
-  for (int d = 0; d < 2; ++d) {
+  for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
     for (int q = 0; q < LOADS; ++q) load(q, space + d * STEP);
     loaded();
@@ -354,15 +366,15 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
 #pragma unroll
     for (int p = 0; p < (ONE ? 1 : 2); ++p)
 #pragma unroll
-      for (int j = 0; j < RN; ++j) fb[d][p][j] = B::fragment(space + d * STEP + A::bytes, laneB, p, j);
+      for (int j = 0; j < RN; ++j) fb[d % 2][p][j] = B::fragment(space + d * STEP + A::bytes, laneB, p, j);
   };
-  static_assert(RM % 2 == 0, "two turns of fragments");
-  arrive<LOADS>();
+  static_assert(RM % 2 == 0 && DEPTH % 2 == 0, "two turns of fragments");
+  arrive<(DEPTH - 1) * LOADS>();
   readB(0);
   readA(0, 0, 0);
   auto round = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 0; d < 2; ++d) {
+    for (int d = 0; d < DEPTH; ++d) {
 #pragma unroll
       for (int i = 0; i < RM; ++i) {
         const int turn = i % 2;
@@ -370,20 +382,20 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
           readA(turn ^ 1, i + 1, d);
         } else {
           // every wave has this step's fragments, so that its place is free, and the next step's operands are there
-          arrive<0>();
-          readB(d ^ 1);
-          readA(turn ^ 1, 0, d ^ 1);
+          arrive<(DEPTH - 2) * LOADS>();
+          readB((d + 1) % DEPTH);
+          readA(turn ^ 1, 0, (d + 1) % DEPTH);
         }
         if (!ONE) {
 #pragma unroll
-          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d][1][j], fa[turn][0], sum[i][j]);
+          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d % 2][1][j], fa[turn][0], sum[i][j]);
         }
         if (ONE != 3) {
 #pragma unroll
-          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d][0][j], fa[turn][1], sum[i][j]);
+          for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d % 2][0][j], fa[turn][1], sum[i][j]);
         }
 #pragma unroll
-        for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d][0][j], fa[turn][0], sum[i][j]);
+        for (int j = 0; j < RN; ++j) sum[i][j] = multiply(fb[d % 2][0][j], fa[turn][0], sum[i][j]);
         if (i + 1 == RM) {
 #pragma unroll
           for (int q = 0; q < LOADS; ++q) load(q, space + d * STEP);
@@ -391,7 +403,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
         __builtin_amdgcn_sched_barrier(0);
       }
       loaded();
-      if (left <= -128) return false;  // that was the last step
+      if (left <= -DEPTH * 64) return false;  // that was the last step
     }
     return true;
   };
@@ -401,8 +413,8 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
   // (the loads requested behind the last step write zeros to LDS, which the results now go through)
   arrive<0>();
   constexpr int PITCH = WN + 4;
-  static_assert(32 * PITCH * 4 <= 2 * STEP / WAVES, "a wave's share of LDS holds 32 rows");
-  float* const mine = reinterpret_cast<float*>(space + wave * (2 * STEP / WAVES));
+  static_assert(32 * PITCH * 4 <= DEPTH * STEP / WAVES, "a wave's share of LDS holds 32 rows");
+  float* const mine = reinterpret_cast<float*>(space + wave * (DEPTH * STEP / WAVES));
   auto eight = [&](int row, int c, float(&v)[8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -435,27 +447,27 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
   }
 }
 
-// Results from the sums of `ranges` ranges of k, in their order.  A wave: 32 rows of 64 columns of a tile.
+// Results from the sums of `ranges` ranges of k, in their order.  A wave: 32 rows of up to 64 columns of a tile.
 template <class RESULT, int BM, int BN>
 __global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int ranges, int tiles, int count) {
-  constexpr int ACROSS = BN / 64, BLOCKS = BM / 32 * ACROSS;  // of a tile
-  __shared__ float space[4][32 * 68];
+  constexpr int COLS = BN < 64 ? BN : 64, ACROSS = BN / COLS, BLOCKS = BM / 32 * ACROSS;  // of a tile
+  __shared__ __attribute__((aligned(16))) float space[4][32 * (COLS + 4)];
   const int wave = threadIdx.x / 64, at = (int)blockIdx.x * 4 + wave, index = at / BLOCKS, block = at % BLOCKS;
   if (index >= count) return;
   const long matrix = blockIdx.z;
   int i, j;
   if (g.symmetric) {
-    belowDiagonal(index, i, j);
+    belowDiagonal(index, (int)((g.M + BM - 1) / BM), i, j);
   } else {
     const int across = (int)((g.N + BN - 1) / BN);
     i = index / across, j = index % across;
   }
-  const int row0 = block / ACROSS * 32, col0 = block % ACROSS * 64;
+  const int row0 = block / ACROSS * 32, col0 = block % ACROSS * COLS;
   const long m0 = (long)i * BM + row0, n0 = (long)j * BN + col0;
   if (m0 >= g.M || n0 >= g.N) return;
   const long far = (long)tiles * BM * BN;  // from a range to the next
   const float* const from = g.parts + matrix * ranges * far + ((long)index * BM + row0) * BN + col0;
-  leavePairs<64>(g, result, matrix, m0, n0, g.symmetric ? i != j : g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
+  leavePairs<COLS>(g, result, matrix, m0, n0, g.symmetric ? i != j : g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = 0.f;
     for (int r = 0; r < ranges; ++r) {
@@ -467,33 +479,43 @@ __global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int range
   });
 }
 
-// Small products.  A workgroup: 32 x 32 results, its waves a range of k each, straight from memory to the matrix instructions;
-// their sums meet in LDS.
-template <class RESULT, int WAVES, int AHEAD>
+// Small products.  A workgroup: SIDE x SIDE results over one range of k, its waves a part of that each, straight from memory to
+// the matrix instructions; their sums meet in LDS.
+template <class RESULT, int SIDE, int WAVES, int AHEAD>
 __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
-  constexpr int PITCH = 36;
+  constexpr int PITCH = SIDE + 4, R = SIDE / 16, LANES = SIDE / 4;
   constexpr bool LAST = !__is_same(RESULT, Nothing);
-  __shared__ __attribute__((aligned(16))) float sums[WAVES][32 * PITCH];
+  __shared__ __attribute__((aligned(16))) float sums[WAVES][SIDE * PITCH];
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const PairTile<32, 32> tile(g);
+  const PairTile<SIDE, SIDE> tile(g);
   if (!tile.any) return;
   const long m0 = tile.m0, n0 = tile.n0, matrix = blockIdx.z;
-  const long share = (g.K / 32 + WAVES - 1) / WAVES * 32, first = wave * share, end = min(first + share, g.K);
-  const half16* a[2];
-  const half16* b[2];
+  // (four neighbouring results to a lane of the first ones, which what stands beside them is on its way to already)
+  const int row = threadIdx.x / LANES, c = threadIdx.x % LANES * 4;
+  const long m = m0 + row, n = n0 + c;
+  halfx4 oldLead{}, oldRest{};
+  if (row < SIDE && g.old.data && !g.parts) {
+    const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m, n);
+    oldLead = *reinterpret_cast<const halfx4*>(from), oldRest = *reinterpret_cast<const halfx4*>(from + 32);
+  }
+  const float factor = g.factors ? g.factors[matrix] : 1.f;
+  const long begin = blockIdx.y * g.range, stop = min(begin + g.range, g.K);
+  const long share = ((stop - begin) / 32 + WAVES - 1) / WAVES * 32, first = begin + wave * share, end = min(first + share, stop);
+  const half16* a[R];
+  const half16* b[R];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < R; ++i) {
     a[i] = g.a.data + matrix * g.a.batch + 2 * (m0 + 16 * i + lane % 16) * g.a.cols + lane / 16 * 8;
     b[i] = g.b.data + matrix * g.b.batch + 2 * (n0 + 16 * i + lane % 16) * g.b.cols + lane / 16 * 8;
   }
-  floatx4 sum[2][2] = {};
+  floatx4 sum[R][R] = {};
   for (long k0 = first; k0 < end; k0 += 32 * AHEAD) {
-    uintx4 fa[AHEAD][2][2], fb[AHEAD][2][2];  // [step][rows][piece]
+    uintx4 fa[AHEAD][R][2], fb[AHEAD][R][2];  // [step][rows][piece]
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) {
       const long k = min(k0 + 32 * s, end - 32);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
           fa[s][i][p] = *reinterpret_cast<const uintx4*>(a[i] + 2 * k + 32 * p);
@@ -504,46 +526,45 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
     for (int s = 0; s < AHEAD; ++s) {
       if (k0 + 32 * s >= end) break;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sum[i][j] = multiply(fb[s][j][1], fa[s][i][0], sum[i][j]);
+        for (int j = 0; j < R; ++j) sum[i][j] = multiply(fb[s][j][1], fa[s][i][0], sum[i][j]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sum[i][j] = multiply(fb[s][j][0], fa[s][i][1], sum[i][j]);
+        for (int j = 0; j < R; ++j) sum[i][j] = multiply(fb[s][j][0], fa[s][i][1], sum[i][j]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) sum[i][j] = multiply(fb[s][j][0], fa[s][i][0], sum[i][j]);
+        for (int j = 0; j < R; ++j) sum[i][j] = multiply(fb[s][j][0], fa[s][i][0], sum[i][j]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < R; ++j)
       *reinterpret_cast<floatx4*>(&sums[wave][(16 * i + lane % 16) * PITCH + 16 * j + lane / 16 * 4]) = sum[i][j];
   __syncthreads();
-  // four neighbours to a lane of the first 256
-  const int row = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
-  const long m = m0 + row, n = n0 + c;
-  bool turns = tile.mirror;
-  if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1;
+  bool turns = tile.mirror && !g.parts;
+  if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1 && !g.parts;
   float z[4] = {};
-  if (row < 32) {
-    const float factor = g.factors ? g.factors[matrix] : 1.f, by = g.by * factor * (g.power == 2 ? factor : 1.f), beta = g.beta * factor;
+  if (row < SIDE) {
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const floatx4 q = *reinterpret_cast<const floatx4*>(&sums[w][row * PITCH + c]);
 #pragma unroll
       for (int v = 0; v < 4; ++v) z[v] += q[v];
     }
+    if (g.parts) {
+      storePack(g.parts + (((matrix * gridDim.y + blockIdx.y) * gridDim.x + tile.index) * SIDE + row) * SIDE + c, z);
+      return;
+    }
+    const float by = g.by * factor * (g.power == 2 ? factor : 1.f), beta = g.beta * factor;
 #pragma unroll
     for (int v = 0; v < 4; ++v) z[v] *= by;
     if (g.old.data) {
-      const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m, n);
-      const halfx4 lead = *reinterpret_cast<const halfx4*>(from), rest = *reinterpret_cast<const halfx4*>(from + 32);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) z[v] += beta * ((float)lead[v] + (float)rest[v]);
+      for (int v = 0; v < 4; ++v) z[v] += beta * ((float)oldLead[v] + (float)oldRest[v]);
     }
     if constexpr (LAST) {
 #pragma unroll
@@ -559,7 +580,7 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
   }
   if (!turns) return;
   __syncthreads();
-  if (row < 32) {
+  if (row < SIDE) {
     // now a column, four of its rows
 #pragma unroll
     for (int v = 0; v < 4; ++v) z[v] = sums[0][(c + v) * PITCH + row];
@@ -576,51 +597,65 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
 
 long padded(long n) { return (n + 31) / 32 * 32; }
 
-// What lies in the workspace, for so many matrices of P x Q.
-struct Space {
-  double* sums;
-  float* factors;
-  Pairs x, xt[2], gram, poly;
-  float* parts;
-  size_t bytes;
-
-  Space(void* workspace, long batch, long P, long Q) {
-    char* at = static_cast<char*>(workspace);
-    sums = reinterpret_cast<double*>(at);
-    at += rounded((size_t)batch * kShares * sizeof(double));
-    factors = reinterpret_cast<float*>(at);
-    at += rounded((size_t)batch * sizeof(float));
-    auto pairs = [&](long rows, long cols) {
-      const Pairs m{reinterpret_cast<half16*>(at), cols, 2 * rows * cols};
-      at += rounded((size_t)batch * 2 * rows * cols * sizeof(half16));
-      return m;
-    };
-    x = pairs(P, Q), xt[0] = pairs(Q, P), xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
-    parts = reinterpret_cast<float*>(at);
-    at += (size_t)batch * 17 * ((P + 255) / 256 + 8) * 256 * ((Q + 255) / 256) * 256 * 4;
-    bytes = at - static_cast<char*>(workspace);
-  }
-};
-
 // The kernel of a product, and the ranges that its k is cut into.
+enum PairKind { Small16, Small32, Deep64, Wide64, Deep128, Wide128, Wide256 };
 struct PairPlan {
-  int side;  // of a tile
+  int kind, side;  // side: of a tile
   long tiles, ranges, range;
 };
 
-static long forced(const char* k) { const char* f = getenv(k); return f ? atol(f) : 0; }
+// The kernel with the least expected time, in us, from what each takes for a step of 32 k: `alone` where workgroups have compute
+// units to themselves, else `each` for every one that a compute unit gets (in whole rounds where few fit it), and besides for
+// results, more of them where they are left both ways round.  Ranges add a launch, and their sums' way to memory and back.
+// Measured in every kernel on products from 64 x 64 x 64 to 2048 x 8192 x 8192: 1024 x 1024 x 1024 with half of it a mirror
+// image: Deep64 11.4, Wide64 18.4, Wide128 28; 2048 x 2048 x 2048 so: Wide64 40, Deep128 42, Wide128 in three ranges 44;
+// 2048 x 8192 x 2048: Wide256 167, Wide128 189, Wide64 240; 256 x 256 x 8192: Small32 in one range 58, in eight 17.
+PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
+  struct Option {
+    int kind, side, most;  // most: ranges
+    double alone, each;
+    bool whole;
+    double results;
+  };
+  static const Option options[] = {
+      {Small16, 16, 1, 0.136, 0.148, false, 3}, {Small32, 32, 16, 0.24, 0.243, false, 3}, {Deep64, 64, 8, 0.18, 0.24, true, 5},
+      {Wide64, 64, 8, 0.4, 0.25, false, 5},     {Deep128, 128, 8, 0.56, 0.68, true, 6},   {Wide128, 128, 8, 0.62, 0.63, true, 6},
+      {Wide256, 256, 8, 1.8, 2.4, true, 10}};
+  PairPlan best{};
+  double least = 0;
+  const long steps = K / 32;
+  const double units = computeUnits();
+  for (const Option& o : options) {
+    const long down = ceilDivLong(M, o.side), across = ceilDivLong(N, o.side);
+    const long tiles = symmetric ? down * (down + 1) / 2 : down * across;
+    for (long ranges = 1; ranges <= o.most; ranges += ranges < 4 ? 1 : ranges / 2) {
+      const long range = ceilDivLong(steps, ranges), used = ceilDivLong(steps, range);
+      if (ranges > 1 && range < 8) break;
+      const double share = (double)batch * tiles * used / units, rounds = o.whole && share < 8 ? std::ceil(share) : share;
+      double time = o.results + (symmetric ? 0 : 2) + range * (share <= 0.75 ? o.alone : std::max(o.alone, rounds * o.each));
+      if (used > 1) time += 4.5 + (double)batch * tiles * used * o.side * o.side * 8 / 4e6;
+      if (least == 0 || time < least) {
+        least = time;
+        best = PairPlan{o.kind, o.side, (tiles + 7) / 8 * 8, used, 32 * range};
+      }
+    }
+  }
+  return best;
+}
 
-PairPlan planOf(int which, long M, long N, long K) {
-  const char* sides[] = {"S0", "S1", "S2"}; const char* rs[] = {"R0", "R1", "R2"};
-  const bool symmetric = which < 2;
-  PairPlan p;
-  p.side = forced(sides[which]) ? (int)forced(sides[which]) : M >= 1024 ? 128 : 32;
-  const long down = ceilDivLong(M, p.side), across = ceilDivLong(N, p.side);
-  p.tiles = ((symmetric ? down * (down + 1) / 2 : down * across) + 7) / 8 * 8;
-  p.ranges = p.side == 32 ? 1 : forced(rs[which]) ? forced(rs[which]) : 1;
-  p.range = ceilDivLong(K / 32, p.ranges) * 32;
-  p.ranges = ceilDivLong(K, p.range);
-  return p;
+size_t partsBytes(const PairPlan& p, long batch) {
+  return p.ranges > 1 ? (size_t)batch * p.ranges * p.tiles * p.side * p.side * sizeof(float) : 0;
+}
+
+template <class RESULT, int SIDE>
+void launchSmall(const PairArgs& g, const RESULT& result, dim3 grid, hipStream_t s) {
+  // (as many waves as there are steps for, two or four ahead)
+  if (g.range <= 256)
+    small<RESULT, SIDE, 4, 2><<<grid, 256, 0, s>>>(g, result);
+  else if (g.range <= 512)
+    small<RESULT, SIDE, 8, 2><<<grid, 512, 0, s>>>(g, result);
+  else
+    small<RESULT, SIDE, 8, 4><<<grid, 512, 0, s>>>(g, result);
 }
 
 // one: see product's ONE
@@ -629,25 +664,24 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
   const dim3 grid((unsigned)plan.tiles, (unsigned)plan.ranges, batch);
   g.range = plan.range;
   if (plan.ranges > 1) g.parts = parts;
-  if (plan.side == 32) {
-    if (g.K <= 256)
-      small<RESULT, 4, 2><<<grid, 256, 0, s>>>(g, result);
-    else if (g.K <= 512)
-      small<RESULT, 8, 2><<<grid, 512, 0, s>>>(g, result);
-    else
-      small<RESULT, 8, 4><<<grid, 512, 0, s>>>(g, result);
-    return;
-  }
   auto tiles = [&](auto pieces) {
     constexpr int ONE = decltype(pieces)::value;
-    if (plan.side == 64)
-      product<RESULT, ONE, 64, 64, 32, 32><<<grid, 256, 0, s>>>(g, result);
-    else if (plan.side == 128)
-      product<RESULT, ONE, 128, 128, 64, 64><<<grid, 256, 0, s>>>(g, result);
+    if (plan.kind == Deep64)
+      product<RESULT, ONE, 64, 64, 32, 32, 4><<<grid, 256, 0, s>>>(g, result);
+    else if (plan.kind == Wide64)
+      product<RESULT, ONE, 64, 64, 32, 32, 2><<<grid, 256, 0, s>>>(g, result);
+    else if (plan.kind == Deep128)
+      product<RESULT, ONE, 128, 128, 32, 64, 4><<<grid, 512, 0, s>>>(g, result);
+    else if (plan.kind == Wide128)
+      product<RESULT, ONE, 128, 128, 64, 32, 2><<<grid, 512, 0, s>>>(g, result);
     else
-      product<RESULT, ONE, 256, 256, 128, 64><<<grid, 512, 0, s>>>(g, result);
+      product<RESULT, ONE, 256, 256, 128, 64, 2><<<grid, 512, 0, s>>>(g, result);
   };
-  if (one == 3)
+  if (plan.kind == Small16)
+    launchSmall<RESULT, 16>(g, result, grid, s);
+  else if (plan.kind == Small32)
+    launchSmall<RESULT, 32>(g, result, grid, s);
+  else if (one == 3)
     tiles(std::integral_constant<int, 3>());
   else if (one == 1)
     tiles(std::integral_constant<int, 1>());
@@ -655,15 +689,48 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
     tiles(std::integral_constant<int, 0>());
   if (plan.ranges > 1) {
     const long down = ceilDivLong(g.M, plan.side), count = g.symmetric ? down * (down + 1) / 2 : down * ceilDivLong(g.N, plan.side);
-    const dim3 blocks((unsigned)ceilDivLong(count * (plan.side / 32) * (plan.side / 64), 4), 1, batch);
-    if (plan.side == 64)
-      join<RESULT, 64, 64><<<blocks, 256, 0, s>>>(g, result, (int)plan.ranges, (int)plan.tiles, (int)count);
+    const dim3 blocks((unsigned)ceilDivLong(count * (plan.side / 32) * (plan.side > 32 ? plan.side / 64 : 1), 4), 1, batch);
+    const int ranges = (int)plan.ranges, rounded = (int)plan.tiles;
+    if (plan.side == 32)
+      join<RESULT, 32, 32><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
+    else if (plan.side == 64)
+      join<RESULT, 64, 64><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
     else if (plan.side == 128)
-      join<RESULT, 128, 128><<<blocks, 256, 0, s>>>(g, result, (int)plan.ranges, (int)plan.tiles, (int)count);
+      join<RESULT, 128, 128><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
     else
-      join<RESULT, 256, 256><<<blocks, 256, 0, s>>>(g, result, (int)plan.ranges, (int)plan.tiles, (int)count);
+      join<RESULT, 256, 256><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
   }
 }
+
+// What lies in the workspace, for so many matrices of P x Q, and how the three products of a step run.
+struct Space {
+  double* sums;
+  float* factors;
+  Pairs x, xt[2], gram, poly;
+  float* parts;
+  size_t bytes;
+  PairPlan plans[3];
+
+  Space(void* workspace, long batch, long P, long Q)
+      : plans{planOf(true, batch, P, P, Q), planOf(true, batch, P, P, P), planOf(false, batch, P, Q, P)} {
+    char* at = static_cast<char*>(workspace);
+    auto take = [&](size_t size) {
+      char* const from = at;
+      at += rounded(size);
+      return from;
+    };
+    sums = reinterpret_cast<double*>(take((size_t)batch * kShares * sizeof(double)));
+    factors = reinterpret_cast<float*>(take((size_t)batch * sizeof(float)));
+    auto pairs = [&](long rows, long cols) {
+      return Pairs{reinterpret_cast<half16*>(take((size_t)batch * 2 * rows * cols * sizeof(half16))), cols, 2 * rows * cols};
+    };
+    x = pairs(P, Q), xt[0] = pairs(Q, P), xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
+    size_t most = 0;
+    for (const PairPlan& p : plans) most = std::max(most, partsBytes(p, batch));
+    parts = reinterpret_cast<float*>(take(most));
+    bytes = at - static_cast<char*>(workspace);
+  }
+};
 
 template <class T>
 int run(const OrthogonalProblem& p, hipStream_t s) {
@@ -673,15 +740,18 @@ int run(const OrthogonalProblem& p, hipStream_t s) {
   const Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
   const Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
   Space w(p.workspace, p.batch, P, Q);
-  const PairPlan gram = planOf(0, P, P, Q), poly = planOf(1, P, P, P), last = planOf(2, P, Q, P);
-  if (p.batch > 65535) return FBFFT_UNSUPPORTED_SIZE;
+  const PairPlan &gram = w.plans[0], &poly = w.plans[1], &last = w.plans[2];
+  const long squared = ceilDivLong(P, 64) * ceilDivLong(Q, 64);
+  if (p.batch > 65535 || !launches((double)squared * p.batch, 256)) return FBFFT_UNSUPPORTED_SIZE;
+  for (const PairPlan& plan : w.plans)
+    if (!launches((double)plan.tiles * plan.ranges * p.batch, 512)) return FBFFT_UNSUPPORTED_SIZE;
   const unsigned batch = (unsigned)p.batch;
   // lines of neighbours, for the squares
   const bool lines = g.row == 1 && g.col != 1;
   const Given<const T> by{g.data, lines ? g.col : g.row, lines ? g.row : g.col, g.batch};
   const long count = lines ? rows : cols;
   squares<T><<<dim3(kShares, batch), 256, 0, s>>>(by, lines ? cols : rows, count, divisorOf(ceilDivLong(count, 8)), w.sums);
-  const dim3 grid((unsigned)(ceilDivLong(P, 64) * ceilDivLong(Q, 64)), batch);
+  const dim3 grid((unsigned)squared, batch);
   if (lines)
     begin<T, true><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
   else
