@@ -24,6 +24,8 @@ namespace {
 typedef half16 halfx4 __attribute__((ext_vector_type(4)));
 
 constexpr float kUnit = 1024.f;  // what stands for 1 in pieces
+constexpr float kWide = 64.f;    // the same for products of factors, which reach growth
+constexpr long kAloneFrom = 3;   // columns to a row of X from which on alone() may run
 
 struct Pairs {
   half16* data;
@@ -145,15 +147,22 @@ __global__ __launch_bounds__(256) void begin(Given<const T> g, long rows, long c
   }
 }
 
-__device__ __forceinline__ void storeFour(half16* to, const float (&z)[4]) {
+// Of four neighbours those from `first` up to `end`, as pieces.
+__device__ __forceinline__ void storeFour(half16* to, const float (&z)[4], int first, int end) {
   halfx4 lead, rest;
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
     lead[v] = (half16)z[v];
     rest[v] = (half16)(z[v] - (float)lead[v]);
   }
-  *reinterpret_cast<halfx4*>(to) = lead;
-  *reinterpret_cast<halfx4*>(to + 32) = rest;
+  if (first <= 0 && end >= 4) {
+    *reinterpret_cast<halfx4*>(to) = lead;
+    *reinterpret_cast<halfx4*>(to + 32) = rest;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (v >= first && v < end) to[v] = lead[v], to[v + 32] = rest[v];
+  }
 }
 
 // ---- products ----
@@ -170,7 +179,9 @@ struct PairArgs {
   const float* factors;  // not null: of each matrix; `power` times in by, once in beta
   int power;
   Pairs old, out, turned;  // old, turned: data may be null
-  bool symmetric;          // out is: tiles below the diagonal, and their mirror images
+  // out is: what lies on and below the diagonal, and its mirror image.  (Exactly: of matrices whose sides differ by roundings,
+  // the part that is not symmetric grows tenfold with every step of products that take them to commute.)
+  bool symmetric;
   float* parts;            // not null: sums of each range, [matrix][range][tile][BM][BN], in place of results
 };
 
@@ -182,6 +193,20 @@ struct Result {
   float scale;
 };
 struct Nothing {};
+
+// Of eight neighbours those from `first` up to `end`.
+__device__ __forceinline__ void storeEight(half16* to, const float (&z)[8], int first, int end) {
+  halfx8 lead, rest;
+  splitEight(z, lead, rest);
+  if (first <= 0 && end >= 8) {
+    *reinterpret_cast<halfx8*>(to) = lead;
+    *reinterpret_cast<halfx8*>(to + 32) = rest;
+  } else {
+#pragma unroll
+    for (int v = 0; v < 8; ++v)
+      if (v >= first && v < end) to[v] = lead[v], to[v + 32] = rest[v];
+  }
+}
 
 // 32 rows by COLS (64) columns of results from row m0 and column n0, both multiples of 32, by one wave: eight(row, column, v)
 // gives eight neighbouring sums.  Results that go the other way round meet in LDS, 32 x (COLS + 4) numbers.
@@ -223,11 +248,7 @@ __device__ __forceinline__ void leavePairs(const PairArgs& g, const RESULT& resu
           }
         }
       } else {
-        halfx8 lead, rest;
-        splitEight(z, lead, rest);
-        half16* const to = g.out.data + matrix * g.out.batch + placeOf(g.out, m, n);
-        *reinterpret_cast<halfx8*>(to) = lead;
-        *reinterpret_cast<halfx8*>(to + 32) = rest;
+        storeEight(g.out.data + matrix * g.out.batch + placeOf(g.out, m, n), z, 0, g.symmetric ? (int)min(m - n + 1, 8l) : 8);
       }
     }
     if (turns) {
@@ -258,11 +279,8 @@ __device__ __forceinline__ void leavePairs(const PairArgs& g, const RESULT& resu
           }
         }
       } else {
-        halfx8 lead, rest;
-        splitEight(z, lead, rest);
-        half16* const to = g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n, m0) + 8 * q;
-        *reinterpret_cast<halfx8*>(to) = lead;
-        *reinterpret_cast<halfx8*>(to + 32) = rest;
+        storeEight(g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n, m0) + 8 * q, z,
+                   g.symmetric ? (int)max(n + 1 - (m0 + 8 * q), 0l) : 0, 8);
       }
     }
   }
@@ -302,7 +320,7 @@ struct PairTile {
       int i, j;
       belowDiagonal(any ? index : 0, side, i, j);
       m0 = (long)i * BM, n0 = (long)j * BN;
-      mirror = i != j;
+      mirror = true;
     } else {
       const Tile<BM, BN> t(g.M, g.N);
       m0 = t.m0, n0 = t.n0, any = t.any;
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int range
   if (m0 >= g.M || n0 >= g.N) return;
   const long far = (long)tiles * BM * BN;  // from a range to the next
   const float* const from = g.parts + matrix * ranges * far + ((long)index * BM + row0) * BN + col0;
-  leavePairs<COLS>(g, result, matrix, m0, n0, g.symmetric ? i != j : g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
+  leavePairs<COLS>(g, result, matrix, m0, n0, g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = 0.f;
     for (int r = 0; r < ranges; ++r) {
@@ -574,7 +592,7 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
           storePack(result.y.data + matrix * result.y.batch + m * result.y.row + (n + v) * result.y.col, {z[v]});
       }
     } else {
-      storeFour(g.out.data + matrix * g.out.batch + placeOf(g.out, m, n), z);
+      storeFour(g.out.data + matrix * g.out.batch + placeOf(g.out, m, n), z, 0, g.symmetric ? (int)min(m - n + 1, 4l) : 4);
     }
     if (turns) *reinterpret_cast<floatx4*>(&sums[0][row * PITCH + c]) = floatx4{z[0], z[1], z[2], z[3]};
   }
@@ -590,7 +608,8 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
         if (n0 + row < result.cols && m0 + c + v < result.rows)
           storePack(result.y.data + matrix * result.y.batch + (n0 + row) * result.y.col + (m0 + c + v) * result.y.row, {z[v]});
     } else {
-      storeFour(g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n0 + row, m0 + c), z);
+      storeFour(g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n0 + row, m0 + c), z,
+                g.symmetric ? (int)max(n0 + row + 1 - (m0 + c), 0l) : 0, 4);
     }
   }
 }
@@ -602,6 +621,7 @@ enum PairKind { Small16, Small32, Deep64, Wide64, Deep128, Wide128, Wide256 };
 struct PairPlan {
   int kind, side;  // side: of a tile
   long tiles, ranges, range;
+  double time;  // expected
 };
 
 // The kernel with the least expected time, in us, from what each takes for a step of 32 k: `alone` where workgroups have compute
@@ -636,7 +656,7 @@ PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
       if (used > 1) time += 4.5 + (double)batch * tiles * used * o.side * o.side * 8 / 4e6;
       if (least == 0 || time < least) {
         least = time;
-        best = PairPlan{o.kind, o.side, (tiles + 7) / 8 * 8, used, 32 * range};
+        best = PairPlan{o.kind, o.side, (tiles + 7) / 8 * 8, used, 32 * range, time};
       }
     }
   }
@@ -702,17 +722,21 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
   }
 }
 
-// What lies in the workspace, for so many matrices of P x Q, and how the three products of a step run.
+// What lies in the workspace, for so many matrices of P x Q, and how the products run: of X with its transpose, of the P x P
+// matrices, of them with X, and of two of them at once.
 struct Space {
   double* sums;
   float* factors;
   Pairs x, xt[2], gram, poly;
+  Pairs turns[4];  // in the place of xt[1], gram and poly: what alone() takes
+  Pairs alonePoly;
   float* parts;
   size_t bytes;
-  PairPlan plans[3];
+  PairPlan gramPlan, polyPlan, lastPlan, twoPlan;
 
   Space(void* workspace, long batch, long P, long Q)
-      : plans{planOf(true, batch, P, P, Q), planOf(true, batch, P, P, P), planOf(false, batch, P, Q, P)} {
+      : gramPlan(planOf(true, batch, P, P, Q)), polyPlan(planOf(true, batch, P, P, P)), lastPlan(planOf(false, batch, P, Q, P)),
+        twoPlan(planOf(true, 2 * batch, P, P, P)) {
     char* at = static_cast<char*>(workspace);
     auto take = [&](size_t size) {
       char* const from = at;
@@ -724,55 +748,150 @@ struct Space {
     auto pairs = [&](long rows, long cols) {
       return Pairs{reinterpret_cast<half16*>(take((size_t)batch * 2 * rows * cols * sizeof(half16))), cols, 2 * rows * cols};
     };
-    x = pairs(P, Q), xt[0] = pairs(Q, P), xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
+    x = pairs(P, Q), xt[0] = pairs(Q, P);
+    char* const shared = at;
+    xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
+    char* const end = at;
+    at = shared;
+    for (Pairs& t : turns) t = pairs(P, P);
+    alonePoly = pairs(P, P);
+    if (Q < kAloneFrom * P) at = end;
+    at = std::max(at, end);
     size_t most = 0;
-    for (const PairPlan& p : plans) most = std::max(most, partsBytes(p, batch));
+    for (const PairPlan* p : {&gramPlan, &polyPlan, &lastPlan}) most = std::max(most, partsBytes(*p, batch));
+    if (Q >= kAloneFrom * P) most = std::max(most, partsBytes(twoPlan, 2 * batch));
     parts = reinterpret_cast<float*>(take(most));
     bytes = at - static_cast<char*>(workspace);
+  }
+
+  bool fits(long batch) const {
+    for (const PairPlan* p : {&gramPlan, &polyPlan, &lastPlan, &twoPlan})
+      if (!launches((double)p->tiles * p->ranges * batch * (p == &twoPlan ? 2 : 1), 512)) return false;
+    return true;
+  }
+  // whether the P x P matrices alone, which X meets in the last product, are expected to take less time
+  bool takesLessAlone(int steps, long P, long Q) const {
+    const double all = steps * (gramPlan.time + polyPlan.time + lastPlan.time);
+    const double alone = gramPlan.time + 8 + (3 * steps - 1) * polyPlan.time + std::max(0, steps - 2) * (twoPlan.time - polyPlan.time) + lastPlan.time;
+    return Q >= kAloneFrom * P && alone < all;
+  }
+};
+
+// m = a I + poly, in units of kWide
+__global__ __launch_bounds__(256) void firstFactor(Pairs poly, Pairs m, long rows, float a) {
+  const long words = poly.cols / 8, at = (long)blockIdx.x * 256 + threadIdx.x, i = at / words, j = (at - i * words) * 8;
+  if (i >= rows) return;
+  const half16* const from = poly.data + blockIdx.y * poly.batch + placeOf(poly, i, j);
+  halfx8 lead = *reinterpret_cast<const halfx8*>(from), rest = *reinterpret_cast<const halfx8*>(from + 32);
+  float z[8];
+#pragma unroll
+  for (int v = 0; v < 8; ++v) z[v] = ((float)lead[v] + (float)rest[v]) * (kWide / kUnit) + (i == j + v ? a * kWide : 0.f);
+  splitEight(z, lead, rest);
+  half16* const to = m.data + blockIdx.y * m.batch + placeOf(m, i, j);
+  *reinterpret_cast<halfx8*>(to) = lead;
+  *reinterpret_cast<halfx8*>(to + 32) = rest;
+}
+
+// One call: the matrices, and the launches of both ways.
+template <class T>
+struct Call {
+  const OrthogonalProblem& p;
+  hipStream_t s;
+  bool turn;
+  long rows, cols, P, Q;  // X has no more rows than columns; filled up
+  Given<const T> g;
+  Given<T> y;
+  Space w;
+
+  Call(const OrthogonalProblem& problem, hipStream_t stream)
+      : p(problem), s(stream), turn(p.rows > p.cols), rows(turn ? p.cols : p.rows), cols(turn ? p.rows : p.cols), P(padded(rows)),
+        Q(padded(cols)), g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch},
+        y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch}, w(p.workspace, p.batch, P, Q) {}
+
+  static constexpr bool SHORT = sizeof(T) == 2;  // X is single pieces at first
+  static constexpr float one = 1.f / kUnit;
+  unsigned batch() const { return (unsigned)p.batch; }
+  float coefficient(int step, int i) const { return p.coefficients[3 * step + i]; }
+  Result<T> result() const { return {y, rows, cols, p.scale / kUnit}; }
+
+  void squaresAndX(long squared) {
+    // lines of neighbours, for the squares
+    const bool lines = g.row == 1 && g.col != 1;
+    const Given<const T> by{g.data, lines ? g.col : g.row, lines ? g.row : g.col, g.batch};
+    const long count = lines ? rows : cols;
+    squares<T><<<dim3(kShares, batch()), 256, 0, s>>>(by, lines ? cols : rows, count, divisorOf(ceilDivLong(count, 8)), w.sums);
+    const dim3 grid((unsigned)squared, batch());
+    if (lines)
+      begin<T, true><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
+    else
+      begin<T, false><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
+  }
+
+  void gramOf(const Pairs& to, bool first) {
+    launchProduct(PairArgs{w.x, w.x, P, P, Q, 0, one, 0.f, first ? w.factors : nullptr, 2, Pairs{}, to, to, true, nullptr}, Nothing{},
+                  w.gramPlan, SHORT && first ? 3 : 0, w.parts, batch(), s);
+  }
+
+  // to = beta from + by a from, P x P matrices that commute, so that it is symmetric, too; of `count` matrices each
+  void commuting(const Pairs& a, const Pairs& from, const Pairs& to, float by, float beta, const PairPlan& plan, unsigned count) {
+    launchProduct(PairArgs{a, from, P, P, P, 0, by, beta, nullptr, 0, from, to, to, true, nullptr}, Nothing{}, plan, 0, w.parts, count, s);
+  }
+
+  // step after step
+  void steps() {
+    for (int i = 0; i < p.steps; ++i) {
+      const float a = coefficient(i, 0), b = coefficient(i, 1), c = coefficient(i, 2);
+      const bool first = i == 0;
+      gramOf(w.gram, first);
+      commuting(w.gram, w.gram, w.poly, c * one, b, w.polyPlan, batch());
+      const PairArgs x{w.poly, w.xt[i % 2], P, Q, P, 0, one, a, first ? w.factors : nullptr, 1, w.x, w.x, w.xt[(i + 1) % 2], false, nullptr};
+      if (i + 1 < p.steps)
+        launchProduct(x, Nothing{}, w.lastPlan, SHORT && first ? 1 : 0, w.parts, batch(), s);
+      else
+        launchProduct(x, result(), w.lastPlan, SHORT && first ? 1 : 0, w.parts, batch(), s);
+    }
+  }
+
+  // The factors a I + B of all steps first, which are polynomials of the first A as every later A is, and their product with X.
+  void alone() {
+    const Pairs &gram = w.turns[0], &next = w.turns[1], &poly = w.alonePoly;
+    gramOf(gram, true);
+    int m = 2;  // where the factors' product lies
+    for (int i = 0; i < p.steps; ++i) {
+      const float a = coefficient(i, 0), b = coefficient(i, 1), c = coefficient(i, 2);
+      const bool last = i + 1 == p.steps;
+      commuting(gram, gram, poly, c * one, b, w.polyPlan, batch());
+      const Pairs &from = w.turns[m], &to = w.turns[5 - m];
+      if (i == 0) {
+        firstFactor<<<dim3((unsigned)ceilDivLong(P * P / 8, 256), batch()), 256, 0, s>>>(poly, from, P, a);
+        if (!last) commuting(poly, gram, next, one, a, w.polyPlan, batch());
+      } else if (last || p.batch > 1) {
+        if (!last) commuting(poly, gram, next, one, a, w.polyPlan, batch());
+        commuting(poly, from, to, one, a, w.polyPlan, batch());
+        m = 5 - m;
+      } else {
+        // both at once: a matrix's place is the distance between them
+        const Pairs same{poly.data, P, 0}, sources{gram.data, P, from.data - gram.data}, results{next.data, P, to.data - next.data};
+        commuting(same, sources, results, one, a, w.twoPlan, 2);
+        m = 5 - m;
+      }
+      if (!last) commuting(poly, next, gram, one, a, w.polyPlan, batch());
+    }
+    const PairArgs x{w.turns[m], w.xt[0], P, Q, P, 0, 1.f / kWide, 0.f, w.factors, 1, Pairs{}, Pairs{}, Pairs{}, false, nullptr};
+    launchProduct(x, result(), w.lastPlan, SHORT ? 1 : 0, w.parts, batch(), s);
   }
 };
 
 template <class T>
 int run(const OrthogonalProblem& p, hipStream_t s) {
-  // (X has no more rows than columns)
-  const bool turn = p.rows > p.cols;
-  const long rows = turn ? p.cols : p.rows, cols = turn ? p.rows : p.cols, P = padded(rows), Q = padded(cols);
-  const Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
-  const Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
-  Space w(p.workspace, p.batch, P, Q);
-  const PairPlan &gram = w.plans[0], &poly = w.plans[1], &last = w.plans[2];
-  const long squared = ceilDivLong(P, 64) * ceilDivLong(Q, 64);
-  if (p.batch > 65535 || !launches((double)squared * p.batch, 256)) return FBFFT_UNSUPPORTED_SIZE;
-  for (const PairPlan& plan : w.plans)
-    if (!launches((double)plan.tiles * plan.ranges * p.batch, 512)) return FBFFT_UNSUPPORTED_SIZE;
-  const unsigned batch = (unsigned)p.batch;
-  // lines of neighbours, for the squares
-  const bool lines = g.row == 1 && g.col != 1;
-  const Given<const T> by{g.data, lines ? g.col : g.row, lines ? g.row : g.col, g.batch};
-  const long count = lines ? rows : cols;
-  squares<T><<<dim3(kShares, batch), 256, 0, s>>>(by, lines ? cols : rows, count, divisorOf(ceilDivLong(count, 8)), w.sums);
-  const dim3 grid((unsigned)squared, batch);
-  if (lines)
-    begin<T, true><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
+  Call<T> call(p, s);
+  const long squared = ceilDivLong(call.P, 64) * ceilDivLong(call.Q, 64);
+  if (p.batch > 65535 || !launches((double)squared * p.batch, 256) || !call.w.fits(p.batch)) return FBFFT_UNSUPPORTED_SIZE;
+  call.squaresAndX(squared);
+  if (__is_same(T, brain16) && p.growth * kWide <= 32768 && call.w.takesLessAlone(p.steps, call.P, call.Q))
+    call.alone();
   else
-    begin<T, false><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
-  constexpr bool SHORT = sizeof(T) == 2;
-  const float one = 1.f / kUnit;
-  for (int i = 0; i < p.steps; ++i) {
-    const float a = p.coefficients[3 * i], b = p.coefficients[3 * i + 1], c = p.coefficients[3 * i + 2];
-    const Pairs from = w.xt[i % 2], to = w.xt[(i + 1) % 2], none{};
-    const float* const factors = i == 0 ? w.factors : nullptr;
-    const bool shorter = SHORT && i == 0;
-    launchProduct(PairArgs{w.x, w.x, P, P, Q, 0, one, 0.f, factors, 2, none, w.gram, w.gram, true, nullptr}, Nothing{}, gram,
-                  shorter ? 3 : 0, w.parts, batch, s);
-    launchProduct(PairArgs{w.gram, w.gram, P, P, P, 0, c * one, b, nullptr, 0, w.gram, w.poly, w.poly, true, nullptr}, Nothing{}, poly, 0,
-                  w.parts, batch, s);
-    const PairArgs x{w.poly, from, P, Q, P, 0, one, a, factors, 1, w.x, w.x, to, false, nullptr};
-    if (i + 1 < p.steps)
-      launchProduct(x, Nothing{}, last, shorter ? 1 : 0, w.parts, batch, s);
-    else
-      launchProduct(x, Result<T>{y, rows, cols, p.scale / kUnit}, last, shorter ? 1 : 0, w.parts, batch, s);
-  }
+    call.steps();
   return launchStatus();
 }
 

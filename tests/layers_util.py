@@ -57,38 +57,53 @@ def layer_norm_grads(x, weight, mean, rstd, g):
 QUINTIC = (3.4445, -4.7750, 2.0315)
 
 
-def orthogonal(g, triples, eps, scale, moved=None):
-    """The formula on [batch][rows][cols]; moved(v, k): what becomes of a value that is held between products, from sums
-    of k products."""
-    moved = moved or (lambda v, k: v)
+def orthogonal(g, triples, eps, scale, moved=None, alone=False):
+    """The formula on [batch][rows][cols]; moved(v, k, unit): what becomes of a value that is held between products, from
+    sums of k products, in pieces whose unit is `unit`.  alone: the factors a I + B of all steps first, and X in the end."""
+    moved = moved or (lambda v, k, unit=1024: v)
     x = g.detach().cpu().double()
     turn = x.shape[1] > x.shape[2]
     x = x.transpose(1, 2) if turn else x
     x = x / (x.square().sum((1, 2), keepdim=True).sqrt() + eps)
     p, q = x.shape[1:]
-    for i, (a, b, c) in enumerate(triples):
-        x = moved(x, 1 if i == 0 else p)
-        gram = moved(x @ x.transpose(1, 2), q)
-        poly = moved(b * gram + c * (gram @ gram), p)
-        x = a * x + poly @ x
+    if alone:
+        same = lambda v, k, unit=1024: (lambda w: w.tril() + w.tril(-1).transpose(1, 2))(moved(v, k, unit))  # noqa: E731
+        x = moved(x, 1)
+        gram, m = same(x @ x.transpose(1, 2), q), None
+        for i, (a, b, c) in enumerate(triples):
+            poly = same(b * gram + c * (gram @ gram), p)
+            m = same(poly + a * torch.eye(p, dtype=torch.float64) if m is None else a * m + poly @ m, p, 64)
+            if i + 1 < len(triples):
+                half = same(a * gram + poly @ gram, p)
+                gram = same(a * half + poly @ half, p)
+        x = m @ x
+    else:
+        for i, (a, b, c) in enumerate(triples):
+            x = moved(x, 1 if i == 0 else p)
+            gram = moved(x @ x.transpose(1, 2), q)
+            poly = moved(b * gram + c * (gram @ gram), p)
+            x = a * x + poly @ x
     x = moved(x, p) * scale
     return x.transpose(1, 2) if turn else x
 
 
 def orthogonal_bound(g, triples, eps, scale):
     """How far 22 bits of every value between the products, and 32-bit sums of them, may leave the result off: the formula
-    with every such value moved by a random part of its rounding, 2^-22 of itself and 2^-35 (the smallest second piece),
-    and of its sum's, 2^-24 sqrt(k) of its row's and column's size, which the root of the matrix's mean square stands for.
-    Eight such moves, three times the largest; (the rounding to the result's type apart)."""
+    with every such value moved by a random part of its rounding, 2^-22 of itself and 2^-25 of the pieces' unit (the smallest
+    second piece), and of its sum's, 2^-24 sqrt(k) of its row's and column's size, which the root of the matrix's mean square
+    stands for.  Eight such moves, three times the largest; (the rounding to the result's type apart).  bfloat16 matrices
+    with three times as many columns as rows, or rows as columns, may be computed alone."""
     gen = torch.Generator().manual_seed(1)
 
-    def moved(v, k):
-        unit = lambda: torch.rand(v.shape, generator=gen, dtype=torch.float64) * 2 - 1  # noqa: E731
+    def moved(v, k, unit=1024):
+        part = lambda: torch.rand(v.shape, generator=gen, dtype=torch.float64) * 2 - 1  # noqa: E731
         size = v.square().mean((1, 2), keepdim=True).sqrt()
-        return v + unit() * (2.0 ** -22 * v.abs() + 2.0 ** -35) + unit() * 2.0 ** -24 * math.sqrt(k) * size
+        return v + part() * (2.0 ** -22 * v.abs() + 2.0 ** -25 / unit) + part() * 2.0 ** -24 * math.sqrt(k) * size
 
     want = orthogonal(g, triples, eps, scale)
-    offs = [orthogonal(g, triples, eps, scale, moved) - want for _ in range(8)]
+    short, long = (-(-n // 32) for n in sorted(g.shape[1:]))
+    forms = [False, True] if g.dtype == torch.bfloat16 and long >= 3 * short else [False]
+    offs = [orthogonal(g, triples, eps, scale, moved, form) - want for form in forms for _ in range(8)]
     norms = torch.stack([o.square().sum((1, 2)).sqrt() for o in offs]).amax(0)
     return want, 3 * norms, 3 * torch.stack([o.abs().amax((1, 2)) for o in offs]).amax(0)
 

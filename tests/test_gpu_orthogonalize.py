@@ -72,9 +72,34 @@ def test_batches_and_strides(shape, form, dtype):
     check(stored(g, dtype, form), form=form)
 
 
-def test_large():
+@pytest.mark.parametrize("shape", [(1280, 2100), (500, 2100), (2100, 700)], ids=str)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=NAMES.get)
+def test_large(shape, dtype):
     gen = torch.Generator().manual_seed(3)
-    check(gradient(gen, 1, 1280, 2100)[0].to(torch.bfloat16).to(dev()))
+    check(gradient(gen, 1, *shape)[0].to(dtype).to(dev()))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("noise", [1e-1, 1e-2, 1e-4])
+@pytest.mark.parametrize("shape", [(90, 100), (100, 700), (640, 96)], ids=str)
+def test_few_strong_directions(shape, noise, dtype):
+    """One direction over noise: small singular values that the first steps multiply by 3.4 each, and what rounding put beside
+    them.  The result stays within a rounding of bfloat16 (2.3e-3 of its norm on average) of the formula."""
+    gen = torch.Generator().manual_seed(11)
+    g = (randn(gen, shape[0], 1) @ randn(gen, 1, shape[1]) + noise * randn(gen, *shape)).to(dtype).to(dev())
+    y = check(g).cpu().double()
+    want = orthogonal(g[None], [QUINTIC] * 5, 1e-7, 1.0)[0]
+    assert float((y - want).norm() / want.norm()) < {torch.float32: 2e-4, torch.float16: 5e-4, torch.bfloat16: 2.3e-3}[dtype]
+
+
+@pytest.mark.parametrize("batch", [1, 3])
+@pytest.mark.parametrize("steps", [1, 2, 3, 7])
+def test_steps_of_long_matrices(steps, batch):
+    gen = torch.Generator().manual_seed(12)
+    g = gradient(gen, batch, 64, 1000).to(torch.bfloat16).to(dev())
+    check(g, steps=steps)
+    check(g.transpose(1, 2).contiguous(), steps=steps, scale=0.5)
+    check(g, steps=steps, coefficients=(1.5, -0.5, 0.0))
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
