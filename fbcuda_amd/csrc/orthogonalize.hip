@@ -614,6 +614,199 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
   }
 }
 
+// ---- small matrices: all steps in one launch ----
+
+// A workgroup to a matrix, whose X, A and B stay in LDS: pair lines of 32 columns as in memory, rows 16 bytes further apart, so that
+// the 16 rows of a fragment take all banks.  Waves take blocks of 16 x 16 results in turn; X's columns, which the last product
+// of a step sums over X's rows, come by the transposing read.
+constexpr int kWholeLanes = 1024, kWholeSteps = 3;  // of 32 rows of X, at most
+constexpr int kWholeSmall = 64 << 10, kWholeLarge = 156 << 10;  // bytes of LDS
+
+struct WholeArgs {
+  long rows, cols;
+  int P, Q, steps;
+  float eps, scale;
+  float coefficients[96];
+};
+
+inline long wholeBytes(long P, long Q) { return P * (4 * Q + 16) + 2 * P * (4 * P + 16); }
+
+// Eight k from 32 kb + 8 (lane / 16) of row first + lane % 16.
+__device__ __forceinline__ uintx4 wholeFragment(const char* m, int pitch, int first, int kb, int piece) {
+  const int lane = threadIdx.x % 64;
+  return *reinterpret_cast<const uintx4*>(m + (first + lane % 16) * pitch + kb * 128 + piece * 64 + lane / 16 * 16);
+}
+// The same of a matrix that lies the other way round, [k][row].  (Of sixteen lanes, lane l gives the address of four rows (l % 4)
+// of k (l / 4) and gets four k of row l.)
+__device__ __forceinline__ uintx4 wholeTurned(const char* m, int pitch, int first, int kb, int piece) {
+  const int lane = threadIdx.x % 64, at = first + lane % 4 * 4;
+  uintx4 f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int k = 32 * kb + lane / 16 * 8 + lane % 16 / 4 + 4 * h;
+    const char* const from = m + k * pitch + at / 32 * 128 + piece * 64 + at % 32 * 2;
+    const uintx2 u = __builtin_bit_cast(
+        uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) shortx4*)const_cast<char*>(from)));
+    f[2 * h] = u[0];
+    f[2 * h + 1] = u[1];
+  }
+  return f;
+}
+
+// a block's sums, of kbs steps: a(kb, piece) and b(kb, piece) give the fragments.  (Three sums, which do not wait for each other.)
+template <class A, class B>
+__device__ __forceinline__ floatx4 wholeSums(int kbs, A a, B b) {
+  floatx4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0, s2 = s0;
+  for (int kb = 0; kb < kbs; ++kb) {
+    const uintx4 a0 = a(kb, 0), a1 = a(kb, 1), b0 = b(kb, 0), b1 = b(kb, 1);
+    s1 = multiply(b1, a0, s1);
+    s2 = multiply(b0, a1, s2);
+    s0 = multiply(b0, a0, s0);
+  }
+  return s0 + (s1 + s2);
+}
+
+__device__ __forceinline__ void wholePair(char* m, int pitch, int i, int j, half16& lead, half16& rest) {
+  const half16* const at = reinterpret_cast<const half16*>(m + i * pitch + j / 32 * 128) + j % 32;
+  lead = at[0], rest = at[32];
+}
+
+// This lane's four results of block (i, j), of row m = 16 i + lane % 16 and columns from n = 16 j + 4 (lane / 16), of a symmetric
+// matrix: what lies on and below the diagonal, and its mirror image.
+__device__ __forceinline__ void wholeSymmetric(char* to, int pitch, int i, int j, const float (&z)[4]) {
+  const int lane = threadIdx.x % 64, m = 16 * i + lane % 16, n = 16 * j + lane / 16 * 4;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    if (n + v > m) continue;
+    const half16 lead = (half16)z[v], rest = (half16)(z[v] - (float)lead);
+    half16* const here = reinterpret_cast<half16*>(to + m * pitch + (n + v) / 32 * 128) + (n + v) % 32;
+    half16* const there = reinterpret_cast<half16*>(to + (n + v) * pitch + m / 32 * 128) + m % 32;
+    here[0] = lead, here[32] = rest;
+    there[0] = lead, there[32] = rest;
+  }
+}
+
+template <class T, int BYTES>
+__global__ __launch_bounds__(kWholeLanes) void whole(Given<const T> g, Given<T> y, WholeArgs w) {
+  constexpr int WAVES = kWholeLanes / 64;
+  __shared__ __attribute__((aligned(128))) char space[BYTES];
+  __shared__ double sums[WAVES];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, P = w.P, Q = w.Q;
+  const int pitchX = 4 * Q + 16, pitchA = 4 * P + 16;
+  char *const x = space, *const gram = x + P * pitchX, *const poly = gram + P * pitchA;
+  const T* const from = g.data + blockIdx.x * g.batch;
+  T* const to = y.data + blockIdx.x * y.batch;
+
+  // G as numbers of 32 bits, in the place of their pairs, and its squares
+  double sum = 0;
+  const bool lines = g.row == 1 && g.col != 1;  // columns are the lines of neighbours
+  const int words = (lines ? P : Q) / 8, total = (lines ? Q : P) * words;
+  for (int at = threadIdx.x; at < total; at += kWholeLanes) {
+    const int line = at / words, in = (at - line * words) * 8;
+    const long here = lines ? w.cols : w.rows, count = lines ? w.rows : w.cols;
+    float v[8] = {};
+    if (line < here) loadEight(from + line * (lines ? g.col : g.row), lines ? g.row : g.col, in, count, v);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      sum += (double)v[q] * (double)v[q];
+      const int i = lines ? in + q : line, j = lines ? line : in + q;
+      *reinterpret_cast<float*>(x + i * pitchX + 4 * j) = v[q];
+    }
+  }
+  sum = waveSum(sum);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int q = 0; q < WAVES; ++q) sum += sums[q];
+  const double by = (double)kUnit / (__builtin_sqrt(sum) + (double)w.eps);
+  // (eight lanes to a line of 32 numbers, all of a wave's before any of its pairs)
+  for (int first = 0; first < P * (Q / 32); first += kWholeLanes / 8) {
+    const int at = first + threadIdx.x / 8, i = at / (Q / 32), in = threadIdx.x % 8 * 4;
+    char* const line = x + i * pitchX + (at - i * (Q / 32)) * 128;
+    float z[4] = {};
+    if (i < P) {
+      const floatx4 v = *reinterpret_cast<const floatx4*>(line + in * 4);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) z[q] = (float)((double)v[q] * by);
+    }
+    waveExchange();
+    if (i < P) storeFour(reinterpret_cast<half16*>(line) + in, z, 0, 4);
+    waveExchange();
+  }
+  __syncthreads();
+
+  const float one = 1.f / kUnit;
+  const int down = P / 16, triangle = down * (down + 1) / 2;
+  for (int step = 0; step < w.steps; ++step) {
+    const float a = w.coefficients[3 * step], b = w.coefficients[3 * step + 1], c = w.coefficients[3 * step + 2];
+    for (int t = wave; t < triangle; t += WAVES) {
+      int i, j;
+      belowDiagonal(t, down, i, j);
+      const floatx4 s = wholeSums(
+          Q / 32, [&](int kb, int p) { return wholeFragment(x, pitchX, 16 * i, kb, p); },
+          [&](int kb, int p) { return wholeFragment(x, pitchX, 16 * j, kb, p); });
+      wholeSymmetric(gram, pitchA, i, j, {s[0] * one, s[1] * one, s[2] * one, s[3] * one});
+    }
+    __syncthreads();
+    for (int t = wave; t < triangle; t += WAVES) {
+      int i, j;
+      belowDiagonal(t, down, i, j);
+      const floatx4 s = wholeSums(
+          P / 32, [&](int kb, int p) { return wholeFragment(gram, pitchA, 16 * i, kb, p); },
+          [&](int kb, int p) { return wholeFragment(gram, pitchA, 16 * j, kb, p); });
+      const int m = 16 * i + lane % 16, n = 16 * j + lane / 16 * 4;
+      float z[4];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        half16 lead, rest;
+        wholePair(gram, pitchA, m, n + v, lead, rest);
+        z[v] = c * one * s[v] + b * ((float)lead + (float)rest);
+      }
+      wholeSymmetric(poly, pitchA, i, j, z);
+    }
+    __syncthreads();
+    // 16 columns of X at a time, which nobody else takes, so that they are overwritten where they lie
+    const bool last = step + 1 == w.steps;
+#pragma unroll 1
+    for (int j = wave; j < Q / 16; j += WAVES) {
+      uintx4 columns[kWholeSteps][2];
+#pragma unroll
+      for (int kb = 0; kb < kWholeSteps; ++kb)
+        if (kb < P / 32)
+#pragma unroll
+          for (int piece = 0; piece < 2; ++piece) columns[kb][piece] = wholeTurned(x, pitchX, 16 * j, kb, piece);
+      waveExchange();
+#pragma unroll 1
+      for (int i = 0; i < down; ++i) {
+        floatx4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0, s2 = s0;
+#pragma unroll
+        for (int kb = 0; kb < kWholeSteps; ++kb)
+          if (kb < P / 32) {
+            const uintx4 a0 = wholeFragment(poly, pitchA, 16 * i, kb, 0), a1 = wholeFragment(poly, pitchA, 16 * i, kb, 1);
+            s1 = multiply(columns[kb][1], a0, s1);
+            s2 = multiply(columns[kb][0], a1, s2);
+            s0 = multiply(columns[kb][0], a0, s0);
+          }
+        const int m = 16 * i + lane % 16, n = 16 * j + lane / 16 * 4;
+        half16* const here = reinterpret_cast<half16*>(x + m * pitchX + n / 32 * 128) + n % 32;
+        const halfx4 lead = *reinterpret_cast<const halfx4*>(here), rest = *reinterpret_cast<const halfx4*>(here + 32);
+        float z[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) z[v] = one * (s0[v] + (s1[v] + s2[v])) + a * ((float)lead[v] + (float)rest[v]);
+        if (!last) {
+          storeFour(here, z, 0, 4);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (m < w.rows && n + v < w.cols) storePack(to + m * y.row + (n + v) * y.col, {z[v] * w.scale});
+        }
+      }
+    }
+    if (!last) __syncthreads();
+  }
+}
+
 long padded(long n) { return (n + 31) / 32 * 32; }
 
 // The kernel of a product, and the ranges that its k is cut into.
@@ -883,7 +1076,24 @@ struct Call {
 };
 
 template <class T>
+bool launchWhole(const OrthogonalProblem& p, hipStream_t s) {
+  const bool turn = p.rows > p.cols;
+  const long rows = turn ? p.cols : p.rows, cols = turn ? p.rows : p.cols, P = padded(rows), Q = padded(cols), bytes = wholeBytes(P, Q);
+  if (bytes > kWholeLarge || P > 32 * kWholeSteps) return false;
+  const Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
+  const Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
+  WholeArgs w{rows, cols, (int)P, (int)Q, p.steps, p.eps, p.scale / kUnit, {}};
+  for (int i = 0; i < 3 * p.steps; ++i) w.coefficients[i] = p.coefficients[i];
+  if (bytes <= kWholeSmall)
+    whole<T, kWholeSmall><<<dim3((unsigned)p.batch), kWholeLanes, 0, s>>>(g, y, w);
+  else
+    whole<T, kWholeLarge><<<dim3((unsigned)p.batch), kWholeLanes, 0, s>>>(g, y, w);
+  return true;
+}
+
+template <class T>
 int run(const OrthogonalProblem& p, hipStream_t s) {
+  if (p.batch <= 0x3fffff && launchWhole<T>(p, s)) return launchStatus();
   Call<T> call(p, s);
   const long squared = ceilDivLong(call.P, 64) * ceilDivLong(call.Q, 64);
   if (p.batch > 65535 || !launches((double)squared * p.batch, 256) || !call.w.fits(p.batch)) return FBFFT_UNSUPPORTED_SIZE;
