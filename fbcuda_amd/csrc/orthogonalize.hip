@@ -619,7 +619,8 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
 // A workgroup to a matrix, whose X, A and B stay in LDS: pair lines of 32 columns as in memory, rows 16 bytes further apart, so that
 // the 16 rows of a fragment take all banks.  Waves take blocks of 16 x 16 results in turn; X's columns, which the last product
 // of a step sums over X's rows, come by the transposing read.
-constexpr int kWholeLanes = 1024, kWholeSteps = 3;  // of 32 rows of X, at most
+constexpr int kWholeLanes = 1024;
+constexpr int kWholeSteps = 3, kWholeBlocks = 2;  // of 32 rows of X, at most, and of a symmetric matrix to a wave
 constexpr int kWholeSmall = 64 << 10, kWholeLarge = 156 << 10;  // bytes of LDS
 
 struct WholeArgs {
@@ -657,6 +658,7 @@ __device__ __forceinline__ uintx4 wholeTurned(const char* m, int pitch, int firs
 template <class A, class B>
 __device__ __forceinline__ floatx4 wholeSums(int kbs, A a, B b) {
   floatx4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0, s2 = s0;
+#pragma unroll 4
   for (int kb = 0; kb < kbs; ++kb) {
     const uintx4 a0 = a(kb, 0), a1 = a(kb, 1), b0 = b(kb, 0), b1 = b(kb, 1);
     s1 = multiply(b1, a0, s1);
@@ -691,7 +693,7 @@ __global__ __launch_bounds__(kWholeLanes) void whole(Given<const T> g, Given<T> 
   constexpr int WAVES = kWholeLanes / 64;
   __shared__ __attribute__((aligned(128))) char space[BYTES];
   __shared__ double sums[WAVES];
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, P = w.P, Q = w.Q;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64, P = w.P, Q = w.Q;
   const int pitchX = 4 * Q + 16, pitchA = 4 * P + 16;
   char *const x = space, *const gram = x + P * pitchX, *const poly = gram + P * pitchA;
   const T* const from = g.data + blockIdx.x * g.batch;
@@ -737,21 +739,31 @@ __global__ __launch_bounds__(kWholeLanes) void whole(Given<const T> g, Given<T> 
   __syncthreads();
 
   const float one = 1.f / kUnit;
-  const int down = P / 16, triangle = down * (down + 1) / 2;
+  const int down = P / 16, triangle = down * (down + 1) / 2, across = Q / 16;
+  int rows[kWholeBlocks], cols[kWholeBlocks];  // of this wave's blocks of a symmetric matrix
+#pragma unroll
+  for (int q = 0; q < kWholeBlocks; ++q) {
+    const int t = wave + WAVES * q;
+    belowDiagonal(t < triangle ? t : 0, down, rows[q], cols[q]);
+  }
+  // waves that share 16 columns of X, where there are fewer of those than waves
+  const int shares = across >= WAVES ? 1 : across >= WAVES / 2 ? 2 : 4, rounds = (across * shares + WAVES - 1) / WAVES;
   for (int step = 0; step < w.steps; ++step) {
     const float a = w.coefficients[3 * step], b = w.coefficients[3 * step + 1], c = w.coefficients[3 * step + 2];
-    for (int t = wave; t < triangle; t += WAVES) {
-      int i, j;
-      belowDiagonal(t, down, i, j);
+#pragma unroll
+    for (int q = 0; q < kWholeBlocks; ++q) {
+      if (wave + WAVES * q >= triangle) break;
+      const int i = rows[q], j = cols[q];
       const floatx4 s = wholeSums(
           Q / 32, [&](int kb, int p) { return wholeFragment(x, pitchX, 16 * i, kb, p); },
           [&](int kb, int p) { return wholeFragment(x, pitchX, 16 * j, kb, p); });
       wholeSymmetric(gram, pitchA, i, j, {s[0] * one, s[1] * one, s[2] * one, s[3] * one});
     }
     __syncthreads();
-    for (int t = wave; t < triangle; t += WAVES) {
-      int i, j;
-      belowDiagonal(t, down, i, j);
+#pragma unroll
+    for (int q = 0; q < kWholeBlocks; ++q) {
+      if (wave + WAVES * q >= triangle) break;
+      const int i = rows[q], j = cols[q];
       const floatx4 s = wholeSums(
           P / 32, [&](int kb, int p) { return wholeFragment(gram, pitchA, 16 * i, kb, p); },
           [&](int kb, int p) { return wholeFragment(gram, pitchA, 16 * j, kb, p); });
@@ -766,19 +778,26 @@ __global__ __launch_bounds__(kWholeLanes) void whole(Given<const T> g, Given<T> 
       wholeSymmetric(poly, pitchA, i, j, z);
     }
     __syncthreads();
-    // 16 columns of X at a time, which nobody else takes, so that they are overwritten where they lie
+    // 16 columns of X at a time, overwritten where they lie, when all that they are summed from is in registers
     const bool last = step + 1 == w.steps;
 #pragma unroll 1
-    for (int j = wave; j < Q / 16; j += WAVES) {
+    for (int round = 0; round < rounds; ++round) {
+      const int task = wave + WAVES * round, j = task / shares;
       uintx4 columns[kWholeSteps][2];
+      if (j < across) {
 #pragma unroll
-      for (int kb = 0; kb < kWholeSteps; ++kb)
-        if (kb < P / 32)
+        for (int kb = 0; kb < kWholeSteps; ++kb)
+          if (kb < P / 32)
 #pragma unroll
-          for (int piece = 0; piece < 2; ++piece) columns[kb][piece] = wholeTurned(x, pitchX, 16 * j, kb, piece);
-      waveExchange();
-#pragma unroll 1
-      for (int i = 0; i < down; ++i) {
+            for (int piece = 0; piece < 2; ++piece) columns[kb][piece] = wholeTurned(x, pitchX, 16 * j, kb, piece);
+      }
+      if (shares > 1)
+        __syncthreads();
+      else
+        waveExchange();
+      if (j >= across) continue;
+#pragma unroll 2
+      for (int i = task % shares; i < down; i += shares) {
         floatx4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0, s2 = s0;
 #pragma unroll
         for (int kb = 0; kb < kWholeSteps; ++kb)
