@@ -399,6 +399,9 @@ int launchRowsBack(const LayerNormProblem& p, float* parts, hipStream_t s) {
   FBFFT_ROWS(512, 1)
   FBFFT_ROWS(1024, 1)
   FBFFT_ROWS(1024, 2)
+  if constexpr (sizeof(T) == 4) {
+    FBFFT_ROWS(1024, 4)
+  }
 #undef FBFFT_ROWS
   return 0;
 }
