@@ -12,13 +12,14 @@ namespace {
 constexpr int kLanes = 256;
 
 // the sum over a workgroup, in every lane
+template <int LANES>
 __device__ __forceinline__ float groupSum(float v, float* space) {
   v = waveSum(v);
   if (threadIdx.x % 64 == 0) space[threadIdx.x / 64] = v;
   __syncthreads();
   v = 0.f;
 #pragma unroll
-  for (int q = 0; q < kLanes / 64; ++q) v += space[q];
+  for (int q = 0; q < LANES / 64; ++q) v += space[q];
   __syncthreads();
   return v;
 }
@@ -28,21 +29,24 @@ __device__ __forceinline__ float valueOf(const Matrix& m, long i, long j) {
   return (float)static_cast<const T*>(m.data)[i * m.row + j * m.col];
 }
 
-// any strides: a workgroup to a row
-template <class T>
-__global__ __launch_bounds__(kLanes) void anyForward(LayerNormProblem p) {
-  __shared__ float space[kLanes / 64];
+// any strides and lengths: a workgroup to a row
+template <class T, int LANES>
+__global__ __launch_bounds__(LANES) void anyForward(LayerNormProblem p) {
+  __shared__ float space[LANES / 64];
   for (long i = blockIdx.x; i < p.M; i += gridDim.x) {
     float sum = 0.f;
-    for (long j = threadIdx.x; j < p.N; j += kLanes) sum += valueOf<T>(p.x, i, j);
-    const float mean = groupSum(sum, space) / p.N;
+#pragma unroll 4
+    for (long j = threadIdx.x; j < p.N; j += LANES) sum += valueOf<T>(p.x, i, j);
+    const float mean = groupSum<LANES>(sum, space) / p.N;
     sum = 0.f;
-    for (long j = threadIdx.x; j < p.N; j += kLanes) {
+#pragma unroll 4
+    for (long j = threadIdx.x; j < p.N; j += LANES) {
       const float d = valueOf<T>(p.x, i, j) - mean;
       sum += d * d;
     }
-    const float rstd = 1.f / __builtin_sqrtf(groupSum(sum, space) / p.N + p.eps);
-    for (long j = threadIdx.x; j < p.N; j += kLanes)
+    const float rstd = 1.f / __builtin_sqrtf(groupSum<LANES>(sum, space) / p.N + p.eps);
+#pragma unroll 4
+    for (long j = threadIdx.x; j < p.N; j += LANES)
       static_cast<T*>(p.y.data)[i * p.y.row + j * p.y.col] =
           (T)((valueOf<T>(p.x, i, j) - mean) * rstd * lineOr(p.weight, j, 1.f) + lineOr(p.bias, j, 0.f));
     if (threadIdx.x == 0) {
@@ -52,20 +56,22 @@ __global__ __launch_bounds__(kLanes) void anyForward(LayerNormProblem p) {
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(kLanes) void anyBackward(LayerNormProblem p) {
-  __shared__ float space[kLanes / 64];
+template <class T, int LANES>
+__global__ __launch_bounds__(LANES) void anyBackward(LayerNormProblem p) {
+  __shared__ float space[LANES / 64];
   for (long i = blockIdx.x; i < p.M; i += gridDim.x) {
     const float mean = p.mean[i * p.meanStride], rstd = p.rstd[i * p.rstdStride];
     float s1 = 0.f, s2 = 0.f;
-    for (long j = threadIdx.x; j < p.N; j += kLanes) {
+#pragma unroll 4
+    for (long j = threadIdx.x; j < p.N; j += LANES) {
       const float h = valueOf<T>(p.g, i, j) * lineOr(p.weight, j, 1.f);
       s1 += h;
       s2 += h * ((valueOf<T>(p.x, i, j) - mean) * rstd);
     }
-    s1 = groupSum(s1, space) / p.N;
-    s2 = groupSum(s2, space) / p.N;
-    for (long j = threadIdx.x; j < p.N; j += kLanes) {
+    s1 = groupSum<LANES>(s1, space) / p.N;
+    s2 = groupSum<LANES>(s2, space) / p.N;
+#pragma unroll 4
+    for (long j = threadIdx.x; j < p.N; j += LANES) {
       const float h = valueOf<T>(p.g, i, j) * lineOr(p.weight, j, 1.f), xh = (valueOf<T>(p.x, i, j) - mean) * rstd;
       static_cast<T*>(p.y.data)[i * p.y.row + j * p.y.col] = (T)(rstd * (h - s1 - xh * s2));
     }
@@ -324,21 +330,68 @@ __global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* 
   }
 }
 
-// The workgroups' sums, joined in their order: 16 columns of [2][N] to a workgroup, 64 lanes to each.
+// Columns' sums by themselves: a wave takes 64 words of a row and every kColumnWaves-th row of a band.  A band's go to parts
+// [band][2][N], those of one band to the gradients.
+constexpr int kColumnWaves = 8;
+
+template <class T, int VEC>
+__global__ __launch_bounds__(kColumnWaves * 64) void columnSums(LayerNormProblem p, float* parts, long rows) {
+  __shared__ __attribute__((aligned(16))) float sums[kColumnWaves][64 * VEC];
+  typedef Row<T, VEC, 64, 1> R;
+  const long from = (long)blockIdx.x * 64 * VEC, first = (long)blockIdx.y * rows, end = min(first + rows, p.M);
+  Matrix x = p.x, g = p.g;
+  x.data = static_cast<T*>(x.data) + from, g.data = static_cast<T*>(g.data) + from;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  float sumW[VEC] = {}, sumB[VEC] = {};
+#pragma unroll 4
+  for (long i = first + wave; i < end; i += kColumnWaves) {
+    R a, b;
+    a.load(x, i, p.N - from);
+    b.load(g, i, p.N - from);
+    const float mean = p.mean[i * p.meanStride], rstd = p.rstd[i * p.rstdStride];
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) {
+      const float dy = (float)b.v[0][q];
+      sumB[q] += dy;
+      sumW[q] = __builtin_fmaf(dy, ((float)a.v[0][q] - mean) * rstd, sumW[q]);
+    }
+  }
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) sums[wave][threadIdx.x % 64 * VEC + q] = part ? sumB[q] : sumW[q];
+    __syncthreads();
+    const Line& to = part ? p.gradBias : p.gradWeight;
+    for (int j = threadIdx.x; j < 64 * VEC && from + j < p.N; j += kColumnWaves * 64) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < kColumnWaves; ++q) v += sums[q][j];
+      if (parts)
+        parts[(2 * blockIdx.y + part) * p.N + from + j] = v;
+      else if (to.data)
+        storeAny(to.data, to.type, (from + j) * to.stride, v);
+    }
+  }
+}
+
+// Parts' sums, joined in their order: 1024 / SLICES columns of [2][N] to a workgroup, SLICES lanes to each.
+template <int SLICES>
 __global__ __launch_bounds__(1024) void joinRows(LayerNormProblem p, const float* parts, int bands) {
-  __shared__ float sums[64][17];
-  const int column = threadIdx.x % 16, slice = threadIdx.x / 16;
-  const long j = (long)blockIdx.x * 16 + column;
+  constexpr int COLUMNS = 1024 / SLICES;
+  __shared__ float sums[SLICES][COLUMNS + 1];
+  const int column = threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS;
+  const long j = (long)blockIdx.x * COLUMNS + column;
   float sum = 0.f;
   if (j < 2 * p.N)
 #pragma unroll 8
-    for (int r = slice; r < bands; r += 64) sum += parts[r * 2 * p.N + j];
+    for (int r = slice; r < bands; r += SLICES) sum += parts[r * 2 * p.N + j];
   sums[slice][column] = sum;
   __syncthreads();
   if (slice > 0 || j >= 2 * p.N) return;
   sum = 0.f;
 #pragma unroll
-  for (int q = 0; q < 64; ++q) sum += sums[q][column];
+  for (int q = 0; q < SLICES; ++q) sum += sums[q][column];
   const Line& to = j < p.N ? p.gradWeight : p.gradBias;
   if (to.data) storeAny(to.data, to.type, (j < p.N ? j : j - p.N) * to.stride, sum);
 }
@@ -347,6 +400,14 @@ __global__ __launch_bounds__(1024) void joinRows(LayerNormProblem p, const float
 // of 256, 512 and 1024 parts: 8192 x 2048 bf16 25.0, 29.4, 37.6; 4096 x 8192 bf16 43.5, 54.4, 71.8; 67712 x 192 f32 33.6, 29.1,
 // 30.8).
 long bandsOf(long M, long N) { return std::min(M, N < 256 ? 512L : 256L); }
+
+// Whether the columns are summed by themselves, from x and g once more: for few long rows, of which each workgroup has one or two
+// and leaves sums as long as they are (us apart and together: 256 x 16384 bf16 13.9, 28.3; 64 x 8192 f16 10.0, 11.0; 512 x 8192 bf16
+// 13.6, 18.1; 1024 x 8192 bf16 21.2, 20.5; 512 x 4096 f32 13.1, 14.5; 64 x 8192 f32 11.6, 10.6).
+// Rows that no workgroup holds are read again as it is.
+bool apart(long M, long N, size_t valueBytes) {
+  return N > 16384 || (std::min(M, 256L) * N >= 3 << 18 && M * (long)valueBytes <= 1024);
+}
 
 // Lanes to a row: as many as it has words, so that a lane holds one; wider rows take more words to a lane.
 template <class T, bool STREAM>
@@ -406,31 +467,62 @@ int launchRowsBack(const LayerNormProblem& p, float* parts, hipStream_t s) {
   return 0;
 }
 
+// Lanes of the workgroups that read a row several times: 1024 for few long rows (gradients of 1 x 20000 bf16 15.5 us and by 256
+// lanes 36.4, 1024 x 20000 80.6 and 91.2, 2048 x 20000 150 and 138).
+bool manyLanes(const LayerNormProblem& p) { return p.N > 4096 && p.M <= 4 * computeUnits(); }
+
 template <class T>
 int forward(const LayerNormProblem& p, hipStream_t s) {
   if (p.x.col == 1 && p.y.col == 1 && (streams((double)p.M * p.N, p.type) ? launchRows<T, true>(p, s) : launchRows<T, false>(p, s)))
     return launchStatus();
-  anyForward<T><<<dim3((unsigned)std::min(p.M, 1L << 20)), kLanes, 0, s>>>(p);
+  const dim3 grid((unsigned)std::min(p.M, 1L << 20));
+  if (!manyLanes(p))
+    anyForward<T, 256><<<grid, 256, 0, s>>>(p);
+  else
+    anyForward<T, 1024><<<grid, 1024, 0, s>>>(p);
   return launchStatus();
+}
+
+void launchJoinRows(const LayerNormProblem& p, const float* parts, int bands, hipStream_t s) {
+  if (bands > 32)
+    joinRows<64><<<dim3((unsigned)((2 * p.N + 15) / 16)), 1024, 0, s>>>(p, parts, bands);
+  else
+    joinRows<8><<<dim3((unsigned)((2 * p.N + 127) / 128)), 1024, 0, s>>>(p, parts, bands);
 }
 
 template <class T>
 int backward(const LayerNormProblem& p, hipStream_t s) {
   float* const parts = static_cast<float*>(p.workspace);
-  const bool sums = p.gradWeight.data || p.gradBias.data;
+  bool sums = p.gradWeight.data || p.gradBias.data;
   const long across = (p.N + kLanes - 1) / kLanes;
   long bands = p.M > 0 ? bandsOf(p.M, p.N) : 0;
   if (sums && (!launches((double)across * std::max(bands, 1L), kLanes) || !launches((2.0 * p.N + 15) / 16, 1024))) return FBFFT_UNSUPPORTED_SIZE;
   bool done = p.M == 0;
   if (!done && p.x.col == 1 && p.g.col == 1 && (!p.y.data || p.y.col == 1)) {
-    float* const to = sums ? parts : nullptr;
+    float* to = sums ? parts : nullptr;
+    if (sums && apart(p.M, p.N, sizeof(T))) {
+      constexpr int V = 16 / sizeof(T);
+      const long over = (p.N + 64 * V - 1) / (64 * V), most = std::min(std::max(512 / over, 1L), (p.M + 31) / 32);
+      const long rows = (p.M + most - 1) / most;
+      bands = (p.M + rows - 1) / rows;
+      if (!launches((double)over * bands, kColumnWaves * 64)) return FBFFT_UNSUPPORTED_SIZE;
+      columnSums<T, V><<<dim3((unsigned)over, (unsigned)bands), kColumnWaves * 64, 0, s>>>(p, bands > 1 ? parts : nullptr, rows);
+      if (bands > 1) launchJoinRows(p, parts, (int)bands, s);
+      if (!p.y.data) return launchStatus();
+      sums = false;
+      to = nullptr;
+    }
     const int groups = streams((double)p.M * p.N, p.type) ? launchRowsBack<T, true>(p, to, s) : launchRowsBack<T, false>(p, to, s);
     if (groups) done = true, bands = groups;
   }
   // (before gradInput, which may be one of the operands)
   if (!done && sums) anyParameters<T><<<dim3((unsigned)(across * bands)), kLanes, 0, s>>>(p, parts, bands);
-  if (!done && p.y.data) anyBackward<T><<<dim3((unsigned)std::min(p.M, 1L << 20)), kLanes, 0, s>>>(p);
-  if (sums) joinRows<<<dim3((unsigned)((2 * p.N + 15) / 16)), 1024, 0, s>>>(p, parts, (int)bands);
+  const dim3 grid((unsigned)std::min(p.M, 1L << 20));
+  if (!done && p.y.data && !manyLanes(p))
+    anyBackward<T, 256><<<grid, 256, 0, s>>>(p);
+  else if (!done && p.y.data)
+    anyBackward<T, 1024><<<grid, 1024, 0, s>>>(p);
+  if (sums) launchJoinRows(p, parts, (int)bands, s);
   return launchStatus();
 }
 

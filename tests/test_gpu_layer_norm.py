@@ -251,3 +251,22 @@ def test_many(m, n):
     x, w, b, g = make(m, n, torch.bfloat16, 12)
     _, mean, rstd = check_forward(x, w, b)
     check_backward(x, w, mean, rstd, g)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(64, 12801), (120, 8192), (33, 24000), (250, 4100), (260, 4100), (500, 3300), (520, 3300), (96, 16384)],
+                         ids=str)
+@pytest.mark.parametrize("form", ["rows", "pitch"])
+def test_few_long_rows(shape, form, dtype):  # (whose columns are summed by themselves, or not quite)
+    m, n = shape
+    x, w, b, g = make(m, n, dtype, 8, form)
+    _, mean, rstd = check_forward(x, w, b, form=form)
+    gx, gw, gb = check_backward(x, w, mean, rstd, g, form=form)
+    ws = space(1, m, n)
+    w2, b2 = torch.full_like(gw, 7.0), torch.full_like(gb, 7.0)
+    assert F.layer_norm_bprop(x, w, mean, rstd, g, None, w2, None, ws) == F.Success
+    assert F.layer_norm_bprop(x, w, mean, rstd, g, None, None, b2, ws) == F.Success
+    into = g.clone() if form == "rows" else g
+    assert F.layer_norm_bprop(x, w, mean, rstd, into, into, gw.zero_(), gb.zero_(), ws) == F.Success
+    torch.cuda.synchronize()
+    assert torch.equal(into, gx) and torch.equal(w2, gw) and torch.equal(b2, gb)
