@@ -201,7 +201,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
   char* const scales = space + 2 * STEP;
   const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
-  const Tile<BM, BN> tile(g.M, g.N);
+  const Tile<BM, BN> tile(g.M, g.N, gridDim.x < 8 ? 0 : (int)blockIdx.y);
   if (!tile.any) return;
   const long m0 = tile.m0, n0 = tile.n0, first = blockIdx.y * g.range, end = min(first + g.range, g.blocks);
 
@@ -540,7 +540,7 @@ int run(const LinearMx4Problem& p, hipStream_t s) {
   char* space = static_cast<char*>(p.workspace);
   const bool tiles = plan.kind == Mx4Plan::Tiles;
   const long rows = tiles ? plan.rows : 16 * plan.rows, cols = tiles ? plan.cols : 16 * plan.cols;
-  const long groups = ceilDivLong(p.M, rows) * ceilDivLong(p.N, cols) + (tiles ? 7 : 0), blocks = tiles ? groups / 8 * 8 : groups;
+  const long groups = ceilDivLong(p.M, rows) * ceilDivLong(p.N, cols), blocks = tiles && groups >= 8 ? (groups + 7) / 8 * 8 : groups;
   const JoinPlan join = plan.ranges > 1 ? joinOf(g.e.dense, p.M, p.N, plan.ranges) : JoinPlan{};
   const int lanes = tiles ? plan.rows * 2 : kFewWaves * 64;
   if (!launches((double)blocks * plan.ranges, lanes) || !launches(join.blocks, 256)) return FBFFT_UNSUPPORTED_SIZE;

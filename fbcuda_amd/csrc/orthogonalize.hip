@@ -313,16 +313,17 @@ struct PairTile {
   bool any, mirror;
 
   __device__ __forceinline__ PairTile(const PairArgs& g) {
+    const int turn = gridDim.x < 8 ? 0 : (int)(blockIdx.y + blockIdx.z) % 8;
     if (g.symmetric) {
       const int side = (int)((g.M + BM - 1) / BM), total = side * (side + 1) / 2, per = (total + 7) / 8;
-      index = (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
+      index = ((int)blockIdx.x + turn) % 8 * per + (int)blockIdx.x / 8;
       any = (int)blockIdx.x / 8 < per && index < total;
       int i, j;
       belowDiagonal(any ? index : 0, side, i, j);
       m0 = (long)i * BM, n0 = (long)j * BN;
       mirror = true;
     } else {
-      const Tile<BM, BN> t(g.M, g.N);
+      const Tile<BM, BN> t(g.M, g.N, turn);
       m0 = t.m0, n0 = t.n0, any = t.any;
       index = (int)(m0 / BM * ((g.N + BN - 1) / BN) + n0 / BN);
       mirror = g.turned.data != nullptr;
@@ -465,12 +466,14 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
   }
 }
 
-// Results from the sums of `ranges` ranges of k, in their order.  A wave: 32 rows of up to 64 columns of a tile.
+// Results from the sums of `ranges` ranges of k, in their order.  A wave: 32 rows of up to 64 columns of a tile; tiles of 32, whose
+// matrices are small and whose ranges are many, a workgroup to a tile and all loads at once (one of 60 x 60 in 13 ranges 2.9 us, by
+// single waves 11.9).
 template <class RESULT, int BM, int BN>
 __global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int ranges, int tiles, int count) {
   constexpr int COLS = BN < 64 ? BN : 64, ACROSS = BN / COLS, BLOCKS = BM / 32 * ACROSS;  // of a tile
   __shared__ __attribute__((aligned(16))) float space[4][32 * (COLS + 4)];
-  const int wave = threadIdx.x / 64, at = (int)blockIdx.x * 4 + wave, index = at / BLOCKS, block = at % BLOCKS;
+  const int wave = threadIdx.x / 64, at = BM == 32 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, index = at / BLOCKS, block = at % BLOCKS;
   if (index >= count) return;
   const long matrix = blockIdx.z;
   int i, j;
@@ -485,16 +488,40 @@ __global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int range
   if (m0 >= g.M || n0 >= g.N) return;
   const long far = (long)tiles * BM * BN;  // from a range to the next
   const float* const from = g.parts + matrix * ranges * far + ((long)index * BM + row0) * BN + col0;
-  leavePairs<COLS>(g, result, matrix, m0, n0, g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
+  if constexpr (BM == 32) {
+    __shared__ __attribute__((aligned(16))) float sums[32 * 36];
+    const int row = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
+    float v[4] = {};
+    for (int first = 0; first < ranges; first += 16) {
+      float u[16][4];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = 0.f;
-    for (int r = 0; r < ranges; ++r) {
-      float u[8];
-      loadPack<float, 8>(from + r * far + row * BN + c, u);
+      for (int r = 0; r < 16; ++r) loadPack<float, 4>(from + min(first + r, ranges - 1) * far + row * BN + c, u[r]);
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] += u[q];
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += first + r < ranges ? u[r][q] : 0.f;
     }
-  });
+    storePack(sums + row * 36 + c, v);
+    __syncthreads();
+    if (wave == 0)
+      leavePairs<COLS>(g, result, matrix, m0, n0, g.turned.data != nullptr, space[0], [&](int row, int c, float(&v)[8]) {
+        loadPack<float, 8>(sums + row * 36 + c, v);
+      });
+  } else {
+    leavePairs<COLS>(g, result, matrix, m0, n0, g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] = 0.f;
+      for (int first = 0; first < ranges; first += 4) {
+        float u[4][8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) loadPack<float, 8>(from + min(first + r, ranges - 1) * far + row * BN + c, u[r]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] += first + r < ranges ? u[r][q] : 0.f;
+      }
+    });
+  }
 }
 
 // Small products.  A workgroup: SIDE x SIDE results over one range of k, its waves a part of that each, straight from memory to
@@ -868,7 +895,7 @@ PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
       if (used > 1) time += 4.5 + (double)batch * tiles * used * o.side * o.side * 8 / 4e6;
       if (least == 0 || time < least) {
         least = time;
-        best = PairPlan{o.kind, o.side, (tiles + 7) / 8 * 8, used, 32 * range, time};
+        best = PairPlan{o.kind, o.side, tiles < 8 ? tiles : (tiles + 7) / 8 * 8, used, 32 * range, time};
       }
     }
   }
@@ -887,7 +914,7 @@ void launchSmall(const PairArgs& g, const RESULT& result, dim3 grid, hipStream_t
   else if (g.range <= 512)
     small<RESULT, SIDE, 8, 2><<<grid, 512, 0, s>>>(g, result);
   else
-    small<RESULT, SIDE, 8, 4><<<grid, 512, 0, s>>>(g, result);
+    small<RESULT, SIDE, 16, 2><<<grid, 1024, 0, s>>>(g, result);
 }
 
 // one: see product's ONE
@@ -921,7 +948,7 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
     tiles(std::integral_constant<int, 0>());
   if (plan.ranges > 1) {
     const long down = ceilDivLong(g.M, plan.side), count = g.symmetric ? down * (down + 1) / 2 : down * ceilDivLong(g.N, plan.side);
-    const dim3 blocks((unsigned)ceilDivLong(count * (plan.side / 32) * (plan.side > 32 ? plan.side / 64 : 1), 4), 1, batch);
+    const dim3 blocks((unsigned)(plan.side == 32 ? count : ceilDivLong(count * (plan.side / 32) * (plan.side / 64), 4)), 1, batch);
     const int ranges = (int)plan.ranges, rounded = (int)plan.tiles;
     if (plan.side == 32)
       join<RESULT, 32, 32><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);

@@ -163,16 +163,17 @@ __device__ __forceinline__ void leave(const ARGS& g, long range, long m0, long n
 }
 
 // Where a workgroup's tile lies.  Neighbouring tiles go to one XCD (workgroups are dealt out to the eight in turn), in
-// strips of four rows of tiles, so that those that run together share lines of both operands in its L2.
+// strips of four rows of tiles, so that those that run together share lines of both operands in its L2.  `turn`: by so much
+// further XCDs, for what else than a tile a grid's workgroups differ in, so that a few tiles' ranges and matrices go to all eight.
 template <int BM, int BN>
 struct Tile {
   long m0, n0;
   bool any;
 
-  __device__ __forceinline__ Tile(long M, long N) {
+  __device__ __forceinline__ Tile(long M, long N, int turn = 0) {
     constexpr int tall = 4;
     const int across = (int)((N + BN - 1) / BN), down = (int)((M + BM - 1) / BM), total = across * down, per = (total + 7) / 8;
-    int tile = (int)blockIdx.x % 8 * per + (int)blockIdx.x / 8;
+    int tile = ((int)blockIdx.x + turn) % 8 * per + (int)blockIdx.x / 8;
     any = (int)blockIdx.x / 8 < per && tile < total;
     const int strip = tile / (tall * across), height = max(1, min(tall, down - strip * tall));
     tile -= strip * tall * across;
