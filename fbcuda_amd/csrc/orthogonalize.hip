@@ -10,6 +10,17 @@
 // to 6e-3, pairs about 2e-6, as 32-bit arithmetic does: the first steps multiply small singular values by 3.4 each, and what
 // rounding put beside them, too.)
 //
+// Three ways:
+//   whole     one launch, a workgroup to a matrix in LDS: up to 96 rows (or columns) and 156 KB of pairs.  16 of 131 x 81 bf16
+//             46 us, 64 x 64 f32 19; step by step 80 and 52, of which each launch's way through memory is 2.5 to 4
+//   steps()   three products a step.  What bounds them: launches and latency below about 10^9 operations a product (192 x 1600
+//             f32 110 us, 17 launches), above it the matrix instructions, three for what one 16-bit product takes (8192 x 2048 f32
+//             1.78 ms, 0.92 PFLOP/s of the three)
+//   alone()   of long bfloat16 matrices: every A and B is a polynomial of the first A, so that the steps are products of P x P
+//             matrices alone, half of each by symmetry, and X is met by one product at the end.  8192 x 2048 bf16 in 0.95 ms, step
+//             by step 1.57.  It takes the later A from the first, not from the rounded X, which puts small singular values off
+//             more (9e-4 of the norm at worst, where float32 results could not hide it)
+//
 // A pair matrix has rows of a multiple of 32 columns, 32 leading pieces and then their 32 second pieces, 128 bytes: what a
 // matrix instruction takes of a row.  Rows and columns are filled up with zeros.
 #include "product.h"
@@ -685,7 +696,6 @@ __device__ __forceinline__ uintx4 wholeTurned(const char* m, int pitch, int firs
 template <class A, class B>
 __device__ __forceinline__ floatx4 wholeSums(int kbs, A a, B b) {
   floatx4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0, s2 = s0;
-#pragma unroll 4
   for (int kb = 0; kb < kbs; ++kb) {
     const uintx4 a0 = a(kb, 0), a1 = a(kb, 1), b0 = b(kb, 0), b1 = b(kb, 1);
     s1 = multiply(b1, a0, s1);
@@ -823,7 +833,6 @@ __global__ __launch_bounds__(kWholeLanes) void whole(Given<const T> g, Given<T> 
       else
         waveExchange();
       if (j >= across) continue;
-#pragma unroll 2
       for (int i = task % shares; i < down; i += shares) {
         floatx4 s0{0.f, 0.f, 0.f, 0.f}, s1 = s0, s2 = s0;
 #pragma unroll
@@ -917,7 +926,7 @@ void launchSmall(const PairArgs& g, const RESULT& result, dim3 grid, hipStream_t
     small<RESULT, SIDE, 16, 2><<<grid, 1024, 0, s>>>(g, result);
 }
 
-// one: see product's ONE
+// one: see product's ONE (float32 matrices have second pieces everywhere, the last product's first operand always has)
 template <class RESULT>
 void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int one, float* parts, unsigned batch, hipStream_t s) {
   const dim3 grid((unsigned)plan.tiles, (unsigned)plan.ranges, batch);
@@ -940,12 +949,13 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
     launchSmall<RESULT, 16>(g, result, grid, s);
   else if (plan.kind == Small32)
     launchSmall<RESULT, 32>(g, result, grid, s);
-  else if (one == 3)
-    tiles(std::integral_constant<int, 3>());
-  else if (one == 1)
-    tiles(std::integral_constant<int, 1>());
-  else
+  else if (one == 0)
     tiles(std::integral_constant<int, 0>());
+  else if constexpr (!__is_same(RESULT, Result<float>)) {
+    if (one == 1) tiles(std::integral_constant<int, 1>());
+    if constexpr (__is_same(RESULT, Nothing))
+      if (one == 3) tiles(std::integral_constant<int, 3>());
+  }
   if (plan.ranges > 1) {
     const long down = ceilDivLong(g.M, plan.side), count = g.symmetric ? down * (down + 1) / 2 : down * ceilDivLong(g.N, plan.side);
     const dim3 blocks((unsigned)(plan.side == 32 ? count : ceilDivLong(count * (plan.side / 32) * (plan.side / 64), 4)), 1, batch);
@@ -1121,11 +1131,12 @@ struct Call {
   }
 };
 
+bool inOneLaunch(long batch, long P, long Q) { return batch <= 0x3fffff && P <= 32 * kWholeSteps && wholeBytes(P, Q) <= kWholeLarge; }
+
 template <class T>
-bool launchWhole(const OrthogonalProblem& p, hipStream_t s) {
+void launchWhole(const OrthogonalProblem& p, hipStream_t s) {
   const bool turn = p.rows > p.cols;
   const long rows = turn ? p.cols : p.rows, cols = turn ? p.rows : p.cols, P = padded(rows), Q = padded(cols), bytes = wholeBytes(P, Q);
-  if (bytes > kWholeLarge || P > 32 * kWholeSteps) return false;
   const Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
   const Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
   WholeArgs w{rows, cols, (int)P, (int)Q, p.steps, p.eps, p.scale / kUnit, {}};
@@ -1134,12 +1145,14 @@ bool launchWhole(const OrthogonalProblem& p, hipStream_t s) {
     whole<T, kWholeSmall><<<dim3((unsigned)p.batch), kWholeLanes, 0, s>>>(g, y, w);
   else
     whole<T, kWholeLarge><<<dim3((unsigned)p.batch), kWholeLanes, 0, s>>>(g, y, w);
-  return true;
 }
 
 template <class T>
 int run(const OrthogonalProblem& p, hipStream_t s) {
-  if (p.batch <= 0x3fffff && launchWhole<T>(p, s)) return launchStatus();
+  if (inOneLaunch(p.batch, padded(std::min(p.rows, p.cols)), padded(std::max(p.rows, p.cols)))) {
+    launchWhole<T>(p, s);
+    return launchStatus();
+  }
   Call<T> call(p, s);
   const long squared = ceilDivLong(call.P, 64) * ceilDivLong(call.Q, 64);
   if (p.batch > 65535 || !launches((double)squared * p.batch, 256) || !call.w.fits(p.batch)) return FBFFT_UNSUPPORTED_SIZE;
