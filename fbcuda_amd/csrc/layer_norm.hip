@@ -2,6 +2,10 @@
 //
 //   forward    y = (x - mean) rstd w + b,  rstd = 1 / sqrt(var + eps)
 //   backward   xh = (x - mean) rstd, h = w g;  dx = rstd (h - mean(h) - xh mean(h xh)),  dw = sum g xh,  db = sum g over rows
+//
+// Memory bounds all of it: every operand is read once, rows stay in registers between their sums and their results.  (16384 x 2048
+// bf16 forward 23.6 us, 5.7 TB/s; 8192 x 2048 bf16 backward 24.5, where 101 MB take 19 at the rate of a copy and the join of the
+// columns' sums is a launch of 3 to 4; 67712 x 192 f32 backward 33.1, 156 MB 29.)  Few rows are a launch: 1 x 2048 4.1 us.
 #include "operators.h"
 
 #include <algorithm>
@@ -167,7 +171,7 @@ __device__ __forceinline__ void rowSums(float& s1, float& s2, float (*space)[THR
   }
 }
 
-// A workgroup takes THREADS / LANES rows at a time, the next ones on their way.  The variance is that of the values in registers
+// A workgroup takes THREADS / LANES rows at a time, the next ones on their way where registers allow it.  The variance is that of the values in registers
 // around their mean: nothing cancels.
 template <class T, int VEC, int LANES, int WORDS, int THREADS, bool STREAM>
 __global__ __launch_bounds__(THREADS) void rowsForward(LayerNormProblem p) {
