@@ -219,32 +219,40 @@ __device__ __forceinline__ void storeEight(half16* to, const float (&z)[8], int 
   }
 }
 
-// 32 rows by COLS (64) columns of results from row m0 and column n0, both multiples of 32, by one wave: eight(row, column, v)
-// gives eight neighbouring sums.  Results that go the other way round meet in LDS, 32 x (COLS + 4) numbers.
-template <int COLS, class RESULT, class EIGHT>
+// 32 rows by COLS columns of results from row m0 and column n0, both multiples of 32, by WAVES waves, one or a workgroup's:
+// eight(row, column, v) gives eight neighbouring sums.  What stands beside them is on its way for all rows at once (a row after the
+// other, each waits for memory).  Results that go the other way round meet in LDS, 32 x (COLS + 4) numbers.
+template <int COLS, int WAVES, class RESULT, class EIGHT>
 __device__ __forceinline__ void leavePairs(const PairArgs& g, const RESULT& result, long matrix, long m0, long n0, bool mirror,
                                            float* space, EIGHT eight) {
-  constexpr int LANES = COLS / 8, ROWS = 64 / LANES, PITCH = COLS + 4;
+  constexpr int LANES = COLS / 8, ROWS = WAVES * 64 / LANES, TIMES = ROWS < 32 ? 32 / ROWS : 1, PITCH = COLS + 4;
   constexpr bool LAST = !__is_same(RESULT, Nothing);
-  const int lane = threadIdx.x % 64, c = lane % LANES * 8;
+  const int lane = threadIdx.x % (WAVES * 64), c = lane % LANES * 8;
   bool turns = mirror;
   if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1;
-  const bool inside = n0 + c < g.N;  // (N is a multiple of 32)
+  const long n = n0 + c;
+  const bool inside = n < g.N;  // (N is a multiple of 32)
   const float factor = g.factors ? g.factors[matrix] : 1.f, by = g.by * factor * (g.power == 2 ? factor : 1.f), beta = g.beta * factor;
-#pragma unroll 1
-  for (int row = lane / LANES; row < 32; row += ROWS) {
-    const long m = m0 + row, n = n0 + c;
+  halfx8 old[TIMES][2] = {};
+  if (g.old.data && inside) {
+#pragma unroll
+    for (int t = 0; t < TIMES; ++t) {
+      const int row = t * ROWS + lane / LANES;
+      if (row >= 32 || m0 + row >= g.M) continue;
+      const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m0 + row, n);
+      old[t][0] = *reinterpret_cast<const halfx8*>(from), old[t][1] = *reinterpret_cast<const halfx8*>(from + 32);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TIMES; ++t) {
+    const int row = t * ROWS + lane / LANES;
+    if (row >= 32) continue;
+    const long m = m0 + row;
     float z[8];
     eight(row, c, z);
 #pragma unroll
-    for (int v = 0; v < 8; ++v) z[v] *= by;
+    for (int v = 0; v < 8; ++v) z[v] = z[v] * by + beta * ((float)old[t][0][v] + (float)old[t][1][v]);
     if (inside && m < g.M) {
-      if (g.old.data) {
-        const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m, n);
-        const halfx8 lead = *reinterpret_cast<const halfx8*>(from), rest = *reinterpret_cast<const halfx8*>(from + 32);
-#pragma unroll
-        for (int v = 0; v < 8; ++v) z[v] += beta * ((float)lead[v] + (float)rest[v]);
-      }
       if constexpr (LAST) {
 #pragma unroll
         for (int v = 0; v < 8; ++v) z[v] *= result.scale;
@@ -269,30 +277,32 @@ __device__ __forceinline__ void leavePairs(const PairArgs& g, const RESULT& resu
     }
   }
   if (!turns) return;
-  waveExchange();
-  for (int column = lane; column < COLS; column += 64) {
+  if constexpr (WAVES == 1)
+    waveExchange();
+  else
+    __syncthreads();
+#pragma unroll 4
+  for (int at = lane; at < COLS * 4; at += WAVES * 64) {
+    const int column = at % COLS, q = at / COLS;
     const long n = n0 + column;
     if (n >= g.N || m0 >= g.M) continue;
+    float z[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float z[8];
+    for (int v = 0; v < 8; ++v) z[v] = space[(8 * q + v) * PITCH + column];
+    if constexpr (LAST) {
+      auto* const to = result.y.data + matrix * result.y.batch + n * result.y.col + m0 + 8 * q;
+      if (n < result.cols) {
+        if (m0 + 8 * q + 8 <= result.rows) {
+          storePack(to, z);
+        } else {
 #pragma unroll
-      for (int v = 0; v < 8; ++v) z[v] = space[(8 * q + v) * PITCH + column];
-      if constexpr (LAST) {
-        auto* const to = result.y.data + matrix * result.y.batch + n * result.y.col + m0 + 8 * q;
-        if (n < result.cols) {
-          if (m0 + 8 * q + 8 <= result.rows) {
-            storePack(to, z);
-          } else {
-#pragma unroll
-            for (int v = 0; v < 8; ++v)
-              if (m0 + 8 * q + v < result.rows) storePack(to + v, {z[v]});
-          }
+          for (int v = 0; v < 8; ++v)
+            if (m0 + 8 * q + v < result.rows) storePack(to + v, {z[v]});
         }
-      } else {
-        storeEight(g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n, m0) + 8 * q, z,
-                   g.symmetric ? (int)max(n + 1 - (m0 + 8 * q), 0l) : 0, 8);
       }
+    } else {
+      storeEight(g.turned.data + matrix * g.turned.batch + placeOf(g.turned, n, m0) + 8 * q, z,
+                 g.symmetric ? (int)max(n + 1 - (m0 + 8 * q), 0l) : 0, 8);
     }
   }
 }
@@ -472,20 +482,18 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
         storePack(to + row * BN + lane % (WN / 8) * 8, v);
       }
     } else {
-      leavePairs<WN>(g, result, matrix, m0 + row0, n0 + wn, tile.mirror, mine, eight);
+      leavePairs<WN, 1>(g, result, matrix, m0 + row0, n0 + wn, tile.mirror, mine, eight);
     }
   }
 }
 
-// Results from the sums of `ranges` ranges of k, in their order.  A wave: 32 rows of up to 64 columns of a tile; tiles of 32, whose
-// matrices are small and whose ranges are many, a workgroup to a tile and all loads at once (one of 60 x 60 in 13 ranges 2.9 us, by
-// single waves 11.9).
+// Results from the sums of `ranges` ranges of k, in their order: a workgroup to 32 rows of up to 64 columns of a tile, eight ranges'
+// sums on their way at once (60 x 60 in 13 ranges 5.5 us, by a wave and range after range 11.9).
 template <class RESULT, int BM, int BN>
-__global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int ranges, int tiles, int count) {
-  constexpr int COLS = BN < 64 ? BN : 64, ACROSS = BN / COLS, BLOCKS = BM / 32 * ACROSS;  // of a tile
-  __shared__ __attribute__((aligned(16))) float space[4][32 * (COLS + 4)];
-  const int wave = threadIdx.x / 64, at = BM == 32 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, index = at / BLOCKS, block = at % BLOCKS;
-  if (index >= count) return;
+__global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int ranges, int tiles) {
+  constexpr int COLS = BN < 64 ? BN : 64, ACROSS = BN / COLS, BLOCKS = BM / 32 * ACROSS, AHEAD = 8;  // BLOCKS: of a tile
+  __shared__ __attribute__((aligned(16))) float space[32 * (COLS + 4)];
+  const int index = (int)blockIdx.x / BLOCKS, block = (int)blockIdx.x % BLOCKS;
   const long matrix = blockIdx.z;
   int i, j;
   if (g.symmetric) {
@@ -499,40 +507,19 @@ __global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int range
   if (m0 >= g.M || n0 >= g.N) return;
   const long far = (long)tiles * BM * BN;  // from a range to the next
   const float* const from = g.parts + matrix * ranges * far + ((long)index * BM + row0) * BN + col0;
-  if constexpr (BM == 32) {
-    __shared__ __attribute__((aligned(16))) float sums[32 * 36];
-    const int row = threadIdx.x / 8, c = threadIdx.x % 8 * 4;
-    float v[4] = {};
-    for (int first = 0; first < ranges; first += 16) {
-      float u[16][4];
+  leavePairs<COLS, 4>(g, result, matrix, m0, n0, g.turned.data != nullptr, space, [&](int row, int c, float(&v)[8]) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) loadPack<float, 4>(from + min(first + r, ranges - 1) * far + row * BN + c, u[r]);
+    for (int q = 0; q < 8; ++q) v[q] = 0.f;
+    for (int first = 0; first < ranges; first += AHEAD) {
+      float u[AHEAD][8];
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
+      for (int r = 0; r < AHEAD; ++r) loadPack<float, 8>(from + min(first + r, ranges - 1) * far + row * BN + c, u[r]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] += first + r < ranges ? u[r][q] : 0.f;
+      for (int r = 0; r < AHEAD; ++r)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += first + r < ranges ? u[r][q] : 0.f;
     }
-    storePack(sums + row * 36 + c, v);
-    __syncthreads();
-    if (wave == 0)
-      leavePairs<COLS>(g, result, matrix, m0, n0, g.turned.data != nullptr, space[0], [&](int row, int c, float(&v)[8]) {
-        loadPack<float, 8>(sums + row * 36 + c, v);
-      });
-  } else {
-    leavePairs<COLS>(g, result, matrix, m0, n0, g.turned.data != nullptr, space[wave], [&](int row, int c, float(&v)[8]) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] = 0.f;
-      for (int first = 0; first < ranges; first += 4) {
-        float u[4][8];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) loadPack<float, 8>(from + min(first + r, ranges - 1) * far + row * BN + c, u[r]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] += first + r < ranges ? u[r][q] : 0.f;
-      }
-    });
-  }
+  });
 }
 
 // Small products.  A workgroup: SIDE x SIDE results over one range of k, its waves a part of that each, straight from memory to
@@ -877,7 +864,8 @@ struct PairPlan {
 // results, more of them where they are left both ways round.  Ranges add a launch, and their sums' way to memory and back.
 // Measured in every kernel on products from 64 x 64 x 64 to 2048 x 8192 x 8192: 1024 x 1024 x 1024 with half of it a mirror
 // image: Deep64 11.4, Wide64 18.4, Wide128 28; 2048 x 2048 x 2048 so: Wide64 40, Deep128 42, Wide128 in three ranges 44;
-// 2048 x 8192 x 2048: Wide256 167, Wide128 189, Wide64 240; 256 x 256 x 8192: Small32 in one range 58, in eight 17.
+// 2048 x 8192 x 2048: Wide256 167, Wide128 189, Wide64 240; 256 x 256 x 8192: Small32 in one range 58, in eight 17; 256 x 256 x
+// 6432: Small32 in nine 20, Deep64 in eight 13.
 PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
   struct Option {
     int kind, side, most;  // most: ranges
@@ -886,7 +874,7 @@ PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
     double results;
   };
   static const Option options[] = {
-      {Small16, 16, 1, 0.136, 0.148, false, 3}, {Small32, 32, 16, 0.24, 0.243, false, 3}, {Deep64, 64, 8, 0.18, 0.24, true, 5},
+      {Small16, 16, 1, 0.136, 0.148, false, 3}, {Small32, 32, 16, 0.24, 0.42, false, 3}, {Deep64, 64, 8, 0.18, 0.24, true, 5},
       {Wide64, 64, 8, 0.4, 0.25, false, 5},     {Deep128, 128, 8, 0.56, 0.68, true, 6},   {Wide128, 128, 8, 0.62, 0.63, true, 6},
       {Wide256, 256, 8, 1.8, 2.4, true, 10}};
   PairPlan best{};
@@ -896,7 +884,7 @@ PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
   for (const Option& o : options) {
     const long down = ceilDivLong(M, o.side), across = ceilDivLong(N, o.side);
     const long tiles = symmetric ? down * (down + 1) / 2 : down * across;
-    for (long ranges = 1; ranges <= o.most; ranges += ranges < 4 ? 1 : ranges / 2) {
+    for (long ranges = 1; ranges <= o.most; ranges += ranges < 4 ? 1 : ranges < 8 ? 2 : 4) {
       const long range = ceilDivLong(steps, ranges), used = ceilDivLong(steps, range);
       if (ranges > 1 && range < 8) break;
       const double share = (double)batch * tiles * used / units, rounds = o.whole && share < 8 ? std::ceil(share) : share;
@@ -958,16 +946,16 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
   }
   if (plan.ranges > 1) {
     const long down = ceilDivLong(g.M, plan.side), count = g.symmetric ? down * (down + 1) / 2 : down * ceilDivLong(g.N, plan.side);
-    const dim3 blocks((unsigned)(plan.side == 32 ? count : ceilDivLong(count * (plan.side / 32) * (plan.side / 64), 4)), 1, batch);
+    const dim3 blocks((unsigned)(count * (plan.side / 32) * (plan.side > 32 ? plan.side / 64 : 1)), 1, batch);
     const int ranges = (int)plan.ranges, rounded = (int)plan.tiles;
     if (plan.side == 32)
-      join<RESULT, 32, 32><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
+      join<RESULT, 32, 32><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
     else if (plan.side == 64)
-      join<RESULT, 64, 64><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
+      join<RESULT, 64, 64><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
     else if (plan.side == 128)
-      join<RESULT, 128, 128><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
+      join<RESULT, 128, 128><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
     else
-      join<RESULT, 256, 256><<<blocks, 256, 0, s>>>(g, result, ranges, rounded, (int)count);
+      join<RESULT, 256, 256><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
   }
 }
 
@@ -1015,7 +1003,8 @@ struct Space {
 
   bool fits(long batch) const {
     for (const PairPlan* p : {&gramPlan, &polyPlan, &lastPlan, &twoPlan})
-      if (!launches((double)p->tiles * p->ranges * batch * (p == &twoPlan ? 2 : 1), 512)) return false;
+      // (workgroups of up to 1024 lanes, or of 256 to 32 x 32 or 32 x 64 of the results)
+      if (!launches((double)p->tiles * std::max(p->ranges, p->ranges > 1 ? p->side * p->side / 4096 + 1l : 1l) * batch * (p == &twoPlan ? 2 : 1), 1024)) return false;
     return true;
   }
   // whether the P x P matrices alone, which X meets in the last product, are expected to take less time
