@@ -430,8 +430,8 @@ int fbfft_dropout_bprop(const fbfft_array* gradOutput, const fbfft_array* gradIn
  *   mean, var: over the N values of a row (var divides by N)
  *   output = (input - mean) / sqrt(var + eps) * weight[n] + bias[n]
  * weight, bias: [N] of any type, or NULL for 1 and 0.  mean, rstd (= 1 / sqrt(var + eps)): float32 [M], written for the
- * backward pass, or NULL.  M and N are below 2^31.  output may be input itself (same address and strides); any other
- * overlap is not defined.  workspace: fbfft_layer_norm_workspace(0, ...) bytes, 256-byte aligned, NULL where that is 0;
+ * backward pass, or NULL; nothing is written where M or N is 0.  M and N are below 2^31.  output may be input itself (same
+ * address and strides); any other overlap is not defined.  workspace: fbfft_layer_norm_workspace(0, ...) bytes, 256-byte aligned, NULL where that is 0;
  * its contents need not survive. */
 size_t fbfft_layer_norm_workspace(int pass, long long rows, long long cols);
 int fbfft_layer_norm_fprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* bias,
@@ -442,7 +442,7 @@ int fbfft_layer_norm_fprop(const fbfft_array* input, const fbfft_array* weight, 
  *   gradBias[n] = sum_m gradOutput,  gradWeight[n] = sum_m gradOutput xh
  *   gradInput = rstd (weight gradOutput - sum_n(weight gradOutput) / N - xh sum_n(weight gradOutput xh) / N)
  * gradInput, gradWeight, gradBias: any of them NULL where it is not wanted; the latter two are overwritten.  gradInput
- * may be gradOutput or input itself.  Reproducible bit for bit.  workspace: fbfft_layer_norm_workspace(1, ...). */
+ * may be gradOutput or input itself (same address and strides).  Reproducible bit for bit.  workspace: fbfft_layer_norm_workspace(1, ...). */
 int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, const fbfft_array* mean,
                            const fbfft_array* rstd, const fbfft_array* gradOutput, const fbfft_array* gradInput,
                            const fbfft_array* gradWeight, const fbfft_array* gradBias, void* workspace,
@@ -463,8 +463,10 @@ int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, 
  * the result's norm, half of what its rounding to bfloat16 is off by.  A matrix of zeros gives zeros where
  * eps > 0; values that are not finite make all of their matrix NaN.
  * steps from 1 to 32; eps and scale finite, eps >= 0; coefficients under which a singular value in [0, 1] or what the
- * products make of it could pass 32 are refused (UnsupportedSize): the pieces end at 64.  rows, cols up to 65536.
- * workspace: fbfft_orthogonalize_workspace bytes, 256-byte aligned.  Reproducible bit for bit. */
+ * products make of it could pass 32 are refused (UnsupportedSize): the pieces end at 64.  rows, cols up to 65536;
+ * a batch up to 65535 matrices, of small ones (32 x 1152, 64 x 480, 96 x 192) 2^22 - 1.
+ * workspace: fbfft_orthogonalize_workspace bytes, 256-byte aligned; its contents need not survive, and calls that overlap in
+ * time need one each.  Reproducible bit for bit. */
 size_t fbfft_orthogonalize_workspace(long long batch, long long rows, long long cols);
 int fbfft_orthogonalize(const fbfft_array* input, const fbfft_array* output, const float* coefficients, int steps,
                         float eps, float scale, void* workspace, size_t workspaceBytes, fbfft_stream_t stream);
@@ -489,7 +491,8 @@ typedef struct fbfft_mx4 {
  * A block of zeros has the scale 2^-127; one that holds NaN or an infinity has the scale NaN. */
 int fbfft_mx4_quantize(const fbfft_array* input, const fbfft_mx4* output, fbfft_stream_t stream);
 
-/* output [M][K] = what the format stands for, rounded to output's type (bfloat16 and float32 hold it exactly). */
+/* output [M][K] = what the format stands for, rounded to output's type (bfloat16 and float32 hold
+ * it exactly up to their largest number; beyond it, infinity). */
 int fbfft_mx4_dequantize(const fbfft_mx4* input, const fbfft_array* output, fbfft_stream_t stream);
 
 /* Rows times a weight matrix held in that format, for serving:
