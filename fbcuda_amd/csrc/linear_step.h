@@ -1,5 +1,5 @@
 // Where the 16-byte words of one step of an operand lie, in memory and in LDS, when they go straight from the one to the
-// other (linear.hip).  Arithmetic only, which a host compiler runs, too.
+// other (product.h).  Arithmetic only, which a host compiler runs, too.
 #pragma once
 
 #include <hip/hip_runtime.h>

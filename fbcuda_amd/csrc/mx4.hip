@@ -193,7 +193,7 @@ struct Packed : Direct<ROWS, 64, true, WAVES> {
 // side by side for each pair of blocks: a lane's scales of two fragments in both instructions are one word.
 // Bound by the matrix instructions and their fragments' way from LDS where k is long (4096 x 16384 x 4096 125 to 146 us, 3.8 to
 // 4.4 PFLOP/s), and by the results where it is not: 8192 x 2048 x 8192 88 us without an activation, of which the products are 62;
-// GELU adds 18, whose exponentials wait on nothing but find two waves to a SIMD, a bias and the residual of 134 MB 44 more.  Tiles
+// GELU adds 18, whose exponentials wait on nothing but find two waves to a SIMD, a bias and the residual of 134 MB 26 to 44 more.  Tiles
 // of 256 need half of the operands' way from L2 that those of 128 do, and fill the chip only with large products.
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(Mx4Args g) {
@@ -366,10 +366,8 @@ struct FewArgs {
   int pitch, scales;      // of x in LDS: bytes from a row to the next, and in front of the scales
 };
 
-// RB fragments of 16 rows by NB of 16 columns of w to a workgroup, whose eight waves share k and meet in LDS: few rows are bound by
-// w's way from memory, which needs many loads under way and no tile, 8192 x 2048 codes of w and scales in 4.6 us (1 row; 1.6 at the
-// rate of a copy, 3.5 an empty launch in a graph).  WAY: every workgroup quantises x to LDS for itself, which saves a launch and
-// the codes' way through memory.
+// Bound by w's way from memory, which needs many loads under way and no tile, and by the launch: 1 x 2048 x 8192 4.6 us, of which
+// the bytes are 1.6 at the rate of a copy and an empty launch 3.5.  Quantising on the way saves a launch, 2.5 us there.
 template <class T, bool WAY, int RB, int NB, int AHEAD>
 __global__ __launch_bounds__(kFewWaves * 64) void fewRows(FewArgs f) {
   static_assert(!WAY || RB == 1, "quantised on the way: 16 rows at most");

@@ -187,3 +187,14 @@ def test_python_wrappers_refuse():
             F.packed_rows(codes, scales)
     assert F.packed_rows(None, None) is None
     assert ctypes.sizeof(F.Mx4) == 48
+
+
+def test_words_that_products_read_lie_in_their_operands():
+    """tests/cpp/steps_check.cpp: every word that products of pairs and of 4-bit rows move straight to LDS, over ragged rows and
+    k and ranges of k."""
+    import os
+    import subprocess
+    at = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp")
+    subprocess.check_call(["make", "-C", at, "-B", "steps_check"], stdout=subprocess.DEVNULL, stderr=subprocess.DEVNULL)
+    out = subprocess.run([os.path.join(at, "steps_check")], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.strip() == "OK", out.stdout
