@@ -113,8 +113,11 @@ struct Row {
       if (j + VEC <= N) {
         v[w] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(from + j);
       } else {
+        v[w] = {};
+        if (j < N) {  // (only where a row ends inside a word do waves take one value after the other)
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) v[w][q] = j + q < N ? from[j + q] : (T)0.f;
+          for (int q = 0; q < VEC; ++q) v[w][q] = j + q < N ? from[j + q] : (T)0.f;
+        }
       }
     }
   }
@@ -239,17 +242,75 @@ __global__ __launch_bounds__(THREADS) void rowsForward(LayerNormProblem p) {
   }
 }
 
-// Rows as above, 1024 lanes to a workgroup; the columns' sums of its rows stay in registers, meet in LDS and go to parts
-// [workgroup][2][N].
-template <class T, int VEC, int LANES, int WORDS, bool STREAM>
-__global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* parts) {
-  constexpr int GROUPS = 1024 / LANES;
+// The columns' sums of all rows over LANES words of a row (up to 64) from word `first`, by a workgroup of 1024 lanes, to the
+// gradients.
+template <class T, int VEC, int LANES>
+__device__ __forceinline__ void leaveColumns(const LayerNormProblem& p, long first, float* space) {
+  constexpr int GROUPS = 1024 / LANES, COLUMNS = LANES * VEC;
+  typedef Row<T, VEC, LANES, 1> R;
+  const long from = first * VEC;
+  Matrix x = p.x, g = p.g;
+  x.data = static_cast<T*>(x.data) + from, g.data = static_cast<T*>(g.data) + from;
+  float sumW[VEC] = {}, sumB[VEC] = {};
+#pragma unroll 4
+  for (long i = threadIdx.x / LANES; i < p.M; i += GROUPS) {
+    R a, b;
+    a.load(x, i, p.N - from);
+    b.load(g, i, p.N - from);
+    const float mean = p.mean[i * p.meanStride], rstd = p.rstd[i * p.rstdStride];
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) {
+      const float dy = (float)b.v[0][q];
+      sumB[q] += dy;
+      sumW[q] = __builtin_fmaf(dy, ((float)a.v[0][q] - mean) * rstd, sumW[q]);
+    }
+  }
+  // over a wave's rows, then over the waves
+#pragma unroll
+  for (int q = 0; q < VEC; ++q)
+#pragma unroll
+    for (int far = LANES; far < 64; far *= 2) {
+      sumW[q] += __shfl_xor(sumW[q], far);
+      sumB[q] += __shfl_xor(sumB[q], far);
+    }
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    __syncthreads();
+    if (lane < LANES) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) space[wave * COLUMNS + lane * VEC + q] = part ? sumB[q] : sumW[q];
+    }
+    __syncthreads();
+    const Line& to = part ? p.gradBias : p.gradWeight;
+    for (int j = threadIdx.x; j < COLUMNS && from + j < p.N; j += 1024) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) v += space[w * COLUMNS + j];
+      if (to.data) storeAny(to.data, to.type, (from + j) * to.stride, v);
+    }
+  }
+}
+
+// Rows as above, 1024 lanes to a workgroup; SUMS: the columns' sums of its rows stay in registers, meet in LDS and go to parts
+// [workgroup][2][N], where parts is not null.  Else the workgroups behind the first `groups` take the columns' sums of all rows, 64
+// words of a row each.
+template <class T, int VEC, int LANES, int WORDS, bool STREAM, bool SUMS>
+__global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* parts, int groups) {
+  constexpr int GROUPS = 1024 / LANES, ACROSS = LANES < 64 ? LANES : 64;
+  if constexpr (!SUMS) {
+    __shared__ __attribute__((aligned(16))) float columns[16 * ACROSS * VEC];
+    if ((int)blockIdx.x >= groups) {
+      leaveColumns<T, VEC, ACROSS>(p, (long)((int)blockIdx.x - groups) * ACROSS, columns);
+      return;
+    }
+  }
   __shared__ float space[2][16][2];
   typedef Row<T, VEC, LANES, WORDS> R;
   constexpr bool HOLDS = WORDS == 1;  // the parameters, and the next row
   float weight[VEC], sumW[WORDS][VEC] = {}, sumB[WORDS][VEC] = {};
   if constexpr (HOLDS) loadLine(p.weight, R::at(0), p.N, 1.f, weight);
-  const long step = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  const long step = (long)groups * GROUPS, first = (long)blockIdx.x * GROUPS + threadIdx.x / LANES;
   const float each = 1.f / (float)p.N;
   R nextX, nextG;
   float nextMean, nextRstd;
@@ -278,8 +339,10 @@ __global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* 
           const float dy = (float)g.v[w][q], xh = ((float)x.v[w][q] - mean) * rstd, h = dy * weight[q];
           s1 += h;
           s2 = __builtin_fmaf(h, xh, s2);
-          sumB[w][q] += dy;
-          sumW[w][q] = __builtin_fmaf(dy, xh, sumW[w][q]);
+          if constexpr (SUMS) {
+            sumB[w][q] += dy;
+            sumW[w][q] = __builtin_fmaf(dy, xh, sumW[w][q]);
+          }
         }
       }
     }
@@ -306,7 +369,7 @@ __global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* 
     }
     turn ^= 1;
   }
-  if (!parts) return;
+  if (!SUMS || !parts) return;
   float* const to = parts + (long)blockIdx.x * 2 * p.N;
   if constexpr (GROUPS == 1) {
 #pragma unroll
@@ -405,6 +468,15 @@ __global__ __launch_bounds__(1024) void joinRows(LayerNormProblem p, const float
 // 30.8).
 long bandsOf(long M, long N) { return std::min(M, N < 256 ? 512L : 256L); }
 
+// Whether a workgroup may sum its columns of all rows in twelve turns: then workgroups for rows and for columns run in one launch,
+// without parts (128 x 2048 bf16 5.6 us, 7.6 in two launches; 128 x 8192 6.0, 10.4; 256 x 512 7.2 either way).
+bool together(long M, long N, size_t valueBytes) {
+  const long words = (N * (long)valueBytes + 15) / 16;
+  long lanes = 8;
+  while (lanes < 64 && lanes < words) lanes *= 2;
+  return N <= 16384 && M * lanes <= 12288;
+}
+
 // Whether the columns are summed by themselves, from x and g once more: for few long rows, of which each workgroup has one or two
 // and leaves sums as long as they are (us apart and together: 256 x 16384 bf16 13.9, 28.3; 64 x 8192 f16 10.0, 11.0; 512 x 8192 bf16
 // 13.6, 18.1; 1024 x 8192 bf16 21.2, 20.5; 512 x 4096 f32 13.1, 14.5; 64 x 8192 f32 11.6, 10.6).
@@ -447,15 +519,18 @@ bool launchRows(const LayerNormProblem& p, hipStream_t s) {
   return false;
 }
 
-template <class T, bool STREAM>
-int launchRowsBack(const LayerNormProblem& p, float* parts, hipStream_t s) {
+// Workgroups for the rows of a backward pass, with the columns' sums of each in parts (SUMS), or without them and `columns` more for
+// the columns of all rows; 0 where no registers hold a row.  rows: whether gradInput is wanted, or not yet.
+template <class T, bool STREAM, bool SUMS>
+int launchRowsBack(const LayerNormProblem& p, float* parts, bool rows, bool columns, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const long words = (p.N + V - 1) / V, bands = bandsOf(p.M, p.N);
-#define FBFFT_ROWS(LANES, WORDS)                                                        \
-  if (words <= LANES * WORDS) {                                                         \
-    const long groups = std::min(bands, (p.M + 1024 / LANES - 1) / (1024 / LANES));     \
-    rowsBackward<T, V, LANES, WORDS, STREAM><<<dim3((unsigned)groups), 1024, 0, s>>>(p, parts); \
-    return (int)groups;                                                                 \
+#define FBFFT_ROWS(LANES, WORDS)                                                                                   \
+  if (words <= LANES * WORDS) {                                                                                    \
+    const long most = (p.M + 1024 / LANES - 1) / (1024 / LANES), groups = rows ? std::min(SUMS ? bands : 65536L, most) : 0; \
+    const long more = columns ? (words + 63) / 64 : 0;                                                             \
+    rowsBackward<T, V, LANES, WORDS, STREAM, SUMS><<<dim3((unsigned)(groups + more)), 1024, 0, s>>>(p, parts, (int)groups); \
+    return (int)(groups + more);                                                                                   \
   }
   FBFFT_ROWS(8, 1)
   FBFFT_ROWS(16, 1)
@@ -505,7 +580,12 @@ int backward(const LayerNormProblem& p, hipStream_t s) {
   if (sums && (!launches((double)across * std::max(bands, 1L), kLanes) || !launches((2.0 * p.N + 15) / 16, 1024))) return FBFFT_UNSUPPORTED_SIZE;
   bool done = p.M == 0;
   if (!done && p.x.col == 1 && p.g.col == 1 && (!p.y.data || p.y.col == 1)) {
-    float* to = sums ? parts : nullptr;
+    if (sums && together(p.M, p.N, sizeof(T))) {
+      const bool over = p.y.data && (p.y.data == p.x.data || p.y.data == p.g.data);  // (what the columns read)
+      launchRowsBack<T, false, false>(p, nullptr, p.y.data && !over, true, s);
+      if (over) launchRowsBack<T, false, false>(p, nullptr, true, false, s);
+      return launchStatus();
+    }
     if (sums && apart(p.M, p.N, sizeof(T))) {
       constexpr int V = 16 / sizeof(T);
       const long over = (p.N + 64 * V - 1) / (64 * V), most = std::min(std::max(512 / over, 1L), (p.M + 31) / 32);
@@ -516,10 +596,13 @@ int backward(const LayerNormProblem& p, hipStream_t s) {
       if (bands > 1) launchJoinRows(p, parts, (int)bands, s);
       if (!p.y.data) return launchStatus();
       sums = false;
-      to = nullptr;
+      done = launchRowsBack<T, false, false>(p, nullptr, true, false, s) > 0;
+    } else {
+      float* const to = sums ? parts : nullptr;
+      const int groups = streams((double)p.M * p.N, p.type) ? launchRowsBack<T, true, true>(p, to, true, false, s)
+                                                            : launchRowsBack<T, false, true>(p, to, true, false, s);
+      if (groups) done = true, bands = groups;
     }
-    const int groups = streams((double)p.M * p.N, p.type) ? launchRowsBack<T, true>(p, to, s) : launchRowsBack<T, false>(p, to, s);
-    if (groups) done = true, bands = groups;
   }
   // (before gradInput, which may be one of the operands)
   if (!done && sums) anyParameters<T><<<dim3((unsigned)(across * bands)), kLanes, 0, s>>>(p, parts, bands);
