@@ -497,6 +497,7 @@ bool launchRows(const LayerNormProblem& p, hipStream_t s) {
     rowsForward<T, V, LANES, WORDS, THREADS, STREAM><<<grid(THREADS / LANES), THREADS, 0, s>>>(p); \
     return true;                                                                                 \
   }
+  FBFFT_ROWS(4, 1, 256)
   FBFFT_ROWS(8, 1, 256)
   FBFFT_ROWS(16, 1, 256)
   FBFFT_ROWS(32, 1, 256)
