@@ -874,7 +874,7 @@ PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
     double results;
   };
   static const Option options[] = {
-      {Small16, 16, 1, 0.136, 0.148, false, 3}, {Small32, 32, 16, 0.24, 0.42, false, 3}, {Deep64, 64, 8, 0.18, 0.24, true, 5},
+      {Small16, 16, 1, 0.136, 0.148, false, 3}, {Small32, 32, 16, 0.24, 0.42, false, 3}, {Deep64, 64, 8, 0.18, 0.24, true, 4},
       {Wide64, 64, 8, 0.4, 0.25, false, 5},     {Deep128, 128, 8, 0.56, 0.68, true, 6},   {Wide128, 128, 8, 0.62, 0.63, true, 6},
       {Wide256, 256, 8, 1.8, 2.4, true, 10}};
   PairPlan best{};
