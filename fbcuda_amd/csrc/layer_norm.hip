@@ -105,6 +105,8 @@ struct Row {
   typename Pack<T, VEC>::type v[WORDS];
 
   static __device__ __forceinline__ long at(int w) { return (long)(w * LANES + threadIdx.x % LANES) * VEC; }
+  // SKIP: lanes behind a row's end pass by (of rows that reach all lanes that costs 2 %)
+  template <bool SKIP>
   __device__ __forceinline__ void load(const Matrix& m, long i, long N) {
     const T* const from = static_cast<const T*>(m.data) + i * m.row;
 #pragma unroll
@@ -113,8 +115,8 @@ struct Row {
       if (j + VEC <= N) {
         v[w] = *reinterpret_cast<const typename Pack<T, VEC>::type*>(from + j);
       } else {
-        v[w] = {};
-        if (j < N) {  // (only where a row ends inside a word do waves take one value after the other)
+        if (SKIP) v[w] = typename Pack<T, VEC>::type{};
+        if (!SKIP || j < N) {
 #pragma unroll
           for (int q = 0; q < VEC; ++q) v[w][q] = j + q < N ? from[j + q] : (T)0.f;
         }
@@ -193,14 +195,14 @@ __global__ __launch_bounds__(THREADS) void rowsForward(LayerNormProblem p) {
   const long step = (long)gridDim.x * GROUPS, first = (long)blockIdx.x * GROUPS + threadIdx.x / LANES;
   const float each = 1.f / (float)p.N;
   R next;
-  if constexpr (HOLDS) next.load(p.x, min(first, p.M - 1), p.N);
+  if constexpr (HOLDS) next.template load<false>(p.x, min(first, p.M - 1), p.N);
   for (long i = first; i - threadIdx.x / LANES < p.M; i += step) {  // (as often for all rows of a workgroup)
     R x;
     if constexpr (HOLDS) {
       x = next;
-      if (i - threadIdx.x / LANES + step < p.M) next.load(p.x, min(i + step, p.M - 1), p.N);
+      if (i - threadIdx.x / LANES + step < p.M) next.template load<false>(p.x, min(i + step, p.M - 1), p.N);
     } else {
-      x.load(p.x, min(i, p.M - 1), p.N);
+      x.template load<false>(p.x, min(i, p.M - 1), p.N);
     }
     float sum = 0.f, none = 0.f;
 #pragma unroll
@@ -255,8 +257,8 @@ __device__ __forceinline__ void leaveColumns(const LayerNormProblem& p, long fir
 #pragma unroll 4
   for (long i = threadIdx.x / LANES; i < p.M; i += GROUPS) {
     R a, b;
-    a.load(x, i, p.N - from);
-    b.load(g, i, p.N - from);
+    a.template load<true>(x, i, p.N - from);
+    b.template load<true>(g, i, p.N - from);
     const float mean = p.mean[i * p.meanStride], rstd = p.rstd[i * p.rstdStride];
 #pragma unroll
     for (int q = 0; q < VEC; ++q) {
@@ -316,8 +318,8 @@ __global__ __launch_bounds__(1024) void rowsBackward(LayerNormProblem p, float* 
   float nextMean, nextRstd;
   auto load = [&](long row) __attribute__((always_inline)) {
     const long i = min(row, p.M - 1);
-    nextX.load(p.x, i, p.N);
-    nextG.load(p.g, i, p.N);
+    nextX.template load<true>(p.x, i, p.N);
+    nextG.template load<true>(p.g, i, p.N);
     nextMean = p.mean[i * p.meanStride], nextRstd = p.rstd[i * p.rstdStride];
   };
   if constexpr (HOLDS) load(first);
@@ -413,8 +415,8 @@ __global__ __launch_bounds__(kColumnWaves * 64) void columnSums(LayerNormProblem
 #pragma unroll 4
   for (long i = first + wave; i < end; i += kColumnWaves) {
     R a, b;
-    a.load(x, i, p.N - from);
-    b.load(g, i, p.N - from);
+    a.template load<true>(x, i, p.N - from);
+    b.template load<true>(g, i, p.N - from);
     const float mean = p.mean[i * p.meanStride], rstd = p.rstd[i * p.rstdStride];
 #pragma unroll
     for (int q = 0; q < VEC; ++q) {

@@ -14,10 +14,10 @@
 //   whole     one launch, a workgroup to a matrix in LDS: up to 96 rows (or columns) and 156 KB of pairs.  16 of 131 x 81 bf16
 //             46 us, 64 x 64 f32 19; step by step 80 and 52, of which each launch's way through memory is 2.5 to 4
 //   steps()   three products a step.  What bounds them: launches and latency below about 10^9 operations a product (192 x 1600
-//             f32 110 us, 17 launches), above it the matrix instructions, three for what one 16-bit product takes (8192 x 2048 f32
+//             f32 104 us, 17 launches), above it the matrix instructions, three for what one 16-bit product takes (8192 x 2048 f32
 //             1.78 ms, 0.92 PFLOP/s of the three)
 //   alone()   of long bfloat16 matrices: every A and B is a polynomial of the first A, so that the steps are products of P x P
-//             matrices alone, half of each by symmetry, and X is met by one product at the end.  8192 x 2048 bf16 in 0.95 ms, step
+//             matrices alone, half of each by symmetry, and X is met by one product at the end.  8192 x 2048 bf16 in 0.92 ms, step
 //             by step 1.57.  It takes the later A from the first, not from the rounded X, which puts small singular values off
 //             more (9e-4 of the norm at worst, where float32 results could not hide it)
 //
