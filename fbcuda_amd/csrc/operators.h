@@ -335,7 +335,6 @@ struct OrthogonalProblem {
   const float* coefficients;
   int steps;
   float eps, scale;
-  double growth;  // what the steps' polynomials multiply a singular value by, at most
   void* workspace;
 };
 size_t orthogonalWorkspaceBytes(long batch, long rows, long cols);

@@ -294,20 +294,17 @@ constexpr long long kMostSide = 65536;  // of a matrix that is orthogonalised
 constexpr double kMostSingular = 32;    // of what its products meet: pieces hold numbers below 64
 
 // Whether singular values that start in [0, 1] and what the products make of them stay within kMostSingular under these
-// polynomials: the greatest magnitude of each over the interval so far, at its ends and where its derivative is 0.  growth: what
-// they multiply one by at most, all steps together.
-bool staysInside(const float* coefficients, int steps, double& growth) {
+// polynomials: the greatest magnitude of each over the interval so far, at its ends and where its derivative is 0.
+bool staysInside(const float* coefficients, int steps) {
   double most = 1;
-  growth = 1;
   for (int i = 0; i < steps; ++i) {
     const double a = coefficients[3 * i], b = coefficients[3 * i + 1], c = coefficients[3 * i + 2];
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-    double next = 0, inner = 0, factor = std::fabs(a);
+    double next = 0, inner = 0;
     auto at = [&](double u) {  // u: the singular value's square
       if (!(u >= 0 && u <= most * most)) return;
       next = std::fmax(next, std::fabs(std::sqrt(u) * (a + u * (b + u * c))));
       inner = std::fmax(inner, std::fabs(u * (b + u * c)));
-      factor = std::fmax(factor, std::fabs(a + u * (b + u * c)));
     };
     at(most * most);
     if (c != 0) at(-b / (2 * c));
@@ -321,7 +318,6 @@ bool staysInside(const float* coefficients, int steps, double& growth) {
     }
     if (!(next <= kMostSingular && inner <= kMostSingular && most * most <= kMostSingular)) return false;
     most = next;
-    growth *= factor;
   }
   return true;
 }
@@ -340,8 +336,7 @@ extern "C" int fbfft_orthogonalize(const fbfft_array* input, const fbfft_array* 
     return FBFFT_UNSUPPORTED_DIMENSION;
   const long long batch = dim == 3 ? input->size[0] : 1, rows = input->size[dim - 2], cols = input->size[dim - 1];
   if (steps < 1 || steps > 32 || !(eps >= 0.f) || std::isinf(eps) || !std::isfinite(scale)) return FBFFT_UNSUPPORTED_SIZE;
-  double growth;
-  if (!staysInside(coefficients, steps, growth)) return FBFFT_UNSUPPORTED_SIZE;
+  if (!staysInside(coefficients, steps)) return FBFFT_UNSUPPORTED_SIZE;
   if (batch * rows * cols == 0) return FBFFT_SUCCESS;
   if (rows > kMostSide || cols > kMostSide) return FBFFT_UNSUPPORTED_SIZE;
   if (!okWorkspace(workspace, workspaceBytes, fbfft_orthogonalize_workspace(batch, rows, cols))) return FBFFT_UNSUPPORTED_DIMENSION;
@@ -350,7 +345,7 @@ extern "C" int fbfft_orthogonalize(const fbfft_array* input, const fbfft_array* 
   p.y = Matrix{output->data, (long)output->stride[dim - 2], (long)output->stride[dim - 1]};
   if (dim == 3) p.xBatch = input->stride[0], p.yBatch = output->stride[0];
   p.batch = batch, p.rows = rows, p.cols = cols, p.type = input->type;
-  p.coefficients = coefficients, p.steps = steps, p.eps = eps, p.scale = scale, p.growth = growth, p.workspace = workspace;
+  p.coefficients = coefficients, p.steps = steps, p.eps = eps, p.scale = scale, p.workspace = workspace;
   return launchOrthogonalize(p, stream);
 }
 

@@ -10,16 +10,16 @@
 // to 6e-3, pairs about 2e-6, as 32-bit arithmetic does: the first steps multiply small singular values by 3.4 each, and what
 // rounding put beside them, too.)
 //
-// Three ways:
+// Two ways:
 //   whole     one launch, a workgroup to a matrix in LDS: up to 96 rows (or columns) and 156 KB of pairs.  16 of 131 x 81 bf16
 //             46 us, 64 x 64 f32 19; step by step 80 and 52, of which each launch's way through memory is 2.5 to 4
 //   steps()   three products a step.  What bounds them: launches and latency below about 10^9 operations a product (192 x 1600
 //             f32 104 us, 17 launches), above it the matrix instructions, three for what one 16-bit product takes (8192 x 2048 f32
 //             1.78 ms, 0.92 PFLOP/s of the three)
-//   alone()   of long bfloat16 matrices: every A and B is a polynomial of the first A, so that the steps are products of P x P
-//             matrices alone, half of each by symmetry, and X is met by one product at the end.  8192 x 2048 bf16 in 0.92 ms, step
-//             by step 1.57.  It takes the later A from the first, not from the rounded X, which puts small singular values off
-//             more (9e-4 of the norm at worst, where float32 results could not hide it)
+//             (The P x P matrices of all steps first, every A from the first, and X met by them once at the end, took 0.92 ms for
+//             8192 x 2048 bf16.  But a rounding of the first A grows by up to a^2 with every step that only looks at A, where X
+//             itself would have set it right: five times the error of 32-bit arithmetic there, and up to half a rounding to bfloat16
+//             on matrices of one strong direction.)
 //
 // A pair matrix has rows of a multiple of 32 columns, 32 leading pieces and then their 32 second pieces, 128 bytes: what a
 // matrix instruction takes of a row.  Rows and columns are filled up with zeros.
@@ -35,8 +35,6 @@ namespace {
 typedef half16 halfx4 __attribute__((ext_vector_type(4)));
 
 constexpr float kUnit = 1024.f;  // what stands for 1 in pieces
-constexpr float kWide = 64.f;    // the same for products of factors, which reach growth
-constexpr long kAloneFrom = 3;   // columns to a row of X from which on alone() may run
 
 struct Pairs {
   half16* data;
@@ -190,8 +188,7 @@ struct PairArgs {
   const float* factors;  // not null: of each matrix; `power` times in by, once in beta
   int power;
   Pairs old, out, turned;  // old, turned: data may be null
-  // out is: what lies on and below the diagonal, and its mirror image.  (Exactly: of matrices whose sides differ by roundings,
-  // the part that is not symmetric grows tenfold with every step of products that take them to commute.)
+  // out is: what lies on and below the diagonal, and its mirror image.  (Exactly: A A is computed as A A^T.)
   bool symmetric;
   float* parts;            // not null: sums of each range, [matrix][range][tile][BM][BN], in place of results
 };
@@ -960,20 +957,17 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
 }
 
 // What lies in the workspace, for so many matrices of P x Q, and how the products run: of X with its transpose, of the P x P
-// matrices, of them with X, and of two of them at once.
+// matrices, and of them with X.
 struct Space {
   double* sums;
   float* factors;
   Pairs x, xt[2], gram, poly;
-  Pairs turns[4];  // in the place of xt[1], gram and poly: what alone() takes
-  Pairs alonePoly;
   float* parts;
   size_t bytes;
-  PairPlan gramPlan, polyPlan, lastPlan, twoPlan;
+  PairPlan gramPlan, polyPlan, lastPlan;
 
   Space(void* workspace, long batch, long P, long Q)
-      : gramPlan(planOf(true, batch, P, P, Q)), polyPlan(planOf(true, batch, P, P, P)), lastPlan(planOf(false, batch, P, Q, P)),
-        twoPlan(planOf(true, 2 * batch, P, P, P)) {
+      : gramPlan(planOf(true, batch, P, P, Q)), polyPlan(planOf(true, batch, P, P, P)), lastPlan(planOf(false, batch, P, Q, P)) {
     char* at = static_cast<char*>(workspace);
     auto take = [&](size_t size) {
       char* const from = at;
@@ -985,52 +979,22 @@ struct Space {
     auto pairs = [&](long rows, long cols) {
       return Pairs{reinterpret_cast<half16*>(take((size_t)batch * 2 * rows * cols * sizeof(half16))), cols, 2 * rows * cols};
     };
-    x = pairs(P, Q), xt[0] = pairs(Q, P);
-    char* const shared = at;
-    xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
-    char* const end = at;
-    at = shared;
-    for (Pairs& t : turns) t = pairs(P, P);
-    alonePoly = pairs(P, P);
-    if (Q < kAloneFrom * P) at = end;
-    at = std::max(at, end);
+    x = pairs(P, Q), xt[0] = pairs(Q, P), xt[1] = pairs(Q, P), gram = pairs(P, P), poly = pairs(P, P);
     size_t most = 0;
     for (const PairPlan* p : {&gramPlan, &polyPlan, &lastPlan}) most = std::max(most, partsBytes(*p, batch));
-    if (Q >= kAloneFrom * P) most = std::max(most, partsBytes(twoPlan, 2 * batch));
     parts = reinterpret_cast<float*>(take(most));
     bytes = at - static_cast<char*>(workspace);
   }
 
   bool fits(long batch) const {
-    for (const PairPlan* p : {&gramPlan, &polyPlan, &lastPlan, &twoPlan})
+    for (const PairPlan* p : {&gramPlan, &polyPlan, &lastPlan})
       // (workgroups of up to 1024 lanes, or of 256 to 32 x 32 or 32 x 64 of the results)
-      if (!launches((double)p->tiles * std::max(p->ranges, p->ranges > 1 ? p->side * p->side / 4096 + 1l : 1l) * batch * (p == &twoPlan ? 2 : 1), 1024)) return false;
+      if (!launches((double)p->tiles * std::max(p->ranges, p->ranges > 1 ? p->side * p->side / 4096 + 1l : 1l) * batch, 1024)) return false;
     return true;
-  }
-  // whether the P x P matrices alone, which X meets in the last product, are expected to take less time
-  bool takesLessAlone(int steps, long P, long Q) const {
-    const double all = steps * (gramPlan.time + polyPlan.time + lastPlan.time);
-    const double alone = gramPlan.time + 8 + (3 * steps - 1) * polyPlan.time + std::max(0, steps - 2) * (twoPlan.time - polyPlan.time) + lastPlan.time;
-    return Q >= kAloneFrom * P && alone < all;
   }
 };
 
-// m = a I + poly, in units of kWide
-__global__ __launch_bounds__(256) void firstFactor(Pairs poly, Pairs m, long rows, float a) {
-  const long words = poly.cols / 8, at = (long)blockIdx.x * 256 + threadIdx.x, i = at / words, j = (at - i * words) * 8;
-  if (i >= rows) return;
-  const half16* const from = poly.data + blockIdx.y * poly.batch + placeOf(poly, i, j);
-  halfx8 lead = *reinterpret_cast<const halfx8*>(from), rest = *reinterpret_cast<const halfx8*>(from + 32);
-  float z[8];
-#pragma unroll
-  for (int v = 0; v < 8; ++v) z[v] = ((float)lead[v] + (float)rest[v]) * (kWide / kUnit) + (i == j + v ? a * kWide : 0.f);
-  splitEight(z, lead, rest);
-  half16* const to = m.data + blockIdx.y * m.batch + placeOf(m, i, j);
-  *reinterpret_cast<halfx8*>(to) = lead;
-  *reinterpret_cast<halfx8*>(to + 32) = rest;
-}
-
-// One call: the matrices, and the launches of both ways.
+// One call: the matrices, and its launches.
 template <class T>
 struct Call {
   const OrthogonalProblem& p;
@@ -1065,58 +1029,20 @@ struct Call {
       begin<T, false><<<grid, 256, 0, s>>>(g, rows, cols, w.sums, p.eps, w.x, w.xt[0], w.factors);
   }
 
-  void gramOf(const Pairs& to, bool first) {
-    launchProduct(PairArgs{w.x, w.x, P, P, Q, 0, one, 0.f, first ? w.factors : nullptr, 2, Pairs{}, to, to, true, nullptr}, Nothing{},
-                  w.gramPlan, SHORT && first ? 3 : 0, w.parts, batch(), s);
-  }
-
-  // to = beta from + by a from, P x P matrices that commute, so that it is symmetric, too; of `count` matrices each
-  void commuting(const Pairs& a, const Pairs& from, const Pairs& to, float by, float beta, const PairPlan& plan, unsigned count) {
-    launchProduct(PairArgs{a, from, P, P, P, 0, by, beta, nullptr, 0, from, to, to, true, nullptr}, Nothing{}, plan, 0, w.parts, count, s);
-  }
-
-  // step after step
   void steps() {
     for (int i = 0; i < p.steps; ++i) {
       const float a = coefficient(i, 0), b = coefficient(i, 1), c = coefficient(i, 2);
       const bool first = i == 0;
-      gramOf(w.gram, first);
-      commuting(w.gram, w.gram, w.poly, c * one, b, w.polyPlan, batch());
+      launchProduct(PairArgs{w.x, w.x, P, P, Q, 0, one, 0.f, first ? w.factors : nullptr, 2, Pairs{}, w.gram, w.gram, true, nullptr}, Nothing{},
+                    w.gramPlan, SHORT && first ? 3 : 0, w.parts, batch(), s);
+      launchProduct(PairArgs{w.gram, w.gram, P, P, P, 0, c * one, b, nullptr, 0, w.gram, w.poly, w.poly, true, nullptr}, Nothing{}, w.polyPlan, 0,
+                    w.parts, batch(), s);
       const PairArgs x{w.poly, w.xt[i % 2], P, Q, P, 0, one, a, first ? w.factors : nullptr, 1, w.x, w.x, w.xt[(i + 1) % 2], false, nullptr};
       if (i + 1 < p.steps)
         launchProduct(x, Nothing{}, w.lastPlan, SHORT && first ? 1 : 0, w.parts, batch(), s);
       else
         launchProduct(x, result(), w.lastPlan, SHORT && first ? 1 : 0, w.parts, batch(), s);
     }
-  }
-
-  // The factors a I + B of all steps first, which are polynomials of the first A as every later A is, and their product with X.
-  void alone() {
-    const Pairs &gram = w.turns[0], &next = w.turns[1], &poly = w.alonePoly;
-    gramOf(gram, true);
-    int m = 2;  // where the factors' product lies
-    for (int i = 0; i < p.steps; ++i) {
-      const float a = coefficient(i, 0), b = coefficient(i, 1), c = coefficient(i, 2);
-      const bool last = i + 1 == p.steps;
-      commuting(gram, gram, poly, c * one, b, w.polyPlan, batch());
-      const Pairs &from = w.turns[m], &to = w.turns[5 - m];
-      if (i == 0) {
-        firstFactor<<<dim3((unsigned)ceilDivLong(P * P / 8, 256), batch()), 256, 0, s>>>(poly, from, P, a);
-        if (!last) commuting(poly, gram, next, one, a, w.polyPlan, batch());
-      } else if (last || p.batch > 1) {
-        if (!last) commuting(poly, gram, next, one, a, w.polyPlan, batch());
-        commuting(poly, from, to, one, a, w.polyPlan, batch());
-        m = 5 - m;
-      } else {
-        // both at once: a matrix's place is the distance between them
-        const Pairs same{poly.data, P, 0}, sources{gram.data, P, from.data - gram.data}, results{next.data, P, to.data - next.data};
-        commuting(same, sources, results, one, a, w.twoPlan, 2);
-        m = 5 - m;
-      }
-      if (!last) commuting(poly, next, gram, one, a, w.polyPlan, batch());
-    }
-    const PairArgs x{w.turns[m], w.xt[0], P, Q, P, 0, 1.f / kWide, 0.f, w.factors, 1, Pairs{}, Pairs{}, Pairs{}, false, nullptr};
-    launchProduct(x, result(), w.lastPlan, SHORT ? 1 : 0, w.parts, batch(), s);
   }
 };
 
@@ -1146,10 +1072,7 @@ int run(const OrthogonalProblem& p, hipStream_t s) {
   const long squared = ceilDivLong(call.P, 64) * ceilDivLong(call.Q, 64);
   if (p.batch > 65535 || !launches((double)squared * p.batch, 256) || !call.w.fits(p.batch)) return FBFFT_UNSUPPORTED_SIZE;
   call.squaresAndX(squared);
-  if (__is_same(T, brain16) && p.growth * kWide <= 32768 && call.w.takesLessAlone(p.steps, call.P, call.Q))
-    call.alone();
-  else
-    call.steps();
+  call.steps();
   return launchStatus();
 }
 

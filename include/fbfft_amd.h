@@ -457,11 +457,8 @@ int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, 
  * input, output: [rows][cols] or [batch][rows][cols] of one type, any strides, not overlapping; each matrix of a batch
  * by itself.  coefficients: 3 steps numbers in host memory, read during the call.  Products are summed in 32 bits;
  * between them X, A and b A + c A A are held as two 16-bit pieces of a value, 22 bits of it together, and products
- * leave out that of the second pieces: about what 32-bit arithmetic gives.  bfloat16 matrices with three times as
- * many columns as rows, or rows as columns, may be computed as the product of all steps' a I + b A + c A A with X, the
- * later A from the first: small singular values are then off by more, on matrices of one strong direction up to 9e-4 of
- * the result's norm, half of what its rounding to bfloat16 is off by.  A matrix of zeros gives zeros where
- * eps > 0; values that are not finite make all of their matrix NaN.
+ * leave out that of the second pieces: about what 32-bit arithmetic gives, for all types and shapes.  A matrix of zeros
+ * gives zeros where eps > 0; values that are not finite make all of their matrix NaN.
  * steps from 1 to 32; eps and scale finite, eps >= 0; coefficients under which a singular value in [0, 1] or what the
  * products make of it could pass 32 are refused (UnsupportedSize): the pieces end at 64.  rows, cols up to 65536;
  * a batch up to 65535 matrices, of small ones (32 x 1152, 64 x 480, 96 x 192) 2^22 - 1.
