@@ -1046,25 +1046,30 @@ struct Call {
   }
 };
 
-bool inOneLaunch(long batch, long P, long Q) { return batch <= 0x3fffff && P <= 32 * kWholeSteps && wholeBytes(P, Q) <= kWholeLarge; }
+bool inOneLaunch(long P, long Q) { return P <= 32 * kWholeSteps && wholeBytes(P, Q) <= kWholeLarge; }
 
 template <class T>
 void launchWhole(const OrthogonalProblem& p, hipStream_t s) {
   const bool turn = p.rows > p.cols;
   const long rows = turn ? p.cols : p.rows, cols = turn ? p.rows : p.cols, P = padded(rows), Q = padded(cols), bytes = wholeBytes(P, Q);
-  const Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
-  const Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
+  Given<const T> g{static_cast<const T*>(p.x.data), turn ? p.x.col : p.x.row, turn ? p.x.row : p.x.col, p.xBatch};
+  Given<T> y{static_cast<T*>(p.y.data), turn ? p.y.col : p.y.row, turn ? p.y.row : p.y.col, p.yBatch};
   WholeArgs w{rows, cols, (int)P, (int)Q, p.steps, p.eps, p.scale / kUnit, {}};
   for (int i = 0; i < 3 * p.steps; ++i) w.coefficients[i] = p.coefficients[i];
-  if (bytes <= kWholeSmall)
-    whole<T, kWholeSmall><<<dim3((unsigned)p.batch), kWholeLanes, 0, s>>>(g, y, w);
-  else
-    whole<T, kWholeLarge><<<dim3((unsigned)p.batch), kWholeLanes, 0, s>>>(g, y, w);
+  // (as many matrices at a time as a launch, which counts its lanes in 32 bits, holds)
+  constexpr long most = 0xffffffffl / kWholeLanes;
+  for (long first = 0; first < p.batch; first += most, g.data += most * g.batch, y.data += most * y.batch) {
+    const dim3 grid((unsigned)std::min(most, p.batch - first));
+    if (bytes <= kWholeSmall)
+      whole<T, kWholeSmall><<<grid, kWholeLanes, 0, s>>>(g, y, w);
+    else
+      whole<T, kWholeLarge><<<grid, kWholeLanes, 0, s>>>(g, y, w);
+  }
 }
 
 template <class T>
 int run(const OrthogonalProblem& p, hipStream_t s) {
-  if (inOneLaunch(p.batch, padded(std::min(p.rows, p.cols)), padded(std::max(p.rows, p.cols)))) {
+  if (inOneLaunch(padded(std::min(p.rows, p.cols)), padded(std::max(p.rows, p.cols)))) {
     launchWhole<T>(p, s);
     return launchStatus();
   }
@@ -1079,7 +1084,9 @@ int run(const OrthogonalProblem& p, hipStream_t s) {
 }  // namespace
 
 size_t orthogonalWorkspaceBytes(long batch, long rows, long cols) {
-  return Space(nullptr, batch, padded(std::min(rows, cols)), padded(std::max(rows, cols))).bytes;
+  const long P = padded(std::min(rows, cols)), Q = padded(std::max(rows, cols));
+  // (matrices in LDS leave it alone, whatever their number: one matrix's)
+  return Space(nullptr, inOneLaunch(P, Q) ? 1 : batch, P, Q).bytes;
 }
 
 int launchOrthogonalize(const OrthogonalProblem& p, hipStream_t s) {

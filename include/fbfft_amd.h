@@ -461,9 +461,9 @@ int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, 
  * gives zeros where eps > 0; values that are not finite make all of their matrix NaN.
  * steps from 1 to 32; eps and scale finite, eps >= 0; coefficients under which a singular value in [0, 1] or what the
  * products make of it could pass 32 are refused (UnsupportedSize): the pieces end at 64.  rows, cols up to 65536;
- * a batch up to 65535 matrices, of small ones (32 x 1152, 64 x 480, 96 x 192) 2^22 - 1.
- * workspace: fbfft_orthogonalize_workspace bytes, 256-byte aligned; its contents need not survive, and calls that overlap in
- * time need one each.  Reproducible bit for bit. */
+ * a batch up to 65535 matrices, of small ones (up to 32 x 1152, 64 x 480, 96 x 192) any number.
+ * workspace: fbfft_orthogonalize_workspace bytes (for small ones the same whatever the batch), 256-byte aligned; its contents
+ * need not survive, and calls that overlap in time need one each.  Reproducible bit for bit. */
 size_t fbfft_orthogonalize_workspace(long long batch, long long rows, long long cols);
 int fbfft_orthogonalize(const fbfft_array* input, const fbfft_array* output, const float* coefficients, int steps,
                         float eps, float scale, void* workspace, size_t workspaceBytes, fbfft_stream_t stream);

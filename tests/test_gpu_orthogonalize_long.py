@@ -64,3 +64,16 @@ def test_a_step_that_shrinks_after_steps_that_grew(shape, rank):
     assert bool(torch.isfinite(y).all())
     want, norms, _ = orthogonal_bound(g.float()[None], triples, 1e-7, 1.0)
     assert float((y - want[0]).norm()) <= float(norms) + U[torch.bfloat16] * float(want.norm())
+
+
+def test_more_small_matrices_than_a_launch_holds():
+    gen = torch.Generator().manual_seed(3)
+    few, many = 1031, (1 << 22) + 77
+    base = randn(gen, few, 2, 3).float().to(dev())
+    want = torch.empty_like(base)
+    assert F.orthogonalize(base, want, torch.empty(F.orthogonalize_workspace(few, 2, 3), dtype=torch.uint8, device=dev())) == F.Success
+    g = base[torch.arange(many, device=dev()) % few]
+    y = torch.full_like(g, 7.0)
+    assert F.orthogonalize(g, y, torch.empty(F.orthogonalize_workspace(many, 2, 3), dtype=torch.uint8, device=dev())) == F.Success
+    torch.cuda.synchronize()
+    assert torch.equal(y, want[torch.arange(many, device=dev()) % few])
