@@ -444,13 +444,13 @@ __global__ __launch_bounds__(kColumnWaves * 64) void columnSums(LayerNormProblem
   }
 }
 
-// Parts' sums, joined in their order: 1024 / SLICES columns of [2][N] to a workgroup, SLICES lanes to each.
+// Parts' sums, joined in their order, from column `first` of [2][N] on: 1024 / SLICES columns to a workgroup, SLICES lanes to each.
 template <int SLICES>
-__global__ __launch_bounds__(1024) void joinRows(LayerNormProblem p, const float* parts, int bands) {
+__global__ __launch_bounds__(1024) void joinRows(LayerNormProblem p, const float* parts, int bands, long first) {
   constexpr int COLUMNS = 1024 / SLICES;
   __shared__ float sums[SLICES][COLUMNS + 1];
   const int column = threadIdx.x % COLUMNS, slice = threadIdx.x / COLUMNS;
-  const long j = (long)blockIdx.x * COLUMNS + column;
+  const long j = first + (long)blockIdx.x * COLUMNS + column;
   float sum = 0.f;
   if (j < 2 * p.N)
 #pragma unroll 8
@@ -567,11 +567,17 @@ int forward(const LayerNormProblem& p, hipStream_t s) {
   return launchStatus();
 }
 
+constexpr long kMostLanes = 0xffffffffl;  // of a launch
+
 void launchJoinRows(const LayerNormProblem& p, const float* parts, int bands, hipStream_t s) {
-  if (bands > 32)
-    joinRows<64><<<dim3((unsigned)((2 * p.N + 15) / 16)), 1024, 0, s>>>(p, parts, bands);
-  else
-    joinRows<8><<<dim3((unsigned)((2 * p.N + 127) / 128)), 1024, 0, s>>>(p, parts, bands);
+  const long columns = bands > 32 ? 16 : 128, most = kMostLanes / 1024;  // of a workgroup; workgroups of a launch
+  for (long first = 0; first < 2 * p.N; first += most * columns) {
+    const dim3 grid((unsigned)std::min(most, (2 * p.N - first + columns - 1) / columns));
+    if (bands > 32)
+      joinRows<64><<<grid, 1024, 0, s>>>(p, parts, bands, first);
+    else
+      joinRows<8><<<grid, 1024, 0, s>>>(p, parts, bands, first);
+  }
 }
 
 template <class T>
@@ -579,8 +585,7 @@ int backward(const LayerNormProblem& p, hipStream_t s) {
   float* const parts = static_cast<float*>(p.workspace);
   bool sums = p.gradWeight.data || p.gradBias.data;
   const long across = (p.N + kLanes - 1) / kLanes;
-  long bands = p.M > 0 ? bandsOf(p.M, p.N) : 0;
-  if (sums && (!launches((double)across * std::max(bands, 1L), kLanes) || !launches((2.0 * p.N + 15) / 16, 1024))) return FBFFT_UNSUPPORTED_SIZE;
+  long bands = p.M > 0 ? std::min(bandsOf(p.M, p.N), kMostLanes / kLanes / across) : 0;  // (of the element by element way)
   bool done = p.M == 0;
   if (!done && p.x.col == 1 && p.g.col == 1 && (!p.y.data || p.y.col == 1)) {
     if (sums && together(p.M, p.N, sizeof(T))) {
@@ -589,12 +594,13 @@ int backward(const LayerNormProblem& p, hipStream_t s) {
       if (over) launchRowsBack<T, false, false>(p, nullptr, true, false, s);
       return launchStatus();
     }
-    if (sums && apart(p.M, p.N, sizeof(T))) {
-      constexpr int V = 16 / sizeof(T);
-      const long over = (p.N + 64 * V - 1) / (64 * V), most = std::min(std::max(512 / over, 1L), (p.M + 31) / 32);
+    constexpr int V = 16 / sizeof(T);
+    const long over = (p.N + 64 * V - 1) / (64 * V);
+    // (one band where there are 512 workgroups across; of float32 rows of 2^31 - 256 values and more they do not fit a launch)
+    if (sums && apart(p.M, p.N, sizeof(T)) && launches((double)over, kColumnWaves * 64)) {
+      const long most = std::min(std::max(512 / over, 1L), (p.M + 31) / 32);
       const long rows = (p.M + most - 1) / most;
       bands = (p.M + rows - 1) / rows;
-      if (!launches((double)over * bands, kColumnWaves * 64)) return FBFFT_UNSUPPORTED_SIZE;
       columnSums<T, V><<<dim3((unsigned)over, (unsigned)bands), kColumnWaves * 64, 0, s>>>(p, bands > 1 ? parts : nullptr, rows);
       if (bands > 1) launchJoinRows(p, parts, (int)bands, s);
       if (!p.y.data) return launchStatus();
