@@ -6,6 +6,8 @@
 
 namespace fbfft_amd {
 
+inline long ceilDivLong(long a, long b) { return (a + b - 1) / b; }
+
 constexpr unsigned kOutside = 0x80000000u;  // the place of a word that is not there: behind every buffer
 constexpr int kReach = 0x7fffffff;          // bytes of a buffer, which ends in front of it
 

@@ -4,6 +4,7 @@
 //   product                               y = activation(sum_k x w + bias) + residual
 //
 // The scaled matrix instruction takes 128 k of 16 rows of both operands: a lane a whole block, 16 bytes, and the byte of its scale.
+#include "mx4_plan.h"
 #include "product.h"
 
 #include <algorithm>
@@ -459,9 +460,6 @@ __global__ __launch_bounds__(kFewWaves * 64) void fewRows(FewArgs f) {
   }
 }
 
-// of x in LDS: rows of codes 16 bytes apart, and their scales
-size_t fewBytes(long M, long blocks) { return std::min(M, 16l) * 17 * (blocks + 1); }
-
 template <class T, bool WAY, int RB, int NB>
 void launchFew(FewArgs f, hipStream_t s) {
   const long across = ceilDivLong(f.g.N, 16 * NB);
@@ -481,68 +479,9 @@ void launchFew(FewArgs f, hipStream_t s) {
 
 // ---- what runs ----
 
-// The kernel of a product: its tile, or its fragments of x and w, and the ranges that k is cut into.
-struct Mx4Plan {
-  enum Kind { Way, Few, Tiles };
-  int kind, rows, cols;  // Way, Few: RB and NB; Tiles: of a tile
-  long ranges, range;    // blocks
-};
-
-constexpr size_t kWayMost = 64 << 10;  // of LDS, for x that a workgroup quantises
-
-// The kernel with the least expected time, in us.  Few rows: a base, for each block of k and workgroup the numbers below in ns,
-// but no less than 230 workgroups' (fewer leave compute units idle), and as much again for the results of every workgroup after
-// those.  Tiles: a base, and for each round of workgroups its steps of eight blocks and its results.  (`way`: whether the
-// workgroups may quantise x, which rows one by one are read for: 0.07 ns of a block at one row, 0.144 at 16.)
-// Measured on rows from 1 to 6476 and weights of 256 x 256 to 32000 x 4096, each kernel with each number of ranges, x quantised
-// by the workgroups or in front: 1 x 2048 x 8192 5.5 us on the way and 7.2 in two launches, 128 x 1151 x 1000 6.0 and 7.0,
-// tiles 11.6; 32 x 8192 x 8192 21.8 and tiles in four ranges 19.6; 8192 x 8192 x 8192 in tiles of 256 282, of 128 377.
-// x quantised already: 64 x 4096 x 4096 9.8 by few rows, 13.0 in tiles; 256 x 1152 x 4608 10.0 and 7.9; 6476 x 96 x 4576, most
-// of it results, 70 and 24.
-Mx4Plan planOf(long M, long blocks, long N, bool way) {
-  if (blocks == 0) return {Mx4Plan::Few, 1, 1, 1, 0};
-  Mx4Plan best{};
-  double least = 0;
-  auto offer = [&](const Mx4Plan& plan, double time) {
-    if (least == 0 || time < least) least = time, best = plan;
-  };
-  const double x = (double)std::min(M, 16l);
-  auto few = [&](int kind, int rows, int cols, double base, double each, double results) {
-    const double groups = (double)ceilDivLong(M, 16 * rows) * ceilDivLong(N, 16 * cols), many = std::max(groups, 230.0);
-    offer({kind, rows, cols, 1, blocks}, base + (many * blocks * each + (many - 230) * results * x / 16) / 1e3);
-  };
-  if (way && fewBytes(M, blocks) <= kWayMost) {
-    few(Mx4Plan::Way, 1, 1, 3.3, 0.068 + 0.0047 * x, 0.6);
-    few(Mx4Plan::Way, 1, 2, 3.3, 0.15 + 0.0046 * x, 1.5);
-  }
-  static const double each[3][2] = {{0.106, 0.157}, {0.157, 0.226}, {0.32, 0.42}}, results[3][2] = {{0.6, 1.5}, {0.8, 3.5}, {1.4, 10.8}};
-  for (int r = 0; r < 3; ++r)
-    for (int c = 0; c < 2; ++c) few(Mx4Plan::Few, 1 << r, 1 << c, 5.7, each[r][c], results[r][c]);
-  struct Option {
-    int side, together;  // together: workgroups that share a compute unit
-    double alone, last, shared, results;  // 256 k and the results: of a lone workgroup, of one among many
-  };
-  static const Option options[] = {{128, 2, 0.9, 2, 1.34, 4.4}, {256, 1, 1.9, 4.9, 1.9, 8}};
-  const int units = computeUnits();
-  for (const Option& a : options) {
-    const long tiles = ceilDivLong(M, a.side) * ceilDivLong(N, a.side);
-    for (long ranges = 1; ranges <= 32; ranges *= 2) {
-      const long range = ceilDivLong(ceilDivLong(blocks, ranges), 8) * 8, used = ceilDivLong(blocks, range);
-      if (ranges > 1 && range < 16) break;
-      const long groups = tiles * used, slots = (long)units * a.together;
-      const bool lone = groups <= units;
-      const double rounds = groups <= slots ? 1.0 : std::max((double)groups / slots, groups < 4 * slots ? (double)ceilDivLong(groups, slots) : 1.0);
-      double time = 6.5 + rounds * (range / 8 * (lone ? a.alone : a.shared) + (lone ? a.last : a.results));
-      if (used > 1) time += 2.5 + (double)M * N * used * 4 / 4e6;
-      offer({Mx4Plan::Tiles, a.side, a.side, used, range}, time);
-    }
-  }
-  return best;
-}
-
 template <class T>
 int run(const LinearMx4Problem& p, hipStream_t s) {
-  const Mx4Plan plan = planOf(p.M, p.blocks, p.N, p.x.data && p.x.col == 1);
+  const Mx4Plan plan = planOf(p.M, p.blocks, p.N, p.x.data && p.x.col == 1, computeUnits());
   Mx4Args g{p.xq, p.w, p.M, p.N, p.blocks, plan.range, Epilogue{p.y, p.residual, {}, p.bias, p.activation, false, nullptr}};
   g.e.dense = p.y.col == 1 && (!p.residual.data || p.residual.col == 1);
   char* space = static_cast<char*>(p.workspace);
@@ -614,7 +553,8 @@ int launchMx4Dequantize(const Mx4& from, const Matrix& y, int type, long M, long
 
 size_t linearMx4WorkspaceBytes(long M, long blocks, long N) {
   // (x, quantised in front of the product, and ranges' sums, whichever way x comes)
-  const long ranges = std::max(planOf(M, blocks, N, true).ranges, planOf(M, blocks, N, false).ranges);
+  const int units = computeUnits();
+  const long ranges = std::max(planOf(M, blocks, N, true, units).ranges, planOf(M, blocks, N, false, units).ranges);
   return rounded((size_t)M * blocks * 16) + rounded((size_t)M * blocks) + (ranges > 1 ? rounded((size_t)ranges * M * N * sizeof(float)) : 0);
 }
 

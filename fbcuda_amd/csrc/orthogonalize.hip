@@ -23,6 +23,7 @@
 //
 // A pair matrix has rows of a multiple of 32 columns, 32 leading pieces and then their 32 second pieces, 128 bytes: what a
 // matrix instruction takes of a row.  Rows and columns are filled up with zeros.
+#include "pair_plan.h"
 #include "product.h"
 
 #include <algorithm>
@@ -642,8 +643,8 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
 // the 16 rows of a fragment take all banks.  Waves take blocks of 16 x 16 results in turn; X's columns, which the last product
 // of a step sums over X's rows, come by the transposing read.
 constexpr int kWholeLanes = 1024;
-constexpr int kWholeSteps = 3, kWholeBlocks = 2;  // of 32 rows of X, at most, and of a symmetric matrix to a wave
-constexpr int kWholeSmall = 64 << 10, kWholeLarge = 156 << 10;  // bytes of LDS
+constexpr int kWholeBlocks = 2;        // of a symmetric matrix to a wave
+constexpr int kWholeSmall = 64 << 10;  // bytes of LDS
 
 struct WholeArgs {
   long rows, cols;
@@ -651,8 +652,6 @@ struct WholeArgs {
   float eps, scale;
   float coefficients[96];
 };
-
-inline long wholeBytes(long P, long Q) { return P * (4 * Q + 16) + 2 * P * (4 * P + 16); }
 
 // Eight k from 32 kb + 8 (lane / 16) of row first + lane % 16.
 __device__ __forceinline__ uintx4 wholeFragment(const char* m, int pitch, int first, int kb, int piece) {
@@ -846,56 +845,6 @@ __global__ __launch_bounds__(kWholeLanes) void whole(Given<const T> g, Given<T> 
   }
 }
 
-long padded(long n) { return (n + 31) / 32 * 32; }
-
-// The kernel of a product, and the ranges that its k is cut into.
-enum PairKind { Small16, Small32, Deep64, Wide64, Deep128, Wide128, Wide256 };
-struct PairPlan {
-  int kind, side;  // side: of a tile
-  long tiles, ranges, range;
-  double time;  // expected
-};
-
-// The kernel with the least expected time, in us, from what each takes for a step of 32 k: `alone` where workgroups have compute
-// units to themselves, else `each` for every one that a compute unit gets (in whole rounds where few fit it), and besides for
-// results, more of them where they are left both ways round.  Ranges add a launch, and their sums' way to memory and back.
-// Measured in every kernel on products from 64 x 64 x 64 to 2048 x 8192 x 8192: 1024 x 1024 x 1024 with half of it a mirror
-// image: Deep64 11.4, Wide64 18.4, Wide128 28; 2048 x 2048 x 2048 so: Wide64 40, Deep128 42, Wide128 in three ranges 44;
-// 2048 x 8192 x 2048: Wide256 167, Wide128 189, Wide64 240; 256 x 256 x 8192: Small32 in one range 58, in eight 17; 256 x 256 x
-// 6432: Small32 in nine 20, Deep64 in eight 13.
-PairPlan planOf(bool symmetric, long batch, long M, long N, long K) {
-  struct Option {
-    int kind, side, most;  // most: ranges
-    double alone, each;
-    bool whole;
-    double results;
-  };
-  static const Option options[] = {
-      {Small16, 16, 1, 0.136, 0.148, false, 3}, {Small32, 32, 16, 0.24, 0.42, false, 3}, {Deep64, 64, 8, 0.18, 0.24, true, 4},
-      {Wide64, 64, 8, 0.4, 0.25, false, 5},     {Deep128, 128, 8, 0.56, 0.68, true, 6},   {Wide128, 128, 8, 0.62, 0.63, true, 6},
-      {Wide256, 256, 8, 1.8, 2.4, true, 10}};
-  PairPlan best{};
-  double least = 0;
-  const long steps = K / 32;
-  const double units = computeUnits();
-  for (const Option& o : options) {
-    const long down = ceilDivLong(M, o.side), across = ceilDivLong(N, o.side);
-    const long tiles = symmetric ? down * (down + 1) / 2 : down * across;
-    for (long ranges = 1; ranges <= o.most; ranges += ranges < 4 ? 1 : ranges < 8 ? 2 : 4) {
-      const long range = ceilDivLong(steps, ranges), used = ceilDivLong(steps, range);
-      if (ranges > 1 && range < 8) break;
-      const double share = (double)batch * tiles * used / units, rounds = o.whole && share < 8 ? std::ceil(share) : share;
-      double time = o.results + (symmetric ? 0 : 2) + range * (share <= 0.75 ? o.alone : std::max(o.alone, rounds * o.each));
-      if (used > 1) time += 4.5 + (double)batch * tiles * used * o.side * o.side * 8 / 4e6;
-      if (least == 0 || time < least) {
-        least = time;
-        best = PairPlan{o.kind, o.side, tiles < 8 ? tiles : (tiles + 7) / 8 * 8, used, 32 * range, time};
-      }
-    }
-  }
-  return best;
-}
-
 size_t partsBytes(const PairPlan& p, long batch) {
   return p.ranges > 1 ? (size_t)batch * p.ranges * p.tiles * p.side * p.side * sizeof(float) : 0;
 }
@@ -967,7 +916,8 @@ struct Space {
   PairPlan gramPlan, polyPlan, lastPlan;
 
   Space(void* workspace, long batch, long P, long Q)
-      : gramPlan(planOf(true, batch, P, P, Q)), polyPlan(planOf(true, batch, P, P, P)), lastPlan(planOf(false, batch, P, Q, P)) {
+      : gramPlan(planOf(true, batch, P, P, Q, computeUnits())), polyPlan(planOf(true, batch, P, P, P, computeUnits())),
+        lastPlan(planOf(false, batch, P, Q, P, computeUnits())) {
     char* at = static_cast<char*>(workspace);
     auto take = [&](size_t size) {
       char* const from = at;
@@ -1045,8 +995,6 @@ struct Call {
     }
   }
 };
-
-bool inOneLaunch(long P, long Q) { return P <= 32 * kWholeSteps && wholeBytes(P, Q) <= kWholeLarge; }
 
 template <class T>
 void launchWhole(const OrthogonalProblem& p, hipStream_t s) {

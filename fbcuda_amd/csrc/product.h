@@ -324,7 +324,6 @@ void launchJoin(const JoinPlan& plan, const Epilogue& e, long M, long N, int ran
     joinRanges<T, 8><<<grid, 256, 0, s>>>(e, M, N, ranges);
 }
 
-long ceilDivLong(long a, long b) { return (a + b - 1) / b; }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
 }  // namespace
