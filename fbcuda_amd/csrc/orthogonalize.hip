@@ -191,7 +191,7 @@ struct PairArgs {
   Pairs old, out, turned;  // old, turned: data may be null
   // out is: what lies on and below the diagonal, and its mirror image.  (Exactly: A A is computed as A A^T.)
   bool symmetric;
-  float* parts;            // not null: sums of each range, [matrix][range][tile][BM][BN], in place of results
+  float* parts;            // not null: sums of each range of a symmetric product, [matrix][range][tile][BM][BN], in place of results
 };
 
 // where the last product leaves its results, times a factor
@@ -328,7 +328,7 @@ __device__ __forceinline__ void belowDiagonal(int tile, int down, int& i, int& j
 template <int BM, int BN>
 struct PairTile {
   long m0, n0;
-  int index;  // among all tiles
+  int index;  // among the tiles of a symmetric product
   bool any, mirror;
 
   __device__ __forceinline__ PairTile(const PairArgs& g) {
@@ -343,8 +343,7 @@ struct PairTile {
       mirror = true;
     } else {
       const Tile<BM, BN> t(g.M, g.N, turn);
-      m0 = t.m0, n0 = t.n0, any = t.any;
-      index = (int)(m0 / BM * ((g.N + BN - 1) / BN) + n0 / BN);
+      m0 = t.m0, n0 = t.n0, any = t.any, index = 0;
       mirror = g.turned.data != nullptr;
     }
   }
@@ -470,7 +469,7 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
       for (int j = 0; j < RN; ++j) *reinterpret_cast<floatx4*>(mine + (16 * i + lane % 16) * PITCH + 16 * j + lane / 16 * 4) = sum[i0 + i][j];
     waveExchange();
     const int row0 = wm + 16 * i0;
-    if (g.parts) {
+    if (__is_same(RESULT, Nothing) && g.parts) {
       const long tiles = gridDim.x;
       float* const to = g.parts + (((matrix * gridDim.y + blockIdx.y) * tiles + tile.index) * BM + row0) * BN + wn;
 #pragma unroll 1
@@ -485,27 +484,22 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
   }
 }
 
-// Results from the sums of `ranges` ranges of k, in their order: a workgroup to 32 rows of up to 64 columns of a tile, eight ranges'
+// Results of a symmetric product from the sums of `ranges` ranges of k, in their order: a workgroup to 32 rows of up to 64 columns of a tile, eight ranges'
 // sums on their way at once (60 x 60 in 13 ranges 5.5 us, by a wave and range after range 11.9).
-template <class RESULT, int BM, int BN>
-__global__ __launch_bounds__(256) void join(PairArgs g, RESULT result, int ranges, int tiles) {
+template <int BM, int BN>
+__global__ __launch_bounds__(256) void join(PairArgs g, int ranges, int tiles) {
   constexpr int COLS = BN < 64 ? BN : 64, ACROSS = BN / COLS, BLOCKS = BM / 32 * ACROSS, AHEAD = 8;  // BLOCKS: of a tile
   __shared__ __attribute__((aligned(16))) float space[32 * (COLS + 4)];
   const int index = (int)blockIdx.x / BLOCKS, block = (int)blockIdx.x % BLOCKS;
   const long matrix = blockIdx.z;
   int i, j;
-  if (g.symmetric) {
-    belowDiagonal(index, (int)((g.M + BM - 1) / BM), i, j);
-  } else {
-    const int across = (int)((g.N + BN - 1) / BN);
-    i = index / across, j = index % across;
-  }
+  belowDiagonal(index, (int)((g.M + BM - 1) / BM), i, j);
   const int row0 = block / ACROSS * 32, col0 = block % ACROSS * COLS;
   const long m0 = (long)i * BM + row0, n0 = (long)j * BN + col0;
   if (m0 >= g.M || n0 >= g.N) return;
   const long far = (long)tiles * BM * BN;  // from a range to the next
   const float* const from = g.parts + matrix * ranges * far + ((long)index * BM + row0) * BN + col0;
-  leavePairs<COLS, 4>(g, result, matrix, m0, n0, g.turned.data != nullptr, space, [&](int row, int c, float(&v)[8]) {
+  leavePairs<COLS, 4>(g, Nothing{}, matrix, m0, n0, true, space, [&](int row, int c, float(&v)[8]) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = 0.f;
     for (int first = 0; first < ranges; first += AHEAD) {
@@ -535,7 +529,7 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
   const int row = threadIdx.x / LANES, c = threadIdx.x % LANES * 4;
   const long m = m0 + row, n = n0 + c;
   halfx4 oldLead{}, oldRest{};
-  if (row < SIDE && g.old.data && !g.parts) {
+  if (row < SIDE && g.old.data && (LAST || !g.parts)) {
     const half16* const from = g.old.data + matrix * g.old.batch + placeOf(g.old, m, n);
     oldLead = *reinterpret_cast<const halfx4*>(from), oldRest = *reinterpret_cast<const halfx4*>(from + 32);
   }
@@ -587,7 +581,7 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
       *reinterpret_cast<floatx4*>(&sums[wave][(16 * i + lane % 16) * PITCH + 16 * j + lane / 16 * 4]) = sum[i][j];
   __syncthreads();
   bool turns = tile.mirror && !g.parts;
-  if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1 && !g.parts;
+  if constexpr (LAST) turns = result.y.row == 1 && result.y.col != 1;
   float z[4] = {};
   if (row < SIDE) {
 #pragma unroll
@@ -596,7 +590,7 @@ __global__ __launch_bounds__(WAVES * 64) void small(PairArgs g, RESULT result) {
 #pragma unroll
       for (int v = 0; v < 4; ++v) z[v] += q[v];
     }
-    if (g.parts) {
+    if (!LAST && g.parts) {
       storePack(g.parts + (((matrix * gridDim.y + blockIdx.y) * gridDim.x + tile.index) * SIDE + row) * SIDE + c, z);
       return;
     }
@@ -890,18 +884,18 @@ void launchProduct(PairArgs g, const RESULT& result, const PairPlan& plan, int o
     if constexpr (__is_same(RESULT, Nothing))
       if (one == 3) tiles(std::integral_constant<int, 3>());
   }
-  if (plan.ranges > 1) {
-    const long down = ceilDivLong(g.M, plan.side), count = g.symmetric ? down * (down + 1) / 2 : down * ceilDivLong(g.N, plan.side);
+  if (plan.ranges > 1) {  // (symmetric products)
+    const long down = ceilDivLong(g.M, plan.side), count = down * (down + 1) / 2;
     const dim3 blocks((unsigned)(count * (plan.side / 32) * (plan.side > 32 ? plan.side / 64 : 1)), 1, batch);
     const int ranges = (int)plan.ranges, rounded = (int)plan.tiles;
     if (plan.side == 32)
-      join<RESULT, 32, 32><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
+      join<32, 32><<<blocks, 256, 0, s>>>(g, ranges, rounded);
     else if (plan.side == 64)
-      join<RESULT, 64, 64><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
+      join<64, 64><<<blocks, 256, 0, s>>>(g, ranges, rounded);
     else if (plan.side == 128)
-      join<RESULT, 128, 128><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
+      join<128, 128><<<blocks, 256, 0, s>>>(g, ranges, rounded);
     else
-      join<RESULT, 256, 256><<<blocks, 256, 0, s>>>(g, result, ranges, rounded);
+      join<256, 256><<<blocks, 256, 0, s>>>(g, ranges, rounded);
   }
 }
 

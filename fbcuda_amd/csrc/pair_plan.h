@@ -53,7 +53,8 @@ inline PairPlan planOf(bool symmetric, long batch, long M, long N, long K, doubl
   for (const Option& o : options) {
     const long down = ceilDivLong(M, o.side), across = ceilDivLong(N, o.side);
     const long tiles = symmetric ? down * (down + 1) / 2 : down * across;
-    for (long ranges = 1; ranges <= o.most; ranges += ranges < 4 ? 1 : ranges < 8 ? 2 : 4) {
+    // (B X has at least as many columns as rows, and its k are its rows: where ranges of 256 k could be cut, tiles fill the chip)
+    for (long ranges = 1; ranges <= (symmetric ? o.most : 1); ranges += ranges < 4 ? 1 : ranges < 8 ? 2 : 4) {
       const long range = ceilDivLong(steps, ranges), used = ceilDivLong(steps, range);
       if (ranges > 1 && range < 8) break;
       const double share = (double)batch * tiles * used / units, rounds = o.whole && share < 8 ? std::ceil(share) : share;
