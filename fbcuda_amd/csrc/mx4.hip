@@ -15,8 +15,8 @@ namespace {
 typedef int intx8 __attribute__((ext_vector_type(8)));
 
 // The scale's byte of a block from the bits of its largest magnitude as float32 (numbers without sign, which order like the
-// values), 255 for what is not finite.  floor(log2) is the exponent's field; numbers without one are below 2^-125, as
-// are all that take the least scale.
+// values), 255 for what is not finite.  floor(log2) is the exponent's field; the least scale is that of all numbers below 2^-124,
+// those without an exponent of their own among them.
 __device__ __forceinline__ int scaleOf(unsigned most) {
   const int exponent = (int)(most >> 23);
   return exponent == 255 ? 255 : max(exponent - 2, 0);

@@ -15,7 +15,7 @@
 //             46 us, 64 x 64 f32 19; step by step 80 and 52, of which each launch's way through memory is 2.5 to 4
 //   steps()   three products a step.  What bounds them: launches and latency below about 10^9 operations a product (192 x 1600
 //             f32 104 us, 17 launches), above it the matrix instructions, three for what one 16-bit product takes (8192 x 2048 f32
-//             1.78 ms, 0.92 PFLOP/s of the three)
+//             1.63 ms, 1.03 PFLOP/s of the three; bf16, whose first step has fewer pieces, 1.55)
 //             (The P x P matrices of all steps first, every A from the first, and X met by them once at the end, took 0.92 ms for
 //             8192 x 2048 bf16.  But a rounding of the first A grows by up to a^2 with every step that only looks at A, where X
 //             itself would have set it right: five times the error of 32-bit arithmetic there, and up to half a rounding to bfloat16
@@ -845,7 +845,7 @@ size_t partsBytes(const PairPlan& p, long batch) {
 
 template <class RESULT, int SIDE>
 void launchSmall(const PairArgs& g, const RESULT& result, dim3 grid, hipStream_t s) {
-  // (as many waves as there are steps for, two or four ahead)
+  // (as many waves as there are steps for, two steps of each ahead)
   if (g.range <= 256)
     small<RESULT, SIDE, 4, 2><<<grid, 256, 0, s>>>(g, result);
   else if (g.range <= 512)
