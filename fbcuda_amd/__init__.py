@@ -442,8 +442,7 @@ def FFTIteratedConvolutionWS(fftSize, ins, outs, weight, pass_, scale, batchSize
     rc = _entry().fbfft_iterated_conv_ws(fftSize, ins.data_ptr(), outs.data_ptr(),
                                          _desc(weight), int(pass_),
                                          float(scale), int(batchSize), int(numTiles),
-                                         workspace.data_ptr(),
-                                         workspace.numel() * workspace.element_size(), _stream(stream))
+                                         *_space(workspace), _stream(stream))
     if rc < 0:
         raise RuntimeError("fbfft_iterated_conv_ws: %s" % error_string(-rc))
     return rc == 1
@@ -461,8 +460,7 @@ def conv_fprop(input, weight, output, fftSize, workspace, stream=None):
             return rc
     _on_gpu(input, weight, output, workspace)
     return _entry().fbfft_conv_fprop(_desc(input), _desc(weight), _desc(output), fftSize,
-                                     workspace.data_ptr(),
-                                     workspace.numel() * workspace.element_size(), _stream(stream))
+                                     *_space(workspace), _stream(stream))
 
 
 STATIC_SCRATCH_BYTES = 32 << 20
@@ -502,8 +500,7 @@ def conv_bprop(gradOutput, weight, gradInput, fftSize, workspace, stream=None):
             return rc
     _on_gpu(gradOutput, weight, gradInput, workspace)
     return _entry().fbfft_conv_bprop(_desc(gradOutput), _desc(weight), _desc(gradInput), fftSize,
-                                     workspace.data_ptr(),
-                                     workspace.numel() * workspace.element_size(), _stream(stream))
+                                     *_space(workspace), _stream(stream))
 
 
 def conv_accgrad(input, gradOutput, gradWeight, fftSize, workspace, scale=1.0, accumulate=False,
@@ -517,8 +514,7 @@ def conv_accgrad(input, gradOutput, gradWeight, fftSize, workspace, scale=1.0, a
     _on_gpu(input, gradOutput, gradWeight, workspace)
     return _entry().fbfft_conv_accgrad(_desc(input), _desc(gradOutput), _desc(gradWeight), fftSize,
                                        scale, int(bool(accumulate)),
-                                       workspace.data_ptr(),
-                                       workspace.numel() * workspace.element_size(), _stream(stream))
+                                       *_space(workspace), _stream(stream))
 
 
 # ---- operators around a convolution layer: float32, float16 and bfloat16, any strides ----
@@ -550,8 +546,13 @@ def _activation(name):
 
 
 def _space(workspace):
-    """(address, bytes) of a workspace, which may be None."""
-    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    """(address, bytes) of a workspace, which may be None: of an expanded one, those that it has."""
+    if workspace is None or workspace.numel() == 0:
+        return None, 0
+    _on_gpu(workspace)
+    size = workspace.element_size()
+    behind = workspace.untyped_storage().nbytes() - workspace.storage_offset() * size
+    return workspace.data_ptr(), min(workspace.numel() * size, behind)
 
 
 def _given(*ts):

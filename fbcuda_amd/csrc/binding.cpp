@@ -15,6 +15,7 @@
 
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <limits>
 
 #include "../../include/fbfft_amd.h"
@@ -56,13 +57,14 @@ bool real(PyObject* o, float* v) {
   return true;
 }
 
-// device memory of any type: address and bytes
+// device memory of any type: address and bytes (of an expanded tensor those that it has)
 bool memory(PyObject* o, void** p, size_t* bytes) {
   if (!THPVariable_CheckExact(o)) return false;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.layout() != at::kStrided) return false;
   *p = t.data_ptr();
-  *bytes = (size_t)t.numel() * (size_t)t.element_size();
+  const int64_t size = t.element_size(), behind = (int64_t)t.storage().nbytes() - t.storage_offset() * size;
+  *bytes = (size_t)std::max<int64_t>(0, std::min<int64_t>(t.numel() * size, behind));
   return true;
 }
 

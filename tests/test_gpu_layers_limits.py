@@ -7,6 +7,7 @@ from gpu_util import dev
 from layers_util import quantized, values_of
 from operators_util import NAMES, TYPES, linear, randn, rounded, within
 from test_gpu_mx4 import matrix, packed, quantize
+from test_gpu_orthogonalize import check as updates
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +125,27 @@ def replays_are_eager(x, y, call, size):
         assert call(want, spaces[1]) == F.Success
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+def test_workspaces_that_are_no_memory_of_the_gpu_are_refused():
+    g = torch.ones((300, 300), device=dev())
+    y = torch.full_like(g, 7.0)
+    small, host = torch.empty(256, dtype=torch.uint8, device=dev())[:1].expand(1 << 30), torch.empty(1 << 24, dtype=torch.uint8)
+    for stream in (None, torch.cuda.current_stream()):  # (the native call, and the general way)
+        assert F.orthogonalize(g, y, small, stream=stream) == F.UnsupportedDimension
+        with pytest.raises(ValueError):
+            F.orthogonalize(g, y, host, stream=stream)
+        with pytest.raises(ValueError):
+            F.layer_norm_bprop(g, None, g[0], g[0], g, y, y[0], y[0], host, stream=stream)
+    torch.cuda.synchronize()
+    assert bool((y == 7).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape", [(20, 40), (130, 150), (300, 1200)], ids=str)
+def test_matrices_far_smaller_than_eps(shape, dtype):
+    """X is then small in front of every step, and the least step of what is held between products, 2^-35, counts."""
+    gen = torch.Generator().manual_seed(7)
+    g = randn(gen, *shape).to(dtype).to(dev())
+    for eps in (1e1, 1e4, 1e6, 1e9):
+        updates(g, eps=eps * float(g.norm()))
