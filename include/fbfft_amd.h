@@ -457,8 +457,9 @@ int fbfft_layer_norm_bprop(const fbfft_array* input, const fbfft_array* weight, 
  * input, output: [rows][cols] or [batch][rows][cols] of one type, any strides, not overlapping; each matrix of a batch
  * by itself.  coefficients: 3 steps numbers in host memory, read during the call.  Products are summed in 32 bits;
  * between them X, A and b A + c A A are held as two 16-bit pieces of a value, 22 bits of it together, and products
- * leave out that of the second pieces: about what 32-bit arithmetic gives, for all types and shapes.  A matrix of zeros
- * gives zeros where eps > 0; values that are not finite make all of their matrix NaN.
+ * leave out that of the second pieces: about what 32-bit arithmetic gives, for all types and shapes (the pieces' least
+ * step is 2^-35: of X far below that, as where |input| is 2^-20 eps and less, few bits are left).  A matrix of zeros gives
+ * zeros where eps > 0; values that are not finite make all of their matrix NaN.
  * steps from 1 to 32; eps and scale finite, eps >= 0; coefficients under which a singular value in [0, 1] or what the
  * products make of it could pass 32 are refused (UnsupportedSize): the pieces end at 64.  rows, cols up to 65536;
  * a batch up to 65535 matrices, of small ones (up to 32 x 1152, 64 x 480, 96 x 192) any number.
