@@ -484,8 +484,8 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void product(PairArgs g, 
   }
 }
 
-// Results of a symmetric product from the sums of `ranges` ranges of k, in their order: a workgroup to 32 rows of up to 64 columns of a tile, eight ranges'
-// sums on their way at once (60 x 60 in 13 ranges 5.5 us, by a wave and range after range 11.9).
+// Results of a symmetric product from the sums of `ranges` ranges of k, in their order: a workgroup to 32 rows of up to 64 columns
+// of a tile, eight ranges' sums on their way at once (60 x 60 in 13 ranges 5.5 us, by a wave and range after range 11.9).
 template <int BM, int BN>
 __global__ __launch_bounds__(256) void join(PairArgs g, int ranges, int tiles) {
   constexpr int COLS = BN < 64 ? BN : 64, ACROSS = BN / COLS, BLOCKS = BM / 32 * ACROSS, AHEAD = 8;  // BLOCKS: of a tile

@@ -26,7 +26,6 @@ enum PairKind { Small16, Small32, Deep64, Wide64, Deep128, Wide128, Wide256 };
 struct PairPlan {
   int kind, side;  // side: of a tile
   long tiles, ranges, range;
-  double time;  // expected
 };
 
 // The kernel with the least expected time, in us, from what each takes for a step of 32 k: `alone` where workgroups have compute
@@ -62,7 +61,7 @@ inline PairPlan planOf(bool symmetric, long batch, long M, long N, long K, doubl
       if (used > 1) time += 4.5 + (double)batch * tiles * used * o.side * o.side * 8 / 4e6;
       if (least == 0 || time < least) {
         least = time;
-        best = PairPlan{o.kind, o.side, tiles < 8 ? tiles : (tiles + 7) / 8 * 8, used, 32 * range, time};
+        best = PairPlan{o.kind, o.side, tiles < 8 ? tiles : (tiles + 7) / 8 * 8, used, 32 * range};
       }
     }
   }
